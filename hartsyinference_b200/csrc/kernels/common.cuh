@@ -45,6 +45,7 @@ enum KernelId : uint32_t {
   kKernelAllToAll = 10,
   kKernelWaitProbe = 11,
   kKernelDpExchange = 12,
+  kKernelKv4 = 13,
 };
 
 struct DeviceStatus {

@@ -60,6 +60,7 @@ from .core import (  # noqa: F401
     sample_tokens,
     selective_scan,
 )
+from .kv4 import attn_decode_kv4, attn_prefill_kv4, kv4_cache, kv4_gather, rope_kv4  # noqa: F401
 from .mixers import (  # noqa: F401
     ChannelScanWeights,
     DeltaWeights,
@@ -104,7 +105,7 @@ from . import reference  # noqa: F401
 def _install_ranges() -> None:
     import sys
     from ..utils.profiling import traced
-    from . import core, mixers
+    from . import core, kv4, mixers
     mod = sys.modules[__name__]
     for name in ("linear", "norm", "glu", "rope_kv", "attn_decode", "attn_prefill_paged", "attn_paged_biased", "attention",
                  "embedding", "argmax", "quant_fp8_act", "grouped_linear", "grouped_linear_dynamic", "moe_route",
@@ -121,6 +122,8 @@ def _install_ranges() -> None:
                  "head_linear", "head_scan", "kv_store", "latent_attn", "latent_gather", "latent_prep", "pair_linear_f32", "poly_norm",
                  "qk_rope_store", "residual_norm", "rope_table", "router", "short_conv", "side_gate"):
         setattr(mod, name, traced(name)(getattr(mixers, name)))
+    for name in ("attn_decode_kv4", "attn_prefill_kv4", "kv4_gather", "rope_kv4"):
+        setattr(mod, name, traced(name)(getattr(kv4, name)))
 
 
 _install_ranges()

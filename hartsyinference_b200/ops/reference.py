@@ -431,6 +431,89 @@ def gather_paged(cache: torch.Tensor, table: torch.Tensor, length: int) -> torch
 
 
 # --------------------------------------------------------------------------------------------
+# 4-bit K/V cache (see ops/kv4.py and csrc/kernels/kv4.cuh)
+# --------------------------------------------------------------------------------------------
+KV4_KEY_EXP, KV4_VALUE_EXP = -6, -10
+
+
+def kv4_blocks(x: torch.Tensor, exp: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """fp32 [..., d] -> codes 1 .. 15 [..., d] and scale bytes [..., d / 32]: per block of 32 the scale is max|x| / 7 with three bits of
+    mantissa (nearest, ties to even), a code the nearest multiple plus 8. The scale of byte b is the half with bits b << 7, times 2^exp."""
+    b = torch.nan_to_num(x.float(), nan=0.0, posinf=math.inf, neginf=-math.inf).unflatten(-1, (-1, 32))
+    f = b.abs().amax(-1)
+    f = f / torch.full_like(f, 7.0) * 2.0 ** -exp
+    bits = f.view(torch.int32)
+    byte = (((bits + 0x7ffff + ((bits >> 20) & 1)) >> 20) - (112 << 3)).clamp(8, 247)
+    code = torch.round(b / kv4_scales(byte, exp)[..., None]).clamp(-7, 7) + 8
+    return code.to(torch.uint8).flatten(-2), byte.to(torch.uint8)
+
+
+def kv4_scales(byte: torch.Tensor, exp: int) -> torch.Tensor:
+    return (byte.to(torch.int32) << 7).to(torch.int16).view(torch.float16).float() * 2.0 ** exp
+
+
+def kv4_held(x: torch.Tensor, exp: int) -> torch.Tensor:
+    """The values that x [..., d] is held as, fp32."""
+    code, byte = kv4_blocks(x, exp)
+    return ((code.float() - 8).unflatten(-1, (-1, 32)) * kv4_scales(byte, exp)[..., None]).flatten(-2)
+
+
+def kv4_places(d: int, values: bool) -> torch.Tensor:
+    """Which nibble of a token's row holds each value, [16, d] (the token of the unit, the value)."""
+    c = torch.arange(d)
+    if not values:
+        return ((c % 8 // 2 * (d // 32) + c // 32) * 8 + c % 32 // 8 + 4 * (c % 2)).expand(16, d)
+    turn = (torch.arange(16)[:, None] & 2) * (2 if d == 128 else 0)
+    return ((c % 8 ^ turn) * (d // 64) + c // 64) * 8 + c % 64 // 8
+
+
+def kv4_store(cache: torch.Tensor, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+    """k, v fp32 [T, hkv, d] to their slots (below 0, or behind the pool: not stored)."""
+    d, page = k.shape[-1], cache.shape[2] * 16
+    on = (slots >= 0) & (slots < cache.shape[0] * page)
+    s = slots[on].long()
+    pg, unit, t = s // page, s % page // 16, s % 16
+    for plane, (x, exp) in enumerate(((k, KV4_KEY_EXP), (v, KV4_VALUE_EXP))):
+        code, byte = kv4_blocks(x[on], exp)
+        nib = torch.empty_like(code).scatter_(-1, kv4_places(d, plane == 1)[t][:, None].expand(code.shape), code)
+        for i in range(s.numel()):
+            row = cache[pg[i], :, unit[i], plane]
+            row[:, t[i] * (d // 2):(t[i] + 1) * (d // 2)] = nib[i, :, 0::2] | (nib[i, :, 1::2] << 4)
+            row[:, 8 * d + t[i] * (d // 32):8 * d + (t[i] + 1) * (d // 32)] = byte[i]
+
+
+def kv4_sequence(cache: torch.Tensor, table: torch.Tensor, length: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of the first ``length`` tokens of a sequence, fp32 [length, hkv, d]."""
+    pages, hkv, units, _, nbytes = cache.shape
+    d, out = 2 * nbytes // 17, []
+    used = cache[table[:(length + units * 16 - 1) // (units * 16)].long()]
+    for plane, exp in enumerate((KV4_KEY_EXP, KV4_VALUE_EXP)):
+        rows = used[:, :, :, plane]                                     # [n, hkv, units, bytes]
+        code = rows[..., :8 * d].unflatten(-1, (16, d // 2))
+        nib = torch.stack([code & 15, code >> 4], -1).flatten(-2)
+        x = torch.gather(nib, -1, kv4_places(d, plane == 1).expand(nib.shape)).float() - 8
+        x = (x.unflatten(-1, (-1, 32)) * kv4_scales(rows[..., 8 * d:].unflatten(-1, (16, d // 32)), exp)[..., None]).flatten(-2)
+        out.append(x.permute(0, 2, 3, 1, 4).reshape(-1, hkv, d)[:length])
+    return out[0], out[1]
+
+
+def rope64(qkv: torch.Tensor, positions: torch.Tensor, hq: int, hkv: int, d: int, inv_freq: Optional[torch.Tensor], style: int,
+           q_norm_w: Optional[torch.Tensor], k_norm_w: Optional[torch.Tensor], eps: float) -> tuple:
+    """q, k, v fp32 [T, heads, d] of packed rows: RMS norm of the heads of q and k (sums in 64 bits) and rotation by angles formed
+    in 64 bits."""
+    x = qkv.float().reshape(qkv.shape[0], hq + 2 * hkv, d)
+    out = []
+    for y, w in ((x[:, :hq], q_norm_w), (x[:, hq:hq + hkv], k_norm_w)):
+        if w is not None:
+            y = y * (1 / (y.double().square().mean(-1, keepdim=True) + eps).sqrt()).float() * w.float()
+        if inv_freq is not None:
+            ang = positions.double()[:, None] * inv_freq.double()
+            y = turn(y, torch.stack([ang.cos(), ang.sin()], -1).float(), style == 1)
+        out.append(y)
+    return out[0], out[1], x[:, hq + hkv:]
+
+
+# --------------------------------------------------------------------------------------------
 # diffusion scheduler step
 # --------------------------------------------------------------------------------------------
 def cfg_euler(z: torch.Tensor, cond: torch.Tensor, uncond: Optional[torch.Tensor], g: float, dt: float) -> torch.Tensor:
