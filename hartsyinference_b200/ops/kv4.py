@@ -172,21 +172,22 @@ def attn_decode_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Ten
         with _on(q.device):
             q = _dense(q)
             out = torch.empty_like(q)
-            rc = _attend(q, out, cache, block_table, kv_lens, None, 1, hkv, page, pages, True, window, scale, softcap)
-            N.check(rc, "b200_attn_kv4")
+            if block_table.shape[1] == 0 or pages == 0:
+                out.zero_()
+            elif b:
+                L, longest = N.lib(), block_table.shape[1] * page
+                longest = longest if max_kv_len is None else min(max_kv_len, longest)
+                # parts of sequences: memory of this call alone, since other streams may be in the same op
+                need = L.b200_attn_decode_kv4_workspace(b, hq, hkv, d, longest)
+                ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+                rc = L.b200_attn_decode_kv4(q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), b, hq, hkv, d,
+                                            page, block_table.shape[1], pages, longest, int(window), float(scale), float(softcap), N.ptr(ws), need,
+                                            N.state(q.device).status.data_ptr(), N.stream())
+                N.check(min(rc, 0), "b200_attn_decode_kv4", rc)
     if not emit_fp8:
         return out
     with _on(q.device) if q.is_cuda else contextlib.nullcontext():
         return out if emit_bf16 else None, quant_fp8_act(out.reshape(b, hq * d))
-
-
-def _attend(q, out, cache, block_table, kv_lens, cu_q, max_q_len, hkv, page, pages, causal, window, scale, softcap) -> int:
-    if block_table.shape[1] == 0 or pages == 0:
-        out.zero_()
-        return 0
-    return N.lib().b200_attn_kv4(q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), N.ptr(cu_q), kv_lens.numel(),
-                                 max_q_len, q.shape[1], hkv, q.shape[2], page, block_table.shape[1], pages, int(causal), int(window), float(scale),
-                                 float(softcap), N.state(q.device).status.data_ptr(), N.stream())
 
 
 def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: torch.Tensor,
@@ -205,6 +206,10 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     with _on(q.device):
         q = _dense(q)
         out = torch.empty_like(q)
-        rc = _attend(q, out, cache, block_table, kv_lens, cu_q, int(max_q_len), hkv, page, pages, causal, window, scale, softcap)
+        if block_table.shape[1] == 0 or pages == 0:
+            return out.zero_()
+        rc = N.lib().b200_attn_kv4(q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(),
+                                   kv_lens.numel(), int(max_q_len), q.shape[1], hkv, q.shape[2], page, block_table.shape[1], pages, int(causal),
+                                   int(window), float(scale), float(softcap), N.state(q.device).status.data_ptr(), N.stream())
         N.check(rc, "b200_attn_kv4")
     return out

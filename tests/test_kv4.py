@@ -50,15 +50,23 @@ def _filled(lens, hkv, d, page, seed=0, fill=0xFF):
     return cache, table
 
 
+def _value_scales(cache, table, n):
+    """The scale of every value of a sequence, [n, hkv, d] in 64 bits."""
+    d = 2 * cache.shape[-1] // 17
+    rows = cache[table[:-(-n // (cache.shape[2] * 16))].long()][:, :, :, 1, 8 * d:].unflatten(-1, (16, d // 32))
+    return R.kv4_scales(rows, R.KV4_VALUE_EXP).double().permute(0, 2, 3, 1, 4).reshape(-1, cache.shape[1], d // 32)[:n].repeat_interleave(32, -1)
+
+
 def _plain(q, cache, table, lens, cuts, causal=True, scale=None, softcap=0.0, window=0):
-    """Attention in 64 bits: (out, sum of p |v|)."""
+    """Attention in 64 bits: (out, sum of p |v|, sum of p times v's scale)."""
     hq, d = q.shape[1:]
-    out, size = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    out, size, scales = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(3))
     for i, n in enumerate(lens):
         a, b = cuts[i], cuts[i + 1]
         if not n or a == b:
             continue
-        k, v = (x.double().repeat_interleave(hq // x.shape[1], 1) for x in R.kv4_sequence(cache, table[i], n))
+        k, v = (x.double() for x in R.kv4_sequence(cache, table[i], n))
+        k, v, c = (x.repeat_interleave(hq // x.shape[1], 1) for x in (k, v, _value_scales(cache, table[i], n)))
         s = torch.einsum("qhd,khd->hqk", q[a:b].double(), k) * (1 / math.sqrt(d) if scale is None else scale)
         if softcap:
             s = softcap * torch.tanh(s / softcap)
@@ -67,17 +75,20 @@ def _plain(q, cache, table, lens, cuts, causal=True, scale=None, softcap=0.0, wi
         if window > 0:
             seen = seen & (key > pos - window)
         p = torch.nan_to_num(torch.softmax(s.masked_fill(~seen, -math.inf), -1))
-        out[a:b], size[a:b] = torch.einsum("hqk,khd->qhd", p, v), torch.einsum("hqk,khd->qhd", p, v.abs())
-    return out, size
+        out[a:b], size[a:b], scales[a:b] = (torch.einsum("hqk,khd->qhd", p, x) for x in (v, v.abs(), c))
+    return out, size, scales
 
 
-def _close(got, want, size):
-    """Probabilities are rounded to bf16 or finer before the product with the values (half a step of each: 2^-8 of sum p |v| together), the
-    result to bf16 (2^-8 of it). Scores are sums of 128 products in 32 bits, of which sum |q k| scale is below 2^9 here: off by less than
-    2^9 * 2^-24 * 2 * 2^3 = 2^-11, and so are probabilities and their sum."""
+def _close(got, want, size, scales):
+    """Probabilities are rounded to bf16 before and after the product with a scale (half a step each, 2^-9 twice, of sum p |v|), the
+    result to bf16 (2^-9 of it): 2^-8 of both holds with a half to spare. Scores are sums of 128 products in 32 bits, of
+    which sum |q k| scale is below 2^9 here: off by less than 2^9 * 2^-24 * 2 * 2^3 = 2^-11, and so are probabilities and their sum.
+    Values enter as 128 + code, and 136 is taken off again, 16 keys at a time: two sums of at most 143 p s that are cut to 24 bits,
+    2 * 2^-22 * 143 < 2^-13 of sum p s with two bits to spare."""
     off = (got.double().cpu() - want).abs()
     assert torch.isfinite(got).all()
-    assert (off <= 2.0 ** -8 * (size + want.abs()) + 2.0 ** -10 * size + 1e-30).all(), float((off / (size + 1e-30)).max())
+    bound = 2.0 ** -8 * (size + want.abs()) + 2.0 ** -10 * size + 2.0 ** -13 * scales + 1e-30
+    assert (off <= bound).all(), float((off / bound).max())
 
 
 # ------------------------------------------------------------------------------------------ format (CPU)
@@ -197,8 +208,8 @@ def test_attention_on_cpu(hq, hkv, d):
     cuts = [0, 4, 5, 45]
     q = _normal(45, hq, d, seed=8).to(torch.bfloat16)
     got = ops.attn_prefill_kv4(q, cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor(cuts, dtype=torch.int32), max(each), window=7, softcap=20.0)
-    want, size = _plain(q, cache, table, lens, cuts, window=7, softcap=20.0)
-    _close(got, want, size)
+    want = _plain(q, cache, table, lens, cuts, window=7, softcap=20.0)
+    _close(got, *want)
 
 
 # ------------------------------------------------------------------------------------------ kernels
@@ -285,12 +296,12 @@ def test_decode_kernel(hq, hkv, d, kw, page):
     lens = [1, 0, 15, 16, 17, 64, 65, 400, 1777]
     cache, table = _filled(lens, hkv, d, page)
     q = _normal(len(lens), hq, d, seed=9).to(torch.bfloat16)
-    want, size = _plain(q, cache, table, lens, list(range(len(lens) + 1)), **kw)
+    want = _plain(q, cache, table, lens, list(range(len(lens) + 1)), **kw)
     dev = _cuda(q, cache, table, torch.tensor(lens, dtype=torch.int32))
     got = ops.attn_decode_kv4(*dev, **kw)
-    _close(got, want, size)
+    _close(got, *want)
     for most in (max(lens), 40000):                                                    # how the work is cut
-        _close(ops.attn_decode_kv4(*dev, max_kv_len=most, **kw), want, size)
+        _close(ops.attn_decode_kv4(*dev, max_kv_len=most, **kw), *want)
     assert torch.equal(got, ops.attn_decode_kv4(*dev, **kw))
 
 
@@ -303,8 +314,8 @@ def test_prefill_kernel(hq, hkv, d, kw):
     cache, table = _filled(lens, hkv, d, 16)
     cuts = torch.tensor([0, *each]).cumsum(0).tolist()
     q = _normal(sum(each), hq, d, seed=9).to(torch.bfloat16)
-    want, size = _plain(q, cache, table, lens, cuts, **kw)
+    want = _plain(q, cache, table, lens, cuts, **kw)
     dev = _cuda(q, cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor(cuts, dtype=torch.int32))
     got = ops.attn_prefill_kv4(*dev, max(each), **kw)
-    _close(got, want, size)
-    _close(ops.attn_prefill_kv4(*dev, max(each) + 300, max_kv_len=333, **kw), want, size)
+    _close(got, *want)
+    _close(ops.attn_prefill_kv4(*dev, max(each) + 300, max_kv_len=333, **kw), *want)
