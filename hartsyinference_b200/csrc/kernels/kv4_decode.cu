@@ -28,8 +28,8 @@ int num_sms();      // of the current device, see gemm_tcgen05.cu
 
 constexpr int kDec4Warps = 8;
 constexpr int kDec4Threads = kDec4Warps * 32;
-constexpr int kDec4Stages = 4;
-constexpr int kDec4MaxSeqs = 2048;         // of a batch that is cut into shares: their unit counts are in shared memory
+constexpr int kDec4Stages = 2;            // of a warp's ring, two units each
+constexpr int kDec4MaxSeqs = 256;          // of a batch that is cut into shares: their unit counts are in shared memory
 constexpr float kDec4Gap = 8.f;            // the reference of the exponentials is raised once a score passes it by this many powers of two
 constexpr float kDec4Log2e = 1.4426950408889634f;
 
@@ -49,12 +49,22 @@ __device__ __forceinline__ uint32_t scaled_bf16x2(uint32_t x, uint32_t s) {
   const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&s));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
-__device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+// d += A B. Not volatile: products of one unit's keys and another's values are interleaved.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (x & mask) | bits in one instruction
+__device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -77,9 +87,11 @@ __device__ __forceinline__ int dec4_units(const DecodeKv4Params& p, int len, int
   return len > 0 ? (len + kKv4Unit - 1) / kKv4Unit - first : 0;
 }
 
-// Bytes of dynamic shared memory: rings, the warps' results of one tile of eight heads, the prefix.
-__host__ __device__ constexpr int dec4_ring_bytes(int d) { return kDec4Warps * kDec4Stages * kv4_unit_bytes(d); }
-__host__ __device__ constexpr int dec4_merge_bytes(int d) { return kDec4Warps * 8 * (d + 4) * 4; }
+// Dynamic shared memory: rings, the warps' results of four heads, queries and what the sums of their products start from, the prefix.
+__host__ __device__ constexpr int dec4_ring_bytes(int d) { return kDec4Warps * kDec4Stages * 2 * kv4_unit_bytes(d); }
+__host__ __device__ constexpr int dec4_merge_bytes(int d) { return kDec4Warps * 4 * (d + 4) * 4; }
+__host__ __device__ constexpr int dec4_query_bytes(int d, int nt) { return nt * (d / 32) * 2 * 512; }
+__host__ __device__ constexpr int dec4_smem_bytes(int d, int nt) { return dec4_ring_bytes(d) + dec4_merge_bytes(d) + dec4_query_bytes(d, nt) + (kDec4MaxSeqs + 1) * 4; }
 
 template <int D, int NT, bool kShares>
 __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4_kernel(const DecodeKv4Params p) {
@@ -88,12 +100,14 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
   constexpr int kUnit = kv4_unit_bytes(D), kPlane = kv4_plane_bytes(D), kBlocks = D / 32, kWords = D / 32, kPitch = D + 4;
   __shared__ uint64_t full[kDec4Warps][kDec4Stages];
   __shared__ float merge_ml[kDec4Warps][8][2];
+  __shared__ float head_factor[NT][8];
   __shared__ int warp_units[kDec4Warps];
   __shared__ uint32_t abort_word;
   float* merge = reinterpret_cast<float*>(smem + dec4_ring_bytes(D));
-  int* prefix = reinterpret_cast<int*>(smem + dec4_ring_bytes(D) + dec4_merge_bytes(D));
+  uint4* queries = reinterpret_cast<uint4*>(smem + dec4_ring_bytes(D) + dec4_merge_bytes(D));     // [tile][block][queries | starts][lane]
+  int* prefix = reinterpret_cast<int*>(smem + dec4_ring_bytes(D) + dec4_merge_bytes(D) + dec4_query_bytes(D, NT));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-  uint8_t* ring = smem + warp * kDec4Stages * kUnit;
+  uint8_t* ring = smem + warp * kDec4Stages * 2 * kUnit;
   volatile uint32_t* abort_flag = &abort_word;
   if (lane == 0) {
 #pragma unroll
@@ -161,180 +175,193 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       s = only_seq; h = blockIdx.x - only_seq * heads_v; at = 0; n = only_units; first = only_first;
     }
   };
-  // units of this warp: f0 + warp + 8 i, i below mine
+  // pairs of units of this warp: units 2 (warp + 8 i) and the next of the share, i below mine
   const int share = static_cast<int>(f1 - f0);
-  const int mine = share > warp ? (share - warp + kDec4Warps - 1) / kDec4Warps : 0;
-  const uint8_t* src = nullptr;                      // lane j: address of unit 32 (i / 32) + j of the warp
+  const int mine = share > 2 * warp ? (share - 2 * warp + 2 * kDec4Warps - 1) / (2 * kDec4Warps) : 0;
+  const uint8_t* src = nullptr;                      // lane j: address of unit j % 2 of pair 16 (i / 16) + j / 2 of the warp
   auto addresses = [&](int i0) {
-    const int i = i0 + lane;
-    if (i >= mine) return;
+    const int rel = 2 * (warp + (i0 + (lane >> 1)) * kDec4Warps) + (lane & 1);
+    src = nullptr;
+    if (rel >= share) return;
     int s, h, n, first;
     long long at;
-    const long long f = f0 + warp + static_cast<long long>(i) * kDec4Warps;
-    find(f, s, h, at, n, first);
-    src = kv4_unit<D>(p.pool, p.pool.block_table + static_cast<long long>(s) * p.pool.max_pages, h / p.chunks, first + static_cast<int>(f - at), kKernelKv4);
+    find(f0 + rel, s, h, at, n, first);
+    src = kv4_unit<D>(p.pool, p.pool.block_table + static_cast<long long>(s) * p.pool.max_pages, h / p.chunks, first + static_cast<int>(f0 + rel - at), kKernelKv4);
   };
-  auto fetch = [&](int i) {
+  // pair i into slot `to` of the ring; a unit behind the share is left out
+  auto fetch = [&](int i, int to) {
     if (i >= mine) return;
-    if ((i & 31) == 0 && i > 0) addresses(i);
-    if ((i & 31) == lane) {
-      uint64_t* bar = &full[warp][i % kDec4Stages];
-      mbar_arrive_expect_tx(bar, kUnit);
-      bulk_load(ring + (i % kDec4Stages) * kUnit, src, kUnit, bar);
+    if ((i & 15) == 0 && i > 0) addresses(i);
+    if ((i & 15) == lane >> 1) {
+      if ((lane & 1) == 0) mbar_arrive_expect_tx(&full[warp][to], 2 * (warp + i * kDec4Warps) + 1 < share ? 2 * kUnit : kUnit);
+      if (src) bulk_load(ring + (2 * to + (lane & 1)) * kUnit, src, kUnit, &full[warp][to]);
     }
   };
   addresses(0);
 #pragma unroll
-  for (int i = 0; i < kDec4Stages; ++i) fetch(i);
+  for (int i = 0; i < kDec4Stages; ++i) fetch(i, i);
+
+  const int ka = (g & 1) ? 7 - (g >> 1) : g >> 1;    // keys of rows g and g + 8: ka, ka + 8
+  // where a lane reads in a unit: its words of keys ka and of the values of keys tq and 7 - tq, and their scales
+  const int k_at = ka * (D / 2) + tq * (D / 8), ks_at = 8 * D + ka * (D / 32);
+  const int v_at = kPlane + tq * (D / 2) + (D == 128 ? (g ^ ((tq & 2) << 1)) * 8 : g * 4), vs_at = kPlane + 8 * D + tq * (D / 32);
+  const int w_at = kPlane + (7 - tq) * (D / 2) + (D == 128 ? (g ^ (((7 - tq) & 2) << 1)) * 8 : g * 4), ws_at = kPlane + 8 * D + (7 - tq) * (D / 32);
+  constexpr int kOther = 8 * (D / 2), kOtherScale = 8 * (D / 32);          // eight keys on
 
   bool ok = true;
-  int i = 0;
-  long long f = f0;
-  bool empty = !kShares && f0 == f1;                 // a sequence without keys: zeros
-  while (f < f1 || empty) {
+  int i = 0, slot = 0, phase = 0;                    // pair i of the warp is in `slot`
+  int at_rel = 0;                                    // start of the current sequence's units in the share
+  bool empty = !kShares && share == 0;               // a sequence without keys: zeros
+  for (int done = 0; done < share || empty;) {
     int s, h, n, first;
-    long long at;
-    find(f, s, h, at, n, first);
-    const long long stop = empty ? f1 : min(at + n, f1);
+    {
+      long long at;
+      find(f0 + done, s, h, at, n, first);
+      at_rel = static_cast<int>(at - f0);
+    }
+    const int stop = min(at_rel + n, share);
     const int kv_head = h / p.chunks, head0 = kv_head * p.group + (h - kv_head * p.chunks) * p.chunk_heads;
     const int heads = min(p.chunk_heads, (kv_head + 1) * p.group - head0);
     const int len = empty ? 0 : kv4_length(p.pool, p.kv_lens[s], kKernelKv4);
     const int start = p.window > 0 ? max(0, len - p.window) : 0;
+    const int last = min(len, (first + share - at_rel) * kKv4Unit);      // keys from here on are not this block's
 
-    // queries of heads 8 t + g in half precision, with a power of two taken out so that the largest is in [2^12, 2^13)
-    uint32_t qb[NT][D / 16][2];
-    float init[NT][kBlocks][2], factor[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    // Queries of heads 8 t + g in half precision, with a power of two taken out so that the largest is in [2^12, 2^13); by warp t for all
+    if (warp < NT) {
+      const int t = warp;
       const bool on = 8 * t + g < heads;
       const __nv_bfloat16* qh = p.q + (static_cast<long long>(s) * p.hq + head0 + (on ? 8 * t + g : 0)) * D;
+      uint32_t qb[D / 16][2];
       float amax = 0.f;
 #pragma unroll
       for (int m = 0; m < D / 16; ++m)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          qb[t][m][r] = on ? *reinterpret_cast<const uint32_t*>(qh + m * 16 + r * 8 + tq * 2) : 0u;
-          const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qb[t][m][r]));
+          qb[m][r] = on ? *reinterpret_cast<const uint32_t*>(qh + m * 16 + r * 8 + tq * 2) : 0u;
+          const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qb[m][r]));
           amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
         }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const int e = amax > 0.f ? min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 12, -100), 85) : 0;
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      float sum[kBlocks];
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) sum[b] = 0.f;
-#pragma unroll
-      for (int m = 0; m < D / 16; ++m)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qb[t][m][r]));
-          const float sh = r ? down * 0.0625f : down;                   // places 8 .. 15 meet codes times 16
-          qb[t][m][r] = pack_f16x2(v.x * sh, v.y * sh);
-          const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&qb[t][m][r]));
-          sum[m / 2] += (w.x + w.y) * (r ? 16.f : 1.f);
-        }
-      // what the partial sums start from: -8 * 2^-24 * sum of the block's queries, for the two heads of this lane's results
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
-        float x = sum[b];
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        x *= -4.76837158203125e-7f;
-        init[t][b][0] = __shfl_sync(0xffffffffu, x, 8 * tq);
-        init[t][b][1] = __shfl_sync(0xffffffffu, x, 8 * tq + 4);
+        float sum = 0.f;
+#pragma unroll
+        for (int m = 2 * b; m < 2 * b + 2; ++m)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qb[m][r]));
+            const float sh = r ? down * 0.0625f : down;                 // places 8 .. 15 meet codes times 16
+            qb[m][r] = pack_f16x2(v.x * sh, v.y * sh);
+            const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&qb[m][r]));
+            sum += (w.x + w.y) * (r ? 16.f : 1.f);
+          }
+        queries[((t * kBlocks + b) * 2) * 32 + lane] = make_uint4(qb[2 * b][0], qb[2 * b][1], qb[2 * b + 1][0], qb[2 * b + 1][1]);
+        // what the sums start from: -8 * 2^-24 times the block's queries, for the two heads of a lane's results
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum *= -4.76837158203125e-7f;
+        const uint32_t s0 = __float_as_uint(__shfl_sync(0xffffffffu, sum, 8 * tq)), s1 = __float_as_uint(__shfl_sync(0xffffffffu, sum, 8 * tq + 4));
+        queries[((t * kBlocks + b) * 2 + 1) * 32 + lane] = make_uint4(s0, s1, s0, s1);
       }
       // codes are times 2^24, scales (as fp32 with bits byte << 20 under an exponent of 96) times 2^(16 + key exponent)
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        factor[t][j] = __shfl_sync(0xffffffffu, up, 8 * tq + 4 * j) * __uint_as_float(static_cast<uint32_t>(127 + 24 + 16 + kKv4KeyExp) << 23);
+      if (tq == 0)
+        head_factor[t][g] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (p.cap_out == 0.f ? p.scale_log2 : p.cap_in) *
+                            __uint_as_float(static_cast<uint32_t>(127 + 24 + 16 + kKv4KeyExp) << 23);
     }
-    float o[NT][D / 16][4], mx[NT][2], l[NT][2];
+    __syncthreads();
+
+    float o[NT][D / 16][4], mx[NT][2], line[NT][2], l[NT][2];      // line: what a score has to pass to raise mx
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int m = 0; m < D / 16; ++m)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[t][m][j] = 0.f;
-      mx[t][0] = mx[t][1] = -INFINITY;
+      mx[t][0] = mx[t][1] = line[t][0] = line[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
     }
-
-    for (; ok; ++i) {
-      const long long fi = f0 + warp + static_cast<long long>(i) * kDec4Warps;
-      if (fi >= stop) break;
-      const int slot = i % kDec4Stages;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[warp][slot], (i / kDec4Stages) & 1, abort_flag))) { ok = false; break; }
-      const uint8_t* unit = ring + slot * kUnit;
-      const int key0 = (first + static_cast<int>(fi - at)) * kKv4Unit;
-      const bool whole = key0 >= start && key0 + kKv4Unit <= len;
-      const int ka = (g & 1) ? 7 - (g >> 1) : g >> 1;                   // keys of rows g and g + 8: ka, ka + 8
-      // ---- scores
-      float sc[NT][4];
-      {
-        uint32_t wa[kWords], wb[kWords], sa, sb;
-        if (D == 128) {
-          const uint4 a = *reinterpret_cast<const uint4*>(unit + ka * 64 + tq * 16), b = *reinterpret_cast<const uint4*>(unit + (ka + 8) * 64 + tq * 16);
-          wa[0] = a.x; wa[1] = a.y; wa[kWords - 2] = a.z; wa[kWords - 1] = a.w;
-          wb[0] = b.x; wb[1] = b.y; wb[kWords - 2] = b.z; wb[kWords - 1] = b.w;
-          sa = *reinterpret_cast<const uint32_t*>(unit + 8 * D + ka * 4);
-          sb = *reinterpret_cast<const uint32_t*>(unit + 8 * D + (ka + 8) * 4);
-        } else {
-          const uint2 a = *reinterpret_cast<const uint2*>(unit + ka * 32 + tq * 8), b = *reinterpret_cast<const uint2*>(unit + (ka + 8) * 32 + tq * 8);
-          wa[0] = a.x; wa[1] = a.y;
-          wb[0] = b.x; wb[1] = b.y;
-          sa = *reinterpret_cast<const uint16_t*>(unit + 8 * D + ka * 2);
-          sb = *reinterpret_cast<const uint16_t*>(unit + 8 * D + (ka + 8) * 2);
-        }
+    uint4 q[NT][kBlocks];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          const uint32_t xa = wa[b], xb = wb[b], ya = xa >> 8, yb = xb >> 8;
-          const uint32_t a0[4] = {xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u};
-          const uint32_t a1[4] = {ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u, yb & 0x00f000f0u};
-          const float fa = __uint_as_float((((b < 3 ? sa << (20 - 8 * b) : sa >> 4)) & 0x0ff00000u) | 0x30000000u);
-          const float fb = __uint_as_float((((b < 3 ? sb << (20 - 8 * b) : sb >> 4)) & 0x0ff00000u) | 0x30000000u);
+      for (int b = 0; b < kBlocks; ++b) q[t][b] = queries[((t * kBlocks + b) * 2) * 32 + lane];
+    auto key_products = [&](const uint8_t* unit, float (&sc)[NT][4]) {
+      uint32_t wa[kWords], wb[kWords], sa, sb;
+      if (D == 128) {
+        const uint4 a = *reinterpret_cast<const uint4*>(unit + k_at), b = *reinterpret_cast<const uint4*>(unit + k_at + kOther);
+        wa[0] = a.x; wa[1] = a.y; wa[kWords - 2] = a.z; wa[kWords - 1] = a.w;
+        wb[0] = b.x; wb[1] = b.y; wb[kWords - 2] = b.z; wb[kWords - 1] = b.w;
+        sa = *reinterpret_cast<const uint32_t*>(unit + ks_at);
+        sb = *reinterpret_cast<const uint32_t*>(unit + ks_at + kOtherScale);
+      } else {
+        const uint2 a = *reinterpret_cast<const uint2*>(unit + k_at), b = *reinterpret_cast<const uint2*>(unit + k_at + kOther);
+        wa[0] = a.x; wa[1] = a.y;
+        wb[0] = b.x; wb[1] = b.y;
+        sa = *reinterpret_cast<const uint16_t*>(unit + ks_at);
+        sb = *reinterpret_cast<const uint16_t*>(unit + ks_at + kOtherScale);
+      }
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            float acc[4] = {init[t][b][0], init[t][b][1], init[t][b][0], init[t][b][1]};
-            mma_f16_16816(acc, a0, qb[t][2 * b][0], qb[t][2 * b][1]);
-            mma_f16_16816(acc, a1, qb[t][2 * b + 1][0], qb[t][2 * b + 1][1]);
-            sc[t][0] = fmaf(acc[0], fa, sc[t][0]);
-            sc[t][1] = fmaf(acc[1], fa, sc[t][1]);
-            sc[t][2] = fmaf(acc[2], fb, sc[t][2]);
-            sc[t][3] = fmaf(acc[3], fb, sc[t][3]);
-          }
+      for (int b = 0; b < kBlocks; ++b) {
+        const uint32_t xa = wa[b], xb = wb[b], ya = xa >> 8, yb = xb >> 8;
+        const uint32_t a0[4] = {xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u};
+        const uint32_t a1[4] = {ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u, yb & 0x00f000f0u};
+        const float fa = __uint_as_float(masked_or(b < 3 ? sa << (20 - 8 * b) : sa >> 4, 0x0ff00000u, 0x30000000u));
+        const float fb = __uint_as_float(masked_or(b < 3 ? sb << (20 - 8 * b) : sb >> 4, 0x0ff00000u, 0x30000000u));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float4 from = *reinterpret_cast<const float4*>(&queries[((t * kBlocks + b) * 2 + 1) * 32 + lane]);
+          float acc[4] = {from.x, from.y, from.z, from.w};
+          mma_f16(acc, a0, q[t][b].x, q[t][b].y);
+          mma_f16(acc, a1, q[t][b].z, q[t][b].w);
+          sc[t][0] = b == 0 ? acc[0] * fa : fmaf(acc[0], fa, sc[t][0]);
+          sc[t][1] = b == 0 ? acc[1] * fa : fmaf(acc[1], fa, sc[t][1]);
+          sc[t][2] = b == 0 ? acc[2] * fb : fmaf(acc[2], fb, sc[t][2]);
+          sc[t][3] = b == 0 ? acc[3] * fb : fmaf(acc[3], fb, sc[t][3]);
         }
       }
-      uint32_t pt[NT][2];
+    };
+    // P^T of two units from their scores; key0: the first key of the first one
+    auto softmax = [&](float (&sc)[2][NT][4], uint32_t (&pt)[2][NT][2], int key0) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        const float2 factor = *reinterpret_cast<const float2*>(&head_factor[t][2 * tq]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = sc[t][j] * factor[t][j & 1];
-          if (p.cap_out == 0.f) {
-            sc[t][j] = x * p.scale_log2;
-          } else {                                    // cap tanh(x) = cap - 2 cap / (exp(2 x) + 1)
-            const float e = dec4_exp2(fminf(x * p.cap_in, 126.f));
-            sc[t][j] = p.cap_out - __fdividef(2.f * p.cap_out, e + 1.f);
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[u][t][j] *= j & 1 ? factor.y : factor.x;
+        if (p.cap_out != 0.f)                         // cap tanh(x) = cap - 2 cap / (exp(2 x) + 1)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[u][t][j] = p.cap_out - __fdividef(2.f * p.cap_out, dec4_exp2(fminf(sc[u][t][j], 126.f)) + 1.f);
+      }
+      if (key0 < start || key0 + 2 * kKv4Unit > last)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = key0 + u * kKv4Unit + ka + (j & 2) * 4;
+            if (key < start || key >= last)
+#pragma unroll
+              for (int t = 0; t < NT; ++t) sc[u][t][j] = -INFINITY;
           }
-          if (!whole) {
-            const int key = key0 + ka + (j & 2) * 4;
-            if (key < start || key >= len) sc[t][j] = -INFINITY;
-          }
-        }
-        const bool over = fmaxf(sc[t][0], sc[t][2]) > mx[t][0] + kDec4Gap || fmaxf(sc[t][1], sc[t][3]) > mx[t][1] + kDec4Gap;
-        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float top0 = fmaxf(fmaxf(sc[0][t][0], sc[0][t][2]), fmaxf(sc[1][t][0], sc[1][t][2]));
+        const float top1 = fmaxf(fmaxf(sc[0][t][1], sc[0][t][3]), fmaxf(sc[1][t][1], sc[1][t][3]));
+        if (__any_sync(0xffffffffu, top0 > line[t][0] || top1 > line[t][1])) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(sc[t][j], sc[t][2 + j]);
+            float top = j ? top1 : top0;
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            if (top > mx[t][j]) {
+            if (top > line[t][j]) {
               const float alpha = dec4_exp2(mx[t][j] - top);
               mx[t][j] = top;
+              line[t][j] = top + kDec4Gap;
               l[t][j] *= alpha;
 #pragma unroll
               for (int m = 0; m < D / 16; ++m) {
@@ -344,63 +371,85 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
             }
           }
         }
-        float e[4];
+        // a warp that has seen no key yet: its scores and its reference are both -infinity
+        const float ref0 = mx[t][0] == -INFINITY ? 0.f : mx[t][0], ref1 = mx[t][1] == -INFINITY ? 0.f : mx[t][1];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = dec4_exp2(sc[t][j] - mx[t][j & 1]);
-        l[t][0] += e[0] + e[2];
-        l[t][1] += e[1] + e[3];
-        pt[t][0] = transpose8x8(pack_bf16x2(e[0], e[1]));
-        pt[t][1] = transpose8x8(pack_bf16x2(e[2], e[3]));
-      }
-      // ---- values: keys tq, 7 - tq and the same plus 8
-      {
-        const uint8_t* vp = unit + kPlane;
-        const int r0 = tq, r1 = 7 - tq;
-        uint32_t w[4][D / 64], s4[4];
+        for (int u = 0; u < 2; ++u) {
+          float e[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = (r & 1 ? r1 : r0) + (r >> 1) * 8;
-          if (D == 128) {
-            const uint2 x = *reinterpret_cast<const uint2*>(vp + row * 64 + ((g ^ ((row & 2) << 1)) << 3));
-            w[r][0] = x.x; w[r][D / 64 - 1] = x.y;
-            s4[r] = *reinterpret_cast<const uint32_t*>(vp + 8 * D + row * 4);
-          } else {
-            w[r][0] = *reinterpret_cast<const uint32_t*>(vp + row * 32 + g * 4);
-            s4[r] = *reinterpret_cast<const uint16_t*>(vp + 8 * D + row * 2);
-          }
-        }
-        const uint32_t offset[4] = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};        // -136
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          const uint32_t sel = b == 0 ? 0x4404u : b == 1 ? 0x5414u : b == 2 ? 0x6424u : 0x7434u;
-          // scale bytes of a pair of keys on top of the halves, then where a bf16 has them
-          const uint32_t p0 = ((__byte_perm(s4[0], s4[1], sel) & 0xff00ff00u) >> 4) + kValueBias, p1 = ((__byte_perm(s4[2], s4[3], sel) & 0xff00ff00u) >> 4) + kValueBias;
-          uint32_t a[2][4];
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {              // byte j of this block's half of the words: values of two products' rows g and g + 8
-              const uint32_t x = __byte_perm(w[2 * r][b / 2], w[2 * r + 1][b / 2], (b & 1 ? 0x7632 : 0x5410) + (j ? 0x0101 : 0));
-              a[j][2 * r] = (x & 0x000f000fu) | 0x43004300u;
-              a[j][2 * r + 1] = ((x >> 4) & 0x000f000fu) | 0x43004300u;
-            }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const uint32_t b0 = scaled_bf16x2(pt[t][0], p0), b1 = scaled_bf16x2(pt[t][1], p1);
-            mma_bf16_16816(o[t][2 * b], offset, b0, b1);
-            mma_bf16_16816(o[t][2 * b], a[0], b0, b1);
-            mma_bf16_16816(o[t][2 * b + 1], offset, b0, b1);
-            mma_bf16_16816(o[t][2 * b + 1], a[1], b0, b1);
-          }
+          for (int j = 0; j < 4; ++j) e[j] = dec4_exp2(sc[u][t][j] - (j & 1 ? ref1 : ref0));
+          l[t][0] += e[0] + e[2];
+          l[t][1] += e[1] + e[3];
+          pt[u][t][0] = transpose8x8(pack_bf16x2(e[0], e[1]));
+          pt[u][t][1] = transpose8x8(pack_bf16x2(e[2], e[3]));
         }
       }
+    };
+    // values: keys tq, 7 - tq and the same plus 8. What lies behind the last key has probability 0, and every byte is a finite scale
+    auto value_products = [&](const uint8_t* unit, const uint32_t (&pt)[NT][2]) {
+      uint32_t w[4][D / 64], s4[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint8_t* x = unit + (r & 1 ? w_at : v_at) + (r >> 1) * kOther;
+        const uint8_t* y = unit + (r & 1 ? ws_at : vs_at) + (r >> 1) * kOtherScale;
+        if (D == 128) {
+          const uint2 z = *reinterpret_cast<const uint2*>(x);
+          w[r][0] = z.x; w[r][D / 64 - 1] = z.y;
+          s4[r] = *reinterpret_cast<const uint32_t*>(y);
+        } else {
+          w[r][0] = *reinterpret_cast<const uint32_t*>(x);
+          s4[r] = *reinterpret_cast<const uint16_t*>(y);
+        }
+      }
+      const uint32_t offset[4] = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};        // -136
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        // scale bytes of a pair of keys, then where a bf16 has them
+        const uint32_t sel = 0x0400u + 0x0101u * b;
+        const uint32_t p0 = (__byte_perm(s4[0], s4[1], sel) & 0x00ff00ffu) * 16u + kValueBias, p1 = (__byte_perm(s4[2], s4[3], sel) & 0x00ff00ffu) * 16u + kValueBias;
+        uint32_t a[2][4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {                // byte j of this block's half of the words: values of two products' rows g and g + 8
+            const uint32_t x = __byte_perm(w[2 * r][b / 2], w[2 * r + 1][b / 2], (b & 1 ? 0x7632 : 0x5410) + (j ? 0x0101 : 0));
+            a[j][2 * r] = masked_or(x, 0x000f000fu, 0x43004300u);
+            a[j][2 * r + 1] = masked_or(x >> 4, 0x000f000fu, 0x43004300u);
+          }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const uint32_t b0 = scaled_bf16x2(pt[t][0], p0), b1 = scaled_bf16x2(pt[t][1], p1);
+          mma_bf16(o[t][2 * b], offset, b0, b1);
+          mma_bf16(o[t][2 * b], a[0], b0, b1);
+          mma_bf16(o[t][2 * b + 1], offset, b0, b1);
+          mma_bf16(o[t][2 * b + 1], a[1], b0, b1);
+        }
+      }
+    };
+    // This warp's pairs that have units of this sequence. One that reaches into the next sequence is kept for it.
+    int key0 = (first - at_rel + 2 * (warp + i * kDec4Warps)) * kKv4Unit;
+    for (int rel = 2 * (warp + i * kDec4Warps); ok && rel < stop; key0 += 2 * kDec4Warps * kKv4Unit) {
+      if (!(ok = mbar_wait(&full[warp][slot], phase, abort_flag))) break;
+      const uint8_t* unit = ring + slot * 2 * kUnit;
+      float sc[2][NT][4];
+      uint32_t pt[2][NT][2];
+      key_products(unit, sc[0]);
+      key_products(unit + kUnit, sc[1]);
+      softmax(sc, pt, key0);
+      value_products(unit, pt[0]);
+      value_products(unit + kUnit, pt[1]);
+      rel += 2 * kDec4Warps;
+      if (rel - 2 * kDec4Warps + 1 >= stop && stop < share) break;
       __syncwarp();
-      fetch(i + kDec4Stages);
+      fetch(i + kDec4Stages, slot);
+      ++i;
+      phase ^= slot;
+      slot ^= 1;
     }
 
-    // ---- join the warps' results, eight heads at a time
-    const bool part = kShares && !(at >= f0 && at + n <= f1);
-    float* dst_part = kShares ? p.parts + (static_cast<long long>(blockIdx.x) * 2 + (at < f0 ? 0 : 1)) * p.chunk_heads * (D + 4) : nullptr;
+    // ---- join the warps' results, four heads at a time
+    const bool part = kShares && !(at_rel >= 0 && at_rel + n <= share);
+    float* dst_part = kShares ? p.parts + (static_cast<long long>(blockIdx.x) * 2 + (at_rel < 0 ? 0 : 1)) * p.chunk_heads * (D + 4) : nullptr;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -414,53 +463,60 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
         }
       }
 #pragma unroll
-      for (int m = 0; m < D / 16; ++m)
+      for (int quad = 0; quad < 2; ++quad) {
+        if (8 * t + 4 * quad >= heads) break;
+        if ((tq >> 1) == quad) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float* row = merge + (warp * 8 + 2 * tq + j) * kPitch + m * 16 + g;
-          row[0] = o[t][m][j];
-          row[8] = o[t][m][2 + j];
+          for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float* row = merge + (warp * 4 + 2 * (tq & 1) + j) * kPitch + m * 16 + g;
+              row[0] = o[t][m][j];
+              row[8] = o[t][m][2 + j];
+            }
         }
-      __syncthreads();
-      const int hh = threadIdx.x >> 5;                // a head per warp
-      if (8 * t + hh < heads) {
-        float top = -INFINITY, den = 0.f;
+        __syncthreads();
+        constexpr int kEach = D / 64;                  // values of a thread: two warps per head
+        const int hh = threadIdx.x >> 6, head = 4 * quad + hh, c = (threadIdx.x & 63) * kEach;
+        if (8 * t + head < heads) {
+          float top = -INFINITY, den = 0.f, acc[kEach];
 #pragma unroll
-        for (int w = 0; w < kDec4Warps; ++w) top = fmaxf(top, merge_ml[w][hh][0]);
-        float wt[kDec4Warps];
+          for (int w = 0; w < kDec4Warps; ++w) top = fmaxf(top, merge_ml[w][head][0]);
 #pragma unroll
-        for (int w = 0; w < kDec4Warps; ++w) {
-          wt[w] = merge_ml[w][hh][0] == top ? 1.f : dec4_exp2(merge_ml[w][hh][0] - top);      // a warp without keys: 0, or all are
-          den += wt[w] * merge_ml[w][hh][1];
-        }
-        for (int c = lane * 4; c < D; c += 128) {
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
 #pragma unroll
           for (int w = 0; w < kDec4Warps; ++w) {
-            const float4 x = *reinterpret_cast<const float4*>(merge + (w * 8 + hh) * kPitch + c);
-            acc.x = fmaf(x.x, wt[w], acc.x);
-            acc.y = fmaf(x.y, wt[w], acc.y);
-            acc.z = fmaf(x.z, wt[w], acc.z);
-            acc.w = fmaf(x.w, wt[w], acc.w);
+            const float m = merge_ml[w][head][0], wt = m == top ? 1.f : dec4_exp2(m - top);      // a warp without keys: 0, or all are
+            den = fmaf(wt, merge_ml[w][head][1], den);
+            const float* x = merge + (w * 4 + hh) * kPitch + c;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) acc[j] = fmaf(wt, x[j], acc[j]);
           }
           if (part) {
-            *reinterpret_cast<float4*>(dst_part + (8 * t + hh) * (D + 4) + c) = acc;
+            float* dst = dst_part + (8 * t + head) * (D + 4);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) dst[c + j] = acc[j];
+            if (c == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(top, den);
           } else {
             const float inv = den == 0.f ? 0.f : 1.f / den;
-            *reinterpret_cast<uint2*>(p.out + (static_cast<long long>(s) * p.hq + head0 + 8 * t + hh) * D + c) =
-                make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+            __nv_bfloat16* dst = p.out + (static_cast<long long>(s) * p.hq + head0 + 8 * t + head) * D + c;
+            if (D == 128) *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[kEach - 1] * inv);
+            else dst[0] = __float2bfloat16(acc[0] * inv);
           }
         }
-        if (part && lane == 0) *reinterpret_cast<float2*>(dst_part + (8 * t + hh) * (D + 4) + D) = make_float2(top, den);
+        __syncthreads();
       }
-      __syncthreads();
     }
-    f = stop;
+    done = stop;
     empty = false;
   }
   if (!ok) {
     // copies in flight end before the block does
-    for (int j = i; j < min(i + kDec4Stages, mine); ++j) mbar_wait(&full[warp][j % kDec4Stages], (j / kDec4Stages) & 1, abort_flag, 1 << 22);
+    for (int j = 0; j < kDec4Stages; ++j) {
+      if (i + j < mine) mbar_wait(&full[warp][slot], phase, abort_flag, 1 << 22);
+      phase ^= slot;
+      slot ^= 1;
+    }
     if (lane == 0) report_status(p.pool.status, kWaitTimeout, kKernelKv4, 43, blockIdx.x);
   }
 }
@@ -571,16 +627,16 @@ B200_API int b200_attn_decode_kv4(const void* q, const void* pool, void* out, co
     p.parts = static_cast<float*>(workspace);
     p.prefix = reinterpret_cast<int*>(p.parts + floats);
   }
-  const int fixed = dec4_ring_bytes(d) + dec4_merge_bytes(d), smem = fixed + (shares ? (seqs + 1) * 4 : 0);
+  const bool two = p.chunk_heads > 8;
+  const int most = dec4_smem_bytes(d, two ? 2 : 1), smem = most - (shares ? kDec4MaxSeqs - seqs : kDec4MaxSeqs + 1) * 4;
   static PerDeviceOnce once[8];
   auto go = [&](auto kernel, PerDeviceOnce& o) -> cudaError_t {
     if (o.first_time()) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + (kDec4MaxSeqs + 1) * 4);
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       if (e != cudaSuccess) return e;
     }
     return launch_pdl(kernel, dim3(static_cast<unsigned>(shares ? p.blocks : pairs)), dim3(kDec4Threads), smem, stream, p);
   };
-  const bool two = p.chunk_heads > 8;
   cudaError_t e;
   if (d == 128) {
     if (shares) e = two ? go(attn_decode_kv4_kernel<128, 2, true>, once[0]) : go(attn_decode_kv4_kernel<128, 1, true>, once[1]);
