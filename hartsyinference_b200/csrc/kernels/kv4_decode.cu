@@ -49,16 +49,30 @@ __device__ __forceinline__ uint32_t scaled_bf16x2(uint32_t x, uint32_t s) {
   const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&s));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
-// d += A B. Not volatile: products of one unit's keys and another's values are interleaved.
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = c + A B. Not volatile: products of one unit's keys and another's values are interleaved.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// Codes 8 in all places times the queries of a block, negative. Volatile, or it would be kept from step to step in 4 registers a block.
+__device__ __forceinline__ void mma_f16_offset(float (&d)[4], const uint32_t (&b0)[2], const uint32_t (&b1)[2]) {
+  const uint32_t low = 0x80088008u, high = 0x80808080u;        // rows are alike: -8 * 2^-24, in places 8 .. 15 -8 * 2^-20
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %4, %5, %5}, {%6, %7}, {%8, %8, %8, %8};\n\t"
+               "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %4, %5, %5}, {%9, %10}, {%0, %1, %2, %3};"
+               : "=&f"(d[0]), "=&f"(d[1]), "=&f"(d[2]), "=&f"(d[3])
+               : "r"(low), "r"(high), "r"(b0[0]), "r"(b0[1]), "f"(0.f), "r"(b1[0]), "r"(b1[1]));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// A constant that the compiler keeps in a register: as an immediate next to another one it would take an instruction more.
+__device__ __forceinline__ uint32_t in_register(uint32_t x) {
+  uint32_t y;
+  asm volatile("mov.b32 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 // (x & mask) | bits in one instruction
 __device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t bits) {
@@ -87,11 +101,17 @@ __device__ __forceinline__ int dec4_units(const DecodeKv4Params& p, int len, int
   return len > 0 ? (len + kKv4Unit - 1) / kKv4Unit - first : 0;
 }
 
-// Dynamic shared memory: rings, the warps' results of four heads, queries and what the sums of their products start from, the prefix.
+// Dynamic shared memory: rings, one part of a sequence for every warp, the prefix.
 __host__ __device__ constexpr int dec4_ring_bytes(int d) { return kDec4Warps * kDec4Stages * 2 * kv4_unit_bytes(d); }
-__host__ __device__ constexpr int dec4_merge_bytes(int d) { return kDec4Warps * 4 * (d + 4) * 4; }
-__host__ __device__ constexpr int dec4_query_bytes(int d, int nt) { return nt * (d / 32) * 2 * 512; }
-__host__ __device__ constexpr int dec4_smem_bytes(int d, int nt) { return dec4_ring_bytes(d) + dec4_merge_bytes(d) + dec4_query_bytes(d, nt) + (kDec4MaxSeqs + 1) * 4; }
+__host__ __device__ constexpr int dec4_merge_bytes(int d, int nt) { return kDec4Warps * 8 * nt * (d + 4) * 4; }
+__host__ __device__ constexpr int dec4_smem_bytes(int d, int nt) { return dec4_ring_bytes(d) + dec4_merge_bytes(d, nt) + (kDec4MaxSeqs + 1) * 4; }
+
+// A part of a sequence that a warp could not finish: slot 0 what began before the warp's units, slot 1 what goes on behind them.
+struct Dec4Part {
+  int s, h;          // -1: none
+  int rel;           // first unit of the sequence (and head) in the order, from the block's first one on
+  int n;             // its units
+};
 
 template <int D, int NT, bool kShares>
 __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4_kernel(const DecodeKv4Params p) {
@@ -99,13 +119,11 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
   constexpr uint32_t kValueBias = ((127 - 15 + kKv4ValueExp) << 7) * 0x10001u;
   constexpr int kUnit = kv4_unit_bytes(D), kPlane = kv4_plane_bytes(D), kBlocks = D / 32, kWords = D / 32, kPitch = D + 4;
   __shared__ uint64_t full[kDec4Warps][kDec4Stages];
-  __shared__ float merge_ml[kDec4Warps][8][2];
-  __shared__ float head_factor[NT][8];
+  __shared__ Dec4Part parked[kDec4Warps][2];
   __shared__ int warp_units[kDec4Warps];
   __shared__ uint32_t abort_word;
   float* merge = reinterpret_cast<float*>(smem + dec4_ring_bytes(D));
-  uint4* queries = reinterpret_cast<uint4*>(smem + dec4_ring_bytes(D) + dec4_merge_bytes(D));     // [tile][block][queries | starts][lane]
-  int* prefix = reinterpret_cast<int*>(smem + dec4_ring_bytes(D) + dec4_merge_bytes(D) + dec4_query_bytes(D, NT));
+  int* prefix = reinterpret_cast<int*>(smem + dec4_ring_bytes(D) + dec4_merge_bytes(D, NT));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   uint8_t* ring = smem + warp * kDec4Stages * 2 * kUnit;
   volatile uint32_t* abort_flag = &abort_word;
@@ -113,6 +131,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
 #pragma unroll
     for (int i = 0; i < kDec4Stages; ++i) mbar_init(&full[warp][i], 1);
     fence_mbar_init();
+    parked[warp][0].s = parked[warp][1].s = -1;
   }
   if (threadIdx.x == 0) abort_word = 0;
   pdl_wait();
@@ -175,25 +194,33 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       s = only_seq; h = blockIdx.x - only_seq * heads_v; at = 0; n = only_units; first = only_first;
     }
   };
-  // pairs of units of this warp: units 2 (warp + 8 i) and the next of the share, i below mine
   const int share = static_cast<int>(f1 - f0);
-  const int mine = share > 2 * warp ? (share - 2 * warp + 2 * kDec4Warps - 1) / (2 * kDec4Warps) : 0;
-  const uint8_t* src = nullptr;                      // lane j: address of unit j % 2 of pair 16 (i / 16) + j / 2 of the warp
+  if (!kShares && share == 0) {                      // a sequence without keys
+    const int h = blockIdx.x - only_seq * heads_v, kv_head = h / p.chunks, head0 = kv_head * p.group + (h - kv_head * p.chunks) * p.chunk_heads;
+    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + (static_cast<long long>(only_seq) * p.hq + head0) * D);
+    for (int c = threadIdx.x; c < min(p.chunk_heads, (kv_head + 1) * p.group - head0) * (D / 2); c += kDec4Threads) out[c] = 0u;
+    return;
+  }
+  // this warp's part of the share, in pairs of units
+  const int w0 = static_cast<int>(static_cast<long long>(share) * warp / kDec4Warps), units = static_cast<int>(static_cast<long long>(share) * (warp + 1) / kDec4Warps) - w0;
+  const int mine = (units + 1) >> 1;
+  f0 += w0;
+  const uint8_t* src = nullptr;                      // lane j: address of unit 32 (i / 16) + j of the warp
   auto addresses = [&](int i0) {
-    const int rel = 2 * (warp + (i0 + (lane >> 1)) * kDec4Warps) + (lane & 1);
+    const int rel = 2 * i0 + lane;
     src = nullptr;
-    if (rel >= share) return;
+    if (rel >= units) return;
     int s, h, n, first;
     long long at;
     find(f0 + rel, s, h, at, n, first);
     src = kv4_unit<D>(p.pool, p.pool.block_table + static_cast<long long>(s) * p.pool.max_pages, h / p.chunks, first + static_cast<int>(f0 + rel - at), kKernelKv4);
   };
-  // pair i into slot `to` of the ring; a unit behind the share is left out
+  // pair i into slot `to` of the ring; a unit behind the last is left out
   auto fetch = [&](int i, int to) {
     if (i >= mine) return;
     if ((i & 15) == 0 && i > 0) addresses(i);
     if ((i & 15) == lane >> 1) {
-      if ((lane & 1) == 0) mbar_arrive_expect_tx(&full[warp][to], 2 * (warp + i * kDec4Warps) + 1 < share ? 2 * kUnit : kUnit);
+      if ((lane & 1) == 0) mbar_arrive_expect_tx(&full[warp][to], 2 * i + 1 < units ? 2 * kUnit : kUnit);
       if (src) bulk_load(ring + (2 * to + (lane & 1)) * kUnit, src, kUnit, &full[warp][to]);
     }
   };
@@ -207,38 +234,38 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
   const int v_at = kPlane + tq * (D / 2) + (D == 128 ? (g ^ ((tq & 2) << 1)) * 8 : g * 4), vs_at = kPlane + 8 * D + tq * (D / 32);
   const int w_at = kPlane + (7 - tq) * (D / 2) + (D == 128 ? (g ^ (((7 - tq) & 2) << 1)) * 8 : g * 4), ws_at = kPlane + 8 * D + (7 - tq) * (D / 32);
   constexpr int kOther = 8 * (D / 2), kOtherScale = 8 * (D / 32);          // eight keys on
+  const uint32_t value_bias = in_register(kValueBias);
 
   bool ok = true;
   int i = 0, slot = 0, phase = 0;                    // pair i of the warp is in `slot`
-  int at_rel = 0;                                    // start of the current sequence's units in the share
-  bool empty = !kShares && share == 0;               // a sequence without keys: zeros
-  for (int done = 0; done < share || empty;) {
-    int s, h, n, first;
+  for (int done = 0; done < units;) {
+    int s, h, n, first, at_rel;                        // at_rel: where the sequence's units start, from the warp's first one on
     {
       long long at;
       find(f0 + done, s, h, at, n, first);
       at_rel = static_cast<int>(at - f0);
     }
-    const int stop = min(at_rel + n, share);
+    const int stop = min(at_rel + n, units);
     const int kv_head = h / p.chunks, head0 = kv_head * p.group + (h - kv_head * p.chunks) * p.chunk_heads;
     const int heads = min(p.chunk_heads, (kv_head + 1) * p.group - head0);
-    const int len = empty ? 0 : kv4_length(p.pool, p.kv_lens[s], kKernelKv4);
+    const int len = kv4_length(p.pool, p.kv_lens[s], kKernelKv4);
     const int start = p.window > 0 ? max(0, len - p.window) : 0;
-    const int last = min(len, (first + share - at_rel) * kKv4Unit);      // keys from here on are not this block's
+    const int last = min(len, (first + units - at_rel) * kKv4Unit);      // keys from here on are not this warp's
 
-    // Queries of heads 8 t + g in half precision, with a power of two taken out so that the largest is in [2^12, 2^13); by warp t for all
-    if (warp < NT) {
-      const int t = warp;
+    // queries of heads 8 t + g in half precision, with a power of two taken out so that the largest is in [2^12, 2^13)
+    uint32_t q[NT][D / 16][2];
+    float factor[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
       const bool on = 8 * t + g < heads;
       const __nv_bfloat16* qh = p.q + (static_cast<long long>(s) * p.hq + head0 + (on ? 8 * t + g : 0)) * D;
-      uint32_t qb[D / 16][2];
       float amax = 0.f;
 #pragma unroll
       for (int m = 0; m < D / 16; ++m)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          qb[m][r] = on ? *reinterpret_cast<const uint32_t*>(qh + m * 16 + r * 8 + tq * 2) : 0u;
-          const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qb[m][r]));
+          q[t][m][r] = on ? *reinterpret_cast<const uint32_t*>(qh + m * 16 + r * 8 + tq * 2) : 0u;
+          const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q[t][m][r]));
           amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
         }
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
@@ -246,32 +273,19 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       const int e = amax > 0.f ? min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 12, -100), 85) : 0;
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        float sum = 0.f;
+      for (int m = 0; m < D / 16; ++m)
 #pragma unroll
-        for (int m = 2 * b; m < 2 * b + 2; ++m)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qb[m][r]));
-            const float sh = r ? down * 0.0625f : down;                 // places 8 .. 15 meet codes times 16
-            qb[m][r] = pack_f16x2(v.x * sh, v.y * sh);
-            const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&qb[m][r]));
-            sum += (w.x + w.y) * (r ? 16.f : 1.f);
-          }
-        queries[((t * kBlocks + b) * 2) * 32 + lane] = make_uint4(qb[2 * b][0], qb[2 * b][1], qb[2 * b + 1][0], qb[2 * b + 1][1]);
-        // what the sums start from: -8 * 2^-24 times the block's queries, for the two heads of a lane's results
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= -4.76837158203125e-7f;
-        const uint32_t s0 = __float_as_uint(__shfl_sync(0xffffffffu, sum, 8 * tq)), s1 = __float_as_uint(__shfl_sync(0xffffffffu, sum, 8 * tq + 4));
-        queries[((t * kBlocks + b) * 2 + 1) * 32 + lane] = make_uint4(s0, s1, s0, s1);
-      }
+        for (int r = 0; r < 2; ++r) {
+          const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q[t][m][r]));
+          const float sh = r ? down * 0.0625f : down;                   // places 8 .. 15 meet codes times 16
+          q[t][m][r] = pack_f16x2(v.x * sh, v.y * sh);
+        }
       // codes are times 2^24, scales (as fp32 with bits byte << 20 under an exponent of 96) times 2^(16 + key exponent)
-      if (tq == 0)
-        head_factor[t][g] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (p.cap_out == 0.f ? p.scale_log2 : p.cap_in) *
-                            __uint_as_float(static_cast<uint32_t>(127 + 24 + 16 + kKv4KeyExp) << 23);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (p.cap_out == 0.f ? p.scale_log2 : p.cap_in) *
+                       __uint_as_float(static_cast<uint32_t>(127 + 24 + 16 + kKv4KeyExp) << 23);
+      factor[t][0] = __shfl_sync(0xffffffffu, up, 8 * tq);
+      factor[t][1] = __shfl_sync(0xffffffffu, up, 8 * tq + 4);
     }
-    __syncthreads();
 
     float o[NT][D / 16][4], mx[NT][2], line[NT][2], l[NT][2];      // line: what a score has to pass to raise mx
 #pragma unroll
@@ -283,55 +297,58 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       mx[t][0] = mx[t][1] = line[t][0] = line[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
     }
-    uint4 q[NT][kBlocks];
+    // scores of two units
+    auto key_products = [&](const uint8_t* unit, float (&sc)[2][NT][4]) {
+      uint32_t w[2][2][kWords], scale[2][2];           // [unit][key ka or ka + 8]
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) q[t][b] = queries[((t * kBlocks + b) * 2) * 32 + lane];
-    auto key_products = [&](const uint8_t* unit, float (&sc)[NT][4]) {
-      uint32_t wa[kWords], wb[kWords], sa, sb;
-      if (D == 128) {
-        const uint4 a = *reinterpret_cast<const uint4*>(unit + k_at), b = *reinterpret_cast<const uint4*>(unit + k_at + kOther);
-        wa[0] = a.x; wa[1] = a.y; wa[kWords - 2] = a.z; wa[kWords - 1] = a.w;
-        wb[0] = b.x; wb[1] = b.y; wb[kWords - 2] = b.z; wb[kWords - 1] = b.w;
-        sa = *reinterpret_cast<const uint32_t*>(unit + ks_at);
-        sb = *reinterpret_cast<const uint32_t*>(unit + ks_at + kOtherScale);
-      } else {
-        const uint2 a = *reinterpret_cast<const uint2*>(unit + k_at), b = *reinterpret_cast<const uint2*>(unit + k_at + kOther);
-        wa[0] = a.x; wa[1] = a.y;
-        wb[0] = b.x; wb[1] = b.y;
-        sa = *reinterpret_cast<const uint16_t*>(unit + ks_at);
-        sb = *reinterpret_cast<const uint16_t*>(unit + ks_at + kOtherScale);
-      }
+        for (int r = 0; r < 2; ++r) {
+          const uint8_t* x = unit + u * kUnit + r * kOther + k_at;
+          const uint8_t* y = unit + u * kUnit + r * kOtherScale + ks_at;
+          if (D == 128) {
+            const uint4 z = *reinterpret_cast<const uint4*>(x);
+            w[u][r][0] = z.x; w[u][r][1] = z.y; w[u][r][kWords - 2] = z.z; w[u][r][kWords - 1] = z.w;
+            scale[u][r] = *reinterpret_cast<const uint32_t*>(y);
+          } else {
+            const uint2 z = *reinterpret_cast<const uint2*>(x);
+            w[u][r][0] = z.x; w[u][r][1] = z.y;
+            scale[u][r] = *reinterpret_cast<const uint16_t*>(y);
+          }
+        }
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        const uint32_t xa = wa[b], xb = wb[b], ya = xa >> 8, yb = xb >> 8;
-        const uint32_t a0[4] = {xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u};
-        const uint32_t a1[4] = {ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u, yb & 0x00f000f0u};
-        const float fa = __uint_as_float(masked_or(b < 3 ? sa << (20 - 8 * b) : sa >> 4, 0x0ff00000u, 0x30000000u));
-        const float fb = __uint_as_float(masked_or(b < 3 ? sb << (20 - 8 * b) : sb >> 4, 0x0ff00000u, 0x30000000u));
+      for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float4 from = *reinterpret_cast<const float4*>(&queries[((t * kBlocks + b) * 2 + 1) * 32 + lane]);
-          float acc[4] = {from.x, from.y, from.z, from.w};
-          mma_f16(acc, a0, q[t][b].x, q[t][b].y);
-          mma_f16(acc, a1, q[t][b].z, q[t][b].w);
-          sc[t][0] = b == 0 ? acc[0] * fa : fmaf(acc[0], fa, sc[t][0]);
-          sc[t][1] = b == 0 ? acc[1] * fa : fmaf(acc[1], fa, sc[t][1]);
-          sc[t][2] = b == 0 ? acc[2] * fb : fmaf(acc[2], fb, sc[t][2]);
-          sc[t][3] = b == 0 ? acc[3] * fb : fmaf(acc[3], fb, sc[t][3]);
+          // what the sums start from: the offset of the codes, -8 * 2^-24 and (places 8 .. 15) -8 * 2^-20, times the queries
+          float from[4];
+          mma_f16_offset(from, q[t][2 * b], q[t][2 * b + 1]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t xa = w[u][0][b], xb = w[u][1][b], ya = xa >> 8, yb = xb >> 8;
+            const uint32_t a0[4] = {xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u};
+            const uint32_t a1[4] = {ya & 0x000f000fu, yb & 0x000f000fu, ya & 0x00f000f0u, yb & 0x00f000f0u};
+            const uint32_t sa = scale[u][0], sb = scale[u][1];
+            const float fa = __uint_as_float(masked_or(b < 3 ? sa << (20 - 8 * b) : sa >> 4, 0x0ff00000u, 0x30000000u));
+            const float fb = __uint_as_float(masked_or(b < 3 ? sb << (20 - 8 * b) : sb >> 4, 0x0ff00000u, 0x30000000u));
+            float acc[4];
+            mma_f16(acc, a0, q[t][2 * b], from);
+            mma_f16(acc, a1, q[t][2 * b + 1], acc);
+            sc[u][t][0] = b == 0 ? acc[0] * fa : fmaf(acc[0], fa, sc[u][t][0]);
+            sc[u][t][1] = b == 0 ? acc[1] * fa : fmaf(acc[1], fa, sc[u][t][1]);
+            sc[u][t][2] = b == 0 ? acc[2] * fb : fmaf(acc[2], fb, sc[u][t][2]);
+            sc[u][t][3] = b == 0 ? acc[3] * fb : fmaf(acc[3], fb, sc[u][t][3]);
+          }
         }
-      }
     };
     // P^T of two units from their scores; key0: the first key of the first one
     auto softmax = [&](float (&sc)[2][NT][4], uint32_t (&pt)[2][NT][2], int key0) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float2 factor = *reinterpret_cast<const float2*>(&head_factor[t][2 * tq]);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sc[u][t][j] *= j & 1 ? factor.y : factor.x;
+          for (int j = 0; j < 4; ++j) sc[u][t][j] *= factor[t][j & 1];
         if (p.cap_out != 0.f)                         // cap tanh(x) = cap - 2 cap / (exp(2 x) + 1)
 #pragma unroll
           for (int u = 0; u < 2; ++u)
@@ -371,13 +388,11 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
             }
           }
         }
-        // a warp that has seen no key yet: its scores and its reference are both -infinity
-        const float ref0 = mx[t][0] == -INFINITY ? 0.f : mx[t][0], ref1 = mx[t][1] == -INFINITY ? 0.f : mx[t][1];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           float e[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) e[j] = dec4_exp2(sc[u][t][j] - (j & 1 ? ref1 : ref0));
+          for (int j = 0; j < 4; ++j) e[j] = dec4_exp2(sc[u][t][j] - mx[t][j & 1]);
           l[t][0] += e[0] + e[2];
           l[t][1] += e[1] + e[3];
           pt[u][t][0] = transpose8x8(pack_bf16x2(e[0], e[1]));
@@ -406,7 +421,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       for (int b = 0; b < kBlocks; ++b) {
         // scale bytes of a pair of keys, then where a bf16 has them
         const uint32_t sel = 0x0400u + 0x0101u * b;
-        const uint32_t p0 = (__byte_perm(s4[0], s4[1], sel) & 0x00ff00ffu) * 16u + kValueBias, p1 = (__byte_perm(s4[2], s4[3], sel) & 0x00ff00ffu) * 16u + kValueBias;
+        const uint32_t p0 = (__byte_perm(s4[0], s4[1], sel) & 0x00ff00ffu) * 16u + value_bias, p1 = (__byte_perm(s4[2], s4[3], sel) & 0x00ff00ffu) * 16u + value_bias;
         uint32_t a[2][4];
 #pragma unroll
         for (int r = 0; r < 2; ++r)
@@ -426,20 +441,19 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
         }
       }
     };
-    // This warp's pairs that have units of this sequence. One that reaches into the next sequence is kept for it.
-    int key0 = (first - at_rel + 2 * (warp + i * kDec4Warps)) * kKv4Unit;
-    for (int rel = 2 * (warp + i * kDec4Warps); ok && rel < stop; key0 += 2 * kDec4Warps * kKv4Unit) {
+    // The pairs that have units of this sequence. One that reaches into the next sequence is kept for it.
+    int key0 = (first - at_rel + 2 * i) * kKv4Unit;
+    for (int rel = 2 * i; ok && rel < stop; key0 += 2 * kKv4Unit) {
       if (!(ok = mbar_wait(&full[warp][slot], phase, abort_flag))) break;
       const uint8_t* unit = ring + slot * 2 * kUnit;
       float sc[2][NT][4];
       uint32_t pt[2][NT][2];
-      key_products(unit, sc[0]);
-      key_products(unit + kUnit, sc[1]);
+      key_products(unit, sc);
       softmax(sc, pt, key0);
       value_products(unit, pt[0]);
       value_products(unit + kUnit, pt[1]);
-      rel += 2 * kDec4Warps;
-      if (rel - 2 * kDec4Warps + 1 >= stop && stop < share) break;
+      rel += 2;
+      if (rel > stop && stop < units) break;
       __syncwarp();
       fetch(i + kDec4Stages, slot);
       ++i;
@@ -447,68 +461,48 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       slot ^= 1;
     }
 
-    // ---- join the warps' results, four heads at a time
-    const bool part = kShares && !(at_rel >= 0 && at_rel + n <= share);
-    float* dst_part = kShares ? p.parts + (static_cast<long long>(blockIdx.x) * 2 + (at_rel < 0 ? 0 : 1)) * p.chunk_heads * (D + 4) : nullptr;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float sum = l[t][j];
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (g == 0) {
-          merge_ml[warp][2 * tq + j][0] = mx[t][j];
-          merge_ml[warp][2 * tq + j][1] = sum;
-        }
-      }
+        for (int d = 4; d < 32; d <<= 1) l[t][j] += __shfl_xor_sync(0xffffffffu, l[t][j], d);
+    if (at_rel >= 0 && at_rel + n <= units) {
+      // all of the sequence: neighbouring lane groups exchange a head each, so that both have pairs of neighbouring values
 #pragma unroll
-      for (int quad = 0; quad < 2; ++quad) {
-        if (8 * t + 4 * quad >= heads) break;
-        if ((tq >> 1) == quad) {
+      for (int t = 0; t < NT; ++t) {
+        const float inv0 = l[t][0] == 0.f ? 0.f : 1.f / l[t][0], inv1 = l[t][1] == 0.f ? 0.f : 1.f / l[t][1];
+        const int head = 8 * t + 2 * tq + (g & 1);
+        __nv_bfloat16* dst = p.out + (static_cast<long long>(s) * p.hq + head0 + head) * D + (g & 6);
 #pragma unroll
-          for (int m = 0; m < D / 16; ++m)
+        for (int m = 0; m < D / 16; ++m)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float* row = merge + (warp * 4 + 2 * (tq & 1) + j) * kPitch + m * 16 + g;
-              row[0] = o[t][m][j];
-              row[8] = o[t][m][2 + j];
-            }
-        }
-        __syncthreads();
-        constexpr int kEach = D / 64;                  // values of a thread: two warps per head
-        const int hh = threadIdx.x >> 6, head = 4 * quad + hh, c = (threadIdx.x & 63) * kEach;
-        if (8 * t + head < heads) {
-          float top = -INFINITY, den = 0.f, acc[kEach];
-#pragma unroll
-          for (int w = 0; w < kDec4Warps; ++w) top = fmaxf(top, merge_ml[w][head][0]);
-#pragma unroll
-          for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
-#pragma unroll
-          for (int w = 0; w < kDec4Warps; ++w) {
-            const float m = merge_ml[w][head][0], wt = m == top ? 1.f : dec4_exp2(m - top);      // a warp without keys: 0, or all are
-            den = fmaf(wt, merge_ml[w][head][1], den);
-            const float* x = merge + (w * 4 + hh) * kPitch + c;
-#pragma unroll
-            for (int j = 0; j < kEach; ++j) acc[j] = fmaf(wt, x[j], acc[j]);
+          for (int r = 0; r < 2; ++r) {
+            const float v0 = o[t][m][2 * r] * inv0, v1 = o[t][m][2 * r + 1] * inv1;
+            const float got = __shfl_xor_sync(0xffffffffu, g & 1 ? v0 : v1, 4);
+            if (head < heads) *reinterpret_cast<uint32_t*>(dst + m * 16 + r * 8) = g & 1 ? pack_bf16x2(got, v1) : pack_bf16x2(v0, got);
           }
-          if (part) {
-            float* dst = dst_part + (8 * t + head) * (D + 4);
-#pragma unroll
-            for (int j = 0; j < kEach; ++j) dst[c + j] = acc[j];
-            if (c == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(top, den);
-          } else {
-            const float inv = den == 0.f ? 0.f : 1.f / den;
-            __nv_bfloat16* dst = p.out + (static_cast<long long>(s) * p.hq + head0 + 8 * t + head) * D + c;
-            if (D == 128) *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[kEach - 1] * inv);
-            else dst[0] = __float2bfloat16(acc[0] * inv);
-          }
-        }
-        __syncthreads();
       }
+    } else {
+      // a part of it, kept until the end: the first one in memory of its own, the last one in the ring, which has done its work by then
+      const int which = at_rel < 0 ? 0 : 1;
+      float* park = which ? reinterpret_cast<float*>(ring) : merge + warp * 8 * NT * kPitch;
+      __syncwarp();
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float* row = park + (8 * t + 2 * tq + j) * kPitch;
+#pragma unroll
+          for (int m = 0; m < D / 16; ++m) {
+            row[m * 16 + g] = o[t][m][j];
+            row[m * 16 + 8 + g] = o[t][m][2 + j];
+          }
+          if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(mx[t][j], l[t][j]);
+        }
+      if (lane == 0) parked[warp][which] = Dec4Part{s, h, at_rel + w0, n};
     }
     done = stop;
-    empty = false;
   }
   if (!ok) {
     // copies in flight end before the block does
@@ -518,6 +512,59 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       slot ^= 1;
     }
     if (lane == 0) report_status(p.pool.status, kWaitTimeout, kKernelKv4, 43, blockIdx.x);
+  }
+  __syncthreads();
+
+  // Parts of the same sequence in a row of warps: owned by the warp where it begins, or by the block (job 0) where that is before it
+  for (int job = 0; job <= kDec4Warps; ++job) {
+    int from = job - 1, which = 1;
+    if (job == 0) {
+      for (from = 0; from < kDec4Warps && parked[from][0].s < 0 && parked[from][1].s < 0; ++from) {}       // warps without units
+      which = 0;
+      if (from == kDec4Warps || parked[from][0].s < 0 || parked[from][0].rel >= 0) continue;
+    } else if (parked[from][1].s < 0) {
+      continue;
+    }
+    const Dec4Part seq = parked[from][which];
+    uint32_t in = 1u << from;                          // warps with parts of it, all but the owner's in slot 0
+    for (int w = from + 1; w < kDec4Warps; ++w)
+      if (parked[w][0].s == seq.s && parked[w][0].h == seq.h) in |= 1u << w;
+    const int kv_head = seq.h / p.chunks, head0 = kv_head * p.group + (seq.h - kv_head * p.chunks) * p.chunk_heads;
+    const int heads = min(p.chunk_heads, (kv_head + 1) * p.group - head0);
+    const bool all = seq.rel >= 0 && seq.rel + seq.n <= share;
+    float* dst_part = kShares ? p.parts + (static_cast<long long>(blockIdx.x) * 2 + (seq.rel < 0 ? 0 : 1)) * p.chunk_heads * (D + 4) : nullptr;
+    for (int head = warp; head < heads; head += kDec4Warps) {
+      const int c = lane * (D / 32);
+      float top = -INFINITY, den = 0.f, acc[D / 32];
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) acc[j] = 0.f;
+      auto row = [&](int w) {
+        const float* base = w == from && which ? reinterpret_cast<const float*>(smem + w * kDec4Stages * 2 * kUnit) : merge + w * 8 * NT * kPitch;
+        return base + head * kPitch;
+      };
+      for (int w = from; w < kDec4Warps; ++w)
+        if (in >> w & 1) top = fmaxf(top, row(w)[D]);
+      for (int w = from; w < kDec4Warps; ++w)
+        if (in >> w & 1) {
+          const float* x = row(w);
+          const float2 ml = *reinterpret_cast<const float2*>(x + D);
+          const float wt = ml.x == top ? 1.f : dec4_exp2(ml.x - top);
+          den = fmaf(wt, ml.y, den);
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) acc[j] = fmaf(wt, x[c + j], acc[j]);
+        }
+      if (all) {
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        __nv_bfloat16* dst = p.out + (static_cast<long long>(seq.s) * p.hq + head0 + head) * D + c;
+#pragma unroll
+        for (int j = 0; j < D / 32; j += 2) *reinterpret_cast<uint32_t*>(dst + j) = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
+      } else {
+        float* dst = dst_part + head * (D + 4);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) dst[c + j] = acc[j];
+        if (lane == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(top, den);
+      }
+    }
   }
 }
 
