@@ -55,14 +55,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], c
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-// Codes 8 in all places times the queries of a block, negative. Volatile, or it would be kept from step to step in 4 registers a block.
-__device__ __forceinline__ void mma_f16_offset(float (&d)[4], const uint32_t (&b0)[2], const uint32_t (&b1)[2]) {
-  const uint32_t low = 0x80088008u, high = 0x80808080u;        // rows are alike: -8 * 2^-24, in places 8 .. 15 -8 * 2^-20
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %4, %5, %5}, {%6, %7}, {%8, %8, %8, %8};\n\t"
-               "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %4, %5, %5}, {%9, %10}, {%0, %1, %2, %3};"
-               : "=&f"(d[0]), "=&f"(d[1]), "=&f"(d[2]), "=&f"(d[3])
-               : "r"(low), "r"(high), "r"(b0[0]), "r"(b0[1]), "f"(0.f), "r"(b1[0]), "r"(b1[1]));
-}
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -73,6 +65,12 @@ __device__ __forceinline__ uint32_t in_register(uint32_t x) {
   uint32_t y;
   asm volatile("mov.b32 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+// x * 16 + y on the multiplier; written out, it would become two instructions of the pipe that the masks are bound by
+__device__ __forceinline__ uint32_t times16_plus(uint32_t x, uint32_t y) {
+  uint32_t z;
+  asm("mad.lo.u32 %0, %1, 16, %2;" : "=r"(z) : "r"(x), "r"(y));
+  return z;
 }
 // (x & mask) | bits in one instruction
 __device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t bits) {
@@ -120,6 +118,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
   constexpr int kUnit = kv4_unit_bytes(D), kPlane = kv4_plane_bytes(D), kBlocks = D / 32, kWords = D / 32, kPitch = D + 4;
   __shared__ uint64_t full[kDec4Warps][kDec4Stages];
   __shared__ Dec4Part parked[kDec4Warps][2];
+  __shared__ float4 starts[kDec4Warps][NT][D / 32][4];      // [block][lane quarter]: what the sums of key products start from
   __shared__ int warp_units[kDec4Warps];
   __shared__ uint32_t abort_word;
   float* merge = reinterpret_cast<float*>(smem + dec4_ring_bytes(D));
@@ -187,9 +186,10 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       s = lo;
       n = prefix[s + 1] - prefix[s];
       const long long seq_at = static_cast<long long>(prefix[s]) * heads_v;
-      h = static_cast<int>((f - seq_at) / n);
+      h = static_cast<int>(static_cast<uint32_t>(f - seq_at) / static_cast<uint32_t>(n));
       at = seq_at + static_cast<long long>(h) * n;
-      dec4_units(p, kv4_length(p.pool, p.kv_lens[s], kKernelKv4), first);
+      first = 0;
+      if (p.window > 0) dec4_units(p, kv4_length(p.pool, p.kv_lens[s], kKernelKv4), first);
     } else {
       s = only_seq; h = blockIdx.x - only_seq * heads_v; at = 0; n = only_units; first = only_first;
     }
@@ -219,15 +219,13 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
   auto fetch = [&](int i, int to) {
     if (i >= mine) return;
     if ((i & 15) == 0 && i > 0) addresses(i);
-    if ((i & 15) == lane >> 1) {
-      if ((lane & 1) == 0) mbar_arrive_expect_tx(&full[warp][to], 2 * i + 1 < units ? 2 * kUnit : kUnit);
-      if (src) bulk_load(ring + (2 * to + (lane & 1)) * kUnit, src, kUnit, &full[warp][to]);
+    const unsigned long long a = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), 2 * (i & 15)), b = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), 2 * (i & 15) + 1);
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&full[warp][to], b ? 2 * kUnit : kUnit);
+      bulk_load(ring + 2 * to * kUnit, reinterpret_cast<const void*>(a), kUnit, &full[warp][to]);
+      if (b) bulk_load(ring + (2 * to + 1) * kUnit, reinterpret_cast<const void*>(b), kUnit, &full[warp][to]);
     }
   };
-  addresses(0);
-#pragma unroll
-  for (int i = 0; i < kDec4Stages; ++i) fetch(i, i);
-
   const int ka = (g & 1) ? 7 - (g >> 1) : g >> 1;    // keys of rows g and g + 8: ka, ka + 8
   // where a lane reads in a unit: its words of keys ka and of the values of keys tq and 7 - tq, and their scales
   const int k_at = ka * (D / 2) + tq * (D / 8), ks_at = 8 * D + ka * (D / 32);
@@ -235,6 +233,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
   const int w_at = kPlane + (7 - tq) * (D / 2) + (D == 128 ? (g ^ (((7 - tq) & 2) << 1)) * 8 : g * 4), ws_at = kPlane + 8 * D + (7 - tq) * (D / 32);
   constexpr int kOther = 8 * (D / 2), kOtherScale = 8 * (D / 32);          // eight keys on
   const uint32_t value_bias = in_register(kValueBias);
+  const uint32_t offset[4] = {in_register(0xc308c308u), in_register(0xc308c308u), in_register(0xc308c308u), in_register(0xc308c308u)};
 
   bool ok = true;
   int i = 0, slot = 0, phase = 0;                    // pair i of the warp is in `slot`
@@ -248,9 +247,6 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
     const int stop = min(at_rel + n, units);
     const int kv_head = h / p.chunks, head0 = kv_head * p.group + (h - kv_head * p.chunks) * p.chunk_heads;
     const int heads = min(p.chunk_heads, (kv_head + 1) * p.group - head0);
-    const int len = kv4_length(p.pool, p.kv_lens[s], kKernelKv4);
-    const int start = p.window > 0 ? max(0, len - p.window) : 0;
-    const int last = min(len, (first + units - at_rel) * kKv4Unit);      // keys from here on are not this warp's
 
     // queries of heads 8 t + g in half precision, with a power of two taken out so that the largest is in [2^12, 2^13)
     uint32_t q[NT][D / 16][2];
@@ -259,12 +255,27 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
     for (int t = 0; t < NT; ++t) {
       const bool on = 8 * t + g < heads;
       const __nv_bfloat16* qh = p.q + (static_cast<long long>(s) * p.hq + head0 + (on ? 8 * t + g : 0)) * D;
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) q[t][m][r] = on ? *reinterpret_cast<const uint32_t*>(qh + m * 16 + r * 8 + tq * 2) : 0u;
+    }
+    if (done == 0) {                                   // the first copies, while the queries are on their way
+      addresses(0);
+#pragma unroll
+      for (int j = 0; j < kDec4Stages; ++j) fetch(j, j);
+    }
+    const int len = kv4_length(p.pool, p.kv_lens[s], kKernelKv4);
+    const int start = p.window > 0 ? max(0, len - p.window) : 0;
+    const int last = min(len, (first + units - at_rel) * kKv4Unit);      // keys from here on are not this warp's
+    __syncwarp();                                      // the last sequence's products have read `starts`
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
       float amax = 0.f;
 #pragma unroll
       for (int m = 0; m < D / 16; ++m)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          q[t][m][r] = on ? *reinterpret_cast<const uint32_t*>(qh + m * 16 + r * 8 + tq * 2) : 0u;
           const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q[t][m][r]));
           amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
         }
@@ -273,19 +284,32 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       const int e = amax > 0.f ? min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127 - 12, -100), 85) : 0;
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
-      for (int m = 0; m < D / 16; ++m)
+      for (int b = 0; b < kBlocks; ++b) {
+        float sum = 0.f;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q[t][m][r]));
-          const float sh = r ? down * 0.0625f : down;                   // places 8 .. 15 meet codes times 16
-          q[t][m][r] = pack_f16x2(v.x * sh, v.y * sh);
-        }
+        for (int m = 2 * b; m < 2 * b + 2; ++m)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q[t][m][r]));
+            const float sh = r ? down * 0.0625f : down;                 // places 8 .. 15 meet codes times 16
+            q[t][m][r] = pack_f16x2(v.x * sh, v.y * sh);
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&q[t][m][r]));
+            sum += (x.x + x.y) * (r ? 16.f : 1.f);
+          }
+        // the offset of the codes: -8 * 2^-24 times the block's queries, for the two heads of a lane's results
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum *= -4.76837158203125e-7f;
+        const float s0 = __shfl_sync(0xffffffffu, sum, 8 * tq), s1 = __shfl_sync(0xffffffffu, sum, 8 * tq + 4);
+        if (g == 0) starts[warp][t][b][tq] = make_float4(s0, s1, s0, s1);
+      }
       // codes are times 2^24, scales (as fp32 with bits byte << 20 under an exponent of 96) times 2^(16 + key exponent)
       const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (p.cap_out == 0.f ? p.scale_log2 : p.cap_in) *
                        __uint_as_float(static_cast<uint32_t>(127 + 24 + 16 + kKv4KeyExp) << 23);
       factor[t][0] = __shfl_sync(0xffffffffu, up, 8 * tq);
       factor[t][1] = __shfl_sync(0xffffffffu, up, 8 * tq + 4);
     }
+    __syncwarp();
 
     float o[NT][D / 16][4], mx[NT][2], line[NT][2], l[NT][2];      // line: what a score has to pass to raise mx
 #pragma unroll
@@ -320,9 +344,8 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          // what the sums start from: the offset of the codes, -8 * 2^-24 and (places 8 .. 15) -8 * 2^-20, times the queries
-          float from[4];
-          mma_f16_offset(from, q[t][2 * b], q[t][2 * b + 1]);
+          const float4 from4 = starts[warp][t][b][tq];
+          const float from[4] = {from4.x, from4.y, from4.z, from4.w};
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const uint32_t xa = w[u][0][b], xb = w[u][1][b], ya = xa >> 8, yb = xb >> 8;
@@ -416,12 +439,11 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
           s4[r] = *reinterpret_cast<const uint16_t*>(y);
         }
       }
-      const uint32_t offset[4] = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};        // -136
 #pragma unroll
       for (int b = 0; b < kBlocks; ++b) {
         // scale bytes of a pair of keys, then where a bf16 has them
         const uint32_t sel = 0x0400u + 0x0101u * b;
-        const uint32_t p0 = (__byte_perm(s4[0], s4[1], sel) & 0x00ff00ffu) * 16u + value_bias, p1 = (__byte_perm(s4[2], s4[3], sel) & 0x00ff00ffu) * 16u + value_bias;
+        const uint32_t p0 = times16_plus(__byte_perm(s4[0], s4[1], sel) & 0x00ff00ffu, value_bias), p1 = times16_plus(__byte_perm(s4[2], s4[3], sel) & 0x00ff00ffu, value_bias);
         uint32_t a[2][4];
 #pragma unroll
         for (int r = 0; r < 2; ++r)
@@ -568,10 +590,11 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
   }
 }
 
-// Joins the parts of sequences that several blocks share; zeros for those without keys. One block per (sequence, part of a kv head's heads),
-// one warp per head.
-template <int D>
+// Joins the parts of sequences that several blocks share; zeros for those without keys. One block per (sequence, part of a kv head's heads)
+// with a warp per head, or (kSlices 8, where a sequence has many parts) one block per head whose warps take every eighth part.
+template <int D, int kSlices>
 __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Params p) {
+  __shared__ float sums[kSlices > 1 ? 8 : 1][D + 4];
   pdl_wait();
   pdl_trigger();
   const int heads_v = p.pool.hkv * p.chunks, s = blockIdx.x / heads_v, h = blockIdx.x - s * heads_v;
@@ -583,23 +606,19 @@ __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Par
   // block of unit f: the last whose share starts at or before it
   const int c0 = n > 0 ? static_cast<int>(((at + 1) * p.blocks - 1) / total) : 0, c1 = n > 0 ? static_cast<int>(((at + n) * p.blocks - 1) / total) : 0;
   if (n > 0 && c0 == c1) return;                     // one block had all of it
-  const int lane = threadIdx.x & 31;
-  for (int hh = threadIdx.x >> 5; hh < heads; hh += 8) {
-    __nv_bfloat16* out = p.out + (static_cast<long long>(s) * p.hq + head0 + hh) * D;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kEach = D / 32;                      // values of a lane
+  for (int head = kSlices > 1 ? blockIdx.y : warp; head < heads; head += kSlices > 1 ? heads : 8) {
     // the first part is the second one of its block: the sequence starts in that share
-    auto part = [&](int c) { return p.parts + ((static_cast<long long>(c) * 2 + (c == c0 ? 1 : 0)) * p.chunk_heads + hh) * (D + 4); };
-    float top = -INFINITY, den = 0.f;
+    auto part = [&](int c) { return p.parts + ((static_cast<long long>(c) * 2 + (c == c0 ? 1 : 0)) * p.chunk_heads + head) * (D + 4); };
+    float top = -INFINITY, den = 0.f, acc[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
     if (n > 0) {
       for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, part(c)[D]);
       top = warp_max(top);
-    }
-    constexpr int kEach = D / 32;                    // values of a lane
-    float acc[kEach];
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
-    if (n > 0)
 #pragma unroll 4
-      for (int c = c0; c <= c1; ++c) {
+      for (int c = c0 + (kSlices > 1 ? warp : 0); c <= c1; c += kSlices) {
         const float* x = part(c);
         const float2 ml = *reinterpret_cast<const float2*>(x + D);
         const float w = ml.x == top ? 1.f : dec4_exp2(ml.x - top);
@@ -611,7 +630,25 @@ __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Par
           acc[j + 1] = fmaf(w, v.y, acc[j + 1]);
         }
       }
+    }
+    if (kSlices > 1) {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) sums[warp][lane * kEach + j] = acc[j];
+      if (lane == 0) sums[warp][D] = den;
+      __syncthreads();
+      if (warp) return;
+      den = 0.f;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        den += sums[kSlices > 1 ? w : 0][D];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) acc[j] += sums[kSlices > 1 ? w : 0][lane * kEach + j];
+      }
+    }
     const float inv = den == 0.f ? 0.f : 1.f / den;
+    __nv_bfloat16* out = p.out + (static_cast<long long>(s) * p.hq + head0 + head) * D;
 #pragma unroll
     for (int j = 0; j < kEach; j += 2) *reinterpret_cast<uint32_t*>(out + lane * kEach + j) = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
   }
@@ -694,7 +731,10 @@ B200_API int b200_attn_decode_kv4(const void* q, const void* pool, void* out, co
   }
   if (e != cudaSuccess) return -static_cast<int>(e) - 300;
   if (!shares) return 1;
-  e = d == 128 ? launch_pdl(join_decode_kv4_kernel<128>, dim3(static_cast<unsigned>(pairs)), dim3(256), 0, stream, p)
-               : launch_pdl(join_decode_kv4_kernel<64>, dim3(static_cast<unsigned>(pairs)), dim3(256), 0, stream, p);
+  // a warp takes 0.3 us a part: with a dozen of them a block per head is faster, with a few the blocks' own start is what counts
+  const bool many = p.blocks >= 8 * pairs;
+  const dim3 grid(static_cast<unsigned>(pairs), many ? p.chunk_heads : 1);
+  if (d == 128) e = many ? launch_pdl(join_decode_kv4_kernel<128, 8>, grid, dim3(256), 0, stream, p) : launch_pdl(join_decode_kv4_kernel<128, 1>, grid, dim3(256), 0, stream, p);
+  else e = many ? launch_pdl(join_decode_kv4_kernel<64, 8>, grid, dim3(256), 0, stream, p) : launch_pdl(join_decode_kv4_kernel<64, 1>, grid, dim3(256), 0, stream, p);
   return e == cudaSuccess ? 2 : -static_cast<int>(e) - 400;
 }
