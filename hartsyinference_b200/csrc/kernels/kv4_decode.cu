@@ -49,11 +49,11 @@ __device__ __forceinline__ uint32_t scaled_bf16x2(uint32_t x, uint32_t s) {
   const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&s));
   return *reinterpret_cast<const uint32_t*>(&y);
 }
-// d = c + A B. Not volatile: products of one unit's keys and another's values are interleaved.
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], const float (&c)[4]) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+// d += A B. Not volatile: products of keys and of values of two units may be interleaved.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -66,11 +66,9 @@ __device__ __forceinline__ uint32_t in_register(uint32_t x) {
   asm volatile("mov.b32 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// x * 16 + y on the multiplier; written out, it would become two instructions of the pipe that the masks are bound by
-__device__ __forceinline__ uint32_t times16_plus(uint32_t x, uint32_t y) {
-  uint32_t z;
-  asm("mad.lo.u32 %0, %1, 16, %2;" : "=r"(z) : "r"(x), "r"(y));
-  return z;
+// Four numbers of shared memory, loaded where this stands: two operands that start alike would else be one load and four moves.
+__device__ __forceinline__ void load_here(float (&x)[4], const float4* at) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(smem_u32(at)));
 }
 // (x & mask) | bits in one instruction
 __device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t bits) {
@@ -232,7 +230,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
   const int v_at = kPlane + tq * (D / 2) + (D == 128 ? (g ^ ((tq & 2) << 1)) * 8 : g * 4), vs_at = kPlane + 8 * D + tq * (D / 32);
   const int w_at = kPlane + (7 - tq) * (D / 2) + (D == 128 ? (g ^ (((7 - tq) & 2) << 1)) * 8 : g * 4), ws_at = kPlane + 8 * D + (7 - tq) * (D / 32);
   constexpr int kOther = 8 * (D / 2), kOtherScale = 8 * (D / 32);          // eight keys on
-  const uint32_t value_bias = in_register(kValueBias);
+  const uint32_t value_bias = in_register(kValueBias), sixteen = in_register(16u);     // (a shift by four would be in the pipe of the masks)
   const uint32_t offset[4] = {in_register(0xc308c308u), in_register(0xc308c308u), in_register(0xc308c308u), in_register(0xc308c308u)};
 
   bool ok = true;
@@ -344,8 +342,6 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float4 from4 = starts[warp][t][b][tq];
-          const float from[4] = {from4.x, from4.y, from4.z, from4.w};
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const uint32_t xa = w[u][0][b], xb = w[u][1][b], ya = xa >> 8, yb = xb >> 8;
@@ -355,8 +351,9 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
             const float fa = __uint_as_float(masked_or(b < 3 ? sa << (20 - 8 * b) : sa >> 4, 0x0ff00000u, 0x30000000u));
             const float fb = __uint_as_float(masked_or(b < 3 ? sb << (20 - 8 * b) : sb >> 4, 0x0ff00000u, 0x30000000u));
             float acc[4];
-            mma_f16(acc, a0, q[t][2 * b], from);
-            mma_f16(acc, a1, q[t][2 * b + 1], acc);
+            load_here(acc, &starts[warp][t][b][tq]);
+            mma_f16(acc, a0, q[t][2 * b]);
+            mma_f16(acc, a1, q[t][2 * b + 1]);
             sc[u][t][0] = b == 0 ? acc[0] * fa : fmaf(acc[0], fa, sc[u][t][0]);
             sc[u][t][1] = b == 0 ? acc[1] * fa : fmaf(acc[1], fa, sc[u][t][1]);
             sc[u][t][2] = b == 0 ? acc[2] * fb : fmaf(acc[2], fb, sc[u][t][2]);
@@ -443,7 +440,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       for (int b = 0; b < kBlocks; ++b) {
         // scale bytes of a pair of keys, then where a bf16 has them
         const uint32_t sel = 0x0400u + 0x0101u * b;
-        const uint32_t p0 = times16_plus(__byte_perm(s4[0], s4[1], sel) & 0x00ff00ffu, value_bias), p1 = times16_plus(__byte_perm(s4[2], s4[3], sel) & 0x00ff00ffu, value_bias);
+        const uint32_t p0 = (__byte_perm(s4[0], s4[1], sel) & 0x00ff00ffu) * sixteen + value_bias, p1 = (__byte_perm(s4[2], s4[3], sel) & 0x00ff00ffu) * sixteen + value_bias;
         uint32_t a[2][4];
 #pragma unroll
         for (int r = 0; r < 2; ++r)
@@ -548,32 +545,33 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       continue;
     }
     const Dec4Part seq = parked[from][which];
-    uint32_t in = 1u << from;                          // warps with parts of it, all but the owner's in slot 0
-    for (int w = from + 1; w < kDec4Warps; ++w)
-      if (parked[w][0].s == seq.s && parked[w][0].h == seq.h) in |= 1u << w;
+    bool in[kDec4Warps];                               // warps with parts of it, all but the owner's in slot 0
+#pragma unroll
+    for (int w = 0; w < kDec4Warps; ++w) in[w] = w == from || (w > from && parked[w][0].s == seq.s && parked[w][0].h == seq.h);
     const int kv_head = seq.h / p.chunks, head0 = kv_head * p.group + (seq.h - kv_head * p.chunks) * p.chunk_heads;
     const int heads = min(p.chunk_heads, (kv_head + 1) * p.group - head0);
     const bool all = seq.rel >= 0 && seq.rel + seq.n <= share;
     float* dst_part = kShares ? p.parts + (static_cast<long long>(blockIdx.x) * 2 + (seq.rel < 0 ? 0 : 1)) * p.chunk_heads * (D + 4) : nullptr;
     for (int head = warp; head < heads; head += kDec4Warps) {
       const int c = lane * (D / 32);
+      float2 ml[kDec4Warps];
       float top = -INFINITY, den = 0.f, acc[D / 32];
+      auto row = [&](int w) { return (w == from && which ? reinterpret_cast<const float*>(smem + w * kDec4Stages * 2 * kUnit) : merge + w * 8 * NT * kPitch) + head * kPitch; };
+#pragma unroll
+      for (int w = 0; w < kDec4Warps; ++w) {
+        ml[w] = in[w] ? *reinterpret_cast<const float2*>(row(w) + D) : make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, ml[w].x);
+      }
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) acc[j] = 0.f;
-      auto row = [&](int w) {
-        const float* base = w == from && which ? reinterpret_cast<const float*>(smem + w * kDec4Stages * 2 * kUnit) : merge + w * 8 * NT * kPitch;
-        return base + head * kPitch;
-      };
-      for (int w = from; w < kDec4Warps; ++w)
-        if (in >> w & 1) top = fmaxf(top, row(w)[D]);
-      for (int w = from; w < kDec4Warps; ++w)
-        if (in >> w & 1) {
-          const float* x = row(w);
-          const float2 ml = *reinterpret_cast<const float2*>(x + D);
-          const float wt = ml.x == top ? 1.f : dec4_exp2(ml.x - top);
-          den = fmaf(wt, ml.y, den);
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) acc[j] = fmaf(wt, x[c + j], acc[j]);
+      for (int w = 0; w < kDec4Warps; ++w)
+        if (in[w]) {
+          const float wt = ml[w].x == top ? 1.f : dec4_exp2(ml[w].x - top);
+          const float* x = row(w) + c;
+          den = fmaf(wt, ml[w].y, den);
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) acc[j] = fmaf(wt, x[j], acc[j]);
         }
       if (all) {
         const float inv = den == 0.f ? 0.f : 1.f / den;
@@ -583,7 +581,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       } else {
         float* dst = dst_part + head * (D + 4);
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) dst[c + j] = acc[j];
+        for (int j = 0; j < D / 32; j += 2) *reinterpret_cast<float2*>(dst + c + j) = make_float2(acc[j], acc[j + 1]);
         if (lane == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(top, den);
       }
     }
@@ -594,7 +592,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
 // with a warp per head, or (kSlices 8, where a sequence has many parts) one block per head whose warps take every eighth part.
 template <int D, int kSlices>
 __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Params p) {
-  __shared__ float sums[kSlices > 1 ? 8 : 1][D + 4];
+  __shared__ __align__(8) float sums[kSlices > 1 ? 8 : 1][D + 4];
   pdl_wait();
   pdl_trigger();
   const int heads_v = p.pool.hkv * p.chunks, s = blockIdx.x / heads_v, h = blockIdx.x - s * heads_v;
@@ -604,7 +602,11 @@ __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Par
   const int kv_head = h / p.chunks, head0 = kv_head * p.group + (h - kv_head * p.chunks) * p.chunk_heads;
   const int heads = min(p.chunk_heads, (kv_head + 1) * p.group - head0);
   // block of unit f: the last whose share starts at or before it
-  const int c0 = n > 0 ? static_cast<int>(((at + 1) * p.blocks - 1) / total) : 0, c1 = n > 0 ? static_cast<int>(((at + n) * p.blocks - 1) / total) : 0;
+  const auto block_of = [&](long long f) {
+    const long long x = (f + 1) * p.blocks - 1;
+    return x < (1ll << 32) ? static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(total)) : static_cast<int>(x / total);
+  };
+  const int c0 = n > 0 ? block_of(at) : 0, c1 = n > 0 ? block_of(at + n - 1) : 0;
   if (n > 0 && c0 == c1) return;                     // one block had all of it
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kEach = D / 32;                      // values of a lane
@@ -614,37 +616,59 @@ __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Par
     float top = -INFINITY, den = 0.f, acc[kEach];
 #pragma unroll
     for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
-    if (n > 0) {
-      for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, part(c)[D]);
-      top = warp_max(top);
-#pragma unroll 4
-      for (int c = c0 + (kSlices > 1 ? warp : 0); c <= c1; c += kSlices) {
-        const float* x = part(c);
-        const float2 ml = *reinterpret_cast<const float2*>(x + D);
-        const float w = ml.x == top ? 1.f : dec4_exp2(ml.x - top);
-        den = fmaf(w, ml.y, den);
+    // four parts at a time, all of whose loads are on their way at once; the reference rises as it has to
+    for (int c = n > 0 ? c0 + (kSlices > 1 ? warp : 0) : c1 + 1; c <= c1; c += 4 * kSlices) {
+      float2 ml[4], v[4][kEach / 2];
 #pragma unroll
-        for (int j = 0; j < kEach; j += 2) {
-          const float2 v = *reinterpret_cast<const float2*>(x + lane * kEach + j);
-          acc[j] = fmaf(w, v.x, acc[j]);
-          acc[j + 1] = fmaf(w, v.y, acc[j + 1]);
+      for (int u = 0; u < 4; ++u) {
+        ml[u] = make_float2(-INFINITY, 0.f);
+        if (c + u * kSlices <= c1) {
+          const float* x = part(c + u * kSlices);
+          ml[u] = *reinterpret_cast<const float2*>(x + D);
+#pragma unroll
+          for (int j = 0; j < kEach / 2; ++j) v[u][j] = *reinterpret_cast<const float2*>(x + lane * kEach + 2 * j);
         }
       }
+      const float now = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top);
+      const float alpha = top == now ? 1.f : dec4_exp2(top - now);
+      top = now;
+      den *= alpha;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) acc[j] *= alpha;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c + u * kSlices <= c1) {
+          const float w = ml[u].x == top ? 1.f : dec4_exp2(ml[u].x - top);
+          den = fmaf(w, ml[u].y, den);
+#pragma unroll
+          for (int j = 0; j < kEach / 2; ++j) {
+            acc[2 * j] = fmaf(w, v[u][j].x, acc[2 * j]);
+            acc[2 * j + 1] = fmaf(w, v[u][j].y, acc[2 * j + 1]);
+          }
+        }
     }
     if (kSlices > 1) {
 #pragma unroll
       for (int j = 0; j < kEach; ++j) sums[warp][lane * kEach + j] = acc[j];
-      if (lane == 0) sums[warp][D] = den;
+      if (lane == 0) *reinterpret_cast<float2*>(&sums[warp][D]) = make_float2(top, den);
       __syncthreads();
       if (warp) return;
+      float2 ml[8];
+      top = -INFINITY;
       den = 0.f;
 #pragma unroll
       for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) {
-        den += sums[kSlices > 1 ? w : 0][D];
+        ml[w] = *reinterpret_cast<const float2*>(&sums[kSlices > 1 ? w : 0][D]);
+        top = fmaxf(top, ml[w].x);
+      }
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) acc[j] += sums[kSlices > 1 ? w : 0][lane * kEach + j];
+      for (int w = 0; w < 8; ++w) {
+        const float wt = ml[w].x == top ? 1.f : dec4_exp2(ml[w].x - top);
+        den = fmaf(wt, ml[w].y, den);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) acc[j] = fmaf(wt, sums[kSlices > 1 ? w : 0][lane * kEach + j], acc[j]);
       }
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
