@@ -1,0 +1,410 @@
+// Attention of prompt chunks over a K/V cache held in 4 bits (format: kv4.cuh) on the 5th-generation tensor cores: head size 128.
+//
+// The query heads of a group read the same keys, so rows are (query, head of the group) pairs of one sequence and one kv head, heads fastest: row
+// r is query r / G, head r % G. A block owns two tiles of 128 rows and walks the keys that they see in tiles of 128:
+//   warp 0        one thread issues every tcgen05.mma; TMEM holds S0 | S1 | O0 | O1 (128 columns each), P is written over S and read from there
+//   warps 4..11   softmax of tile 0 and 1, one row per thread: the maximum is raised only where it grows by more than 2^8; tiles that the
+//                 diagonal, a window or the last key crosses are masked before it. Before the first tile they bring the rows of Q
+//   warps 12..15  a thread per key: its row of codes and scales (72 bytes; the next tile's are in flight) becomes 128 bf16 of
+//                 keys, then of values, exactly, in the swizzled rows that the products read: keys along K, values along N, as they lie
+//
+// Packed rows mean that a tile is converted once for 256 rows whatever the group, and that the diagonal crosses few tiles: 256 rows of a
+// group of 8 are 32 queries. Bound by the tensor core and by what a processor issues, about equally.
+#include "kv4.cuh"
+
+namespace b200 {
+
+int num_sms();      // of the current device, see gemm_tcgen05.cu
+
+constexpr int kPf4Tile = 128;
+constexpr int kPf4D = 128;
+constexpr int kPf4Threads = 512;
+constexpr int kPf4Stages = 2;
+constexpr int kPf4Bytes = kPf4Tile * kPf4D * 2;
+constexpr float kPf4Gap = 8.f;            // raise the running maximum only beyond this many powers of two
+constexpr float kPf4Log2e = 1.4426950408889634f;
+
+struct Pf4Barriers {
+  uint64_t q_full;
+  uint64_t k_full[kPf4Stages], k_empty[kPf4Stages];
+  uint64_t v_full[kPf4Stages], v_empty[kPf4Stages];
+  uint64_t s_full[2], p_ready[2], o_done[2];
+  uint32_t tmem_base;
+  uint32_t abort_flag;
+};
+
+struct Pf4Params {
+  const __nv_bfloat16* q;      // [tokens][hq][128]
+  __nv_bfloat16* out;
+  const int* kv_lens;          // [sequences]
+  const int* cu_q;             // [sequences + 1]
+  Kv4Pool pool;
+  int hq, group, causal, window;
+  float scale_log2;            // softmax scale * log2(e)
+  float cap_in, cap_out;       // capped: cap_out * tanh(score * scale / softcap) in log2 units
+};
+
+__device__ __forceinline__ float pf4_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 columns of this warp's 32 lanes: half of the helpers' of common.cuh, for where 128 scores are in registers already.
+__device__ __forceinline__ void pf4_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void pf4_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+               "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+
+template <bool kCap>
+__global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const Pf4Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sq = smem;                                   // two Q tiles, each [half head][128 rows][128 bytes]
+  uint8_t* sk = sq + 2 * kPf4Bytes;
+  uint8_t* sv = sk + kPf4Stages * kPf4Bytes;
+  Pf4Barriers* bars = reinterpret_cast<Pf4Barriers*>(sv + kPf4Stages * kPf4Bytes);
+
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int seq = blockIdx.z, kvh = blockIdx.y, G = p.group;
+  const int q_off = p.cu_q[seq], q_len = p.cu_q[seq + 1] - q_off;
+  const int rows = q_len * G;
+  const int row0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * kPf4Tile;     // the longest rows first
+  if (row0 >= rows) return;
+  const int kv_len = kv4_length(p.pool, p.kv_lens[seq], kKernelKv4);
+  const int ctx = kv_len - q_len;                       // keys in front of the first query
+  const bool tile1 = row0 + kPf4Tile < rows;
+  const int last_query = (min(rows, row0 + 2 * kPf4Tile) - 1) / G;
+  const int n_keys = p.causal ? min(kv_len, ctx + last_query + 1) : kv_len;
+  const int first_tile = p.window > 0 ? max(0, ctx + row0 / G + 1 - p.window) / kPf4Tile : 0;
+  const int n_tiles = n_keys > first_tile * kPf4Tile ? (n_keys + kPf4Tile - 1) / kPf4Tile - first_tile : 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 8);
+    for (int i = 0; i < kPf4Stages; ++i) {
+      mbar_init(&bars->k_full[i], 4);
+      mbar_init(&bars->k_empty[i], 1);
+      mbar_init(&bars->v_full[i], 4);
+      mbar_init(&bars->v_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bars->s_full[t], 1);
+      mbar_init(&bars->p_ready[t], 4);
+      mbar_init(&bars->o_done[t], 1);
+    }
+    bars->abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&bars->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+  volatile uint32_t* abort_flag = &bars->abort_flag;
+  constexpr uint32_t kIdescS = make_idesc(128, 128, kFmtBf16, kFmtBf16);
+  constexpr uint32_t kIdescPV = kIdescS | kIdescBMn;
+
+  // launch: 128 registers a thread, 512 for the four warpgroups' threads of a lane; 56 + 2 * 184 + 88 of them below
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0 && lane == 0 && n_tiles > 0) {
+      // ----------------------------------------------------------------------- MMA issuer
+      const int nq = tile1 ? 2 : 1;
+      bool ok = mbar_wait(&bars->q_full, 0, abort_flag);
+      // S_t(j) = Q_t K_j^T into TMEM columns [t * 128, t * 128 + 128)
+      auto issue_s = [&](int t, int j) {
+        const int s = j % kPf4Stages;
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const uint64_t ad = make_desc_sw128(smem_u32(sq + t * kPf4Bytes + a * (kPf4Bytes / 2)));
+          const uint64_t bd = make_desc_sw128(smem_u32(sk + s * kPf4Bytes + a * (kPf4Bytes / 2)));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_bf16_ss(tmem_base + t * 128, ad + 2 * k, bd + 2 * k, kIdescS, (a | k) != 0);
+        }
+        tc_commit(&bars->s_full[t]);
+      };
+      if (ok) ok = mbar_wait(&bars->k_full[0], 0, abort_flag);
+      if (ok) {
+        tc_fence_after_sync();
+        for (int t = 0; t < nq; ++t) issue_s(t, 0);
+        tc_commit(&bars->k_empty[0]);
+      }
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int s = j % kPf4Stages;
+        const uint32_t ph = static_cast<uint32_t>((j / kPf4Stages) & 1);
+        for (int t = 0; t < nq && ok; ++t) {
+          if (!mbar_wait(&bars->p_ready[t], j & 1, abort_flag)) { ok = false; break; }
+          if (t == 0 && !mbar_wait(&bars->v_full[s], ph, abort_flag)) { ok = false; break; }
+          tc_fence_after_sync();
+          // O_t += P_t V_j: A = P_t in TMEM (16 keys are 8 columns of bf16 pairs), B = 16 rows of the V tile
+          const uint64_t bd = make_desc_sw128_mn(smem_u32(sv + s * kPf4Bytes), kPf4Bytes / 2);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8, bd + k * (2048 >> 4), kIdescPV, (j | k) != 0);
+          tc_commit(&bars->o_done[t]);
+          if (t == nq - 1) tc_commit(&bars->v_empty[s]);
+          if (j + 1 < n_tiles) {
+            const int s1 = (j + 1) % kPf4Stages;
+            if (t == 0 && !mbar_wait(&bars->k_full[s1], static_cast<uint32_t>(((j + 1) / kPf4Stages) & 1), abort_flag)) { ok = false; break; }
+            tc_fence_after_sync();
+            issue_s(t, j + 1);     // executes after the P_t V_j above: it overwrites the columns P_t lives in
+            if (t == nq - 1) tc_commit(&bars->k_empty[s1]);
+          }
+        }
+      }
+      if (!ok) report_status(p.pool.status, kWaitTimeout, kKernelKv4, 51, blockIdx.x);
+    }
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // ------------------------------------------------------------------------- codes to numbers, one key per thread
+    const int key = (warp - 12) * 32 + lane;
+    const int* table = p.pool.block_table + static_cast<long long>(seq) * p.pool.max_pages;
+    const int last = n_keys;
+    auto unit_of = [&](int j) -> const uint8_t* {       // the unit of this thread's key of tile j, or none
+      const int at = (first_tile + j) * kPf4Tile + key;
+      return j < n_tiles && at < last ? kv4_unit<kPf4D>(p.pool, table, kvh, at >> 4, kKernelKv4) : nullptr;
+    };
+    uint32_t kw[16], vw[16], ks = 0, vs = 0;
+    auto load = [&](const uint8_t* unit, bool values, uint32_t (&w)[16], uint32_t& scales) {
+      if (unit) {
+        kv4_load_row<kPf4D>(unit + (values ? kv4_plane_bytes(kPf4D) : 0), key & 15, values, w, scales);
+      } else {
+        scales = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = 0x88888888u;      // zeros: their probabilities are, but what lies there need not be a number
+      }
+    };
+    const uint8_t* unit = unit_of(0);
+    load(unit, false, kw, ks);
+    load(unit, true, vw, vs);
+    unit = unit_of(1);
+    bool ok = true;
+    for (int j = 0; j < n_tiles; ++j) {
+      const int s = j % kPf4Stages;
+      const uint32_t ph = static_cast<uint32_t>((j / kPf4Stages) & 1) ^ 1;
+      auto row_at = [&](uint8_t* tile, int piece) { return tile + (piece >> 3) * (kPf4Bytes / 2) + key * 128 + (((piece & 7) ^ (key & 7)) << 4); };
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty[s], ph, abort_flag)))) break;
+      kv4_key_row<kPf4D>(kw, ks, [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(row_at(sk + s * kPf4Bytes, piece)) = v; });
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->k_full[s]);
+      load(unit, false, kw, ks);
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty[s], ph, abort_flag)))) break;
+      kv4_value_row<kPf4D>(vw, vs, [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(row_at(sv + s * kPf4Bytes, piece)) = v; });
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->v_full[s]);
+      load(unit, true, vw, vs);
+      unit = unit_of(j + 2);
+    }
+    if (!ok && lane == 0) report_status(p.pool.status, kWaitTimeout, kKernelKv4, 52, blockIdx.x);
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    // ------------------------------------------------------------------------- softmax warps
+    const int t = (warp >> 2) - 1;                        // row tile of this warp group
+    const int quarter = warp & 3;                         // TMEM lane quarter this warp may touch
+    const int local = quarter * 32 + lane;                // row inside the tile = TMEM lane
+    const int row_first = row0 + t * kPf4Tile + quarter * 32, row = row_first + lane;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t s_col = lane_base + t * 128, o_col = lane_base + 256 + t * 128;
+    const int query = row / G, head = row - query * G;
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + ((static_cast<long long>(q_off) + query) * p.hq + kvh * G + head) * kPf4D);
+      uint8_t* dst = sq + t * kPf4Bytes + local * 128;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        *reinterpret_cast<uint4*>(dst + (i >> 3) * (kPf4Bytes / 2) + (((i & 7) ^ (local & 7)) << 4)) = row < rows ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->q_full);
+    }
+    if (t == 0 || tile1) {
+      const int pos = ctx + query;
+      const int lim = row >= rows ? 0 : p.causal ? min(kv_len, pos + 1) : kv_len;         // keys [start, lim) are this row's
+      const int start = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+      // keys that every row of the warp sees
+      const int open_from = __reduce_max_sync(0xffffffffu, start), open_to = __reduce_min_sync(0xffffffffu, lim);
+      float m_run = -INFINITY, l_run = 0.f;
+      const float c = kCap ? 1.f : p.scale_log2;
+      bool ok = true;
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], j & 1, abort_flag))) { ok = false; break; }
+        tc_fence_after_sync();
+        uint32_t r[128];
+        float mf[8];
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) tmem_ld_32x32(s_col + cc * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[cc * 32]));
+        tmem_ld_wait();
+#pragma unroll
+        for (int cc = 2; cc < 4; ++cc) tmem_ld_32x32(s_col + cc * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[cc * 32]));
+        const int key0 = (first_tile + j) * kPf4Tile;
+        const bool open = key0 >= open_from && key0 + kPf4Tile <= open_to;
+        if (!kCap && open) {
+          // every row of the warp sees the whole tile; the second half is in flight while the maximum of the first is taken
+#pragma unroll
+          for (int u = 0; u < 8; ++u) mf[u] = __uint_as_float(r[u]);
+#pragma unroll
+          for (int i = 8; i < 64; ++i) mf[i & 7] = fmaxf(mf[i & 7], __uint_as_float(r[i]));
+          tmem_ld_wait();
+        } else {
+          tmem_ld_wait();
+          if (kCap)
+#pragma unroll
+            for (int i = 0; i < 128; ++i)                   // cap tanh(x) = cap - 2 cap / (exp(2 x) + 1)
+              r[i] = __float_as_uint(p.cap_out - __fdividef(2.f * p.cap_out, pf4_exp2(fminf(__uint_as_float(r[i]) * p.cap_in, 126.f)) + 1.f));
+          if (!open) {
+            const int from = start - key0, to = lim - key0;
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (i >= to || i < from) r[i] = 0xff800000u;
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) mf[u] = __uint_as_float(r[u]);
+#pragma unroll
+          for (int i = 8; i < 64; ++i) mf[i & 7] = fmaxf(mf[i & 7], __uint_as_float(r[i]));
+        }
+#pragma unroll
+        for (int i = 64; i < 128; ++i) mf[i & 7] = fmaxf(mf[i & 7], __uint_as_float(r[i]));
+        const float mx = fmaxf(fmaxf(fmaxf(mf[0], mf[1]), fmaxf(mf[2], mf[3])), fmaxf(fmaxf(mf[4], mf[5]), fmaxf(mf[6], mf[7]))) * c;
+        // raise the running maximum only when it would grow by more than the gap (or on the first tile);
+        // a warp decides together because the O rescale below is a warp-wide TMEM access
+        if (__any_sync(0xffffffffu, mx > m_run + kPf4Gap)) {
+          const float m_new = fmaxf(m_run, mx);
+          const float alpha = m_run == -INFINITY ? 0.f : pf4_exp2(m_run - m_new);
+          if (j > 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&bars->o_done[t], (j - 1) & 1, abort_flag))) { ok = false; break; }
+            tc_fence_after_sync();
+#pragma unroll
+            for (int cc = 0; cc < 8; ++cc) {
+              uint32_t o[16];
+              pf4_ld16(o_col + cc * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              pf4_st16(o_col + cc * 16, o);
+            }
+            tmem_st_wait();
+          }
+          l_run *= alpha;
+          m_run = m_new;
+        }
+        const float sub = m_run == -INFINITY ? 0.f : m_run;
+        float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float a = pf4_exp2(fmaf(__uint_as_float(r[cc * 32 + 2 * i]), c, -sub));
+            const float b = pf4_exp2(fmaf(__uint_as_float(r[cc * 32 + 2 * i + 1]), c, -sub));
+            sums[i & 3] += a + b;
+            packed[i] = pack_bf16x2(a, b);
+          }
+          pf4_st16(s_col + cc * 16, packed);             // P_t: columns [0, 64) of S_t
+        }
+        tmem_st_wait();
+        l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_ready[t]);
+      }
+      if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done[t], (n_tiles - 1) & 1, abort_flag));
+      if (!ok) {
+        if (lane == 0) report_status(p.pool.status, kWaitTimeout, kKernelKv4, 53, blockIdx.x);
+      } else {
+        tc_fence_after_sync();
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        // The Q tile is no longer read: 32 rows of 128 bytes per warp turn the rows that the lanes hold into
+        // 128-byte runs. 16-byte pieces are placed by (piece xor row), which keeps the banks apart.
+        uint8_t* strip = sq + t * kPf4Bytes + quarter * 32 * 128;
+#pragma unroll
+        for (int hc = 0; hc < 2; ++hc) {
+          uint32_t o[64];
+          tmem_ld_32x32(o_col + hc * 64, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+          tmem_ld_32x32(o_col + hc * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              w[u] = n_tiles > 0 && inv != 0.f ? pack_bf16x2(__uint_as_float(o[i * 8 + 2 * u]) * inv, __uint_as_float(o[i * 8 + 2 * u + 1]) * inv) : 0u;
+            *reinterpret_cast<uint4*>(strip + lane * 128 + ((i ^ (lane & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = i * 4 + (lane >> 3), piece = lane & 7, out_row = row_first + rr;
+            const uint4 v = *reinterpret_cast<const uint4*>(strip + rr * 128 + ((piece ^ (rr & 7)) * 16));
+            if (out_row < rows) {
+              const int oq = out_row / G;
+              *reinterpret_cast<uint4*>(p.out + ((static_cast<long long>(q_off) + oq) * p.hq + kvh * G + (out_row - oq * G)) * kPf4D + hc * 64 + piece * 8) = v;
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+// Arguments as of b200_attn_kv4 with cu_q. Returns 1, and launches nothing, for sizes that the kernel of small blocks is faster or needed for.
+B200_API int b200_attn_prefill_kv4(const void* q, const void* pool, void* out, const int* block_table, const int* kv_lens, const int* cu_q,
+                                   int seqs, int max_q_len, int max_kv_len, int hq, int hkv, int d, int page, int max_pages, long long pages,
+                                   int causal, int window, float scale, float softcap, void* status, cudaStream_t stream) {
+  if (seqs <= 0 || max_q_len <= 0) return 0;
+  if (hkv < 1 || hq < 1 || hq % hkv || max_pages < 1 || pages < 1 || !kv4_pool_fits(pool, d, page)) return -2;
+  if (seqs > 65535 || hkv > 65535 || static_cast<long long>(max_q_len) * (hq / hkv) >= (1ll << 30)) return -3;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) return -4;
+  if (d != kPf4D || !(scale > 0.f)) return 1;
+  (void)max_kv_len;
+  Pf4Params p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.kv_lens = kv_lens;
+  p.cu_q = cu_q;
+  p.pool = Kv4Pool{static_cast<const uint8_t*>(pool), block_table, pages, hkv, max_pages, kv4_unit_shift(page), static_cast<DeviceStatus*>(status)};
+  p.hq = hq; p.group = hq / hkv; p.causal = causal; p.window = window;
+  p.scale_log2 = scale * kPf4Log2e;
+  if (softcap > 0.f) {
+    p.cap_in = 2.f * kPf4Log2e * scale / softcap;
+    p.cap_out = softcap * kPf4Log2e;
+  }
+  const int smem = (2 + 2 * kPf4Stages) * kPf4Bytes + static_cast<int>(sizeof(Pf4Barriers)) + 1024;
+  static PerDeviceOnce once[2];
+  auto go = [&](auto kernel, PerDeviceOnce& o) -> cudaError_t {
+    if (o.first_time()) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return e;
+    }
+    const dim3 grid(static_cast<unsigned>((static_cast<long long>(max_q_len) * p.group + 2 * kPf4Tile - 1) / (2 * kPf4Tile)), hkv, seqs);
+    return launch_pdl(kernel, grid, dim3(kPf4Threads), smem, stream, p);
+  };
+  const cudaError_t e = softcap > 0.f ? go(attn_prefill_kv4_kernel<true>, once[0]) : go(attn_prefill_kv4_kernel<false>, once[1]);
+  return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
+}

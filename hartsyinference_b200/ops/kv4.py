@@ -194,8 +194,8 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
                      max_q_len: int, causal: bool = True, scale: Optional[float] = None, softcap: float = 0.0, window: int = 0,
                      max_kv_len: Optional[int] = None) -> torch.Tensor:
     """Variable-length (chunked) attention over a 4-bit pool: q [total_q, hq, d] packed by ``cu_q`` int32 [S + 1], the keys of sequence s are
-    its first ``kv_lens[s]`` tokens, the last of them its last query's own. No sequence has more queries than ``max_q_len``. A query
-    without keys gives zeros. Arguments as of :func:`.core.attn_prefill_paged`."""
+    its first ``kv_lens[s]`` tokens, the last of them its last query's own. No sequence has more queries than ``max_q_len``; ``max_kv_len``
+    only chooses between two kernels. A query without keys gives zeros. Arguments as of :func:`.core.attn_prefill_paged`."""
     block_table, kv_lens, pages, hkv, page = _attention_args("attn_prefill_kv4", q, cache, block_table, kv_lens)
     if cu_q.numel() != kv_lens.numel() + 1:
         raise ValueError("attn_prefill_kv4: cu_q [S + 1]")
@@ -208,8 +208,12 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
         out = torch.empty_like(q)
         if block_table.shape[1] == 0 or pages == 0:
             return out.zero_()
-        rc = N.lib().b200_attn_kv4(q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(),
-                                   kv_lens.numel(), int(max_q_len), q.shape[1], hkv, q.shape[2], page, block_table.shape[1], pages, int(causal),
-                                   int(window), float(scale), float(softcap), N.state(q.device).status.data_ptr(), N.stream())
-        N.check(rc, "b200_attn_kv4")
+        L, longest = N.lib(), block_table.shape[1] * page
+        longest = longest if max_kv_len is None else min(max_kv_len, longest)
+        sizes, status = (q.shape[1], hkv, q.shape[2], page, block_table.shape[1], pages, int(causal), int(window), float(scale), float(softcap)), N.state(q.device).status
+        ptrs = (q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr())
+        rc = L.b200_attn_prefill_kv4(*ptrs, kv_lens.numel(), int(max_q_len), longest, *sizes, status.data_ptr(), N.stream())
+        if rc == 1:                                      # few rows or another head size: the kernel of small blocks
+            rc = L.b200_attn_kv4(*ptrs, kv_lens.numel(), int(max_q_len), *sizes, status.data_ptr(), N.stream())
+        N.check(rc, "b200_attn_prefill_kv4")
     return out
