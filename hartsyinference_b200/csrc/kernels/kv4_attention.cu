@@ -201,7 +201,7 @@ B200_API int b200_attn_kv4(const void* q, const void* pool, void* out, const int
                            float scale, float softcap, void* status, cudaStream_t stream) {
   if (seqs <= 0 || max_q_len <= 0) return 0;
   if (hkv < 1 || hq < 1 || hq % hkv || max_pages < 1 || pages < 1 || !kv4_pool_fits(pool, d, page)) return -2;
-  if (seqs > 65535 || hkv > 65535) return -3;
+  if (seqs > 65535 || hkv > 65535 || static_cast<long long>(max_q_len) * (hq / hkv) >= (1ll << 30)) return -3;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) return -4;
   AttnKv4Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q);

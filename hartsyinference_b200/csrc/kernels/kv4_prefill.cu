@@ -5,11 +5,14 @@
 //   warp 0        one thread issues every tcgen05.mma; TMEM holds S0 | S1 | O0 | O1 (128 columns each), P is written over S and read from there
 //   warps 4..11   softmax of tile 0 and 1, one row per thread: the maximum is raised only where it grows by more than 2^8; tiles that the
 //                 diagonal, a window or the last key crosses are masked before it. Before the first tile they bring the rows of Q
-//   warps 12..15  a thread per key: its row of codes and scales (72 bytes; the next tile's are in flight) becomes 128 bf16 of
+//   warps 12..15  a thread per key: its row of codes and scales (68 bytes; the next tile's are in flight) becomes 128 bf16 of
 //                 keys, then of values, exactly, in the swizzled rows that the products read: keys along K, values along N, as they lie
 //
 // Packed rows mean that a tile is converted once for 256 rows whatever the group, and that the diagonal crosses few tiles: 256 rows of a
-// group of 8 are 32 queries. Bound by the tensor core and by what a processor issues, about equally.
+// group of 8 are 32 queries. Bound by the tensor core and by what a processor issues, about equally: a chunk of 2048 queries behind 6144
+// keys takes 315 us for 32 heads over 8 (145 at the rate of the products alone; 284 with warps 12..15 idle; the kernel over a bf16
+// cache takes 245) and 488 us for 64 heads over 8 with 1024 queries per sequence of two (165). A grid that stays and takes blocks
+// from a counter was slower (400): the issuing thread's state then no longer fits its registers.
 #include "kv4.cuh"
 
 namespace b200 {
@@ -118,9 +121,9 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
   constexpr uint32_t kIdescS = make_idesc(128, 128, kFmtBf16, kFmtBf16);
   constexpr uint32_t kIdescPV = kIdescS | kIdescBMn;
 
-  // launch: 128 registers a thread, 512 for the four warpgroups' threads of a lane; 56 + 2 * 184 + 88 of them below
+  // launch: 128 registers a thread, 512 for the four warpgroups' threads of a lane; 72 + 2 * 176 + 88 of them below
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0 && lane == 0 && n_tiles > 0) {
       // ----------------------------------------------------------------------- MMA issuer
       const int nq = tile1 ? 2 : 1;
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
     }
     if (!ok && lane == 0) report_status(p.pool.status, kWaitTimeout, kKernelKv4, 52, blockIdx.x);
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     // ------------------------------------------------------------------------- softmax warps
     const int t = (warp >> 2) - 1;                        // row tile of this warp group
     const int quarter = warp & 3;                         // TMEM lane quarter this warp may touch
@@ -382,7 +385,16 @@ B200_API int b200_attn_prefill_kv4(const void* q, const void* pool, void* out, c
   if (seqs > 65535 || hkv > 65535 || static_cast<long long>(max_q_len) * (hq / hkv) >= (1ll << 30)) return -3;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) return -4;
   if (d != kPf4D || !(scale > 0.f)) return 1;
-  (void)max_kv_len;
+  // Short rows and short caches go to the blocks of 64 rows of b200_attn_kv4, which start faster and read P from registers. Estimates in
+  // units of a key's time here (0.0215 us): a wave of these blocks costs 350 + keys; of the others 150, and 1.2 per key and block of a
+  // processor. Both measured, these / those, in us: one sequence of 32 heads over 8 with 100 queries 13.5 / 7.1, 200: 15.6 / 9.8,
+  // 512: 20.7 / 24.1, 2048: 83 / 192; 16 sequences of 17 queries behind 100 keys 10.7 / 9.5, behind 1000: 35 / 44; 32 heads over 32
+  // there 118 / 83; one of 100 queries behind 8000 189 / 213.
+  const long long rows = static_cast<long long>(max_q_len) * (hq / hkv), lists = static_cast<long long>(seqs) * hkv;
+  const long long here = ((rows + 2 * kPf4Tile - 1) / (2 * kPf4Tile) * lists + num_sms() - 1) / num_sms();
+  const double there = static_cast<double>((rows + 63) / 64 * lists) / num_sms();
+  const double keys = window > 0 && window + static_cast<double>(max_q_len) < max_kv_len ? window + static_cast<double>(max_q_len) : max_kv_len;
+  if (150. + (there > 1. ? there : 1.) * 1.2 * keys <= static_cast<double>(here) * (350. + keys)) return 1;
   Pf4Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.out = static_cast<__nv_bfloat16*>(out);
