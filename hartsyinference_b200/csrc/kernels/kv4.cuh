@@ -25,6 +25,8 @@ constexpr int kKv4KeyExp = -6, kKv4ValueExp = -10;
 __host__ __device__ constexpr int kv4_plane_bytes(int d) { return kKv4Unit * (d / 2 + d / 32); }
 __host__ __device__ constexpr int kv4_unit_bytes(int d) { return 2 * kv4_plane_bytes(d); }
 
+constexpr int kKv4MaxSeqs = 256;          // of a batch whose key axis is cut into equal shares: their unit counts are in shared memory
+
 // The pool of one layer and where sequences lie in it.
 struct Kv4Pool {
   const uint8_t* base;

@@ -1,4 +1,4 @@
-// One query token per sequence over a K/V cache held in 4 bits (format: kv4.cuh).
+// One query token per sequence, or a few, over a K/V cache held in 4 bits (format: kv4.cuh).
 //
 // Bound by the bytes of the cache only as long as a byte costs few instructions: at 6.5 TB/s a processor gets 24 bytes (45 values) a cycle and issues
 // four warp instructions in it. So codes are never turned into numbers one by one; the tensor core multiplies registers that are masked words of a row:
@@ -17,10 +17,12 @@
 //
 // Work: a unit is 16 tokens of one kv head. All units of all sequences and heads in a row are cut into equal shares, one per resident
 // block, whatever the lengths; a share's first and last sequence may be other blocks' too, whose parts the second kernel
-// joins (in the order of the blocks, so results do not depend on timing). Within a share every warp takes each eighth unit and has its own ring of
-// bulk copies, so warps meet only where a sequence ends. Short sequences get one block each and no second kernel.
+// joins (in the order of the blocks, so results do not depend on timing). Within a share every warp takes units side by side and has its own ring of
+// bulk copies, so warps meet only at the end. Short sequences get one block each and no second kernel.
 #include "kv4.cuh"
 #include "mma_sync.cuh"
+
+#include <type_traits>
 
 namespace b200 {
 
@@ -29,18 +31,19 @@ int num_sms();      // of the current device, see gemm_tcgen05.cu
 constexpr int kDec4Warps = 8;
 constexpr int kDec4Threads = kDec4Warps * 32;
 constexpr int kDec4Stages = 2;            // of a warp's ring, two units each
-constexpr int kDec4MaxSeqs = 256;          // of a batch that is cut into shares: their unit counts are in shared memory
+constexpr int kDec4MaxSeqs = kKv4MaxSeqs;
 constexpr float kDec4Gap = 8.f;            // the reference of the exponentials is raised once a score passes it by this many powers of two
 constexpr float kDec4Log2e = 1.4426950408889634f;
 
 struct DecodeKv4Params {
-  const __nv_bfloat16* q;      // [sequences][hq][d]
+  const __nv_bfloat16* q;      // [tokens][hq][d]
   __nv_bfloat16* out;
   const int* kv_lens;
+  const int* cu_q;             // [sequences + 1]: the last tokens of a sequence ask; null: one token a sequence
   Kv4Pool pool;
   float* parts;                // [blocks][2][heads of a chunk][d + 4]: sums, maximum, denominator
   int* prefix;                 // [sequences + 1] units before a sequence, for the second kernel
-  int seqs, hq, group, chunks, chunk_heads;      // heads of a group are walked in `chunks` parts
+  int seqs, hq, group, chunks, chunk_heads;      // columns (query, head of a group), heads fastest, are walked in `chunks` parts
   int window, blocks;
   float scale_log2, cap_in, cap_out;
 };
@@ -91,11 +94,34 @@ __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Units of a sequence that its query sees, and the first of them.
-__device__ __forceinline__ int dec4_units(const DecodeKv4Params& p, int len, int& first) {
-  first = p.window > 0 ? max(0, len - p.window) / kKv4Unit : 0;
-  return len > 0 ? (len + kKv4Unit - 1) / kKv4Unit - first : 0;
+// Tokens of a sequence that ask; few: several of them, else one. Known when compiled except in the joins: decoded tokens would
+// otherwise pay for the other case (4.4 us became 5.7 for 16 short sequences).
+__device__ __forceinline__ int dec4_queries(const DecodeKv4Params& p, bool few, int s) { return few ? p.cu_q[s + 1] - p.cu_q[s] : 1; }
+// Units of a sequence that its queries see, and the first of them.
+__device__ __forceinline__ int dec4_units(const DecodeKv4Params& p, bool few, int s, int& first) {
+  const int len = kv4_length(p.pool, p.kv_lens[s], kKernelKv4), queries = dec4_queries(p, few, s);
+  first = p.window > 0 ? max(0, len - queries + 1 - p.window) / kKv4Unit : 0;
+  return len > 0 && queries > 0 ? (len + kKv4Unit - 1) / kKv4Unit - first : 0;
 }
+// The columns of part h % chunks of kv head h / chunks: how many there are, and the row of q and of the output of one of them.
+struct Dec4Columns {
+  int first, n, group, hq;
+  long long row0;
+  bool few;
+  __device__ __forceinline__ Dec4Columns(const DecodeKv4Params& p, bool few, int s, int h) : few(few) {
+    const int kv_head = h / p.chunks;
+    first = (h - kv_head * p.chunks) * p.chunk_heads;
+    n = min(p.chunk_heads, dec4_queries(p, few, s) * p.group - first);
+    group = p.group;
+    hq = p.hq;
+    row0 = static_cast<long long>(few ? p.cu_q[s] : s) * hq + kv_head * group;
+  }
+  __device__ __forceinline__ int query(int c) const { return static_cast<int>(static_cast<uint32_t>(first + c) / static_cast<uint32_t>(group)); }
+  __device__ __forceinline__ long long row(int c) const {
+    const int i = few ? query(c) : 0;
+    return row0 + static_cast<long long>(i) * hq + first + c - i * group;
+  }
+};
 
 // Dynamic shared memory: rings, one part of a sequence for every warp, the prefix.
 __host__ __device__ constexpr int dec4_ring_bytes(int d) { return kDec4Warps * kDec4Stages * 2 * kv4_unit_bytes(d); }
@@ -109,7 +135,7 @@ struct Dec4Part {
   int n;             // its units
 };
 
-template <int D, int NT, bool kShares>
+template <int D, int NT, bool kShares, bool kFew>
 __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4_kernel(const DecodeKv4Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr uint32_t kValueBias = ((127 - 15 + kKv4ValueExp) << 7) * 0x10001u;
@@ -142,7 +168,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
     int run = 0;
     for (int base = 0; base < p.seqs; base += kDec4Threads) {
       const int s = base + threadIdx.x;
-      int first, n = s < p.seqs ? dec4_units(p, kv4_length(p.pool, p.kv_lens[s], kKernelKv4), first) : 0;
+      int first, n = s < p.seqs ? dec4_units(p, kFew, s, first) : 0;
       int sum = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -168,7 +194,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
     f1 = total * (blockIdx.x + 1) / p.blocks;
   } else {
     only_seq = blockIdx.x / heads_v;
-    only_units = dec4_units(p, kv4_length(p.pool, p.kv_lens[only_seq], kKernelKv4), only_first);
+    only_units = dec4_units(p, kFew, only_seq, only_first);
     f0 = 0;
     f1 = only_units;
     __syncthreads();
@@ -187,16 +213,16 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       h = static_cast<int>(static_cast<uint32_t>(f - seq_at) / static_cast<uint32_t>(n));
       at = seq_at + static_cast<long long>(h) * n;
       first = 0;
-      if (p.window > 0) dec4_units(p, kv4_length(p.pool, p.kv_lens[s], kKernelKv4), first);
+      if (p.window > 0) dec4_units(p, kFew, s, first);
     } else {
       s = only_seq; h = blockIdx.x - only_seq * heads_v; at = 0; n = only_units; first = only_first;
     }
   };
   const int share = static_cast<int>(f1 - f0);
   if (!kShares && share == 0) {                      // a sequence without keys
-    const int h = blockIdx.x - only_seq * heads_v, kv_head = h / p.chunks, head0 = kv_head * p.group + (h - kv_head * p.chunks) * p.chunk_heads;
-    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + (static_cast<long long>(only_seq) * p.hq + head0) * D);
-    for (int c = threadIdx.x; c < min(p.chunk_heads, (kv_head + 1) * p.group - head0) * (D / 2); c += kDec4Threads) out[c] = 0u;
+    const Dec4Columns cols(p, kFew, only_seq, blockIdx.x - only_seq * heads_v);
+    for (int c = warp; c < cols.n; c += kDec4Warps)
+      for (int j = lane; j < D / 2; j += 32) reinterpret_cast<uint32_t*>(p.out + cols.row(c) * D)[j] = 0u;
     return;
   }
   // this warp's part of the share, in pairs of units
@@ -243,16 +269,15 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       at_rel = static_cast<int>(at - f0);
     }
     const int stop = min(at_rel + n, units);
-    const int kv_head = h / p.chunks, head0 = kv_head * p.group + (h - kv_head * p.chunks) * p.chunk_heads;
-    const int heads = min(p.chunk_heads, (kv_head + 1) * p.group - head0);
+    const Dec4Columns cols(p, kFew, s, h);
 
-    // queries of heads 8 t + g in half precision, with a power of two taken out so that the largest is in [2^12, 2^13)
+    // queries of columns 8 t + g in half precision, with a power of two taken out so that the largest is in [2^12, 2^13)
     uint32_t q[NT][D / 16][2];
     float factor[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const bool on = 8 * t + g < heads;
-      const __nv_bfloat16* qh = p.q + (static_cast<long long>(s) * p.hq + head0 + (on ? 8 * t + g : 0)) * D;
+      const bool on = 8 * t + g < cols.n;
+      const __nv_bfloat16* qh = p.q + (on ? cols.row(8 * t + g) * D : 0);
 #pragma unroll
       for (int m = 0; m < D / 16; ++m)
 #pragma unroll
@@ -264,8 +289,11 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       for (int j = 0; j < kDec4Stages; ++j) fetch(j, j);
     }
     const int len = kv4_length(p.pool, p.kv_lens[s], kKernelKv4);
-    const int start = p.window > 0 ? max(0, len - p.window) : 0;
-    const int last = min(len, (first + units - at_rel) * kKv4Unit);      // keys from here on are not this warp's
+    // columns of query i see the keys below len - before + i, where `before` queries are in front of the last one
+    const int before = dec4_queries(p, kFew, s) - 1;
+    const int start = p.window > 0 ? max(0, len - p.window) : 0;       // of the last query: the others' masks begin before it
+    const int stop_key = (first + units - at_rel) * kKv4Unit;          // keys from here on are not this warp's
+    const int last = min(len - before, stop_key);
     __syncwarp();                                      // the last sequence's products have read `starts`
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -316,7 +344,8 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
       for (int m = 0; m < D / 16; ++m)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[t][m][j] = 0.f;
-      mx[t][0] = mx[t][1] = line[t][0] = line[t][1] = -INFINITY;
+      mx[t][0] = mx[t][1] = -1e30f;                    // finite: a column may see nothing of a unit
+      line[t][0] = line[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
     }
     // scores of two units
@@ -375,15 +404,23 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
 #pragma unroll
             for (int j = 0; j < 4; ++j) sc[u][t][j] = p.cap_out - __fdividef(2.f * p.cap_out, dec4_exp2(fminf(sc[u][t][j], 126.f)) + 1.f);
       }
+      // keys below 0 are a pair's first unit where that is the list's before this one
       if (key0 < start || key0 + 2 * kKv4Unit > last)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int key = key0 + u * kKv4Unit + ka + (j & 2) * 4;
-            if (key < start || key >= last)
+            if (kFew) {
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                const int seen = len - before + cols.query(8 * t + 2 * tq + (j & 1));
+                if (key < 0 || key >= min(seen, stop_key) || (p.window > 0 && key < seen - p.window)) sc[u][t][j] = -INFINITY;
+              }
+            } else if (key < start || key >= last) {
 #pragma unroll
               for (int t = 0; t < NT; ++t) sc[u][t][j] = -INFINITY;
+            }
           }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -491,15 +528,15 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const float inv0 = l[t][0] == 0.f ? 0.f : 1.f / l[t][0], inv1 = l[t][1] == 0.f ? 0.f : 1.f / l[t][1];
-        const int head = 8 * t + 2 * tq + (g & 1);
-        __nv_bfloat16* dst = p.out + (static_cast<long long>(s) * p.hq + head0 + head) * D + (g & 6);
+        const int col = 8 * t + 2 * tq + (g & 1);
+        __nv_bfloat16* dst = p.out + (col < cols.n ? cols.row(col) * D : 0) + (g & 6);
 #pragma unroll
         for (int m = 0; m < D / 16; ++m)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const float v0 = o[t][m][2 * r] * inv0, v1 = o[t][m][2 * r + 1] * inv1;
             const float got = __shfl_xor_sync(0xffffffffu, g & 1 ? v0 : v1, 4);
-            if (head < heads) *reinterpret_cast<uint32_t*>(dst + m * 16 + r * 8) = g & 1 ? pack_bf16x2(got, v1) : pack_bf16x2(v0, got);
+            if (col < cols.n) *reinterpret_cast<uint32_t*>(dst + m * 16 + r * 8) = g & 1 ? pack_bf16x2(got, v1) : pack_bf16x2(v0, got);
           }
       }
     } else {
@@ -517,7 +554,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
             row[m * 16 + g] = o[t][m][j];
             row[m * 16 + 8 + g] = o[t][m][2 + j];
           }
-          if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(mx[t][j], l[t][j]);
+          if (g == 0) *reinterpret_cast<float2*>(row + D) = make_float2(l[t][j] == 0.f ? -INFINITY : mx[t][j], l[t][j]);
         }
       if (lane == 0) parked[warp][which] = Dec4Part{s, h, at_rel + w0, n};
     }
@@ -548,15 +585,14 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
     bool in[kDec4Warps];                               // warps with parts of it, all but the owner's in slot 0
 #pragma unroll
     for (int w = 0; w < kDec4Warps; ++w) in[w] = w == from || (w > from && parked[w][0].s == seq.s && parked[w][0].h == seq.h);
-    const int kv_head = seq.h / p.chunks, head0 = kv_head * p.group + (seq.h - kv_head * p.chunks) * p.chunk_heads;
-    const int heads = min(p.chunk_heads, (kv_head + 1) * p.group - head0);
+    const Dec4Columns cols(p, kFew, seq.s, seq.h);
     const bool all = seq.rel >= 0 && seq.rel + seq.n <= share;
     float* dst_part = kShares ? p.parts + (static_cast<long long>(blockIdx.x) * 2 + (seq.rel < 0 ? 0 : 1)) * p.chunk_heads * (D + 4) : nullptr;
-    for (int head = warp; head < heads; head += kDec4Warps) {
+    for (int col = warp; col < cols.n; col += kDec4Warps) {
       const int c = lane * (D / 32);
       float2 ml[kDec4Warps];
       float top = -INFINITY, den = 0.f, acc[D / 32];
-      auto row = [&](int w) { return (w == from && which ? reinterpret_cast<const float*>(smem + w * kDec4Stages * 2 * kUnit) : merge + w * 8 * NT * kPitch) + head * kPitch; };
+      auto row = [&](int w) { return (w == from && which ? reinterpret_cast<const float*>(smem + w * kDec4Stages * 2 * kUnit) : merge + w * 8 * NT * kPitch) + col * kPitch; };
 #pragma unroll
       for (int w = 0; w < kDec4Warps; ++w) {
         ml[w] = in[w] ? *reinterpret_cast<const float2*>(row(w) + D) : make_float2(-INFINITY, 0.f);
@@ -575,11 +611,11 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
         }
       if (all) {
         const float inv = den == 0.f ? 0.f : 1.f / den;
-        __nv_bfloat16* dst = p.out + (static_cast<long long>(seq.s) * p.hq + head0 + head) * D + c;
+        __nv_bfloat16* dst = p.out + cols.row(col) * D + c;
 #pragma unroll
         for (int j = 0; j < D / 32; j += 2) *reinterpret_cast<uint32_t*>(dst + j) = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
       } else {
-        float* dst = dst_part + head * (D + 4);
+        float* dst = dst_part + col * (D + 4);
 #pragma unroll
         for (int j = 0; j < D / 32; j += 2) *reinterpret_cast<float2*>(dst + c + j) = make_float2(acc[j], acc[j + 1]);
         if (lane == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(top, den);
@@ -599,8 +635,7 @@ __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Par
   const long long total = static_cast<long long>(p.prefix[p.seqs]) * heads_v;
   const int n = p.prefix[s + 1] - p.prefix[s];
   const long long at = static_cast<long long>(p.prefix[s]) * heads_v + static_cast<long long>(h) * n;
-  const int kv_head = h / p.chunks, head0 = kv_head * p.group + (h - kv_head * p.chunks) * p.chunk_heads;
-  const int heads = min(p.chunk_heads, (kv_head + 1) * p.group - head0);
+  const Dec4Columns cols(p, p.cu_q != nullptr, s, h);
   // block of unit f: the last whose share starts at or before it
   const auto block_of = [&](long long f) {
     const long long x = (f + 1) * p.blocks - 1;
@@ -610,9 +645,9 @@ __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Par
   if (n > 0 && c0 == c1) return;                     // one block had all of it
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kEach = D / 32;                      // values of a lane
-  for (int head = kSlices > 1 ? blockIdx.y : warp; head < heads; head += kSlices > 1 ? heads : 8) {
+  for (int col = kSlices > 1 ? blockIdx.y : warp; col < cols.n; col += kSlices > 1 ? p.chunk_heads : 8) {
     // the first part is the second one of its block: the sequence starts in that share
-    auto part = [&](int c) { return p.parts + ((static_cast<long long>(c) * 2 + (c == c0 ? 1 : 0)) * p.chunk_heads + head) * (D + 4); };
+    auto part = [&](int c) { return p.parts + ((static_cast<long long>(c) * 2 + (c == c0 ? 1 : 0)) * p.chunk_heads + col) * (D + 4); };
     float top = -INFINITY, den = 0.f, acc[kEach];
 #pragma unroll
     for (int j = 0; j < kEach; ++j) acc[j] = 0.f;
@@ -672,7 +707,7 @@ __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Par
       }
     }
     const float inv = den == 0.f ? 0.f : 1.f / den;
-    __nv_bfloat16* out = p.out + (static_cast<long long>(s) * p.hq + head0 + head) * D;
+    __nv_bfloat16* out = p.out + cols.row(col) * D;
 #pragma unroll
     for (int j = 0; j < kEach; j += 2) *reinterpret_cast<uint32_t*>(out + lane * kEach + j) = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
   }
@@ -685,39 +720,33 @@ static int dec4_blocks(int seqs, int heads_v, int chunk_heads, int max_kv_len) {
   const long long room = (chunk_heads > 8 ? 1ll : 2ll) * num_sms(), shares = (pairs * units + 2 * kDec4Warps - 1) / (2 * kDec4Warps);
   return static_cast<int>(shares < room ? shares : room);
 }
-static void dec4_chunks(int group, int& chunks, int& heads) {
-  chunks = (group + 15) / 16;
-  heads = (group + chunks - 1) / chunks;
+static void dec4_chunks(int columns, int& chunks, int& heads) {
+  chunks = (columns + 15) / 16;
+  heads = (columns + chunks - 1) / chunks;
 }
-
-}  // namespace b200
-
-using namespace b200;
-
-// Bytes of workspace for these sizes (0: none is used).
-B200_API long long b200_attn_decode_kv4_workspace(int seqs, int hq, int hkv, int d, int max_kv_len) {
-  if (seqs <= 0 || hkv < 1 || hq < hkv || hq % hkv) return 0;
+static long long dec4_workspace(int seqs, int columns, int hkv, int d, int max_kv_len) {
   int chunks, heads;
-  dec4_chunks(hq / hkv, chunks, heads);
+  dec4_chunks(columns, chunks, heads);
   const int blocks = dec4_blocks(seqs, hkv * chunks, heads, max_kv_len);
   return blocks == 0 ? 0 : static_cast<long long>(blocks) * 2 * heads * (d + 4) * 4 + (seqs + 1ll) * 4;
 }
 
-// q, out [sequences][hq][d] bf16. window > 0: the last `window` keys. max_kv_len chooses how the work is cut, nothing else; the workspace
-// (16-byte aligned) is of the size that b200_attn_decode_kv4_workspace gives for the same sizes. Returns the number of launches.
-B200_API int b200_attn_decode_kv4(const void* q, const void* pool, void* out, const int* block_table, const int* kv_lens, int seqs, int hq,
-                                  int hkv, int d, int page, int max_pages, long long pages, int max_kv_len, int window, float scale,
-                                  float softcap, void* workspace, long long workspace_bytes, void* status, cudaStream_t stream) {
+static int dec4_run(const void* q, const void* pool, void* out, const int* block_table, const int* kv_lens, const int* cu_q, int seqs, int max_q_len,
+                    int hq, int hkv, int d, int page, int max_pages, long long pages, int max_kv_len, int window, float scale,
+                    float softcap, void* workspace, long long workspace_bytes, void* status, cudaStream_t stream) {
   if (seqs <= 0) return 0;
   if (hkv < 1 || hq < 1 || hq % hkv || max_pages < 1 || pages < 1 || !kv4_pool_fits(pool, d, page)) return -2;
+  const long long columns = static_cast<long long>(max_q_len) * (hq / hkv), units = static_cast<long long>(max_pages) * (page / kKv4Unit);
+  if (columns >= (1ll << 20) || units * seqs >= (1ll << 31) || units * hkv * ((columns + 15) / 16) >= (1ll << 32)) return -3;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15) return -4;
   DecodeKv4Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.out = static_cast<__nv_bfloat16*>(out);
   p.kv_lens = kv_lens;
+  p.cu_q = cu_q;
   p.pool = Kv4Pool{static_cast<const uint8_t*>(pool), block_table, pages, hkv, max_pages, kv4_unit_shift(page), static_cast<DeviceStatus*>(status)};
   p.seqs = seqs; p.hq = hq; p.group = hq / hkv;
-  dec4_chunks(p.group, p.chunks, p.chunk_heads);
+  dec4_chunks(p.group * max_q_len, p.chunks, p.chunk_heads);
   p.window = window;
   p.scale_log2 = scale * kDec4Log2e;
   if (softcap > 0.f) {
@@ -726,9 +755,10 @@ B200_API int b200_attn_decode_kv4(const void* q, const void* pool, void* out, co
   }
   const long long pairs = static_cast<long long>(seqs) * hkv * p.chunks;
   if (pairs >= (1ll << 31)) return -3;
-  if (window > 0 && window < max_kv_len) max_kv_len = window + kKv4Unit;
+  if (window > 0 && window + max_q_len - 1ll < max_kv_len) max_kv_len = min(max_kv_len, window + max_q_len - 1 + kKv4Unit);
   p.blocks = dec4_blocks(seqs, hkv * p.chunks, p.chunk_heads, max_kv_len);
   const bool shares = p.blocks > 0;
+  if (cu_q && !shares) return -6;                    // short caches and many sequences are for the other kernels
   if (shares) {
     const long long floats = static_cast<long long>(p.blocks) * 2 * p.chunk_heads * (d + 4);
     if (!workspace || workspace_bytes < floats * 4 + (seqs + 1ll) * 4) return -5;
@@ -737,21 +767,25 @@ B200_API int b200_attn_decode_kv4(const void* q, const void* pool, void* out, co
   }
   const bool two = p.chunk_heads > 8;
   const int most = dec4_smem_bytes(d, two ? 2 : 1), smem = most - (shares ? kDec4MaxSeqs - seqs : kDec4MaxSeqs + 1) * 4;
-  static PerDeviceOnce once[8];
-  auto go = [&](auto kernel, PerDeviceOnce& o) -> cudaError_t {
-    if (o.first_time()) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-      if (e != cudaSuccess) return e;
-    }
-    return launch_pdl(kernel, dim3(static_cast<unsigned>(shares ? p.blocks : pairs)), dim3(kDec4Threads), smem, stream, p);
+  cudaError_t e = cudaSuccess;
+  auto go = [&](auto kernel, PerDeviceOnce& o) {
+    if (o.first_time()) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess) e = launch_pdl(kernel, dim3(static_cast<unsigned>(shares ? p.blocks : pairs)), dim3(kDec4Threads), smem, stream, p);
   };
-  cudaError_t e;
+  auto pick = [&](auto dim, auto tiles, auto few) {
+    static PerDeviceOnce once[2];
+    if constexpr (few()) go(attn_decode_kv4_kernel<dim(), tiles(), true, true>, once[0]);
+    else if (shares) go(attn_decode_kv4_kernel<dim(), tiles(), true, false>, once[0]);
+    else go(attn_decode_kv4_kernel<dim(), tiles(), false, false>, once[1]);
+  };
+  auto pick_few = [&](auto dim, auto tiles) {
+    if (cu_q) pick(dim, tiles, std::true_type{}); else pick(dim, tiles, std::false_type{});
+  };
+  using std::integral_constant;
   if (d == 128) {
-    if (shares) e = two ? go(attn_decode_kv4_kernel<128, 2, true>, once[0]) : go(attn_decode_kv4_kernel<128, 1, true>, once[1]);
-    else e = two ? go(attn_decode_kv4_kernel<128, 2, false>, once[2]) : go(attn_decode_kv4_kernel<128, 1, false>, once[3]);
+    if (two) pick_few(integral_constant<int, 128>{}, integral_constant<int, 2>{}); else pick_few(integral_constant<int, 128>{}, integral_constant<int, 1>{});
   } else {
-    if (shares) e = two ? go(attn_decode_kv4_kernel<64, 2, true>, once[4]) : go(attn_decode_kv4_kernel<64, 1, true>, once[5]);
-    else e = two ? go(attn_decode_kv4_kernel<64, 2, false>, once[6]) : go(attn_decode_kv4_kernel<64, 1, false>, once[7]);
+    if (two) pick_few(integral_constant<int, 64>{}, integral_constant<int, 2>{}); else pick_few(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   }
   if (e != cudaSuccess) return -static_cast<int>(e) - 300;
   if (!shares) return 1;
@@ -761,4 +795,37 @@ B200_API int b200_attn_decode_kv4(const void* q, const void* pool, void* out, co
   if (d == 128) e = many ? launch_pdl(join_decode_kv4_kernel<128, 8>, grid, dim3(256), 0, stream, p) : launch_pdl(join_decode_kv4_kernel<128, 1>, grid, dim3(256), 0, stream, p);
   else e = many ? launch_pdl(join_decode_kv4_kernel<64, 8>, grid, dim3(256), 0, stream, p) : launch_pdl(join_decode_kv4_kernel<64, 1>, grid, dim3(256), 0, stream, p);
   return e == cudaSuccess ? 2 : -static_cast<int>(e) - 400;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+// Bytes of workspace for these sizes (0: none is used).
+B200_API long long b200_attn_decode_kv4_workspace(int seqs, int hq, int hkv, int d, int max_kv_len) {
+  return seqs <= 0 || hkv < 1 || hq < hkv || hq % hkv ? 0 : dec4_workspace(seqs, hq / hkv, hkv, d, max_kv_len);
+}
+
+// q, out [sequences][hq][d] bf16. window > 0: the last `window` keys. max_kv_len chooses how the work is cut, nothing else; the workspace
+// (16-byte aligned) is of the size that b200_attn_decode_kv4_workspace gives for the same sizes. Returns the number of launches.
+B200_API int b200_attn_decode_kv4(const void* q, const void* pool, void* out, const int* block_table, const int* kv_lens, int seqs, int hq,
+                                  int hkv, int d, int page, int max_pages, long long pages, int max_kv_len, int window, float scale,
+                                  float softcap, void* workspace, long long workspace_bytes, void* status, cudaStream_t stream) {
+  return dec4_run(q, pool, out, block_table, kv_lens, nullptr, seqs, 1, hq, hkv, d, page, max_pages, pages, max_kv_len, window, scale, softcap,
+                  workspace, workspace_bytes, status, stream);
+}
+
+// A few queries per sequence behind a long cache: q, out [tokens][hq][d] packed by cu_q [sequences + 1], causal. Columns of the products are
+// (query, head) pairs, 16 at a time, each time over all units. For more than 512 keys and at most 256 sequences. The workspace is of the size that b200_attn_few_kv4_workspace gives.
+B200_API long long b200_attn_few_kv4_workspace(int seqs, int max_q_len, int hq, int hkv, int d, int max_kv_len) {
+  if (seqs <= 0 || max_q_len < 1 || hkv < 1 || hq < hkv || hq % hkv || static_cast<long long>(max_q_len) * (hq / hkv) >= (1ll << 20)) return 0;
+  return dec4_workspace(seqs, max_q_len * (hq / hkv), hkv, d, max_kv_len);
+}
+B200_API int b200_attn_few_kv4(const void* q, const void* pool, void* out, const int* block_table, const int* kv_lens, const int* cu_q, int seqs,
+                               int max_q_len, int hq, int hkv, int d, int page, int max_pages, long long pages, int max_kv_len, int window,
+                               float scale, float softcap, void* workspace, long long workspace_bytes, void* status, cudaStream_t stream) {
+  if (max_q_len < 1) return 0;
+  if (!cu_q) return -2;
+  return dec4_run(q, pool, out, block_table, kv_lens, cu_q, seqs, max_q_len, hq, hkv, d, page, max_pages, pages, max_kv_len, window, scale, softcap,
+                  workspace, workspace_bytes, status, stream);
 }

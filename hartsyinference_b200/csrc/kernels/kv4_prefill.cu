@@ -376,25 +376,36 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
 
 using namespace b200;
 
-// Arguments as of b200_attn_kv4 with cu_q. Returns 1, and launches nothing, for sizes that the kernel of small blocks is faster or needed for.
+// Which kernel takes a batch of prompt chunks of these sizes: 0 b200_attn_kv4, 1 b200_attn_prefill_kv4, 2 b200_attn_few_kv4.
+B200_API int b200_attn_kv4_choice(int seqs, int max_q_len, int max_kv_len, int hq, int hkv, int d, int causal, int window, float scale) {
+  if (seqs < 1 || max_q_len < 1 || hkv < 1 || hq < hkv) return 0;
+  // Estimates in us from the times below. Blocks of 64 rows (b200_attn_kv4) start fastest and share a processor; blocks of 256 rows (this file's)
+  // come in waves; parts of the key axis (b200_attn_few_kv4) read all units once for every 16 columns.
+  // Measured in us, 64 rows / 256 rows / parts, 32 heads over 8: one sequence of 100 queries 7.1 / 13.4 / 19, of 512 24 / 21 / -, of 2048
+  // 192 / 83 / -; 17 queries behind 1000 keys 30 / 29 / 22, behind 8000 212 / 185 / 36; 100 there 212 / 224 / 98; 8 behind 30000 770 / 675 / 39;
+  // 16 sequences of 17 behind 100 keys 9.7 / 10.6 / 49, behind 1000 44 / 35 / 57, of 5 behind 3000 81 / 85 / 57. 32 heads over 32: 16 of 17
+  // behind 1000 84 / 118 / 76.
+  const long long rows = static_cast<long long>(max_q_len) * (hq / hkv), lists = static_cast<long long>(seqs) * hkv;
+  const long long waves = ((rows + 2 * kPf4Tile - 1) / (2 * kPf4Tile) * lists + num_sms() - 1) / num_sms();
+  const double each = static_cast<double>((rows + 63) / 64 * lists) / num_sms();       // blocks of 64 rows a processor
+  const double keys = window > 0 && window + static_cast<double>(max_q_len) < max_kv_len ? window + static_cast<double>(max_q_len) : max_kv_len;
+  const double units = keys / kKv4Unit * static_cast<double>((rows + 15) / 16 * lists);
+  const double small = 3.3 + (each > 1. ? each : 1.) * 0.026 * keys, wide = static_cast<double>(waves) * (7.5 + 0.0215 * keys);
+  const double parts = 18. + 0.0008 * units;
+  const bool can = d == kPf4D && scale > 0.f, best = can && wide < small;
+  if (causal && keys > 512. && rows < 65536 && seqs <= kKv4MaxSeqs && parts < (best ? wide : small)) return 2;
+  return best;
+}
+
+// Arguments as of b200_attn_kv4 with cu_q; d 128 and a scale above 0.
 B200_API int b200_attn_prefill_kv4(const void* q, const void* pool, void* out, const int* block_table, const int* kv_lens, const int* cu_q,
-                                   int seqs, int max_q_len, int max_kv_len, int hq, int hkv, int d, int page, int max_pages, long long pages,
+                                   int seqs, int max_q_len, int hq, int hkv, int d, int page, int max_pages, long long pages,
                                    int causal, int window, float scale, float softcap, void* status, cudaStream_t stream) {
   if (seqs <= 0 || max_q_len <= 0) return 0;
   if (hkv < 1 || hq < 1 || hq % hkv || max_pages < 1 || pages < 1 || !kv4_pool_fits(pool, d, page)) return -2;
   if (seqs > 65535 || hkv > 65535 || static_cast<long long>(max_q_len) * (hq / hkv) >= (1ll << 30)) return -3;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) return -4;
-  if (d != kPf4D || !(scale > 0.f)) return 1;
-  // Short rows and short caches go to the blocks of 64 rows of b200_attn_kv4, which start faster and read P from registers. Estimates in
-  // units of a key's time here (0.0215 us): a wave of these blocks costs 350 + keys; of the others 150, and 1.2 per key and block of a
-  // processor. Both measured, these / those, in us: one sequence of 32 heads over 8 with 100 queries 13.5 / 7.1, 200: 15.6 / 9.8,
-  // 512: 20.7 / 24.1, 2048: 83 / 192; 16 sequences of 17 queries behind 100 keys 10.7 / 9.5, behind 1000: 35 / 44; 32 heads over 32
-  // there 118 / 83; one of 100 queries behind 8000 189 / 213.
-  const long long rows = static_cast<long long>(max_q_len) * (hq / hkv), lists = static_cast<long long>(seqs) * hkv;
-  const long long here = ((rows + 2 * kPf4Tile - 1) / (2 * kPf4Tile) * lists + num_sms() - 1) / num_sms();
-  const double there = static_cast<double>((rows + 63) / 64 * lists) / num_sms();
-  const double keys = window > 0 && window + static_cast<double>(max_q_len) < max_kv_len ? window + static_cast<double>(max_q_len) : max_kv_len;
-  if (150. + (there > 1. ? there : 1.) * 1.2 * keys <= static_cast<double>(here) * (350. + keys)) return 1;
+  if (d != kPf4D || !(scale > 0.f)) return -5;
   Pf4Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.out = static_cast<__nv_bfloat16*>(out);

@@ -121,7 +121,10 @@ _SIGNATURES = {
     "b200_kv4_gather": (i32, [vp] * 5 + [i32] * 6 + [i64, vp, vp]),
     "b200_attn_decode_kv4_workspace": (i64, [i32] * 5),
     "b200_attn_decode_kv4": (i32, [vp] * 5 + [i32] * 6 + [i64, i32, i32, f32, f32, vp, i64, vp, vp]),
-    "b200_attn_prefill_kv4": (i32, [vp] * 6 + [i32] * 8 + [i64, i32, i32, f32, f32, vp, vp]),
+    "b200_attn_few_kv4_workspace": (i64, [i32] * 6),
+    "b200_attn_few_kv4": (i32, [vp] * 6 + [i32] * 7 + [i64, i32, i32, f32, f32, vp, i64, vp, vp]),
+    "b200_attn_kv4_choice": (i32, [i32] * 8 + [f32]),
+    "b200_attn_prefill_kv4": (i32, [vp] * 6 + [i32] * 7 + [i64, i32, i32, f32, f32, vp, vp]),
     "b200_attn_kv4": (i32, [vp] * 6 + [i32] * 7 + [i64, i32, i32, f32, f32, vp, vp]),
     "b200_attn_prefill": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp]),
 }

@@ -4,7 +4,7 @@ A layer's pool is uint8 ``[pages, kv heads, page / 16, 2, 16 * (d / 2 + d / 32)]
 instead of 32. Every 32 neighbouring values of a head share a scale of 8 bits, ``max|x| / 7`` with three bits of mantissa; a value is held
 as the nearest multiple of it from -7 to 7. Keys up to 6720 and values up to 420 in magnitude are held so, larger ones and
 infinities as the largest multiple, NaN as zero. Head sizes 64 and 128, pages of 16, 32, 64 or 128 tokens, any number
-of query heads per key head. CUDA tensors are bf16; CPU tensors go to the statements in :mod:`.reference`.
+of query heads per key head. CUDA tensors are bf16, block tables and lengths int32; CPU tensors go to the statements in :mod:`.reference`.
 """
 from __future__ import annotations
 
@@ -210,10 +210,16 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
             return out.zero_()
         L, longest = N.lib(), block_table.shape[1] * page
         longest = longest if max_kv_len is None else min(max_kv_len, longest)
-        sizes, status = (q.shape[1], hkv, q.shape[2], page, block_table.shape[1], pages, int(causal), int(window), float(scale), float(softcap)), N.state(q.device).status
-        ptrs = (q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr())
-        rc = L.b200_attn_prefill_kv4(*ptrs, kv_lens.numel(), int(max_q_len), longest, *sizes, status.data_ptr(), N.stream())
-        if rc == 1:                                      # few rows or another head size: the kernel of small blocks
-            rc = L.b200_attn_kv4(*ptrs, kv_lens.numel(), int(max_q_len), *sizes, status.data_ptr(), N.stream())
+        seqs, most, hq, d, window, scale = kv_lens.numel(), int(max_q_len), q.shape[1], q.shape[2], int(window), float(scale)
+        ptrs = (q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(), seqs, most)
+        sizes, status = (hq, hkv, d, page, block_table.shape[1], pages), N.state(q.device).status.data_ptr()
+        kernel = L.b200_attn_kv4_choice(seqs, most, longest, hq, hkv, d, int(causal), window, scale)
+        if kernel == 2:                                  # few queries behind a long cache
+            need = L.b200_attn_few_kv4_workspace(seqs, most, hq, hkv, d, longest)
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+            rc = min(0, L.b200_attn_few_kv4(*ptrs, *sizes, longest, window, scale, float(softcap), N.ptr(ws), need, status, N.stream()))
+        else:
+            run = L.b200_attn_prefill_kv4 if kernel else L.b200_attn_kv4
+            rc = run(*ptrs, *sizes, int(causal), window, scale, float(softcap), status, N.stream())
         N.check(rc, "b200_attn_prefill_kv4")
     return out

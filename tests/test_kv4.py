@@ -80,14 +80,14 @@ def _plain(q, cache, table, lens, cuts, causal=True, scale=None, softcap=0.0, wi
 
 
 def _close(got, want, size, scales):
-    """Probabilities are rounded to bf16 before and after the product with a scale (half a step each, 2^-9 twice, of sum p |v|), the
-    result to bf16 (2^-9 of it): 2^-8 of both holds with a half to spare. Scores are sums of 128 products in 32 bits, of
+    """A rounding to bf16 (8 bits, the first of them 1) is off by at most half of the last one, 2^-8 of the value. Probabilities are rounded before and
+    after the product with a scale: twice 2^-8 of sum p |v|. The result is: 2^-8 of it. Scores are sums of 128 products in 32 bits, of
     which sum |q k| scale is below 2^9 here: off by less than 2^9 * 2^-24 * 2 * 2^3 = 2^-11, and so are probabilities and their sum.
     Values enter as 128 + code, and 136 is taken off again, 16 keys at a time: two sums of at most 143 p s that are cut to 24 bits,
     2 * 2^-22 * 143 < 2^-13 of sum p s with two bits to spare."""
     off = (got.double().cpu() - want).abs()
     assert torch.isfinite(got).all()
-    bound = 2.0 ** -8 * (size + want.abs()) + 2.0 ** -10 * size + 2.0 ** -13 * scales + 1e-30
+    bound = 2.0 ** -7 * size + 2.0 ** -8 * want.abs() + 2.0 ** -10 * size + 2.0 ** -13 * scales + 1e-30
     assert (off <= bound).all(), float((off / bound).max())
 
 
@@ -199,6 +199,17 @@ def test_entry_points_refuse_sizes_before_any_launch():
     assert L.b200_attn_kv4(p, p, p, p, p, None, 1, 1, 5, 2, 64, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -2
     assert L.b200_attn_kv4(p, p, p, p, p, None, 70000, 1, 4, 2, 64, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -3
     assert L.b200_attn_kv4(p, p, p + 8, p, p, None, 1, 1, 4, 2, 64, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -4
+    assert L.b200_attn_kv4(p, p, p, p, p, None, 1, 1 << 29, 8, 2, 64, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -3
+    assert L.b200_attn_prefill_kv4(p, p, p, p, p, p, 1, 1, 5, 2, 128, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -2
+    assert L.b200_attn_prefill_kv4(p, p, p, p, p, p, 70000, 1, 4, 2, 128, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -3
+    assert L.b200_attn_prefill_kv4(p + 4, p, p, p, p, p, 1, 1, 4, 2, 128, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -4
+    assert L.b200_attn_prefill_kv4(p, p, p, p, p, p, 1, 1, 4, 2, 64, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -5
+    assert L.b200_attn_decode_kv4(p, p, p, p, p, 1, 5, 2, 64, 16, 1, 1, 16, 0, 1.0, 0.0, None, 0, None, None) == -2
+    assert L.b200_attn_decode_kv4(p, p, p, p, p, 1, 4, 2, 64, 16, 0, 1, 16, 0, 1.0, 0.0, None, 0, None, None) == -2
+    assert L.b200_attn_decode_kv4(p, p, p, p, p, 200, 4, 2, 64, 128, 1 << 21, 1, 16, 0, 1.0, 0.0, None, 0, None, None) == -3
+    assert L.b200_attn_decode_kv4(p, p, p + 8, p, p, 1, 4, 2, 64, 16, 1, 1, 16, 0, 1.0, 0.0, None, 0, None, None) == -4
+    assert L.b200_attn_few_kv4(p, p, p, p, p, None, 1, 2, 4, 2, 64, 16, 1, 1, 16, 0, 1.0, 0.0, None, 0, None, None) == -2
+    assert L.b200_attn_few_kv4(p, p, p, p, p, p, 1, 2, 4, 2, 64, 16, 1, 1, 16, 0, 1.0, 0.0, None, 0, None, None) == -6
 
 
 @pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 1, 128)])
@@ -319,3 +330,173 @@ def test_prefill_kernel(hq, hkv, d, kw):
     got = ops.attn_prefill_kv4(*dev, max(each), **kw)
     _close(got, *want)
     _close(ops.attn_prefill_kv4(*dev, max(each) + 300, max_kv_len=333, **kw), *want)
+
+
+def _few(q, cache, table, lens, cuts, most, longest, scale=None, softcap=0.0, window=0):
+    """The kernel that cuts the key axis, whatever kernel the op would take."""
+    from hartsyinference_b200.ops import _native as N
+    L, n, hq, d = N.lib(), len(lens), q.shape[1], q.shape[2]
+    hkv, page = cache.shape[1], cache.shape[2] * 16
+    need = L.b200_attn_few_kv4_workspace(n, most, hq, hkv, d, longest)
+    ws, out = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.full_like(q, 7)
+    rc = L.b200_attn_few_kv4(q.data_ptr(), cache.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), cuts.data_ptr(), n, most, hq, hkv, d, page,
+                             table.shape[1], cache.shape[0], longest, window, 1 / math.sqrt(d) if scale is None else scale, softcap, ws.data_ptr(), need,
+                             N.state(q.device).status.data_ptr(), N.stream())
+    assert rc > 0
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+@pytest.mark.parametrize("kw", CASES)
+def test_few_queries_behind_a_long_cache(hq, hkv, d, kw):
+    """One query, none, more than keys, parts of columns that a sequence does not fill, sequences without keys."""
+    lens, each = [700, 0, 5, 2100, 16, 900, 0, 1033], [3, 2, 7, 17, 0, 1, 0, 2]
+    cache, table = _filled(lens, hkv, d, 32)
+    cuts = torch.tensor([0, *each]).cumsum(0).tolist()
+    q = _normal(sum(each), hq, d, seed=9).to(torch.bfloat16)
+    want = _plain(q, cache, table, lens, cuts, **kw)
+    dev = _cuda(q, cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor(cuts, dtype=torch.int32))
+    longest = max(lens) if not kw.get("window") else 40000                              # a window would leave one part
+    if kw.get("window", 1000) > 600:
+        _close(_few(*dev, max(each), longest, **kw), *want)
+        _close(_few(*dev, max(each) + 30, 20000, **kw), *want)
+    _close(ops.attn_prefill_kv4(*dev, max(each), **kw), *want)
+
+
+@gpu
+def test_few_queries_in_a_window():
+    lens, each, kw = [3000, 1500, 611], [5, 3, 9], dict(window=600)
+    for hq, hkv, d in HEADS[:4]:
+        cache, table = _filled(lens, hkv, d, 64)
+        cuts = torch.tensor([0, *each]).cumsum(0).tolist()
+        q = _normal(sum(each), hq, d, seed=9).to(torch.bfloat16)
+        dev = _cuda(q, cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor(cuts, dtype=torch.int32))
+        _close(_few(*dev, 9, 3000, **kw), *_plain(q, cache, table, lens, cuts, **kw))
+
+
+@gpu
+@pytest.mark.parametrize("sizes,kernel", [((1, 100, 100), 0), ((1, 2048, 8192), 1), ((16, 5, 4000), 2)])
+def test_every_prompt_kernel_is_chosen(sizes, kernel):
+    from hartsyinference_b200.ops import _native as N
+    assert N.lib().b200_attn_kv4_choice(*sizes, 32, 8, 128, 1, 0, 0.088) == kernel
+    assert N.lib().b200_attn_kv4_choice(*sizes, 32, 8, 128, 0, 0, 0.088) < 2
+    assert N.lib().b200_attn_kv4_choice(*sizes, 32, 8, 64, 1, 0, 0.125) != 1
+
+
+@gpu
+def test_calls_captured_and_on_two_streams():
+    """Two graphs of the same op replayed side by side, with lengths that change between replays, and a call of its own beside them."""
+    lens = [1900, 1, 700]
+    cache, table = _filled(lens, 2, 128, 16)
+    q = [_normal(3, 8, 128, seed=i).to(torch.bfloat16) for i in range(2)]
+    dev = _cuda(cache, table, torch.tensor(lens, dtype=torch.int32))
+    qd, streams, graphs, outs = _cuda(*q), [torch.cuda.Stream(), torch.cuda.Stream()], [], []
+    cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
+    run = [lambda x: ops.attn_decode_kv4(x, *dev), lambda x: ops.attn_prefill_kv4(x, *dev, cu, 1)]
+    for f, x, st in zip(run, qd, streams):
+        with torch.cuda.stream(st):
+            f(x)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            outs.append(f(x))
+        graphs.append(g)
+    for now in (lens, [5, 0, 640], lens):
+        dev[2].copy_(torch.tensor(now, dtype=torch.int32))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        own = run[0](qd[0])
+        torch.cuda.synchronize()
+        for x, out in zip(q, outs):
+            _close(out, *_plain(x, cache, table, now, [0, 1, 2, 3]))
+        assert torch.equal(own, outs[0])
+
+
+@gpu
+def test_rows_of_another_layout():
+    """Rows with a stride, on an odd address, and integers with a stride; those of another type are refused."""
+    lens, hq, hkv, d = [130, 600], 8, 2, 128
+    cache, table = _filled(lens, hkv, d, 16)
+    wide = _normal(2, 2 * hq, d, seed=3).to(torch.bfloat16)
+    q = wide[:, ::2]
+    odd = torch.empty(2 * hq * d + 1, dtype=torch.bfloat16, device="cuda")[1:].view(2, hq, d)
+    odd.copy_(q)
+    want = _plain(q, cache, table, lens, [0, 1, 2])
+    c, t, n = _cuda(cache, torch.stack([table, table], -1), torch.tensor(lens, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        ops.attn_decode_kv4(odd, c, t[..., 0], n.long())
+    for x in (wide.cuda()[:, ::2], odd):
+        _close(ops.attn_decode_kv4(x, c, t[..., 0], n), *want)
+        _close(ops.attn_prefill_kv4(x, c, t[..., 0], n, torch.tensor([0, 9, 1, 9, 2], dtype=torch.int32, device="cuda")[::2], 1), *want)
+
+
+@gpu
+def test_pages_outside_the_pool_are_reported_and_lengths_cut():
+    """An entry that names no page reads as page 0, a length beyond the row's pages ends there; both leave a word in the status."""
+    from hartsyinference_b200.exceptions import DeviceWaitTimeout
+    from hartsyinference_b200.ops import _native as N
+    lens = [40, 1200]
+    cache, table = _filled(lens, 2, 128, 16)
+    as_read, long = table.clone(), [40, table.shape[1] * 16]
+    as_read[(as_read < 0) | (as_read >= cache.shape[0])] = 0
+    q = _normal(2, 8, 128, seed=1).to(torch.bfloat16)
+    cache.copy_(torch.randint(0, 200, cache.shape, generator=torch.Generator().manual_seed(2), dtype=torch.uint8))      # page 0 and the rest: finite
+    cache.view(-1, cache.shape[-1])[:, 64 * 16:] = 100
+    want = _plain(q, cache, as_read, long, [0, 1, 2])
+    c, t, n = _cuda(cache, table, torch.tensor([40, 1 << 30], dtype=torch.int32))
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for f in (lambda: ops.attn_decode_kv4(q.cuda(), c, t, n), lambda: ops.attn_prefill_kv4(q.cuda(), c, t, n, cu, 1),
+              lambda: ops.attn_prefill_kv4(q.cuda(), c, t, n, cu, 1, max_kv_len=16)):
+        N.check_status()
+        _close(f(), *want)
+        with pytest.raises(DeviceWaitTimeout):
+            N.check_status()
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """A pool of more than 2^32 bytes whose used pages lie at its end."""
+    hkv, d, page, lens = 8, 128, 64, [70, 900]
+    cache, table = _filled(lens, hkv, d, page)
+    each = cache[0].numel()
+    pages = (1 << 32) // each + cache.shape[0] + 5
+    big = torch.empty(pages, *cache.shape[1:], dtype=torch.uint8, device="cuda")
+    big[pages - cache.shape[0]:] = cache.cuda()
+    moved = torch.where(table >= 0, table + (pages - cache.shape[0]), table)
+    q = _normal(2, 32, d, seed=1).to(torch.bfloat16)
+    want = _plain(q, cache, table, lens, [0, 1, 2])
+    qd, t, n, cu = _cuda(q, moved, torch.tensor(lens, dtype=torch.int32), torch.tensor([0, 1, 2], dtype=torch.int32))
+    _close(ops.attn_decode_kv4(qd, big, t, n), *want)
+    _close(ops.attn_prefill_kv4(qd, big, t, n, cu, 1), *want)
+    _close(ops.attn_prefill_kv4(qd, big, t, n, cu, 1, causal=False), *want)
+    kv = torch.tensor([0, 70, 970], dtype=torch.int32)
+    for a, b in zip(ops.kv4_gather(big, t, kv.cuda(), 970), ops.kv4_gather(cache, table, kv, 970)):
+        assert torch.equal(a.cpu(), b)
+    qkv, pos, small, _ = _qkv_args(4, 8, hkv, d, page)
+    slots = torch.tensor([0, 65, 2, -1])
+    ops.rope_kv4(qkv, pos, 8, hkv, d, cache=small, slot_mapping=slots)
+    last = pages - small.shape[0]
+    big[last:] = 0
+    ops.rope_kv4(qkv.cuda(), pos.cuda(), 8, hkv, d, cache=big, inv_freq=R.rope_inv_freq(d, 10000.0).cuda(), slot_mapping=torch.where(slots >= 0, slots + last * page, slots).cuda())
+    assert torch.equal(big[last:].cpu(), small)
+
+
+@gpu
+def test_first_token_that_takes_nearly_all_of_the_weight():
+    """A first key far ahead of the others whose values are zero: the result is made of probabilities near 2^-20."""
+    n, hkv, d = 1500, 2, 128
+    k, v = _normal(n, hkv, d, seed=1), _normal(n, hkv, d, seed=2)
+    q = _normal(1, 8, d, seed=3).to(torch.bfloat16)
+    k[0], v[0] = 0, 0
+    k[0, :, :] = q.float().view(hkv, 4, d).mean(1) * 3
+    cache, table = ops.kv4_cache(100, hkv, 16, d, "cpu"), torch.arange(99, -1, -1, dtype=torch.int32)[None]
+    pos = torch.arange(n)
+    R.kv4_store(cache, table[0, pos // 16].long() * 16 + pos % 16, k, v)
+    want = _plain(q, cache, table, [n], [0, 1])
+    dev = _cuda(cache, table, torch.tensor([n], dtype=torch.int32))
+    _close(ops.attn_decode_kv4(q.cuda(), *dev), *want)
+    _close(ops.attn_prefill_kv4(q.cuda(), *dev, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), 1), *want)
