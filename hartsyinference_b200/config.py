@@ -93,7 +93,7 @@ declare("profile_sync", bool, False, "synchronise after every profiled op so hos
 declare("nvtx", bool, False, "emit NVTX ranges around ops and engine phases")
 declare("kv_page_size", int, 16, "tokens per KV page")
 declare("kv_pool_bytes", int, 0, "KV pool budget in bytes; 0 = size from free device memory")
-declare("kv_dtype", str, "bf16", "KV cache dtype: bf16")
+declare("kv_dtype", str, "bf16", "KV cache dtype: bf16, or int4 (4-bit values with an 8-bit scale per 32, heads of 64 or 128)")
 declare("cuda_graphs", bool, True, "capture the decode step in CUDA graphs")
 declare("max_batch", int, 256, "largest decode batch the scheduler forms")
 declare("prefill_chunk", int, 8192, "tokens per prefill chunk")

@@ -102,8 +102,14 @@ def x_is_cuda(x) -> bool:
 class DecoderModel:
     def __init__(self, cfg: TransformerConfig, device: torch.device | str = "cpu", comm: Optional[Comm] = None,
                  fp8: bool = False, layer_range: Optional[tuple[int, int]] = None, dp_attention: bool = False,
-                 dtype: torch.dtype = torch.bfloat16):
+                 dtype: torch.dtype = torch.bfloat16, kv_dtype: Optional[str] = None):
         self.cfg = cfg
+        # what the cache holds keys and values in: "bf16", or "int4" with a scale of 8 bits per 32 values (ops.kv4)
+        self.kv_dtype = config.get("kv_dtype") if kv_dtype is None else kv_dtype
+        if self.kv_dtype not in ("bf16", "int4"):
+            raise ValueError(f"KV cache dtype bf16 or int4, got '{self.kv_dtype}'")
+        if self.kv_dtype == "int4" and (cfg.mla is not None or cfg.mixed_layers or cfg.head_dim not in (64, 128)):
+            raise ValueError(f"{cfg.arch}: a 4-bit KV cache takes plain attention with heads of 64 or 128")
         # activation dtype: bf16, or fp32 (32-bit products and caches) where the layers have that form
         if dtype != torch.bfloat16 and not (cfg.mixed_layers and dtype == torch.float32):
             raise ValueError(f"{cfg.arch}: activations run in bfloat16")
@@ -586,11 +592,14 @@ class DecoderModel:
                        if hasattr(lw.attn_module, "cache_shape"))
         if self.cfg.mla is not None:
             return (self.layer1 - self.layer0) * page * (self.cfg.mla.kv_lora_rank + self.cfg.mla.qk_rope_head_dim) * 2
+        if self.kv_dtype == "int4":
+            return (self.layer1 - self.layer0) * self.hkv * page * self.cfg.head_dim * 17 // 16
         return (self.layer1 - self.layer0) * 2 * self.hkv * page * self.cfg.head_dim * 2
 
     def alloc_kv(self, num_pages: int, page: int = 16) -> torch.Tensor:
         """[layers, 2, pages, hkv_local, page, head_dim] bf16, or with multi-head latent attention
-        [layers, pages, page, 576] (latent + rotated shared key, replicated on every rank)."""
+        [layers, pages, page, 576] (latent + rotated shared key, replicated on every rank), or in 4 bits a pool of
+        ``ops.kv4_cache`` per layer."""
         if self.cfg.mixed_layers:
             # one pool per attention layer, [planes, pages, kv heads, page, head size] (one plane when values are keys)
             self.kv_cache = [torch.zeros(lw.attn_module.cache_shape(num_pages, page), dtype=self.dtype, device=self.device)
@@ -600,6 +609,10 @@ class DecoderModel:
             row = self.cfg.mla.kv_lora_rank + self.cfg.mla.qk_rope_head_dim
             self.kv_cache = torch.zeros(self.layer1 - self.layer0, num_pages, page, row, dtype=torch.bfloat16,
                                         device=self.device)
+            return self.kv_cache
+        if self.kv_dtype == "int4":
+            one = ops.kv4_cache(1, self.hkv, page, self.cfg.head_dim, "cpu")
+            self.kv_cache = torch.zeros(self.layer1 - self.layer0, num_pages, *one.shape[1:], dtype=torch.uint8, device=self.device)
             return self.kv_cache
         self.kv_cache = torch.zeros(self.layer1 - self.layer0, 2, num_pages, self.hkv, page, self.cfg.head_dim,
                                     dtype=torch.bfloat16, device=self.device)
@@ -686,7 +699,8 @@ class DecoderModel:
             kn, _, _ = ops.norm(qkv[:, nq:nq + nk].contiguous(), k_norm_w, eps=cfg.rms_eps)
             qkv = torch.cat([qn, kn, qkv[:, nq + nk:]], 1)
             q_norm_w = k_norm_w = None
-        kc, vc = (self.kv_cache[li, 0], self.kv_cache[li, 1]) if self.kv_cache is not None else (None, None)
+        kv4 = self.kv_cache[li] if self.kv_cache is not None and self.kv_dtype == "int4" else None
+        kc, vc = (self.kv_cache[li, 0], self.kv_cache[li, 1]) if self.kv_cache is not None and kv4 is None else (None, None)
         window = cfg.layer_window(self.layer0 + li)
         inv_freq = self.inv_freq_local if (window > 0 and self.inv_freq_local is not None) else self.inv_freq
         rot = cfg.rotary_dim if cfg.use_rope and not (cfg.nope_global and window == 0) else 0
@@ -705,6 +719,8 @@ class DecoderModel:
             qkv = torch.cat([qn.reshape(t, -1), kn.reshape(t, -1), vr.reshape(t, -1)], 1).contiguous()
             q_norm_w = k_norm_w = None
             rot = 0
+        if kv4 is not None:
+            return self._attention_kv4(lw, kv4, qkv, q_norm_w, k_norm_w, rot, inv_freq, batch, scale, window)
         q, _, _ = ops.rope_kv(qkv, batch.positions, self.hq, self.hkv, d, k_cache=kc, v_cache=vc,
                               slot_mapping=batch.slot_mapping, rot=rot, theta=cfg.rope_theta,
                               inv_freq=inv_freq, style=cfg.rope_style, q_norm_w=q_norm_w,
@@ -728,6 +744,25 @@ class DecoderModel:
             att = ops.attn_prefill_paged(q, kc, vc, batch.block_table, batch.kv_lens, batch.cu_q,
                                          batch.max_q_len, causal=True, scale=scale,
                                          softcap=cfg.attn_softcap, window=window, max_kv_len=batch.max_kv_len or None)
+        return att.reshape(t, self.hq * d)
+
+    def _attention_kv4(self, lw: LayerWeights, cache: torch.Tensor, qkv, q_norm_w, k_norm_w, rot: int, inv_freq: torch.Tensor,
+                       batch: ForwardBatch, scale: float, window: int):
+        """The rest of ``_attention_core`` over a layer's 4-bit cache."""
+        cfg, d, t = self.cfg, self.cfg.head_dim, qkv.shape[0]
+        q, _, _ = ops.rope_kv4(qkv, batch.positions, self.hq, self.hkv, d, cache=cache, slot_mapping=batch.slot_mapping, rot=rot, theta=cfg.rope_theta,
+                               inv_freq=inv_freq, style=cfg.rope_style, q_norm_w=q_norm_w, k_norm_w=k_norm_w, eps=cfg.rms_eps)
+        kw = dict(scale=scale, softcap=cfg.attn_softcap, window=window)
+        if self.alibi_slopes is not None or lw.sinks is not None:
+            att = ops.attn_biased_kv4(q, cache, batch.block_table, batch.kv_lens, None if batch.is_decode else batch.cu_q, alibi=self.alibi_slopes,
+                                      sinks=lw.sinks, **kw)
+        elif batch.is_decode:
+            fp8 = self.fp8 and q.is_cuda and lw.o is not None and lw.o.is_fp8 and d == 128
+            att = ops.attn_decode_kv4(q, cache, batch.block_table, batch.kv_lens, max_kv_len=batch.max_kv_len or None, emit_fp8=fp8, emit_bf16=not fp8, **kw)
+            if fp8:
+                return att[1]
+        else:
+            att = ops.attn_prefill_kv4(q, cache, batch.block_table, batch.kv_lens, batch.cu_q, batch.max_q_len, max_kv_len=batch.max_kv_len or None, **kw)
         return att.reshape(t, self.hq * d)
 
     def _mrope(self, qkv: torch.Tensor, positions3: torch.Tensor, inv_freq: torch.Tensor) -> torch.Tensor:
@@ -1050,7 +1085,7 @@ class DecoderModel:
         cfg = self.cfg
         if (not x.is_cuda or self.tp > 1 or self.fp8 or cfg.residual_multiplier != 1.0 or cfg.mixed_layers or not (self.first_stage and self.last_stage)
                 or self.alibi_slopes is not None or self.inv_freq_local is not None or batch.slot_mapping is None or self.kv_cache is None
-                or not x.is_contiguous() or batch.positions.dtype != torch.int32 or batch.slot_mapping.dtype != torch.int64
+                or self.kv_dtype != "bf16" or not x.is_contiguous() or batch.positions.dtype != torch.int32 or batch.slot_mapping.dtype != torch.int64
                 or self.inv_freq.dtype != torch.float32 or self.kv_cache.dim() != 6 or not self.kv_cache.is_contiguous() or cfg.rotary_dim % 2):
             return False
         rows = (self.hq + 2 * self.hkv) * cfg.head_dim

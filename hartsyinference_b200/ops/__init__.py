@@ -60,7 +60,7 @@ from .core import (  # noqa: F401
     sample_tokens,
     selective_scan,
 )
-from .kv4 import attn_decode_kv4, attn_prefill_kv4, kv4_cache, kv4_gather, rope_kv4  # noqa: F401
+from .kv4 import attn_biased_kv4, attn_decode_kv4, attn_prefill_kv4, kv4_cache, kv4_gather, rope_kv4  # noqa: F401
 from .mixers import (  # noqa: F401
     ChannelScanWeights,
     DeltaWeights,
@@ -122,7 +122,7 @@ def _install_ranges() -> None:
                  "head_linear", "head_scan", "kv_store", "latent_attn", "latent_gather", "latent_prep", "pair_linear_f32", "poly_norm",
                  "qk_rope_store", "residual_norm", "rope_table", "router", "short_conv", "side_gate"):
         setattr(mod, name, traced(name)(getattr(mixers, name)))
-    for name in ("attn_decode_kv4", "attn_prefill_kv4", "kv4_gather", "rope_kv4"):
+    for name in ("attn_biased_kv4", "attn_decode_kv4", "attn_prefill_kv4", "kv4_gather", "rope_kv4"):
         setattr(mod, name, traced(name)(getattr(kv4, name)))
 
 

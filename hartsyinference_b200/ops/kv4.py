@@ -223,3 +223,24 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
             rc = run(*ptrs, *sizes, int(causal), window, scale, float(softcap), status, N.stream())
         N.check(rc, "b200_attn_prefill_kv4")
     return out
+
+
+def attn_biased_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: Optional[torch.Tensor],
+                    scale: Optional[float] = None, softcap: float = 0.0, window: int = 0, alibi: Optional[torch.Tensor] = None,
+                    sinks: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`.core.attn_paged_biased` over a 4-bit pool: causal attention with ALiBi slopes and / or per-head sink logits, which the kernels
+    do not take. The sequences are read back (:func:`kv4_gather`) and run through tensor ops. ``cu_q`` None: one query token per sequence."""
+    block_table, kv_lens, *_ = _attention_args("attn_biased_kv4", q, cache, block_table, kv_lens)
+    n = kv_lens.numel()
+    if cu_q is not None and cu_q.numel() != n + 1:
+        raise ValueError("attn_biased_kv4: cu_q [S + 1]")
+    cuts = list(range(n + 1)) if cu_q is None else cu_q.tolist()
+    cu_kv = torch.nn.functional.pad(kv_lens.clamp(min=0).cumsum(0, dtype=torch.int32), (1, 0))
+    at = cu_kv.tolist()
+    k, v = kv4_gather(cache, block_table, cu_kv, at[-1])
+    out = torch.zeros_like(q)
+    for i in range(n):
+        a, b, u, w = cuts[i], cuts[i + 1], at[i], at[i + 1]
+        if a < b and u < w:
+            out[a:b] = R.attention(q[a:b], k[u:w], v[u:w], causal=True, scale=scale, softcap=softcap, window=window, alibi=alibi, sinks=sinks).to(q.dtype)
+    return out
