@@ -1,7 +1,7 @@
 """Ops of a K/V cache held in 4 bits: the rotation that stores it, attention over it, and reading it back.
 
-A layer's pool is uint8 ``[pages, kv heads, page / 16, 2, 16 * (d / 2 + d / 32)]`` (:func:`kv4_cache`): 17 bytes per 16 values
-instead of 32. Every 32 neighbouring values of a head share a scale of 8 bits, ``max|x| / 7`` with three bits of mantissa; a value is held
+A layer's pool is uint8 ``[pages, kv heads, page / 16, 2, 16 * (d / 2 + d / 32)]`` (:func:`kv4_cache`): 17 bytes per 32 values
+instead of 64. Every 32 neighbouring values of a head share a scale of 8 bits, ``max|x| / 7`` with three bits of mantissa; a value is held
 as the nearest multiple of it from -7 to 7. Keys up to 6720 and values up to 420 in magnitude are held so, larger ones and
 infinities as the largest multiple, NaN as zero. Head sizes 64 and 128, pages of 16, 32, 64 or 128 tokens, any number
 of query heads per key head. CUDA tensors are bf16, block tables and lengths int32; CPU tensors go to the statements in :mod:`.reference`.
@@ -30,12 +30,14 @@ def _layout(shape, page: int, d: int) -> None:
         raise ValueError(f"4-bit K/V cache: head size 64 or 128 and pages of 16, 32, 64 or 128 tokens, [pages, hkv, page / 16, 2, 17 d / 2]; got {tuple(shape)} for head size {d}")
 
 
-def _pool(cache: torch.Tensor, d: int, device: torch.device) -> tuple:
-    """(pages, kv heads, page) of a pool that an op of this module takes."""
-    if cache.dtype != torch.uint8 or cache.dim() != 5 or not cache.is_contiguous() or cache.device != device or (cache.is_cuda and cache.data_ptr() % 16):
+def _pool(cache: torch.Tensor, d: int, device: int) -> tuple:
+    """(pages, kv heads, page) of a pool that an op of this module takes; ``device``: ``get_device()`` of the other tensors."""
+    shape = cache.shape
+    if cache.dtype is not torch.uint8 or len(shape) != 5 or not cache.is_contiguous() or cache.get_device() != device or (device >= 0 and cache.data_ptr() % 16):
         raise ValueError("4-bit K/V cache: a contiguous uint8 pool on the device of the other tensors (kv4_cache makes one)")
-    _layout(cache.shape, cache.shape[2] * 16, d)
-    return cache.shape[0], cache.shape[1], cache.shape[2] * 16
+    pages, hkv, units, _, _ = shape
+    _layout(shape, units * 16, d)
+    return pages, hkv, units * 16
 
 
 def _dense(x: torch.Tensor) -> torch.Tensor:
@@ -44,17 +46,20 @@ def _dense(x: torch.Tensor) -> torch.Tensor:
     return x.clone() if x.data_ptr() % 16 else x
 
 
-def _ints(what: str, x: Optional[torch.Tensor], like: torch.Tensor, dtype: torch.dtype = torch.int32) -> Optional[torch.Tensor]:
+def _ints(what: str, x: Optional[torch.Tensor], device: int, dtype: torch.dtype = torch.int32) -> Optional[torch.Tensor]:
     if x is None:
         return None
-    if x.device != like.device or (x.is_cuda and x.dtype != dtype):
-        raise ValueError(f"{what}: {dtype} on {like.device}, got {x.dtype} on {x.device}")
+    if x.get_device() != device or (device >= 0 and x.dtype is not dtype):
+        raise ValueError(f"{what}: {dtype} on the device of the other tensors, got {x.dtype} on {x.device}")
     return x.contiguous()
 
 
-def _on(device: torch.device):
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: int):
     """Kernels go to the current device's current stream: make it the tensors' device."""
-    return contextlib.nullcontext() if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def rope_kv4(qkv, positions: torch.Tensor, hq: int, hkv: int, d: int, *, cache: Optional[torch.Tensor] = None,
@@ -72,7 +77,7 @@ def rope_kv4(qkv, positions: torch.Tensor, hq: int, hkv: int, d: int, *, cache: 
     if len(qkv.shape) != 2 or qkv.shape[1] != (hq + 2 * hkv) * d or hq < 1 or hkv < 1 or not 0 <= rot <= d or rot % 2 or style not in (0, 1):
         raise ValueError(f"rope_kv4: [T, (hq + 2 hkv) d] with an even rotated part of at most d, style 0 or 1; got {tuple(qkv.shape)}, rot {rot}, style {style}")
     if cache is not None:
-        pages, heads, page = _pool(cache, d, x.device)
+        pages, heads, page = _pool(cache, d, x.get_device())
         if heads != hkv:
             raise ValueError(f"rope_kv4: a cache of {heads} heads for {hkv}")
     elif slot_mapping is not None:
@@ -96,8 +101,9 @@ def rope_kv4(qkv, positions: torch.Tensor, hq: int, hkv: int, d: int, *, cache: 
         return (q.to(qkv.dtype), *(y.to(qkv.dtype) for y in held)) if want_kv else (q.to(qkv.dtype), None, None)
     if part is None and qkv.dtype != torch.bfloat16:
         raise ValueError(f"rope_kv4: bf16 activations, got {qkv.dtype}")
-    positions, slot_mapping = _ints("positions", positions, x), _ints("slot_mapping", slot_mapping, x, torch.int64)
-    with _on(x.device):
+    device = x.get_device()
+    positions, slot_mapping = _ints("positions", positions, device), _ints("slot_mapping", slot_mapping, device, torch.int64)
+    with _on(device):
         src = None if part is not None else _dense(qkv)
         inv_freq = None if rot == 0 else inv_freq.contiguous()
         q_norm_w, k_norm_w = (None if w is None else w.contiguous() for w in (q_norm_w, k_norm_w))
@@ -116,7 +122,8 @@ def kv4_gather(cache: torch.Tensor, block_table: torch.Tensor, cu_kv: torch.Tens
     """The first tokens of sequences as dense bf16 (k, v) [total, hkv, d]: rows ``cu_kv[s]`` .. ``cu_kv[s + 1]`` (int32 [S + 1], from 0) are
     those of block-table row s, ``total`` is the last of them on the host. What the cache stands for is exact in bf16."""
     d = 2 * cache.shape[-1] // 17
-    pages, hkv, page = _pool(cache, d, block_table.device)
+    device = cache.get_device()
+    pages, hkv, page = _pool(cache, d, device)
     if block_table.dim() != 2 or cu_kv.numel() != block_table.shape[0] + 1 or total < 0:
         raise ValueError("kv4_gather: block_table [S, pages] and cu_kv [S + 1]")
     k = torch.empty(total, hkv, d, dtype=torch.bfloat16, device=cache.device)
@@ -126,10 +133,10 @@ def kv4_gather(cache: torch.Tensor, block_table: torch.Tensor, cu_kv: torch.Tens
         for i, (a, b) in enumerate(zip(cuts, cuts[1:])):
             k[a:b], v[a:b] = R.kv4_sequence(cache, block_table[i], b - a)
         return k, v
-    block_table, cu_kv = _ints("block_table", block_table, cache), _ints("cu_kv", cu_kv, cache)
+    block_table, cu_kv = _ints("block_table", block_table, device), _ints("cu_kv", cu_kv, device)
     if total == 0 or block_table.shape[1] == 0:
         return k.zero_(), v.zero_()
-    with _on(cache.device):
+    with _on(device):
         rc = N.lib().b200_kv4_gather(cache.data_ptr(), block_table.data_ptr(), cu_kv.data_ptr(), k.data_ptr(), v.data_ptr(), block_table.shape[0],
                                      total, hkv, d, page, block_table.shape[1], pages, N.state(cache.device).status.data_ptr(), N.stream())
         N.check(rc, "b200_kv4_gather")
@@ -137,14 +144,16 @@ def kv4_gather(cache: torch.Tensor, block_table: torch.Tensor, cu_kv: torch.Tens
 
 
 def _attention_args(what: str, q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor) -> tuple:
-    if q.dim() != 3 or (q.is_cuda and q.dtype != torch.bfloat16):
+    device = q.get_device()
+    if q.dim() != 3 or (device >= 0 and q.dtype is not torch.bfloat16):
         raise ValueError(f"{what}: q is [tokens, hq, d], bf16 on a device; got {q.dtype} {tuple(q.shape)}")
-    pages, hkv, page = _pool(cache, q.shape[2], q.device)
-    if q.shape[1] < 1 or q.shape[1] % hkv:
-        raise ValueError(f"{what}: {q.shape[1]} query heads on {hkv} key heads")
+    _, hq, d = q.shape
+    pages, hkv, page = _pool(cache, d, device)
+    if hq < 1 or hkv < 1 or hq % hkv:
+        raise ValueError(f"{what}: {hq} query heads on {hkv} key heads")
     if block_table.dim() != 2 or block_table.shape[0] != kv_lens.numel():
         raise ValueError(f"{what}: block_table [S, pages] and kv_lens [S]")
-    return _ints("block_table", block_table, q), _ints("kv_lens", kv_lens, q), pages, hkv, page
+    return _ints("block_table", block_table, device), _ints("kv_lens", kv_lens, device), pages, hkv, page
 
 
 def _on_cpu(q, cache, block_table, kv_lens, cuts, **kw) -> torch.Tensor:
@@ -169,7 +178,7 @@ def attn_decode_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Ten
     if not q.is_cuda:
         out = _on_cpu(q, cache, block_table, kv_lens, list(range(b + 1)), scale=scale, softcap=softcap, window=window)
     else:
-        with _on(q.device):
+        with _on(q.get_device()):
             q = _dense(q)
             out = torch.empty_like(q)
             if block_table.shape[1] == 0 or pages == 0:
@@ -186,7 +195,7 @@ def attn_decode_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Ten
                 N.check(min(rc, 0), "b200_attn_decode_kv4", rc)
     if not emit_fp8:
         return out
-    with _on(q.device) if q.is_cuda else contextlib.nullcontext():
+    with _on(q.get_device()) if q.is_cuda else _HERE:
         return out if emit_bf16 else None, quant_fp8_act(out.reshape(b, hq * d))
 
 
@@ -199,11 +208,11 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     block_table, kv_lens, pages, hkv, page = _attention_args("attn_prefill_kv4", q, cache, block_table, kv_lens)
     if cu_q.numel() != kv_lens.numel() + 1:
         raise ValueError("attn_prefill_kv4: cu_q [S + 1]")
-    cu_q = _ints("cu_q", cu_q, q)
+    cu_q = _ints("cu_q", cu_q, q.get_device())
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
     if not q.is_cuda:
         return _on_cpu(q, cache, block_table, kv_lens, cu_q.tolist(), causal=causal, scale=scale, softcap=softcap, window=window)
-    with _on(q.device):
+    with _on(q.get_device()):
         q = _dense(q)
         out = torch.empty_like(q)
         if block_table.shape[1] == 0 or pages == 0:
