@@ -1,18 +1,19 @@
-// Attention of prompt chunks over a K/V cache held in 4 bits (format: kv4.cuh) on the 5th-generation tensor cores: head size 128.
+// Attention of prompt chunks over a K/V cache held in 4 bits (format: kv4.cuh) on the 5th-generation tensor cores.
 //
 // The query heads of a group read the same keys, so rows are (query, head of the group) pairs of one sequence and one kv head, heads fastest: row
 // r is query r / G, head r % G. A block owns two tiles of 128 rows and walks the keys that they see in tiles of 128:
-//   warp 0        one thread issues every tcgen05.mma; TMEM holds S0 | S1 | O0 | O1 (128 columns each), P is written over S and read from there
+//   warp 0        one thread issues every tcgen05.mma; TMEM holds S0 | S1 | O0 | O1 (128 columns each, of which heads of 64 use half
+//                 in O0 and O1), P is written over S and read from there
 //   warps 4..11   softmax of tile 0 and 1, one row per thread: the maximum is raised only where it grows by more than 2^8; tiles that the
 //                 diagonal, a window or the last key crosses are masked before it. Before the first tile they bring the rows of Q
-//   warps 12..15  a thread per key: its row of codes and scales (68 bytes; the next tile's are in flight) becomes 128 bf16 of
+//   warps 12..15  a thread per key: its row of codes and scales (68 bytes for a head of 128; the next tile's are in flight) becomes bf16 values of
 //                 keys, then of values, exactly, in the swizzled rows that the products read: keys along K, values along N, as they lie
 //
 // Packed rows mean that a tile is converted once for 256 rows whatever the group, and that the diagonal crosses few tiles: 256 rows of a
 // group of 8 are 32 queries. Bound by the tensor core and by what a processor issues, about equally: a chunk of 2048 queries behind 6144
 // keys takes 315 us for 32 heads over 8 (145 at the rate of the products alone; 284 with warps 12..15 idle; the kernel over a bf16
-// cache takes 245) and 488 us for 64 heads over 8 with 1024 queries per sequence of two (165). A grid that stays and takes blocks
-// from a counter was slower (400): the issuing thread's state then no longer fits its registers.
+// cache takes 245), four prompts of 2048 tokens 488 us for 64 heads over 8 (165). A grid that stays and takes blocks
+// from a counter was slower (400): the issuing thread's state then no longer fits its registers. Heads of 64 take 254 us for the first shape.
 #include "kv4.cuh"
 
 namespace b200 {
@@ -20,10 +21,9 @@ namespace b200 {
 int num_sms();      // of the current device, see gemm_tcgen05.cu
 
 constexpr int kPf4Tile = 128;
-constexpr int kPf4D = 128;
 constexpr int kPf4Threads = 512;
 constexpr int kPf4Stages = 2;
-constexpr int kPf4Bytes = kPf4Tile * kPf4D * 2;
+constexpr int kPf4Half = kPf4Tile * 128;    // bytes of a tile's 64 values of a row: 128 bytes a row, swizzled
 constexpr float kPf4Gap = 8.f;            // raise the running maximum only beyond this many powers of two
 constexpr float kPf4Log2e = 1.4426950408889634f;
 
@@ -37,7 +37,7 @@ struct Pf4Barriers {
 };
 
 struct Pf4Params {
-  const __nv_bfloat16* q;      // [tokens][hq][128]
+  const __nv_bfloat16* q;      // [tokens][hq][d]
   __nv_bfloat16* out;
   const int* kv_lens;          // [sequences]
   const int* cu_q;             // [sequences + 1]
@@ -68,14 +68,15 @@ __device__ __forceinline__ void pf4_st16(uint32_t taddr, const uint32_t (&r)[16]
                : "memory");
 }
 
-template <bool kCap>
+template <int D, bool kCap>
 __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const Pf4Params p) {
   extern __shared__ uint8_t smem_raw[];
+  constexpr int kHalves = D / 64, kBytes = kHalves * kPf4Half;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sq = smem;                                   // two Q tiles, each [half head][128 rows][128 bytes]
-  uint8_t* sk = sq + 2 * kPf4Bytes;
-  uint8_t* sv = sk + kPf4Stages * kPf4Bytes;
-  Pf4Barriers* bars = reinterpret_cast<Pf4Barriers*>(sv + kPf4Stages * kPf4Bytes);
+  uint8_t* sk = sq + 2 * kBytes;
+  uint8_t* sv = sk + kPf4Stages * kBytes;
+  Pf4Barriers* bars = reinterpret_cast<Pf4Barriers*>(sv + kPf4Stages * kBytes);
 
   pdl_wait();
   pdl_trigger();
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
   volatile uint32_t* abort_flag = &bars->abort_flag;
   constexpr uint32_t kIdescS = make_idesc(128, 128, kFmtBf16, kFmtBf16);
-  constexpr uint32_t kIdescPV = kIdescS | kIdescBMn;
+  constexpr uint32_t kIdescPV = make_idesc(128, D, kFmtBf16, kFmtBf16) | kIdescBMn;
 
   // launch: 128 registers a thread, 512 for the four warpgroups' threads of a lane; 72 + 2 * 176 + 88 of them below
   if (warp < 4) {
@@ -132,9 +133,9 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
       auto issue_s = [&](int t, int j) {
         const int s = j % kPf4Stages;
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const uint64_t ad = make_desc_sw128(smem_u32(sq + t * kPf4Bytes + a * (kPf4Bytes / 2)));
-          const uint64_t bd = make_desc_sw128(smem_u32(sk + s * kPf4Bytes + a * (kPf4Bytes / 2)));
+        for (int a = 0; a < kHalves; ++a) {
+          const uint64_t ad = make_desc_sw128(smem_u32(sq + t * kBytes + a * kPf4Half));
+          const uint64_t bd = make_desc_sw128(smem_u32(sk + s * kBytes + a * kPf4Half));
 #pragma unroll
           for (int k = 0; k < 4; ++k) mma_bf16_ss(tmem_base + t * 128, ad + 2 * k, bd + 2 * k, kIdescS, (a | k) != 0);
         }
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
           if (t == 0 && !mbar_wait(&bars->v_full[s], ph, abort_flag)) { ok = false; break; }
           tc_fence_after_sync();
           // O_t += P_t V_j: A = P_t in TMEM (16 keys are 8 columns of bf16 pairs), B = 16 rows of the V tile
-          const uint64_t bd = make_desc_sw128_mn(smem_u32(sv + s * kPf4Bytes), kPf4Bytes / 2);
+          const uint64_t bd = make_desc_sw128_mn(smem_u32(sv + s * kBytes), kPf4Half);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
             mma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8, bd + k * (2048 >> 4), kIdescPV, (j | k) != 0);
@@ -179,16 +180,16 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
     const int last = n_keys;
     auto unit_of = [&](int j) -> const uint8_t* {       // the unit of this thread's key of tile j, or none
       const int at = (first_tile + j) * kPf4Tile + key;
-      return j < n_tiles && at < last ? kv4_unit<kPf4D>(p.pool, table, kvh, at >> 4, kKernelKv4) : nullptr;
+      return j < n_tiles && at < last ? kv4_unit<D>(p.pool, table, kvh, at >> 4, kKernelKv4) : nullptr;
     };
-    uint32_t kw[16], vw[16], ks = 0, vs = 0;
-    auto load = [&](const uint8_t* unit, bool values, uint32_t (&w)[16], uint32_t& scales) {
+    uint32_t kw[D / 8], vw[D / 8], ks = 0, vs = 0;
+    auto load = [&](const uint8_t* unit, bool values, uint32_t (&w)[D / 8], uint32_t& scales) {
       if (unit) {
-        kv4_load_row<kPf4D>(unit + (values ? kv4_plane_bytes(kPf4D) : 0), key & 15, values, w, scales);
+        kv4_load_row<D>(unit + (values ? kv4_plane_bytes(D) : 0), key & 15, values, w, scales);
       } else {
         scales = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = 0x88888888u;      // zeros: their probabilities are, but what lies there need not be a number
+        for (int i = 0; i < D / 8; ++i) w[i] = 0x88888888u;      // zeros: their probabilities are, but what lies there need not be a number
       }
     };
     const uint8_t* unit = unit_of(0);
@@ -199,15 +200,15 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
     for (int j = 0; j < n_tiles; ++j) {
       const int s = j % kPf4Stages;
       const uint32_t ph = static_cast<uint32_t>((j / kPf4Stages) & 1) ^ 1;
-      auto row_at = [&](uint8_t* tile, int piece) { return tile + (piece >> 3) * (kPf4Bytes / 2) + key * 128 + (((piece & 7) ^ (key & 7)) << 4); };
+      auto row_at = [&](uint8_t* tile, int piece) { return tile + (piece >> 3) * kPf4Half + key * 128 + (((piece & 7) ^ (key & 7)) << 4); };
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty[s], ph, abort_flag)))) break;
-      kv4_key_row<kPf4D>(kw, ks, [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(row_at(sk + s * kPf4Bytes, piece)) = v; });
+      kv4_key_row<D>(kw, ks, [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(row_at(sk + s * kBytes, piece)) = v; });
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->k_full[s]);
       load(unit, false, kw, ks);
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_empty[s], ph, abort_flag)))) break;
-      kv4_value_row<kPf4D>(vw, vs, [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(row_at(sv + s * kPf4Bytes, piece)) = v; });
+      kv4_value_row<D>(vw, vs, [&](int piece, uint4 v) { *reinterpret_cast<uint4*>(row_at(sv + s * kBytes, piece)) = v; });
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->v_full[s]);
@@ -226,11 +227,11 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
     const uint32_t s_col = lane_base + t * 128, o_col = lane_base + 256 + t * 128;
     const int query = row / G, head = row - query * G;
     {
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + ((static_cast<long long>(q_off) + query) * p.hq + kvh * G + head) * kPf4D);
-      uint8_t* dst = sq + t * kPf4Bytes + local * 128;
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + ((static_cast<long long>(q_off) + query) * p.hq + kvh * G + head) * D);
+      uint8_t* dst = sq + t * kBytes + local * 128;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        *reinterpret_cast<uint4*>(dst + (i >> 3) * (kPf4Bytes / 2) + (((i & 7) ^ (local & 7)) << 4)) = row < rows ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<uint4*>(dst + (i >> 3) * kPf4Half + (((i & 7) ^ (local & 7)) << 4)) = row < rows ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->q_full);
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
             if (!__all_sync(0xffffffffu, mbar_wait(&bars->o_done[t], (j - 1) & 1, abort_flag))) { ok = false; break; }
             tc_fence_after_sync();
 #pragma unroll
-            for (int cc = 0; cc < 8; ++cc) {
+            for (int cc = 0; cc < D / 16; ++cc) {
               uint32_t o[16];
               pf4_ld16(o_col + cc * 16, o);
               tmem_ld_wait();
@@ -333,9 +334,9 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
         const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
         // The Q tile is no longer read: 32 rows of 128 bytes per warp turn the rows that the lanes hold into
         // 128-byte runs. 16-byte pieces are placed by (piece xor row), which keeps the banks apart.
-        uint8_t* strip = sq + t * kPf4Bytes + quarter * 32 * 128;
+        uint8_t* strip = sq + t * kBytes + quarter * 32 * 128;
 #pragma unroll
-        for (int hc = 0; hc < 2; ++hc) {
+        for (int hc = 0; hc < kHalves; ++hc) {
           uint32_t o[64];
           tmem_ld_32x32(o_col + hc * 64, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
           tmem_ld_32x32(o_col + hc * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
             const uint4 v = *reinterpret_cast<const uint4*>(strip + rr * 128 + ((piece ^ (rr & 7)) * 16));
             if (out_row < rows) {
               const int oq = out_row / G;
-              *reinterpret_cast<uint4*>(p.out + ((static_cast<long long>(q_off) + oq) * p.hq + kvh * G + (out_row - oq * G)) * kPf4D + hc * 64 + piece * 8) = v;
+              *reinterpret_cast<uint4*>(p.out + ((static_cast<long long>(q_off) + oq) * p.hq + kvh * G + (out_row - oq * G)) * D + hc * 64 + piece * 8) = v;
             }
           }
           __syncwarp();
@@ -384,20 +385,23 @@ B200_API int b200_attn_kv4_choice(int seqs, int max_q_len, int max_kv_len, int h
   // Measured in us, 64 rows / 256 rows / parts, 32 heads over 8: one sequence of 100 queries 7.1 / 13.4 / 19, of 512 24 / 21 / -, of 2048
   // 192 / 83 / -; 17 queries behind 1000 keys 30 / 29 / 22, behind 8000 212 / 185 / 36; 100 there 212 / 224 / 98; 8 behind 30000 770 / 675 / 39;
   // 16 sequences of 17 behind 100 keys 9.7 / 10.6 / 49, behind 1000 44 / 35 / 57, of 5 behind 3000 81 / 85 / 57. 32 heads over 32: 16 of 17
-  // behind 1000 84 / 118 / 76.
+  // behind 1000 84 / 118 / 76. Heads of 64, 32 over 8: 100 queries 5.2 / 9.9 / -, 512 19 / 17 / -, 2048 behind 6000 619 / 254 / -, 17 behind
+  // 8000 146 / 162 / 26, 100 there 147 / 201 / 67.
   const long long rows = static_cast<long long>(max_q_len) * (hq / hkv), lists = static_cast<long long>(seqs) * hkv;
   const long long waves = ((rows + 2 * kPf4Tile - 1) / (2 * kPf4Tile) * lists + num_sms() - 1) / num_sms();
   const double each = static_cast<double>((rows + 63) / 64 * lists) / num_sms();       // blocks of 64 rows a processor
   const double keys = window > 0 && window + static_cast<double>(max_q_len) < max_kv_len ? window + static_cast<double>(max_q_len) : max_kv_len;
   const double units = keys / kKv4Unit * static_cast<double>((rows + 15) / 16 * lists);
-  const double small = 3.3 + (each > 1. ? each : 1.) * 0.026 * keys, wide = static_cast<double>(waves) * (7.5 + 0.0215 * keys);
-  const double parts = 18. + 0.0008 * units;
-  const bool can = d == kPf4D && scale > 0.f, best = can && wide < small;
+  const bool big = d == 128;
+  const double small = (big ? 3.3 : 3.) + (each > 1. ? each : 1.) * (big ? 0.026 : 0.0178) * keys;
+  const double wide = static_cast<double>(waves) * (big ? 7.5 + 0.0215 * keys : 6. + 0.0193 * keys);
+  const double parts = big ? 18. + 0.0008 * units : 14. + 0.00051 * units;
+  const bool can = scale > 0.f, best = can && wide < small;
   if (causal && keys > 512. && rows < 65536 && seqs <= kKv4MaxSeqs && parts < (best ? wide : small)) return 2;
   return best;
 }
 
-// Arguments as of b200_attn_kv4 with cu_q; d 128 and a scale above 0.
+// Arguments as of b200_attn_kv4 with cu_q; a scale above 0.
 B200_API int b200_attn_prefill_kv4(const void* q, const void* pool, void* out, const int* block_table, const int* kv_lens, const int* cu_q,
                                    int seqs, int max_q_len, int hq, int hkv, int d, int page, int max_pages, long long pages,
                                    int causal, int window, float scale, float softcap, void* status, cudaStream_t stream) {
@@ -405,7 +409,7 @@ B200_API int b200_attn_prefill_kv4(const void* q, const void* pool, void* out, c
   if (hkv < 1 || hq < 1 || hq % hkv || max_pages < 1 || pages < 1 || !kv4_pool_fits(pool, d, page)) return -2;
   if (seqs > 65535 || hkv > 65535 || static_cast<long long>(max_q_len) * (hq / hkv) >= (1ll << 30)) return -3;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) return -4;
-  if (d != kPf4D || !(scale > 0.f)) return -5;
+  if (!(scale > 0.f)) return -5;
   Pf4Params p{};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.out = static_cast<__nv_bfloat16*>(out);
@@ -418,8 +422,8 @@ B200_API int b200_attn_prefill_kv4(const void* q, const void* pool, void* out, c
     p.cap_in = 2.f * kPf4Log2e * scale / softcap;
     p.cap_out = softcap * kPf4Log2e;
   }
-  const int smem = (2 + 2 * kPf4Stages) * kPf4Bytes + static_cast<int>(sizeof(Pf4Barriers)) + 1024;
-  static PerDeviceOnce once[2];
+  const int smem = (2 + 2 * kPf4Stages) * kPf4Half * (d / 64) + static_cast<int>(sizeof(Pf4Barriers)) + 1024;
+  static PerDeviceOnce once[4];
   auto go = [&](auto kernel, PerDeviceOnce& o) -> cudaError_t {
     if (o.first_time()) {
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -428,6 +432,8 @@ B200_API int b200_attn_prefill_kv4(const void* q, const void* pool, void* out, c
     const dim3 grid(static_cast<unsigned>((static_cast<long long>(max_q_len) * p.group + 2 * kPf4Tile - 1) / (2 * kPf4Tile)), hkv, seqs);
     return launch_pdl(kernel, grid, dim3(kPf4Threads), smem, stream, p);
   };
-  const cudaError_t e = softcap > 0.f ? go(attn_prefill_kv4_kernel<true>, once[0]) : go(attn_prefill_kv4_kernel<false>, once[1]);
+  cudaError_t e;
+  if (d == 128) e = softcap > 0.f ? go(attn_prefill_kv4_kernel<128, true>, once[0]) : go(attn_prefill_kv4_kernel<128, false>, once[1]);
+  else e = softcap > 0.f ? go(attn_prefill_kv4_kernel<64, true>, once[2]) : go(attn_prefill_kv4_kernel<64, false>, once[3]);
   return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
 }

@@ -203,7 +203,7 @@ def test_entry_points_refuse_sizes_before_any_launch():
     assert L.b200_attn_prefill_kv4(p, p, p, p, p, p, 1, 1, 5, 2, 128, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -2
     assert L.b200_attn_prefill_kv4(p, p, p, p, p, p, 70000, 1, 4, 2, 128, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -3
     assert L.b200_attn_prefill_kv4(p + 4, p, p, p, p, p, 1, 1, 4, 2, 128, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -4
-    assert L.b200_attn_prefill_kv4(p, p, p, p, p, p, 1, 1, 4, 2, 64, 16, 1, 1, 1, 0, 1.0, 0.0, None, None) == -5
+    assert L.b200_attn_prefill_kv4(p, p, p, p, p, p, 1, 1, 4, 2, 64, 16, 1, 1, 1, 0, -1.0, 0.0, None, None) == -5
     assert L.b200_attn_decode_kv4(p, p, p, p, p, 1, 5, 2, 64, 16, 1, 1, 16, 0, 1.0, 0.0, None, 0, None, None) == -2
     assert L.b200_attn_decode_kv4(p, p, p, p, p, 1, 4, 2, 64, 16, 0, 1, 16, 0, 1.0, 0.0, None, 0, None, None) == -2
     assert L.b200_attn_decode_kv4(p, p, p, p, p, 200, 4, 2, 64, 128, 1 << 21, 1, 16, 0, 1.0, 0.0, None, 0, None, None) == -3
@@ -376,12 +376,31 @@ def test_few_queries_in_a_window():
 
 
 @gpu
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+@pytest.mark.parametrize("kw", CASES + [dict(causal=False)])
+def test_wide_blocks_of_prompts(hq, hkv, d, kw):
+    """The kernel of 256 rows a block, whatever kernel the op would take."""
+    from hartsyinference_b200.ops import _native as N
+    kw = dict(causal=True, scale=1 / math.sqrt(d), softcap=0.0, window=0) | kw
+    lens, each = [700, 0, 70, 333, 1, 200, 5, 128], [140, 0, 3, 130, 1, 200, 9, 2]
+    cache, table = _filled(lens, hkv, d, 32)
+    cuts = torch.tensor([0, *each]).cumsum(0).tolist()
+    q = _normal(sum(each), hq, d, seed=9).to(torch.bfloat16)
+    qd, c, t, n, cu = _cuda(q, cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor(cuts, dtype=torch.int32))
+    out = torch.full_like(qd, 7)
+    rc = N.lib().b200_attn_prefill_kv4(qd.data_ptr(), c.data_ptr(), out.data_ptr(), t.data_ptr(), n.data_ptr(), cu.data_ptr(), len(lens), max(each), hq, hkv, d, 32,
+                                       t.shape[1], c.shape[0], int(kw["causal"]), kw["window"], kw["scale"], kw["softcap"], N.state(qd.device).status.data_ptr(), N.stream())
+    assert rc == 0
+    _close(out, *_plain(q, cache, table, lens, cuts, **kw))
+
+
+@gpu
 @pytest.mark.parametrize("sizes,kernel", [((1, 100, 100), 0), ((1, 2048, 8192), 1), ((16, 5, 4000), 2)])
 def test_every_prompt_kernel_is_chosen(sizes, kernel):
     from hartsyinference_b200.ops import _native as N
     assert N.lib().b200_attn_kv4_choice(*sizes, 32, 8, 128, 1, 0, 0.088) == kernel
     assert N.lib().b200_attn_kv4_choice(*sizes, 32, 8, 128, 0, 0, 0.088) < 2
-    assert N.lib().b200_attn_kv4_choice(*sizes, 32, 8, 64, 1, 0, 0.125) != 1
+    assert N.lib().b200_attn_kv4_choice(*sizes, 32, 8, 128, 1, 0, -0.088) != 1
 
 
 @gpu
