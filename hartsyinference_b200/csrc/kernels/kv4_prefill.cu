@@ -2,18 +2,19 @@
 //
 // The query heads of a group read the same keys, so rows are (query, head of the group) pairs of one sequence and one kv head, heads fastest: row
 // r is query r / G, head r % G. A block owns two tiles of 128 rows and walks the keys that they see in tiles of 128:
-//   warp 0        one thread issues every tcgen05.mma; TMEM holds S0 | S1 | O0 | O1 (128 columns each, of which heads of 64 use half
-//                 in O0 and O1), P is written over S and read from there
-//   warps 4..11   softmax of tile 0 and 1, one row per thread: the maximum is raised only where it grows by more than 2^8; tiles that the
-//                 diagonal, a window or the last key crosses are masked before it. Before the first tile they bring the rows of Q
+//   warps 0, 1    a thread each issues the tcgen05.mma of a row tile; TMEM holds S0 | S1 | O0 | O1 (128 columns each, of which heads of 64
+//                 use half in O0 and O1). S is made in halves of 64 keys, two ahead of the softmax, P is written over S and read from there
+//   warps 4..11   softmax of tile 0 and 1, one row per thread, 64 keys a step: the maximum is raised only where it grows by more than 2^8;
+//                 steps that the diagonal, a window or the last key crosses are masked before it. Before the first they bring the rows of Q
 //   warps 12..15  a thread per key: its row of codes and scales (68 bytes for a head of 128; the next tile's are in flight) becomes bf16 values of
 //                 keys, then of values, exactly, in the swizzled rows that the products read: keys along K, values along N, as they lie
 //
 // Packed rows mean that a tile is converted once for 256 rows whatever the group, and that the diagonal crosses few tiles: 256 rows of a
 // group of 8 are 32 queries. Bound by the tensor core and by what a processor issues, about equally: a chunk of 2048 queries behind 6144
-// keys takes 315 us for 32 heads over 8 (145 at the rate of the products alone; 284 with warps 12..15 idle; the kernel over a bf16
-// cache takes 245), four prompts of 2048 tokens 488 us for 64 heads over 8 (165). A grid that stays and takes blocks
-// from a counter was slower (400): the issuing thread's state then no longer fits its registers. Heads of 64 take 254 us for the first shape.
+// keys takes 282 us for 32 heads over 8 (145 at the rate of the products alone; the kernel over a bf16 cache takes 245), four prompts of 2048
+// tokens 410 us for 64 heads over 8 (165). What counts is how long a row tile waits for its next scores: S of 128 keys at once, made after P V of
+// the ones before, takes 316 and 488; halves with one thread that issues for both row tiles 452 and 571, since it waits for each in turn.
+// A grid that stays and takes blocks from a counter was slower (400): the issuing thread's state then no longer fits its registers.
 #include "kv4.cuh"
 
 namespace b200 {
@@ -21,8 +22,10 @@ namespace b200 {
 int num_sms();      // of the current device, see gemm_tcgen05.cu
 
 constexpr int kPf4Tile = 128;
+constexpr int kPf4Sub = 64;               // keys of a product S: two of them are half a tile's
 constexpr int kPf4Threads = 512;
 constexpr int kPf4Stages = 2;
+constexpr int kPf4Registers = 128;        // of a thread at launch: 65536 / kPf4Threads
 constexpr int kPf4Half = kPf4Tile * 128;    // bytes of a tile's 64 values of a row: 128 bytes a row, swizzled
 constexpr float kPf4Gap = 8.f;            // raise the running maximum only beyond this many powers of two
 constexpr float kPf4Log2e = 1.4426950408889634f;
@@ -31,7 +34,7 @@ struct Pf4Barriers {
   uint64_t q_full;
   uint64_t k_full[kPf4Stages], k_empty[kPf4Stages];
   uint64_t v_full[kPf4Stages], v_empty[kPf4Stages];
-  uint64_t s_full[2], p_ready[2], o_done[2];
+  uint64_t s_full[2][2], p_ready[2][2], o_done[2][2];      // [row tile][half of a key tile]
   uint32_t tmem_base;
   uint32_t abort_flag;
 };
@@ -93,19 +96,22 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
   const int n_keys = p.causal ? min(kv_len, ctx + last_query + 1) : kv_len;
   const int first_tile = p.window > 0 ? max(0, ctx + row0 / G + 1 - p.window) / kPf4Tile : 0;
   const int n_tiles = n_keys > first_tile * kPf4Tile ? (n_keys + kPf4Tile - 1) / kPf4Tile - first_tile : 0;
+  const int n_subs = n_tiles > 0 ? (n_keys + kPf4Sub - 1) / kPf4Sub - 2 * first_tile : 0;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 8);
     for (int i = 0; i < kPf4Stages; ++i) {
       mbar_init(&bars->k_full[i], 4);
-      mbar_init(&bars->k_empty[i], 1);
+      mbar_init(&bars->k_empty[i], tile1 ? 2 : 1);
       mbar_init(&bars->v_full[i], 4);
-      mbar_init(&bars->v_empty[i], 1);
+      mbar_init(&bars->v_empty[i], tile1 ? 2 : 1);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&bars->s_full[t], 1);
-      mbar_init(&bars->p_ready[t], 4);
-      mbar_init(&bars->o_done[t], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars->s_full[t][b], 1);
+        mbar_init(&bars->p_ready[t][b], 4);
+        mbar_init(&bars->o_done[t][b], 1);
+      }
     }
     bars->abort_flag = 0;
     fence_mbar_init();
@@ -119,61 +125,57 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
   tc_fence_after_sync();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
   volatile uint32_t* abort_flag = &bars->abort_flag;
-  constexpr uint32_t kIdescS = make_idesc(128, 128, kFmtBf16, kFmtBf16);
+  constexpr uint32_t kIdescS = make_idesc(128, kPf4Sub, kFmtBf16, kFmtBf16);
   constexpr uint32_t kIdescPV = make_idesc(128, D, kFmtBf16, kFmtBf16) | kIdescBMn;
 
-  // launch: 128 registers a thread, 512 for the four warpgroups' threads of a lane; 72 + 2 * 176 + 88 of them below
+  // launch: 128 registers a thread, 512 for the four warpgroups' threads of a lane; 96 + 2 * 160 + 96 of them below, which the host makes sure of
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 0 && lane == 0 && n_tiles > 0) {
-      // ----------------------------------------------------------------------- MMA issuer
-      const int nq = tile1 ? 2 : 1;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp < (tile1 ? 2 : 1) && lane == 0 && n_tiles > 0) {
+      // ----------------------------------------------------------------------- one issuer per row tile
+      const int t = warp;
+      const uint32_t s_at = tmem_base + t * 128, o_at = tmem_base + 256 + t * 128;
+      const uint64_t qd = make_desc_sw128(smem_u32(sq + t * kBytes)), kd = make_desc_sw128(smem_u32(sk)), vd = make_desc_sw128_mn(smem_u32(sv), kPf4Half);
       bool ok = mbar_wait(&bars->q_full, 0, abort_flag);
-      // S_t(j) = Q_t K_j^T into TMEM columns [t * 128, t * 128 + 128)
-      auto issue_s = [&](int t, int j) {
-        const int s = j % kPf4Stages;
+      // S(u) = Q K_u^T into the columns of half u & 1
+      auto issue_s = [&](int u) {
+        const int s = (u >> 1) % kPf4Stages, b = u & 1;
 #pragma unroll
         for (int a = 0; a < kHalves; ++a) {
-          const uint64_t ad = make_desc_sw128(smem_u32(sq + t * kBytes + a * kPf4Half));
-          const uint64_t bd = make_desc_sw128(smem_u32(sk + s * kBytes + a * kPf4Half));
+          const uint64_t ad = qd + a * (kPf4Half >> 4), bd = kd + ((s * kBytes + a * kPf4Half + b * kPf4Sub * 128) >> 4);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_bf16_ss(tmem_base + t * 128, ad + 2 * k, bd + 2 * k, kIdescS, (a | k) != 0);
+          for (int k = 0; k < 4; ++k) mma_bf16_ss(s_at + b * kPf4Sub, ad + 2 * k, bd + 2 * k, kIdescS, (a | k) != 0);
         }
-        tc_commit(&bars->s_full[t]);
+        tc_commit(&bars->s_full[t][b]);
+        if (b) tc_commit(&bars->k_empty[s]);
       };
       if (ok) ok = mbar_wait(&bars->k_full[0], 0, abort_flag);
       if (ok) {
         tc_fence_after_sync();
-        for (int t = 0; t < nq; ++t) issue_s(t, 0);
-        tc_commit(&bars->k_empty[0]);
+        for (int u = 0; u < min(2, n_subs); ++u) issue_s(u);
       }
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int s = j % kPf4Stages;
-        const uint32_t ph = static_cast<uint32_t>((j / kPf4Stages) & 1);
-        for (int t = 0; t < nq && ok; ++t) {
-          if (!mbar_wait(&bars->p_ready[t], j & 1, abort_flag)) { ok = false; break; }
-          if (t == 0 && !mbar_wait(&bars->v_full[s], ph, abort_flag)) { ok = false; break; }
-          tc_fence_after_sync();
-          // O_t += P_t V_j: A = P_t in TMEM (16 keys are 8 columns of bf16 pairs), B = 16 rows of the V tile
-          const uint64_t bd = make_desc_sw128_mn(smem_u32(sv + s * kBytes), kPf4Half);
+      for (int u = 0; u < n_subs && ok; ++u) {
+        const int j = u >> 1, b = u & 1, s = j % kPf4Stages;
+        if (!(ok = mbar_wait(&bars->p_ready[t][b], j & 1, abort_flag))) break;
+        if (b == 0 && !(ok = mbar_wait(&bars->v_full[s], static_cast<uint32_t>((j / kPf4Stages) & 1), abort_flag))) break;
+        tc_fence_after_sync();
+        // O += P V_u: A = P in TMEM (16 keys are 8 columns of bf16 pairs), B = 16 rows of the V tile
+        const uint64_t bd = vd + ((s * kBytes + b * kPf4Sub * 128) >> 4);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + k * 8, bd + k * (2048 >> 4), kIdescPV, (j | k) != 0);
-          tc_commit(&bars->o_done[t]);
-          if (t == nq - 1) tc_commit(&bars->v_empty[s]);
-          if (j + 1 < n_tiles) {
-            const int s1 = (j + 1) % kPf4Stages;
-            if (t == 0 && !mbar_wait(&bars->k_full[s1], static_cast<uint32_t>(((j + 1) / kPf4Stages) & 1), abort_flag)) { ok = false; break; }
-            tc_fence_after_sync();
-            issue_s(t, j + 1);     // executes after the P_t V_j above: it overwrites the columns P_t lives in
-            if (t == nq - 1) tc_commit(&bars->k_empty[s1]);
-          }
+        for (int k = 0; k < kPf4Sub / 16; ++k) mma_bf16_ts(o_at, s_at + b * kPf4Sub + k * 8, bd + k * (2048 >> 4), kIdescPV, (u | k) != 0);
+        if (b) tc_commit(&bars->v_empty[s]);
+        tc_commit(&bars->o_done[t][b]);
+        if (u + 2 < n_subs) {
+          const int s1 = (j + 1) % kPf4Stages;
+          if (b == 0 && !(ok = mbar_wait(&bars->k_full[s1], static_cast<uint32_t>(((j + 1) / kPf4Stages) & 1), abort_flag))) break;
+          tc_fence_after_sync();
+          issue_s(u + 2);          // executes after the P V_u above: it overwrites the columns P lives in
         }
       }
       if (!ok) report_status(p.pool.status, kWaitTimeout, kKernelKv4, 51, blockIdx.x);
     }
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     // ------------------------------------------------------------------------- codes to numbers, one key per thread
     const int key = (warp - 12) * 32 + lane;
     const int* table = p.pool.block_table + static_cast<long long>(seq) * p.pool.max_pages;
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
     }
     if (!ok && lane == 0) report_status(p.pool.status, kWaitTimeout, kKernelKv4, 52, blockIdx.x);
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
     // ------------------------------------------------------------------------- softmax warps
     const int t = (warp >> 2) - 1;                        // row tile of this warp group
     const int quarter = warp & 3;                         // TMEM lane quarter this warp may touch
@@ -245,52 +247,38 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
       float m_run = -INFINITY, l_run = 0.f;
       const float c = kCap ? 1.f : p.scale_log2;
       bool ok = true;
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars->s_full[t], j & 1, abort_flag))) { ok = false; break; }
+      for (int u = 0; u < n_subs && ok; ++u) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->s_full[t][u & 1], (u >> 1) & 1, abort_flag))) { ok = false; break; }
         tc_fence_after_sync();
-        uint32_t r[128];
+        const uint32_t col = s_col + (u & 1) * kPf4Sub;
+        uint32_t r[kPf4Sub];
         float mf[8];
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) tmem_ld_32x32(s_col + cc * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[cc * 32]));
+        tmem_ld_32x32(col, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        tmem_ld_32x32(col + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
         tmem_ld_wait();
+        const int key0 = first_tile * kPf4Tile + u * kPf4Sub;
+        if (kCap)
 #pragma unroll
-        for (int cc = 2; cc < 4; ++cc) tmem_ld_32x32(s_col + cc * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[cc * 32]));
-        const int key0 = (first_tile + j) * kPf4Tile;
-        const bool open = key0 >= open_from && key0 + kPf4Tile <= open_to;
-        if (!kCap && open) {
-          // every row of the warp sees the whole tile; the second half is in flight while the maximum of the first is taken
+          for (int i = 0; i < kPf4Sub; ++i)               // cap tanh(x) = cap - 2 cap / (exp(2 x) + 1)
+            r[i] = __float_as_uint(p.cap_out - __fdividef(2.f * p.cap_out, pf4_exp2(fminf(__uint_as_float(r[i]) * p.cap_in, 126.f)) + 1.f));
+        if (key0 < open_from || key0 + kPf4Sub > open_to) {
+          const int from = start - key0, to = lim - key0;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) mf[u] = __uint_as_float(r[u]);
-#pragma unroll
-          for (int i = 8; i < 64; ++i) mf[i & 7] = fmaxf(mf[i & 7], __uint_as_float(r[i]));
-          tmem_ld_wait();
-        } else {
-          tmem_ld_wait();
-          if (kCap)
-#pragma unroll
-            for (int i = 0; i < 128; ++i)                   // cap tanh(x) = cap - 2 cap / (exp(2 x) + 1)
-              r[i] = __float_as_uint(p.cap_out - __fdividef(2.f * p.cap_out, pf4_exp2(fminf(__uint_as_float(r[i]) * p.cap_in, 126.f)) + 1.f));
-          if (!open) {
-            const int from = start - key0, to = lim - key0;
-#pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (i >= to || i < from) r[i] = 0xff800000u;
-          }
-#pragma unroll
-          for (int u = 0; u < 8; ++u) mf[u] = __uint_as_float(r[u]);
-#pragma unroll
-          for (int i = 8; i < 64; ++i) mf[i & 7] = fmaxf(mf[i & 7], __uint_as_float(r[i]));
+          for (int i = 0; i < kPf4Sub; ++i)
+            if (i >= to || i < from) r[i] = 0xff800000u;
         }
 #pragma unroll
-        for (int i = 64; i < 128; ++i) mf[i & 7] = fmaxf(mf[i & 7], __uint_as_float(r[i]));
+        for (int i = 0; i < 8; ++i) mf[i] = __uint_as_float(r[i]);
+#pragma unroll
+        for (int i = 8; i < kPf4Sub; ++i) mf[i & 7] = fmaxf(mf[i & 7], __uint_as_float(r[i]));
         const float mx = fmaxf(fmaxf(fmaxf(mf[0], mf[1]), fmaxf(mf[2], mf[3])), fmaxf(fmaxf(mf[4], mf[5]), fmaxf(mf[6], mf[7]))) * c;
         // raise the running maximum only when it would grow by more than the gap (or on the first tile);
         // a warp decides together because the O rescale below is a warp-wide TMEM access
         if (__any_sync(0xffffffffu, mx > m_run + kPf4Gap)) {
           const float m_new = fmaxf(m_run, mx);
           const float alpha = m_run == -INFINITY ? 0.f : pf4_exp2(m_run - m_new);
-          if (j > 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&bars->o_done[t], (j - 1) & 1, abort_flag))) { ok = false; break; }
+          if (u > 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&bars->o_done[t][(u - 1) & 1], ((u - 1) >> 1) & 1, abort_flag))) { ok = false; break; }
             tc_fence_after_sync();
 #pragma unroll
             for (int cc = 0; cc < D / 16; ++cc) {
@@ -309,7 +297,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
         const float sub = m_run == -INFINITY ? 0.f : m_run;
         float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
+        for (int cc = 0; cc < kPf4Sub / 32; ++cc) {
           uint32_t packed[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -318,15 +306,16 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
             sums[i & 3] += a + b;
             packed[i] = pack_bf16x2(a, b);
           }
-          pf4_st16(s_col + cc * 16, packed);             // P_t: columns [0, 64) of S_t
+          pf4_st16(col + cc * 16, packed);               // P_t over the first half of S_t
         }
         tmem_st_wait();
         l_run += (sums[0] + sums[1]) + (sums[2] + sums[3]);
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->p_ready[t]);
+        if (lane == 0) mbar_arrive(&bars->p_ready[t][u & 1]);
       }
-      if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done[t], (n_tiles - 1) & 1, abort_flag));
+      // scores are two ahead, so the last two products may both be outstanding
+      for (int u = max(0, n_subs - 2); u < n_subs && ok; ++u) ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done[t][u & 1], (u >> 1) & 1, abort_flag));
       if (!ok) {
         if (lane == 0) report_status(p.pool.status, kWaitTimeout, kKernelKv4, 53, blockIdx.x);
       } else {
@@ -424,8 +413,16 @@ B200_API int b200_attn_prefill_kv4(const void* q, const void* pool, void* out, c
   }
   const int smem = (2 + 2 * kPf4Stages) * kPf4Half * (d / 64) + static_cast<int>(sizeof(Pf4Barriers)) + 1024;
   static PerDeviceOnce once[4];
-  auto go = [&](auto kernel, PerDeviceOnce& o) -> cudaError_t {
-    if (o.first_time()) {
+  static int registers[4];                             // of the kernels as they were built
+  auto go = [&](auto kernel, int which) -> cudaError_t {
+    if (registers[which] == 0) {
+      cudaFuncAttributes has{};
+      const cudaError_t e = cudaFuncGetAttributes(&has, kernel);
+      if (e != cudaSuccess) return e;
+      registers[which] = has.numRegs;
+    }
+    if (registers[which] != kPf4Registers) return cudaErrorInvalidConfiguration;   // warps would wait for registers that nobody gives back
+    if (once[which].first_time()) {
       const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       if (e != cudaSuccess) return e;
     }
@@ -433,7 +430,7 @@ B200_API int b200_attn_prefill_kv4(const void* q, const void* pool, void* out, c
     return launch_pdl(kernel, grid, dim3(kPf4Threads), smem, stream, p);
   };
   cudaError_t e;
-  if (d == 128) e = softcap > 0.f ? go(attn_prefill_kv4_kernel<128, true>, once[0]) : go(attn_prefill_kv4_kernel<128, false>, once[1]);
-  else e = softcap > 0.f ? go(attn_prefill_kv4_kernel<64, true>, once[2]) : go(attn_prefill_kv4_kernel<64, false>, once[3]);
+  if (d == 128) e = softcap > 0.f ? go(attn_prefill_kv4_kernel<128, true>, 0) : go(attn_prefill_kv4_kernel<128, false>, 1);
+  else e = softcap > 0.f ? go(attn_prefill_kv4_kernel<64, true>, 2) : go(attn_prefill_kv4_kernel<64, false>, 3);
   return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
 }
