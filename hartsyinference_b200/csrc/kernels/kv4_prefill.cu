@@ -371,11 +371,11 @@ B200_API int b200_attn_kv4_choice(int seqs, int max_q_len, int max_kv_len, int h
   if (seqs < 1 || max_q_len < 1 || hkv < 1 || hq < hkv) return 0;
   // Estimates in us from the times below. Blocks of 64 rows (b200_attn_kv4) start fastest and share a processor; blocks of 256 rows (this file's)
   // come in waves; parts of the key axis (b200_attn_few_kv4) read all units once for every 16 columns.
-  // Measured in us, 64 rows / 256 rows / parts, 32 heads over 8: one sequence of 100 queries 7.1 / 13.4 / 19, of 512 24 / 21 / -, of 2048
-  // 192 / 83 / -; 17 queries behind 1000 keys 30 / 29 / 22, behind 8000 212 / 185 / 36; 100 there 212 / 224 / 98; 8 behind 30000 770 / 675 / 39;
-  // 16 sequences of 17 behind 100 keys 9.7 / 10.6 / 49, behind 1000 44 / 35 / 57, of 5 behind 3000 81 / 85 / 57. 32 heads over 32: 16 of 17
-  // behind 1000 84 / 118 / 76. Heads of 64, 32 over 8: 100 queries 5.2 / 9.9 / -, 512 19 / 17 / -, 2048 behind 6000 619 / 254 / -, 17 behind
-  // 8000 146 / 162 / 26, 100 there 147 / 201 / 67.
+  // Measured in us, 64 rows / 256 rows / parts, 32 heads over 8: one sequence of 100 queries 7.1 / 11.4 / -, of 512 24 / 19 / -, of 2048
+  // 191 / 74 / -; 17 queries behind 1000 keys 30 / 23 / 22, behind 8000 210 / 130 / 36; 100 there 213 / 175 / 99; 8 behind 30000 768 / 458 / 39;
+  // 16 sequences of 17 behind 100 keys 9.8 / 10.7 / -, behind 1000 44 / 25 / 57, of 5 behind 3000 81 / 63 / 57. 32 heads over 32: 16 of 17
+  // behind 1000 83 / 98 / 76. Heads of 64, 32 over 8: 100 queries 5.3 / 8.5 / -, 512 18 / 15 / -, 2048 behind 6000 623 / 236 / -, 17 behind
+  // 8000 145 / 123 / 26, 100 there 147 / 164 / 67.
   const long long rows = static_cast<long long>(max_q_len) * (hq / hkv), lists = static_cast<long long>(seqs) * hkv;
   const long long waves = ((rows + 2 * kPf4Tile - 1) / (2 * kPf4Tile) * lists + num_sms() - 1) / num_sms();
   const double each = static_cast<double>((rows + 63) / 64 * lists) / num_sms();       // blocks of 64 rows a processor
@@ -383,7 +383,7 @@ B200_API int b200_attn_kv4_choice(int seqs, int max_q_len, int max_kv_len, int h
   const double units = keys / kKv4Unit * static_cast<double>((rows + 15) / 16 * lists);
   const bool big = d == 128;
   const double small = (big ? 3.3 : 3.) + (each > 1. ? each : 1.) * (big ? 0.026 : 0.0178) * keys;
-  const double wide = static_cast<double>(waves) * (big ? 7.5 + 0.0215 * keys : 6. + 0.0193 * keys);
+  const double wide = static_cast<double>(waves) * (big ? 7.5 + 0.0195 * keys : 6. + 0.018 * keys);
   const double parts = big ? 18. + 0.0008 * units : 14. + 0.00051 * units;
   const bool can = scale > 0.f, best = can && wide < small;
   if (causal && keys > 512. && rows < 65536 && seqs <= kKv4MaxSeqs && parts < (best ? wide : small)) return 2;

@@ -190,7 +190,7 @@ def attn_decode_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Ten
                 need = L.b200_attn_decode_kv4_workspace(b, hq, hkv, d, longest)
                 ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
                 rc = L.b200_attn_decode_kv4(q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), b, hq, hkv, d,
-                                            page, block_table.shape[1], pages, longest, int(window), float(scale), float(softcap), N.ptr(ws), need,
+                                            page, block_table.shape[1], pages, longest, min(int(window), 2 ** 31 - 1), float(scale), float(softcap), N.ptr(ws), need,
                                             N.state(q.device).status.data_ptr(), N.stream())
                 N.check(min(rc, 0), "b200_attn_decode_kv4", rc)
     if not emit_fp8:
@@ -219,7 +219,7 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
             return out.zero_()
         L, longest = N.lib(), block_table.shape[1] * page
         longest = longest if max_kv_len is None else min(max_kv_len, longest)
-        seqs, most, hq, d, window, scale = kv_lens.numel(), int(max_q_len), q.shape[1], q.shape[2], int(window), float(scale)
+        seqs, most, hq, d, window, scale = kv_lens.numel(), int(max_q_len), q.shape[1], q.shape[2], min(int(window), 2 ** 31 - 1), float(scale)
         ptrs = (q.data_ptr(), cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), cu_q.data_ptr(), seqs, most)
         sizes, status = (hq, hkv, d, page, block_table.shape[1], pages), N.state(q.device).status.data_ptr()
         kernel = L.b200_attn_kv4_choice(seqs, most, longest, hq, hkv, d, int(causal), window, scale)
