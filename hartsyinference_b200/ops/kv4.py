@@ -120,22 +120,22 @@ def rope_kv4(qkv, positions: torch.Tensor, hq: int, hkv: int, d: int, *, cache: 
 
 def kv4_gather(cache: torch.Tensor, block_table: torch.Tensor, cu_kv: torch.Tensor, total: int) -> tuple:
     """The first tokens of sequences as dense bf16 (k, v) [total, hkv, d]: rows ``cu_kv[s]`` .. ``cu_kv[s + 1]`` (int32 [S + 1], from 0) are
-    those of block-table row s, ``total`` is the last of them on the host. What the cache stands for is exact in bf16."""
+    those of block-table row s, ``total`` is the last of them on the host. What the cache stands for is exact in bf16. Rows that belong to
+    no sequence are zeros."""
     d = 2 * cache.shape[-1] // 17
     device = cache.get_device()
     pages, hkv, page = _pool(cache, d, device)
     if block_table.dim() != 2 or cu_kv.numel() != block_table.shape[0] + 1 or total < 0:
         raise ValueError("kv4_gather: block_table [S, pages] and cu_kv [S + 1]")
-    k = torch.empty(total, hkv, d, dtype=torch.bfloat16, device=cache.device)
-    v = torch.empty_like(k)
-    if not cache.is_cuda:
-        cuts = cu_kv.tolist()
+    if not cache.is_cuda or total == 0 or block_table.numel() == 0 or pages == 0:
+        k, v = (torch.zeros(total, hkv, d, dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+        cuts = [] if cache.is_cuda else cu_kv.tolist()
         for i, (a, b) in enumerate(zip(cuts, cuts[1:])):
             k[a:b], v[a:b] = R.kv4_sequence(cache, block_table[i], b - a)
         return k, v
+    k = torch.empty(total, hkv, d, dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty_like(k)
     block_table, cu_kv = _ints("block_table", block_table, device), _ints("cu_kv", cu_kv, device)
-    if total == 0 or block_table.shape[1] == 0:
-        return k.zero_(), v.zero_()
     with _on(device):
         rc = N.lib().b200_kv4_gather(cache.data_ptr(), block_table.data_ptr(), cu_kv.data_ptr(), k.data_ptr(), v.data_ptr(), block_table.shape[0],
                                      total, hkv, d, page, block_table.shape[1], pages, N.state(cache.device).status.data_ptr(), N.stream())
@@ -204,10 +204,12 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
                      max_kv_len: Optional[int] = None) -> torch.Tensor:
     """Variable-length (chunked) attention over a 4-bit pool: q [total_q, hq, d] packed by ``cu_q`` int32 [S + 1], the keys of sequence s are
     its first ``kv_lens[s]`` tokens, the last of them its last query's own. No sequence has more queries than ``max_q_len``; ``max_kv_len``
-    only chooses between two kernels. A query without keys gives zeros. Arguments as of :func:`.core.attn_prefill_paged`."""
+    only chooses between two kernels. A query without keys gives zeros; rows behind the last sequence's are undefined. Arguments as of :func:`.core.attn_prefill_paged`."""
     block_table, kv_lens, pages, hkv, page = _attention_args("attn_prefill_kv4", q, cache, block_table, kv_lens)
     if cu_q.numel() != kv_lens.numel() + 1:
         raise ValueError("attn_prefill_kv4: cu_q [S + 1]")
+    if q.shape[0] and max_q_len < 1:
+        raise ValueError(f"attn_prefill_kv4: at most {max_q_len} queries a sequence")
     cu_q = _ints("cu_q", cu_q, q.get_device())
     scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
     if not q.is_cuda:

@@ -218,7 +218,9 @@ def test_attention_on_cpu(hq, hkv, d):
     cache, table = _filled(lens, hkv, d, 16)
     cuts = [0, 4, 5, 45]
     q = _normal(45, hq, d, seed=8).to(torch.bfloat16)
-    got = ops.attn_prefill_kv4(q, cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor(cuts, dtype=torch.int32), max(each), window=7, softcap=20.0)
+    args = (q, cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor(cuts, dtype=torch.int32), max(each))
+    _close(ops.attn_prefill_kv4(*args, causal=False, window=5), *_plain(q, cache, table, lens, cuts, causal=False, window=5))
+    got = ops.attn_prefill_kv4(*args, window=7, softcap=20.0)
     want = _plain(q, cache, table, lens, cuts, window=7, softcap=20.0)
     _close(got, *want)
 
@@ -318,7 +320,7 @@ def test_decode_kernel(hq, hkv, d, kw, page):
 
 @gpu
 @pytest.mark.parametrize("hq,hkv,d", HEADS)
-@pytest.mark.parametrize("kw", CASES + [dict(causal=False)])
+@pytest.mark.parametrize("kw", CASES + [dict(causal=False), dict(causal=False, window=17)])
 def test_prefill_kernel(hq, hkv, d, kw):
     """Chunks behind nothing and behind a prefix, one token, none, and more queries than keys (the first see nothing)."""
     lens, each = [100, 0, 70, 333, 1, 200, 5], [100, 0, 3, 130, 1, 64, 9]
@@ -377,7 +379,7 @@ def test_few_queries_in_a_window():
 
 @gpu
 @pytest.mark.parametrize("hq,hkv,d", HEADS)
-@pytest.mark.parametrize("kw", CASES + [dict(causal=False)])
+@pytest.mark.parametrize("kw", CASES + [dict(causal=False), dict(causal=False, window=17)])
 def test_wide_blocks_of_prompts(hq, hkv, d, kw):
     """The kernel of 256 rows a block, whatever kernel the op would take."""
     from hartsyinference_b200.ops import _native as N
@@ -519,3 +521,22 @@ def test_first_token_that_takes_nearly_all_of_the_weight():
     dev = _cuda(cache, table, torch.tensor([n], dtype=torch.int32))
     _close(ops.attn_decode_kv4(q.cuda(), *dev), *want)
     _close(ops.attn_prefill_kv4(q.cuda(), *dev, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), 1), *want)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_nothing_to_do(dev):
+    """No sequences, no pages, no tokens, and rows that belong to nobody."""
+    cache, none = ops.kv4_cache(2, 2, 16, 64, dev), ops.kv4_cache(0, 2, 16, 64, dev)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    q = torch.ones(3, 4, 64, dtype=torch.bfloat16, device=dev)
+    table = ints([1], [0], [1])
+    assert not ops.attn_decode_kv4(q, none, table, ints(0, 0, 0)).any()
+    assert not ops.attn_decode_kv4(q, cache, table[:, :0], ints(0, 0, 0)).any()
+    assert ops.attn_decode_kv4(q[:0], cache, table[:0], ints()).shape == (0, 4, 64)
+    assert not ops.attn_prefill_kv4(q, none, table, ints(0, 0, 0), ints(0, 1, 2, 3), 1).any()
+    assert ops.attn_prefill_kv4(q[:0], cache, table, ints(0, 0, 0), ints(0, 0, 0, 0), 0).shape == (0, 4, 64)
+    for k in ops.kv4_gather(cache, table[:0], ints(0), 3) + ops.kv4_gather(none, table, ints(0, 0, 0, 0), 3) + ops.kv4_gather(cache, table, ints(0, 0, 1, 1), 4):
+        assert k.shape[1:] == (2, 64) and not k[1:].any()
+    assert ops.rope_kv4(torch.ones(0, 8 * 64, dtype=torch.bfloat16, device=dev), ints(), 4, 2, 64, cache=cache)[0].shape == (0, 4, 64)
+    with pytest.raises(ValueError):
+        ops.attn_prefill_kv4(q, cache, table, ints(1, 1, 1), ints(0, 1, 2, 3), 0)
