@@ -8,7 +8,7 @@ plus the first correction are kept; the KV entries of rejected positions are cut
 allocator's ``truncate``. Every kept token is the greedy token of the same model at its position. A pass over several
 tokens takes other kernels on the device than a decode step (attention of a chunk, products of more rows), which
 round differently, so where two logits are that close together plain greedy decoding may keep the other one; on
-the host the outputs are identical.
+the host the outputs are identical, but for a 4-bit cache, in which a last bit can be a step of a code.
 
 Reference behaviour: src/HartsyInference.LLM/Generation/TextGenerationPipeline.cs
 (GenerateSpeculative:403-463; n-gram 3, draft length 8, look-back 4096).

@@ -151,3 +151,39 @@ def test_gpu_engine_with_graphs_and_without(fp8):
         assert e.alive and (not graphs or (len(e._graphs) >= 1 and not e._graphs_disabled))
     N.check_status()
     assert outs[0] == outs[1]
+
+
+def _drafted(dev, n, **kw):
+    from hartsyinference_b200.engine.speculative import generate_speculative
+    m = _model(dev, seed=5, **kw)
+    part = torch.randint(0, 512, (12,), generator=torch.Generator().manual_seed(5)).tolist()
+    p = SamplingParams(greedy=True, max_tokens=24, ignore_eos=True)
+    engine = lambda: LLMEngine(m, num_pages=96, page_size=16, max_batch=2, prefill_chunk=256, max_model_len=1024)
+    prompt = (part * (n // 12 + 1))[:n]
+    return (m, prompt, *generate_speculative(engine(), prompt, p), engine().generate([prompt], p)[0])
+
+
+def test_drafts_are_verified_over_the_cache():
+    """Every kept token is the greedy one of a pass over the whole sequence where that decision is no near tie: logits are bf16 numbers below 4, whose
+    steps are 2^-6; a step of each of two logits, and of the two ways that hidden states of as many tokens round, are within 0.07."""
+    m, prompt, out, stats, plain = _drafted("cpu", 100)
+    assert len(out) == len(plain) == 24 and stats.drafted > 0
+    for got in (out, plain):
+        tokens = torch.tensor(prompt + got)
+        m.alloc_kv(8, 16)
+        table = torch.arange(8, dtype=torch.int32)[None]
+        n = len(tokens)
+        rows = m.full_logits(m.forward_hidden(ForwardBatch(
+            tokens=tokens.int(), positions=torch.arange(n, dtype=torch.int32), slot_mapping=torch.arange(n), block_table=table, is_decode=False,
+            kv_lens=torch.tensor([n], dtype=torch.int32), cu_q=torch.tensor([0, n], dtype=torch.int32), max_q_len=n, max_kv_len=n))).float()[99:-1]
+        assert rows.abs().max() < 4
+        assert (rows.gather(1, tokens[100:, None])[:, 0] >= rows.amax(1) - 0.07).all()
+
+
+@gpu
+def test_gpu_drafts_are_verified_over_a_long_cache():
+    """Passes of up to nine tokens behind 700 others: the kernel that cuts the key axis. Tokens of plain decoding may differ at near ties."""
+    assert N.lib().b200_attn_kv4_choice(1, 9, 709, 8, 2, 128, 1, 0, 0.088) == 2
+    _, _, out, stats, plain = _drafted("cuda", 700, **GROUPED)
+    N.check_status()
+    assert len(out) == len(plain) == 24 and stats.drafted > 0 and out[0] == plain[0]
