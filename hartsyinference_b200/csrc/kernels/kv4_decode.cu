@@ -16,8 +16,8 @@
 // row 2 i + 1 key 7 - i of eight, which lets every shared-memory read of codes touch each bank once.
 //
 // Work: a unit is 16 tokens of one kv head. All units of all sequences and heads in a row are cut into equal shares, one per resident
-// block, whatever the lengths; a share's first and last sequence may be other blocks' too, whose parts the second kernel
-// joins (in the order of the blocks, so results do not depend on timing). Within a share every warp takes units side by side and has its own ring of
+// block (or one per unit, where there are fewer of them than blocks), whatever the lengths; a share's first and last sequence may be
+// other blocks' too, whose parts the second kernel joins (in the order of the blocks, so results do not depend on timing). Within a share every warp takes units side by side and has its own ring of
 // bulk copies, so warps meet only at the end. Short sequences get one block each and no second kernel.
 #include "kv4.cuh"
 #include "mma_sync.cuh"
@@ -97,6 +97,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
 // Tokens of a sequence that ask; few: several of them, else one. Known when compiled except in the joins: decoded tokens would
 // otherwise pay for the other case (4.4 us became 5.7 for 16 short sequences).
 __device__ __forceinline__ int dec4_queries(const DecodeKv4Params& p, bool few, int s) { return few ? p.cu_q[s + 1] - p.cu_q[s] : 1; }
+// Blocks that have a share of `total` units. The host counts blocks from a bound of the lengths, so there may be more of them than units; those
+// behind these write nothing, and the join must not read what they would have written.
+__device__ __forceinline__ long long dec4_shares(const DecodeKv4Params& p, long long total) { return total < p.blocks ? total : p.blocks; }
 // Units of a sequence that its queries see, and the first of them.
 __device__ __forceinline__ int dec4_units(const DecodeKv4Params& p, bool few, int s, int& first) {
   const int len = kv4_length(p.pool, p.kv_lens[s], kKernelKv4), queries = dec4_queries(p, few, s);
@@ -189,9 +192,10 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
     __syncthreads();
     if (blockIdx.x == 0)
       for (int i = threadIdx.x; i <= p.seqs; i += kDec4Threads) p.prefix[i] = prefix[i];
-    const long long total = static_cast<long long>(run) * heads_v;
-    f0 = total * blockIdx.x / p.blocks;
-    f1 = total * (blockIdx.x + 1) / p.blocks;
+    const long long total = static_cast<long long>(run) * heads_v, shares = dec4_shares(p, total);
+    if (blockIdx.x >= shares) return;
+    f0 = total * blockIdx.x / shares;
+    f1 = total * (blockIdx.x + 1) / shares;
   } else {
     only_seq = blockIdx.x / heads_v;
     only_units = dec4_units(p, kFew, only_seq, only_first);
@@ -632,13 +636,13 @@ __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Par
   pdl_wait();
   pdl_trigger();
   const int heads_v = p.pool.hkv * p.chunks, s = blockIdx.x / heads_v, h = blockIdx.x - s * heads_v;
-  const long long total = static_cast<long long>(p.prefix[p.seqs]) * heads_v;
+  const long long total = static_cast<long long>(p.prefix[p.seqs]) * heads_v, shares = dec4_shares(p, total);
   const int n = p.prefix[s + 1] - p.prefix[s];
   const long long at = static_cast<long long>(p.prefix[s]) * heads_v + static_cast<long long>(h) * n;
   const Dec4Columns cols(p, p.cu_q != nullptr, s, h);
   // block of unit f: the last whose share starts at or before it
   const auto block_of = [&](long long f) {
-    const long long x = (f + 1) * p.blocks - 1;
+    const long long x = (f + 1) * shares - 1;
     return x < (1ll << 32) ? static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(total)) : static_cast<int>(x / total);
   };
   const int c0 = n > 0 ? block_of(at) : 0, c1 = n > 0 ? block_of(at + n - 1) : 0;

@@ -540,3 +540,72 @@ def test_nothing_to_do(dev):
     assert ops.rope_kv4(torch.ones(0, 8 * 64, dtype=torch.bfloat16, device=dev), ints(), 4, 2, 64, cache=cache)[0].shape == (0, 4, 64)
     with pytest.raises(ValueError):
         ops.attn_prefill_kv4(q, cache, table, ints(1, 1, 1), ints(0, 1, 2, 3), 0)
+
+
+# ------------------------------------------------------------------------------------------ few units for many blocks
+def _parts(q, cache, table, lens, longest, fill, cuts=None, most=1, window=0):
+    """The kernels that cut the key axis, with every byte of the workspace set to `fill` before the call."""
+    from hartsyinference_b200.ops import _native as N
+    L, n, hq, d = N.lib(), lens.numel(), q.shape[1], q.shape[2]
+    hkv, page = cache.shape[1], cache.shape[2] * 16
+    need = L.b200_attn_decode_kv4_workspace(n, hq, hkv, d, longest) if cuts is None else L.b200_attn_few_kv4_workspace(n, most, hq, hkv, d, longest)
+    assert need > 0
+    ws, out = torch.full((need,), fill, dtype=torch.uint8, device="cuda"), torch.full_like(q, 7)
+    sizes = (hq, hkv, d, page, table.shape[1], cache.shape[0], longest, window, 1 / math.sqrt(d), 0.0, ws.data_ptr(), need, N.state(q.device).status.data_ptr(), N.stream())
+    ptrs = [x.data_ptr() for x in (q, cache, out, table, lens)]
+    rc = L.b200_attn_decode_kv4(*ptrs, n, *sizes) if cuts is None else L.b200_attn_few_kv4(*ptrs, cuts.data_ptr(), n, most, *sizes)
+    assert rc == 2
+    return out
+
+
+FEW_UNITS = [([17], 32, 8, 128, 8192), ([100], 32, 8, 128, 8192), ([300], 32, 8, 128, 8192), ([300], 14, 2, 64, 8192), ([100] * 16, 8, 1, 128, 131072),
+             ([700] + [12] * 63, 14, 2, 64, 700), ([1], 8, 1, 128, 131072), ([20, 0, 1], 40, 2, 128, 8192), ([0, 0], 4, 2, 64, 8192), ([1, 0, 2, 16, 33], 24, 1, 64, 40000)]
+
+
+@gpu
+@pytest.mark.parametrize("lens,hq,hkv,d,longest", FEW_UNITS)
+@pytest.mark.parametrize("fill", [0xFF, 0x70, 0])                   # as floats: no numbers, 3e29, zeros
+def test_fewer_units_than_blocks(lens, hq, hkv, d, longest, fill):
+    """Blocks are counted from the longest length that the host knows; where the lengths themselves give fewer units, some blocks have none."""
+    cache, table = _filled(lens, hkv, d, 16)
+    wide = torch.full((len(lens), -(-longest // 16)), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table[:, :wide.shape[1]]
+    q = _normal(len(lens), hq, d, seed=9).to(torch.bfloat16)
+    dev = _cuda(q, cache, wide, torch.tensor(lens, dtype=torch.int32))
+    want = _plain(q, cache, table, lens, list(range(len(lens) + 1)))
+    _close(_parts(*dev, longest, fill), *want)
+    _close(_parts(*dev, longest, fill, window=600), *_plain(q, cache, table, lens, list(range(len(lens) + 1)), window=600))
+    each = [min(n + 1, 3 - i % 2) if i % 3 else 4 for i, n in enumerate(lens)]          # a query more than keys among them
+    cuts = torch.tensor([0, *each]).cumsum(0).tolist()
+    q = _normal(sum(each), hq, d, seed=8).to(torch.bfloat16)
+    cu = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    got = _parts(q.cuda(), *dev[1:], longest, fill, cu, 4)
+    _close(got, *_plain(q, cache, table, lens, cuts))
+
+
+@gpu
+def test_captured_over_a_wide_table_and_short_sequences():
+    """A graph made for long sequences and replayed over short ones, in whose memory no number is left by the work before."""
+    lens, hkv, d = [5000, 17, 300], 8, 128
+    cache, table = _filled(lens, hkv, d, 16)
+    q = _normal(3, 32, d, seed=1).to(torch.bfloat16)
+    qd, c, t, n = _cuda(q, cache, table, torch.tensor(lens, dtype=torch.int32))
+    cu = torch.tensor([0, 1, 2, 3], dtype=torch.int32, device="cuda")
+
+    def run():
+        stale = [torch.full((size,), math.nan, device="cuda") for size in (1 << 14, 1 << 17, 1 << 19, 1 << 21)]
+        del stale
+        return ops.attn_decode_kv4(qd, c, t, n), ops.attn_prefill_kv4(qd, c, t, n, cu, 1)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = run()
+    for now in ([17, 1, 0], lens, [0, 0, 0], [100, 16, 33], [1, 0, 0], [5000, 0, 300]):
+        n.copy_(torch.tensor(now, dtype=torch.int32))
+        g.replay()
+        for out in outs + run():
+            _close(out, *_plain(q, cache, table, now, [0, 1, 2, 3]))

@@ -187,3 +187,23 @@ def test_gpu_drafts_are_verified_over_a_long_cache():
     _, _, out, stats, plain = _drafted("cuda", 700, **GROUPED)
     N.check_status()
     assert len(out) == len(plain) == 24 and stats.drafted > 0 and out[0] == plain[0]
+
+
+@gpu
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("heads", [dict(), dict(num_heads=16, num_kv_heads=8)], ids=["2", "8"])
+def test_gpu_engine_decodes_short_sequences_under_a_long_limit(graphs, heads):
+    """An engine for 8192 tokens and a prompt of 17: the tables that decode steps get are as wide as the limit. Logits are those of one pass on the
+    CPU to the fraction that two devices' models agree to above."""
+    m = _model("cuda", seed=3, **GROUPED | heads)
+    tokens = torch.randint(0, 512, (29,), generator=torch.Generator().manual_seed(6))
+    e = LLMEngine(m, num_pages=600, page_size=16, max_batch=2, prefill_chunk=128, max_model_len=8192, use_cuda_graphs=graphs)
+    stale = [torch.full((n,), float("nan"), device="cuda") for n in (1 << 12, 1 << 14, 1 << 16, 1 << 17, 1 << 18) for _ in range(4)]
+    del stale
+    got = [e.replay([("a", tokens[:17].tolist(), [16])])]
+    got += [e.replay([("a", [x], [0])]) for x in tokens[17:].tolist()]
+    assert not graphs or (e._graphs and not e._graphs_disabled)
+    N.check_status()
+    cpu = _twin(m, "cpu")
+    want = _logits(cpu, [_step("cpu", tokens, 0)])[16:]
+    assert torch.nn.functional.cosine_similarity(torch.cat(got).cpu(), want, dim=-1).min().item() > 0.995
