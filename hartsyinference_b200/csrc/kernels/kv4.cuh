@@ -57,6 +57,10 @@ __device__ __forceinline__ int kv4_length(const Kv4Pool& p, int len, uint32_t ke
   return len;
 }
 
+// First of the last `window` keys (at least one) below key `end`. Where queries outnumber keys `end` may be below 0, from which a window near
+// 2^31 must not be taken off.
+__device__ __forceinline__ int kv4_window_start(int end, int window) { return end > window ? end - window : 0; }
+
 // ---- numbers to bytes ---------------------------------------------------------------------------
 // Scale byte of a block whose largest magnitude is amax, and the scale.
 __device__ __forceinline__ uint32_t kv4_scale(float amax, int exp, float& s) {

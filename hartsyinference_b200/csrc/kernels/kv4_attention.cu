@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(128) attn_kv4_kernel(const AttnKv4Params p) {
     head[r] = on ? static_cast<int>(row - static_cast<long long>(query[r]) * G) : 0;
     const int pos = ctx + query[r];
     lim[r] = !on ? 0 : p.causal ? min(kv_len, pos + 1) : kv_len;
-    start[r] = on && p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+    start[r] = on && p.window > 0 ? kv4_window_start(pos + 1, p.window) : 0;
     const __nv_bfloat16* src = p.q + ((static_cast<long long>(q_off) + max(query[r], 0)) * p.hq + kvh * G + head[r]) * D;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(128) attn_kv4_kernel(const AttnKv4Params p) {
   const int first_query = static_cast<int>(block_row / G);
   const int last_query = static_cast<int>(min(rows, block_row + kKv4Rows) - 1) / G;
   const int keys = p.causal ? min(kv_len, ctx + last_query + 1) : kv_len;
-  const int key0 = p.window > 0 ? max(0, ctx + first_query + 1 - p.window) : 0;
+  const int key0 = p.window > 0 ? kv4_window_start(ctx + first_query + 1, p.window) : 0;
   const int tiles = keys > 0 ? (keys + kKv4Tile - 1) / kKv4Tile : 0;
   const int* table = p.pool.block_table + static_cast<long long>(seq) * p.pool.max_pages;
   // this thread's row of a tile: a key (threads 0 .. 63) or a value

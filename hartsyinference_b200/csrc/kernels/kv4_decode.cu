@@ -103,7 +103,7 @@ __device__ __forceinline__ long long dec4_shares(const DecodeKv4Params& p, long 
 // Units of a sequence that its queries see, and the first of them.
 __device__ __forceinline__ int dec4_units(const DecodeKv4Params& p, bool few, int s, int& first) {
   const int len = kv4_length(p.pool, p.kv_lens[s], kKernelKv4), queries = dec4_queries(p, few, s);
-  first = p.window > 0 ? max(0, len - queries + 1 - p.window) / kKv4Unit : 0;
+  first = p.window > 0 ? kv4_window_start(len - queries + 1, p.window) / kKv4Unit : 0;
   return len > 0 && queries > 0 ? (len + kKv4Unit - 1) / kKv4Unit - first : 0;
 }
 // The columns of part h % chunks of kv head h / chunks: how many there are, and the row of q and of the output of one of them.
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
     const int len = kv4_length(p.pool, p.kv_lens[s], kKernelKv4);
     // columns of query i see the keys below len - before + i, where `before` queries are in front of the last one
     const int before = dec4_queries(p, kFew, s) - 1;
-    const int start = p.window > 0 ? max(0, len - p.window) : 0;       // of the last query: the others' masks begin before it
+    const int start = p.window > 0 ? kv4_window_start(len, p.window) : 0;       // of the last query: the others' masks begin before it
     const int stop_key = (first + units - at_rel) * kKv4Unit;          // keys from here on are not this warp's
     const int last = min(len - before, stop_key);
     __syncwarp();                                      // the last sequence's products have read `starts`
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
 #pragma unroll
               for (int t = 0; t < NT; ++t) {
                 const int seen = len - before + cols.query(8 * t + 2 * tq + (j & 1));
-                if (key < 0 || key >= min(seen, stop_key) || (p.window > 0 && key < seen - p.window)) sc[u][t][j] = -INFINITY;
+                if (key < 0 || key >= min(seen, stop_key) || (p.window > 0 && key < kv4_window_start(seen, p.window))) sc[u][t][j] = -INFINITY;
               }
             } else if (key < start || key >= last) {
 #pragma unroll
@@ -762,7 +762,8 @@ static int dec4_run(const void* q, const void* pool, void* out, const int* block
   }
   const long long pairs = static_cast<long long>(seqs) * hkv * p.chunks;
   if (pairs >= (1ll << 31)) return -3;
-  if (window > 0 && window + max_q_len - 1ll < max_kv_len) max_kv_len = min(max_kv_len, window + max_q_len - 1 + kKv4Unit);
+  const long long seen = window + (max_q_len - 1ll);  // keys that some query of a sequence sees
+  if (window > 0 && seen < max_kv_len) max_kv_len = static_cast<int>(min(static_cast<long long>(max_kv_len), seen + kKv4Unit));
   p.blocks = dec4_blocks(seqs, hkv * p.chunks, p.chunk_heads, max_kv_len);
   const bool shares = p.blocks > 0;
   if (cu_q && !shares) return -6;                    // short caches and many sequences are for the other kernels

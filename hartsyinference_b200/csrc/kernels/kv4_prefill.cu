@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
   const bool tile1 = row0 + kPf4Tile < rows;
   const int last_query = (min(rows, row0 + 2 * kPf4Tile) - 1) / G;
   const int n_keys = p.causal ? min(kv_len, ctx + last_query + 1) : kv_len;
-  const int first_tile = p.window > 0 ? max(0, ctx + row0 / G + 1 - p.window) / kPf4Tile : 0;
+  const int first_tile = p.window > 0 ? kv4_window_start(ctx + row0 / G + 1, p.window) / kPf4Tile : 0;
   const int n_tiles = n_keys > first_tile * kPf4Tile ? (n_keys + kPf4Tile - 1) / kPf4Tile - first_tile : 0;
   const int n_subs = n_tiles > 0 ? (n_keys + kPf4Sub - 1) / kPf4Sub - 2 * first_tile : 0;
 
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
     if (t == 0 || tile1) {
       const int pos = ctx + query;
       const int lim = row >= rows ? 0 : p.causal ? min(kv_len, pos + 1) : kv_len;         // keys [start, lim) are this row's
-      const int start = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+      const int start = p.window > 0 ? kv4_window_start(pos + 1, p.window) : 0;
       // keys that every row of the warp sees
       const int open_from = __reduce_max_sync(0xffffffffu, start), open_to = __reduce_min_sync(0xffffffffu, lim);
       float m_run = -INFINITY, l_run = 0.f;

@@ -609,3 +609,34 @@ def test_captured_over_a_wide_table_and_short_sequences():
         g.replay()
         for out in outs + run():
             _close(out, *_plain(q, cache, table, now, [0, 1, 2, 3]))
+
+
+# ------------------------------------------------------------------------------------------ windows near 2^31
+@gpu
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (40, 2, 128)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 8, 2 ** 30])
+@pytest.mark.parametrize("causal", [True, False])
+def test_windows_wider_than_anything(hq, hkv, d, window, causal):
+    """More queries than keys under a window near 2^31, in each kernel: the queries in front of the first key are below 0 already."""
+    from hartsyinference_b200.ops import _native as N
+    L, lens, each = N.lib(), [5, 700, 1, 0, 40], [17, 9, 20, 3, 90]
+    cache, table = _filled(lens, hkv, d, 32)
+    cuts = torch.tensor([0, *each]).cumsum(0).tolist()
+    q = _normal(sum(each), hq, d, seed=9).to(torch.bfloat16)
+    want = _plain(q, cache, table, lens, cuts, causal=causal)
+    dev = _cuda(q, cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor(cuts, dtype=torch.int32))
+    _close(ops.attn_prefill_kv4(*dev, max(each), causal=causal, window=window), *want)
+    _close(ops.attn_prefill_kv4(*dev, max(each), causal=causal, window=window << 9), *want)
+    if causal:
+        _close(_few(*dev, max(each), 700, window=window), *want)
+    qd, c, t, n, cu = dev
+    for run in (L.b200_attn_kv4, L.b200_attn_prefill_kv4):
+        out = torch.full_like(qd, 7)
+        rc = run(qd.data_ptr(), c.data_ptr(), out.data_ptr(), t.data_ptr(), n.data_ptr(), cu.data_ptr(), len(lens), max(each), hq, hkv, d, 32, t.shape[1],
+                 c.shape[0], int(causal), window, 1 / math.sqrt(d), 0.0, N.state(qd.device).status.data_ptr(), N.stream())
+        assert rc == 0
+        _close(out, *want)
+    if causal:
+        last = [c - 1 for c in cuts[1:]]
+        _close(ops.attn_decode_kv4(qd[last], c, t, n, window=window), *(x[last] for x in want))
+    N.check_status()
