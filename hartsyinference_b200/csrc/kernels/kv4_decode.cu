@@ -744,16 +744,17 @@ static int dec4_run(const void* q, const void* pool, void* out, const int* block
   if (seqs <= 0) return 0;
   if (hkv < 1 || hq < 1 || hq % hkv || max_pages < 1 || pages < 1 || !kv4_pool_fits(pool, d, page)) return -2;
   const long long columns = static_cast<long long>(max_q_len) * (hq / hkv), units = static_cast<long long>(max_pages) * (page / kKv4Unit);
-  if (columns >= (1ll << 20) || units * seqs >= (1ll << 31) || units * hkv * ((columns + 15) / 16) >= (1ll << 32)) return -3;
+  if (columns >= (1ll << 20) || units * seqs >= (1ll << 31)) return -3;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15) return -4;
   DecodeKv4Params p{};
+  dec4_chunks(static_cast<int>(columns), p.chunks, p.chunk_heads);
+  if (units * hkv * p.chunks >= (1ll << 32)) return -3;        // the kernels divide the units of a sequence in 32 bits
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.out = static_cast<__nv_bfloat16*>(out);
   p.kv_lens = kv_lens;
   p.cu_q = cu_q;
   p.pool = Kv4Pool{static_cast<const uint8_t*>(pool), block_table, pages, hkv, max_pages, kv4_unit_shift(page), static_cast<DeviceStatus*>(status)};
   p.seqs = seqs; p.hq = hq; p.group = hq / hkv;
-  dec4_chunks(p.group * max_q_len, p.chunks, p.chunk_heads);
   p.window = window;
   p.scale_log2 = scale * kDec4Log2e;
   if (softcap > 0.f) {

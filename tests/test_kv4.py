@@ -640,3 +640,17 @@ def test_windows_wider_than_anything(hq, hkv, d, window, causal):
         last = [c - 1 for c in cuts[1:]]
         _close(ops.attn_decode_kv4(qd[last], c, t, n, window=window), *(x[last] for x in want))
     N.check_status()
+
+
+def test_tables_whose_units_leave_32_bits_are_refused():
+    """2^26 units of 24 kv heads: 17 to 24 columns are walked in three parts, 25 to 32 in two, and the units of a sequence are counted in 32 bits."""
+    from hartsyinference_b200.ops import _native as N
+    if not N.available():
+        pytest.skip("kernels library not built")
+    L, p = N.lib(), 4096
+    decode = lambda columns, max_pages: L.b200_attn_decode_kv4(p, p, p, p, p, 1, 24 * columns, 24, 64, 128, max_pages, 1, 1 << 20, 0, 1.0, 0.0, None, 0, None, None)
+    few = lambda columns, max_pages: L.b200_attn_few_kv4(p, p, p, p, p, p, 1, columns, 24, 24, 64, 128, max_pages, 1, 1 << 20, 0, 1.0, 0.0, None, 0, None, None)
+    for f in (decode, few):
+        assert [f(c, 1 << 23) for c in (16, 17, 20, 24, 25, 32)] == [-5, -3, -3, -3, -5, -5]          # -5: the sizes are taken, no workspace is there
+        assert [f(c, 1 << 22) for c in (16, 17, 20, 24, 25, 32)] == [-5] * 6
+        assert [f(c, 1 << 24) for c in (16, 17, 20, 24, 25, 32)] == [-5] + [-3] * 5
