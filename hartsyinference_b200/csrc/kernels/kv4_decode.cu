@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(256) join_decode_kv4_kernel(const DecodeKv4Par
   // block of unit f: the last whose share starts at or before it
   const auto block_of = [&](long long f) {
     const long long x = (f + 1) * shares - 1;
-    return x < (1ll << 32) ? static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(total)) : static_cast<int>(x / total);
+    return (x | total) >> 32 ? static_cast<int>(x / total) : static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(total));
   };
   const int c0 = n > 0 ? block_of(at) : 0, c1 = n > 0 ? block_of(at + n - 1) : 0;
   if (n > 0 && c0 == c1) return;                     // one block had all of it
