@@ -565,9 +565,10 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
     done = stop;
   }
   if (!ok) {
-    // copies in flight end before the block does
+    // copies in flight end before the block does, whichever warp gave up: the block's flag, which is set by now, would end these waits at once
     for (int j = 0; j < kDec4Stages; ++j) {
-      if (i + j < mine) mbar_wait(&full[warp][slot], phase, abort_flag, 1 << 22);
+      uint32_t alone = 0;
+      if (i + j < mine) mbar_wait(&full[warp][slot], phase, &alone, 1 << 22);
       phase ^= slot;
       slot ^= 1;
     }
