@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
     // The pairs that have units of this sequence. One that reaches into the next sequence is kept for it.
     int key0 = (first - at_rel + 2 * i) * kKv4Unit;
     for (int rel = 2 * i; ok && rel < stop; key0 += 2 * kKv4Unit) {
-      if (!(ok = mbar_wait(&full[warp][slot], phase, abort_flag))) break;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][slot], phase, abort_flag)))) break;
       const uint8_t* unit = ring + slot * 2 * kUnit;
       float sc[2][NT][4];
       uint32_t pt[2][NT][2];
