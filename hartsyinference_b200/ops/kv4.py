@@ -228,11 +228,12 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
         if kernel == 2:                                  # few queries behind a long cache
             need = L.b200_attn_few_kv4_workspace(seqs, most, hq, hkv, d, longest)
             ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-            rc = min(0, L.b200_attn_few_kv4(*ptrs, *sizes, longest, window, scale, float(softcap), N.ptr(ws), need, status, N.stream()))
+            rc = L.b200_attn_few_kv4(*ptrs, *sizes, longest, window, scale, float(softcap), N.ptr(ws), need, status, N.stream())
+            N.check(min(rc, 0), "b200_attn_few_kv4", rc)
         else:
             run = L.b200_attn_prefill_kv4 if kernel else L.b200_attn_kv4
             rc = run(*ptrs, *sizes, int(causal), window, scale, float(softcap), status, N.stream())
-        N.check(rc, "b200_attn_prefill_kv4")
+            N.check(rc, "b200_attn_prefill_kv4")
     return out
 
 

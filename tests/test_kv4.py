@@ -654,3 +654,19 @@ def test_tables_whose_units_leave_32_bits_are_refused():
         assert [f(c, 1 << 23) for c in (16, 17, 20, 24, 25, 32)] == [-5, -3, -3, -3, -5, -5]          # -5: the sizes are taken, no workspace is there
         assert [f(c, 1 << 22) for c in (16, 17, 20, 24, 25, 32)] == [-5] * 6
         assert [f(c, 1 << 24) for c in (16, 17, 20, 24, 25, 32)] == [-5] + [-3] * 5
+
+
+@gpu
+def test_launches_are_counted():
+    """A decode call and a few queries behind a long cache are two kernels each, a call of the other kernels one."""
+    from hartsyinference_b200.ops import _native as N
+    lens = [4000, 3000]
+    cache, table = _filled(lens, 8, 128, 16)
+    q, c, t, n, cu = _cuda(_normal(10, 32, 128).to(torch.bfloat16), cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor([0, 5, 10], dtype=torch.int32))
+    assert N.lib().b200_attn_kv4_choice(2, 5, table.shape[1] * 16, 32, 8, 128, 1, 0, 128 ** -0.5) == 2
+    for call, launches in ((lambda: ops.attn_prefill_kv4(q, c, t, n, cu, 5), 2), (lambda: ops.attn_decode_kv4(q[:2], c, t, n), 2),
+                           (lambda: ops.attn_prefill_kv4(q, c, t, n, cu, 5, causal=False), 1), (lambda: ops.attn_decode_kv4(q[:2], c, t[:, :4], n.clamp(max=64)), 1)):
+        before = N.launch_count
+        call()
+        assert N.launch_count - before == launches
+    N.check_status()
