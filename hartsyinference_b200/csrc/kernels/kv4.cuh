@@ -61,6 +61,13 @@ __device__ __forceinline__ int kv4_length(const Kv4Pool& p, int len, uint32_t ke
 // 2^31 must not be taken off.
 __device__ __forceinline__ int kv4_window_start(int end, int window) { return end > window ? end - window : 0; }
 
+// Exponent of a capped score, cut where exp2 would overflow. A NaN stays one, which fminf would turn into the cut.
+__device__ __forceinline__ float kv4_cut(float x) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(126.f));
+  return y;
+}
+
 // ---- numbers to bytes ---------------------------------------------------------------------------
 // Scale byte of a block whose largest magnitude is amax, and the scale.
 __device__ __forceinline__ uint32_t kv4_scale(float amax, int exp, float& s) {

@@ -35,7 +35,7 @@ __device__ __forceinline__ float kv4_exp2(float x) {
 // Score in log2 units. cap tanh(x) = cap - 2 cap / (exp(2 x) + 1)
 __device__ __forceinline__ float kv4_score(const AttnKv4Params& p, float s) {
   if (p.cap_out == 0.f) return s * p.scale_log2;
-  const float e = kv4_exp2(fminf(s * p.cap_in, 126.f));
+  const float e = kv4_exp2(kv4_cut(s * p.cap_in));
   return p.cap_out - __fdividef(2.f * p.cap_out, e + 1.f);
 }
 

@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kDec4Threads, NT == 1 ? 2 : 1) attn_decode_kv4
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sc[u][t][j] = p.cap_out - __fdividef(2.f * p.cap_out, dec4_exp2(fminf(sc[u][t][j], 126.f)) + 1.f);
+            for (int j = 0; j < 4; ++j) sc[u][t][j] = p.cap_out - __fdividef(2.f * p.cap_out, dec4_exp2(kv4_cut(sc[u][t][j])) + 1.f);
       }
       // keys below 0 are a pair's first unit where that is the list's before this one
       if (key0 < start || key0 + 2 * kKv4Unit > last)

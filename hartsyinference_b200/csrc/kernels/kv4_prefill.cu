@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kPf4Threads, 1) attn_prefill_kv4_kernel(const 
         if (kCap)
 #pragma unroll
           for (int i = 0; i < kPf4Sub; ++i)               // cap tanh(x) = cap - 2 cap / (exp(2 x) + 1)
-            r[i] = __float_as_uint(p.cap_out - __fdividef(2.f * p.cap_out, pf4_exp2(fminf(__uint_as_float(r[i]) * p.cap_in, 126.f)) + 1.f));
+            r[i] = __float_as_uint(p.cap_out - __fdividef(2.f * p.cap_out, pf4_exp2(kv4_cut(__uint_as_float(r[i]) * p.cap_in)) + 1.f));
         if (key0 < open_from || key0 + kPf4Sub > open_to) {
           const int from = start - key0, to = lim - key0;
 #pragma unroll

@@ -670,3 +670,36 @@ def test_launches_are_counted():
         call()
         assert N.launch_count - before == launches
     N.check_status()
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 1, 128)])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_queries_that_are_no_numbers(hq, hkv, d, softcap):
+    """A NaN in a head's query makes that row NaN and no other, capped or not, in every kernel."""
+    from hartsyinference_b200.ops import _native as N
+    L, lens, each = N.lib(), [900, 40, 600], [3, 40, 1]
+    cache, table = _filled(lens, hkv, d, 16)
+    cuts = torch.tensor([0, *each]).cumsum(0).tolist()
+    q = _normal(sum(each), hq, d, seed=9).to(torch.bfloat16)
+    want = _plain(q, cache, table, lens, cuts, softcap=softcap)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool)
+    bad[0, 1] = bad[20, hq - 1] = bad[-1, 0] = True
+    q[..., 5] = torch.where(bad, math.nan, q[..., 5])
+    qd, c, t, n, cu = _cuda(q, cache, table, torch.tensor(lens, dtype=torch.int32), torch.tensor(cuts, dtype=torch.int32))
+
+    def right(out, rows=slice(None)):
+        no = bad[rows]
+        assert out.cpu()[no].isnan().all()
+        _close(out[~no.cuda()], *(x[rows][~no] for x in want))
+
+    right(_few(qd, c, t, n, cu, max(each), 900, softcap=softcap))
+    for run in (L.b200_attn_kv4, L.b200_attn_prefill_kv4):
+        out = torch.full_like(qd, 7)
+        assert run(qd.data_ptr(), c.data_ptr(), out.data_ptr(), t.data_ptr(), n.data_ptr(), cu.data_ptr(), len(lens), max(each), hq, hkv, d, 16, t.shape[1],
+                   c.shape[0], 1, 0, 1 / math.sqrt(d), softcap, N.state(qd.device).status.data_ptr(), N.stream()) == 0
+        right(out)
+    last = [x - 1 for x in cuts[1:]]
+    right(ops.attn_decode_kv4(qd[last], c, t, n, softcap=softcap), last)
+    short = ops.attn_decode_kv4(qd[[20]], c, t[1:2, :3], n[1:2], softcap=softcap)
+    assert short[0, hq - 1].isnan().all() and torch.isfinite(short[0, :hq - 1]).all()
