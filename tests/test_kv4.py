@@ -703,3 +703,22 @@ def test_queries_that_are_no_numbers(hq, hkv, d, softcap):
     right(ops.attn_decode_kv4(qd[last], c, t, n, softcap=softcap), last)
     short = ops.attn_decode_kv4(qd[[20]], c, t[1:2, :3], n[1:2], softcap=softcap)
     assert short[0, hq - 1].isnan().all() and torch.isfinite(short[0, :hq - 1]).all()
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128)])
+def test_decode_into_fp8(dev, hq, hkv, d):
+    """The quantised result is that of the bf16 one, for one kernel and for shares."""
+    lens = [40, 0, 900]
+    cache, table = _filled(lens, hkv, d, 16)
+    q = _normal(3, hq, d, seed=2).to(torch.bfloat16).to(dev)
+    args = [x.to(dev) for x in (cache, table, torch.tensor(lens, dtype=torch.int32))]
+    for n, cut in ((3, slice(None)), (2, slice(0, 4))):
+        a = (q[:n], args[0], args[1][:n, cut], args[2][:n])
+        want = ops.attn_decode_kv4(*a)
+        out, act = ops.attn_decode_kv4(*a, emit_fp8=True)
+        none, only = ops.attn_decode_kv4(*a, emit_fp8=True, emit_bf16=False)
+        held = ops.quant_fp8_act(want.reshape(n, hq * d))
+        assert torch.equal(out, want) and none is None
+        for x in (act, only):
+            assert torch.equal(x.data.view(torch.uint8), held.data.view(torch.uint8)) and torch.equal(x.scales_fp32(), held.scales_fp32())
