@@ -4,7 +4,8 @@
 // fastest: row r is query r / G, head r % G. A tile of 64 keys is turned into bf16 in shared memory once for all of them: one row of
 // keys or values per thread, whose bytes of the next tile are in flight during the products of this one.
 //
-// Products are mma.sync m16n8k16; softmax is the usual one pass with a running maximum, in 32 bits. Bound by how long a block of four warps
+// Products are mma.sync m16n8k16; softmax is the usual one pass with a running maximum, in 32 bits; probabilities enter
+// the second product in bf16, their sum unrounded. Bound by how long a block of four warps
 // takes for a key (26 ns with heads of 128, 18 with 64, whatever else runs until a processor has several blocks): a block starts in
 // 3 us, so short prompts come here (five prompts of about 97 tokens: 5.9 us; 100 queries 7.1, where the blocks of 256 rows take 11.4).
 #include "kv4.cuh"

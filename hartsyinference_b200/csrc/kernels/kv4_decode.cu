@@ -10,15 +10,17 @@
 //   O^T (values x heads) = V^T P^T A = 128 + codes of 16 values of 16 keys (four bits in the mantissa of a bf16 128), B = P^T times the
 //                                  keys' scales of that block. The offset is a second product with a constant matrix of -136.
 //                                  In bf16, since probabilities times scales have no bound from below: a first token that takes nearly
-//                                  all of the weight and has values near zero leaves the rest to probabilities of 2^-24
+//                                  all of the weight and has values near zero leaves the rest to probabilities of 2^-24. A probability is
+//                                  rounded to 8 bits and its product with a scale (4 bits) again; what they are divided by sums unrounded ones
 //
 // P^T is S^T after the softmax with its 8 x 8 blocks transposed (movmatrix). Rows of the tile are not the keys in order: row 2 i is key i and
 // row 2 i + 1 key 7 - i of eight, which lets every shared-memory read of codes touch each bank once.
 //
 // Work: a unit is 16 tokens of one kv head. All units of all sequences and heads in a row are cut into equal shares, one per resident
 // block (or one per unit, where there are fewer of them than blocks), whatever the lengths; a share's first and last sequence may be
-// other blocks' too, whose parts the second kernel joins (in the order of the blocks, so results do not depend on timing). Within a share every warp takes units side by side and has its own ring of
-// bulk copies, so warps meet only at the end. Short sequences get one block each and no second kernel.
+// other blocks' too, whose parts the second kernel joins (in the order of the blocks, so results do not depend on timing). Within a
+// share every warp takes units side by side and has its own ring of bulk copies, so warps meet only at the end. Short sequences get one
+// block each and no second kernel.
 #include "kv4.cuh"
 #include "mma_sync.cuh"
 

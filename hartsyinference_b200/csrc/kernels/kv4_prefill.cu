@@ -3,7 +3,8 @@
 // The query heads of a group read the same keys, so rows are (query, head of the group) pairs of one sequence and one kv head, heads fastest: row
 // r is query r / G, head r % G. A block owns two tiles of 128 rows and walks the keys that they see in tiles of 128:
 //   warps 0, 1    a thread each issues the tcgen05.mma of a row tile; TMEM holds S0 | S1 | O0 | O1 (128 columns each, of which heads of 64
-//                 use half in O0 and O1). S is made in halves of 64 keys, two ahead of the softmax, P is written over S and read from there
+//                 use half in O0 and O1). S is made in halves of 64 keys, two ahead of the softmax, P is written over S
+//                 (in bf16; the sums that the result is divided by are of unrounded ones) and read from there
 //   warps 4..11   softmax of tile 0 and 1, one row per thread, 64 keys a step: the maximum is raised only where it grows by more than 2^8;
 //                 steps that the diagonal, a window or the last key crosses are masked before it. Before the first they bring the rows of Q
 //   warps 12..15  a thread per key: its row of codes and scales (68 bytes for a head of 128; the next tile's are in flight) becomes bf16 values of

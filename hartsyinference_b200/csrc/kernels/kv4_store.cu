@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(256, kRope4Blocks) rope_kv4_kernel(const RopeK
 
 // Four lanes per (token, head): each reads the row's codes whole (16-byte words hold a value of every block, so the lanes take the same
 // addresses) and writes every fourth piece of eight values, so that the four write 64 bytes side by side. Two scattered
-// 4-byte words a lane and a piece a thread took 118 us where this takes 75 (33000 tokens of 8 heads; 57 at the rate of a plain copy).
+// 4-byte words a lane and a piece a thread took 118 us where this takes 75 (33000 tokens of 8 heads; 58 at the rate of a plain copy).
 template <int D>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(const Kv4Pool p, const int* __restrict__ cu_kv, int seqs, int total,
                                                          __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v) {

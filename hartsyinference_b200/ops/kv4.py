@@ -204,7 +204,7 @@ def attn_prefill_kv4(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
                      max_kv_len: Optional[int] = None) -> torch.Tensor:
     """Variable-length (chunked) attention over a 4-bit pool: q [total_q, hq, d] packed by ``cu_q`` int32 [S + 1], the keys of sequence s are
     its first ``kv_lens[s]`` tokens, the last of them its last query's own. No sequence has more queries than ``max_q_len``; ``max_kv_len``
-    only chooses between two kernels. A query without keys gives zeros; rows behind the last sequence's are undefined. Arguments as of :func:`.core.attn_prefill_paged`."""
+    (as of :func:`attn_decode_kv4`) only chooses between three kernels. A query without keys gives zeros; rows behind the last sequence's are undefined. Arguments as of :func:`.core.attn_prefill_paged`."""
     block_table, kv_lens, pages, hkv, page = _attention_args("attn_prefill_kv4", q, cache, block_table, kv_lens)
     if cu_q.numel() != kv_lens.numel() + 1:
         raise ValueError("attn_prefill_kv4: cu_q [S + 1]")
