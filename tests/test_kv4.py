@@ -722,3 +722,28 @@ def test_decode_into_fp8(dev, hq, hkv, d):
         assert torch.equal(out, want) and none is None
         for x in (act, only):
             assert torch.equal(x.data.view(torch.uint8), held.data.view(torch.uint8)) and torch.equal(x.scales_fp32(), held.scales_fp32())
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_probabilities_are_rounded_once(d):
+    """Two keys, the first with score 0 and a value of zero, the second with a probability of nearly half a step between two bf16: the result differs from
+    7 s p / (1 + p) by the rounding of p, at most 2^-8 of it, and its own, 2^-8 again; 2^-12 covers their product (2^-16) and sums and exponentials in 32
+    bits. s are scales of every mantissa. A rounding of p s as well would be off by up to 2.5 times 2^-8 here."""
+    hkv = 512 // d                                                     # 16 blocks of 32 values: every mantissa twice
+    scales = (torch.arange(16) % 8 + 8) / 8.0
+    v = torch.zeros(2, hkv, d)
+    v[1] = (7 * scales).repeat_interleave(32).view(hkv, d)
+    k = torch.zeros(2, hkv, d)
+    k[1] = -0.875
+    cache, table = ops.kv4_cache(1, hkv, 16, d, "cpu"), torch.zeros(1, 1, dtype=torch.int32)
+    R.kv4_store(cache, torch.arange(2), k, v)
+    assert all(torch.equal(a, b) for a, b in zip(R.kv4_sequence(cache, table[0], 2), (k, v)))
+    c, t, n = _cuda(cache, table, torch.tensor([2], dtype=torch.int32))
+    q = torch.ones(1, hkv, d, dtype=torch.bfloat16, device="cuda")
+    for j in range(128):
+        for part in (-0.49, 0.49):
+            p = (128 + j + part) / 256
+            want = v[1].double() * p / (1 + p)
+            got = ops.attn_decode_kv4(q, c, t, n, scale=-math.log(p) / (0.875 * d))[0].double().cpu()
+            assert ((got - want).abs() <= (2.0 ** -7 + 2.0 ** -12) * want).all(), (j, part)
