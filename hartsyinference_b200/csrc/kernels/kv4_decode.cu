@@ -730,9 +730,9 @@ static int dec4_blocks(int seqs, int heads_v, int chunk_heads, int max_kv_len) {
   const long long room = (chunk_heads > 8 ? 1ll : 2ll) * num_sms(), shares = (pairs * units + 2 * kDec4Warps - 1) / (2 * kDec4Warps);
   return static_cast<int>(shares < room ? shares : room);
 }
-// Sixteen columns at a time take one block of a processor, eight two: a walk of eight costs 0.65 of one of sixteen, so three replace two. 20
-// columns behind 16 times 3000 keys 54 us (57 with two of ten), 128 sequences of 6000 tokens and 20 heads over one 56 (64) with
-// heads of 64 and 92 (90) with 128, eight of 100 tokens 6.9 (8.9).
+// Sixteen columns at a time take one block of a processor, eight two: a walk of eight costs 0.6 to 0.7 of one of sixteen, so three replace two. 20
+// columns behind 16 times 3000 keys 55.5 us (55.0 with two of ten), with heads of 64 36.7 (41.8); 128 sequences of 6000 tokens and 20 heads over
+// one 57 (62) with heads of 64 and 90 (86) with 128; 64 of 3000 34 (36); eight of 100 tokens 7.2 (9.0).
 static void dec4_chunks(int columns, int& chunks, int& heads) {
   chunks = columns > 16 && columns <= 24 ? 3 : (columns + 15) / 16;
   heads = (columns + chunks - 1) / chunks;
