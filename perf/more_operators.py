@@ -359,12 +359,12 @@ def run(state):
                                        want_kv=state["slots"] is None)
             return (q, k, v) if state["slots"] is None else (q, state["k_cache"], state["v_cache"])
         step = c["queries"] == 1
-        cuts = (None, 1) if step else (state["cu_q"], state["most"])
+        cu_q = None if step else state["cu_q"]
         if c["kind"] == "pick":
-            ops.key_bounds_(state["bounds"], state["k_cache"], state["table"], state["kv_lens"], *cuts)
-            return ops.pick_pages(state["q"], state["bounds"], state["table"], state["kv_lens"], *cuts, page=c["page"], top=c["top"], first=c["first"], last=c["last"],
+            ops.key_bounds_(state["bounds"], state["k_cache"], state["table"], state["kv_lens"], cu_q, state["most"])
+            return ops.pick_pages(state["q"], state["bounds"], state["table"], state["kv_lens"], cu_q, page=c["page"], top=c["top"], first=c["first"], last=c["last"],
                                   run=c["run"]), state["bounds"]
-        return ops.attn_picked(state["q"], state["k_cache"], state["v_cache"], state["table"], state["kv_lens"], state["picked"], *cuts, run=c["run"], softcap=c["softcap"])
+        return ops.attn_picked(state["q"], state["k_cache"], state["v_cache"], state["table"], state["kv_lens"], state["picked"], cu_q, run=c["run"], softcap=c["softcap"])
     return {"axes": _axes, "pick": _pick, "attend": _attend}[c["kind"]](state)
 
 
