@@ -46,6 +46,8 @@ enum KernelId : uint32_t {
   kKernelWaitProbe = 11,
   kKernelDpExchange = 12,
   kKernelKv4 = 13,
+  kKernelRopeAxes = 14,
+  kKernelPicked = 15,
 };
 
 struct DeviceStatus {

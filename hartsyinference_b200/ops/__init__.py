@@ -60,6 +60,7 @@ from .core import (  # noqa: F401
     sample_tokens,
     selective_scan,
 )
+from .axes import rope_axes, rope_axes_kv  # noqa: F401
 from .kv4 import attn_biased_kv4, attn_decode_kv4, attn_prefill_kv4, kv4_cache, kv4_gather, rope_kv4  # noqa: F401
 from .mixers import (  # noqa: F401
     ChannelScanWeights,
@@ -95,6 +96,7 @@ from .mixers import (  # noqa: F401
     short_conv,
     side_gate,
 )
+from .picked import attn_picked, key_bounds, key_bounds_, pick_pages  # noqa: F401
 from . import reference  # noqa: F401
 
 
@@ -105,7 +107,7 @@ from . import reference  # noqa: F401
 def _install_ranges() -> None:
     import sys
     from ..utils.profiling import traced
-    from . import core, kv4, mixers
+    from . import axes, core, kv4, mixers, picked
     mod = sys.modules[__name__]
     for name in ("linear", "norm", "glu", "rope_kv", "attn_decode", "attn_prefill_paged", "attn_paged_biased", "attention",
                  "embedding", "argmax", "quant_fp8_act", "grouped_linear", "grouped_linear_dynamic", "moe_route",
@@ -124,6 +126,8 @@ def _install_ranges() -> None:
         setattr(mod, name, traced(name)(getattr(mixers, name)))
     for name in ("attn_biased_kv4", "attn_decode_kv4", "attn_prefill_kv4", "kv4_gather", "rope_kv4"):
         setattr(mod, name, traced(name)(getattr(kv4, name)))
+    for part, name in ((axes, "rope_axes_kv"), (picked, "attn_picked"), (picked, "key_bounds_"), (picked, "pick_pages")):
+        setattr(mod, name, traced(name)(getattr(part, name)))
 
 
 _install_ranges()

@@ -513,6 +513,51 @@ def rope64(qkv: torch.Tensor, positions: torch.Tensor, hq: int, hkv: int, d: int
     return out[0], out[1], x[:, hq + hkv:]
 
 
+def rope_axes(qkv: torch.Tensor, positions: torch.Tensor, hq: int, hkv: int, d: int, axes: torch.Tensor, inv_freq: torch.Tensor, style: int,
+              q_norm_w: Optional[torch.Tensor], k_norm_w: Optional[torch.Tensor], eps: float) -> tuple:
+    """:func:`rope64` with a position on every axis, [A, T]: pair j turns by ``positions[axes[j]] * inv_freq[j]``."""
+    q, k, v = rope64(qkv, positions[0], hq, hkv, d, None, style, q_norm_w, k_norm_w, eps)
+    ang = positions.double()[axes.long()].T * inv_freq.double()
+    table = torch.stack([ang.cos(), ang.sin()], -1).float()
+    return turn(q, table, style == 1), turn(k, table, style == 1), v
+
+
+# --------------------------------------------------------------------------------------------
+# pages that queries choose (ops.picked)
+# --------------------------------------------------------------------------------------------
+def bounds_exponent(top: torch.Tensor) -> torch.Tensor:
+    """The smallest e, from -50 to 50, with top <= 127 * 2^e; int32."""
+    m, x = torch.frexp(torch.where(torch.isinf(top), 2.0 ** 100, top.double()))
+    return torch.where(top > 0, x - 7 + (m * 2 > 127 / 64), -50).clamp(-50, 50).to(torch.int32)
+
+
+def page_bounds(k: torch.Tensor) -> torch.Tensor:
+    """Rows of bounds uint8 [..., 2 d + 16] of the keys [..., page, d] of pages."""
+    k = torch.nan_to_num(k.float(), nan=0.0, posinf=math.inf, neginf=-math.inf)
+    high, low = k.amax(-2), k.amin(-2)
+    e = bounds_exponent(torch.maximum(high.abs(), low.abs()).amax(-1))
+    f = torch.exp2(-e.float())[..., None]
+    codes = torch.cat([torch.ceil(high * f), torch.floor(low * f)], -1).clamp(-127, 127).to(torch.int8).view(torch.uint8)
+    tail = torch.zeros(*e.shape, 16, dtype=torch.uint8)
+    tail[..., 0] = (e + 64).to(torch.uint8)
+    return torch.cat([codes, tail.to(codes.device)], -1)
+
+
+def page_scores(q: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+    """Scores fp32 [hkv, pages] of pages with bounds ``rows`` [pages, hkv, 2 d + 16] for queries [m, hq, d] that choose together."""
+    m, hq, d = q.shape
+    hkv = rows.shape[1]
+    q = torch.nan_to_num(q.float(), nan=0.0, posinf=math.inf, neginf=-math.inf)
+    e = bounds_exponent(q.abs().amax(-1))
+    a = torch.round(q * torch.exp2(-e.float())[..., None]).clamp(-127, 127).double()
+    high, low = (rows[..., i * d:(i + 1) * d].contiguous().view(torch.int8).double() for i in (0, 1))
+    a = a.reshape(m, hkv, hq // hkv, d)
+    s = torch.einsum("mhgd,phd->mghp", a.clamp(min=0), high) + torch.einsum("mhgd,phd->mghp", a.clamp(max=0), low)
+    s = s * torch.exp2(e.double()).reshape(m, hkv, -1).transpose(1, 2)[..., None]
+    unit = torch.exp2((rows[..., 2 * d].to(torch.int32) - 64).clamp(-50, 50).double()).T
+    return (s.amax((0, 1)) * unit).float()
+
+
 # --------------------------------------------------------------------------------------------
 # diffusion scheduler step
 # --------------------------------------------------------------------------------------------
