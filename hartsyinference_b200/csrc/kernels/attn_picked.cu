@@ -396,6 +396,12 @@ using namespace b200;
 
 constexpr int kPickedWidth = 4096;
 
+// Whether rows of `cols` columns (queries times heads of a group) go through the tensor-core tiles of attn_picked_tc.cu (1) or b200_attn_picked (0).
+B200_API int b200_attn_picked_form(int rows, int cols, int hkv, int page, int width, long long pages, float scale, float softcap) {
+  if (width > 1024 || !(scale > 0.f) || softcap > 0.f || pages * hkv * page >= (1ll << 31)) return 0;
+  return cols >= 48;
+}
+
 // q, out [tokens][hq][d], k, v [pages][hkv][page][d] bf16; picked int32 [rows][hkv][width] (see picked.cuh), rows = (tokens + seqs (run - 1)) / run.
 // Causal; entries below 0 or behind the run's last query are no pages. A page named twice counts twice.
 B200_API int b200_attn_picked(const void* q, const void* k, const void* v, void* out, const int* picked, const int* block_table, const int* kv_lens,

@@ -1296,6 +1296,20 @@ int make_kmajor_map(CUtensorMap* out, const void* base, int elem_bytes, long lon
   return r == CUDA_SUCCESS ? 0 : -static_cast<int>(r) - 100;
 }
 
+// [tokens][heads][d] bf16 in boxes of 64 values of `box_heads` heads of `box_tokens` tokens.
+int make_heads_map(CUtensorMap* out, const void* base, long long tokens, int heads, int d, int box_tokens, int box_heads) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(d) * 2, static_cast<cuuint64_t>(heads) * d * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -static_cast<int>(r) - 100;
+}
+
 int make_sf_map(CUtensorMap* out, const void* base, long long blocks) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return -1;

@@ -189,9 +189,12 @@ def attn_picked(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
             if block_table.shape[1] == 0 or pages == 0:
                 out.zero_()
             elif seqs:
-                rc = N.lib().b200_attn_picked(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), picked.data_ptr(), block_table.data_ptr(),
-                                              kv_lens.data_ptr(), N.ptr(cu_q), seqs, rows, hq, hkv, d, page, block_table.shape[1], pages, run, picked.shape[2],
-                                              scale, float(softcap), N.state(q.device).status.data_ptr(), N.stream())
+                L, status, width = N.lib(), N.state(q.device).status.data_ptr(), picked.shape[2]
+                ptrs = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), picked.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), N.ptr(cu_q))
+                if run > 1 and L.b200_attn_picked_form(rows, run * (hq // hkv), hkv, page, width, pages, scale, softcap):
+                    rc = L.b200_attn_picked_tc(*ptrs, seqs, rows, tokens, hq, hkv, d, page, block_table.shape[1], pages, run, width, scale, status, N.stream())
+                else:
+                    rc = L.b200_attn_picked(*ptrs, seqs, rows, hq, hkv, d, page, block_table.shape[1], pages, run, width, scale, float(softcap), status, N.stream())
                 N.check(rc, "b200_attn_picked")
     if not emit_fp8:
         return out

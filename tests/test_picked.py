@@ -306,10 +306,36 @@ def test_rows_without_pages_and_queries_in_front_of_their_pages_give_zeros(dev):
     assert not got[:7].any() and got[7, :2].any() and not got[7, 2:].any()
 
 
+@gpu
+@pytest.mark.parametrize("each,lens", BATCHES + [([130, 0, 61, 1], [700, 0, 61, 200])])
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+@pytest.mark.parametrize("page,width", [(16, 30), (32, 5), (64, 9), (128, 7), (16, 1000)])
+def test_attention_of_long_runs(each, lens, hq, hkv, d, page, width):
+    """As many tokens a run as it may have: tiles of up to 128 rows."""
+    run = 128 // (hq // hkv)
+    b = Batch(each, lens, hq, hkv, d, page, seed=width)
+    picked = _some(b, run, width)
+    want = _attention(b, picked, run)
+    _close(b.to("cuda").attend(picked.cuda(), run=run), want)
+    N.check_status()
+
+
+@gpu
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 128)])
+def test_rows_of_a_long_run_that_begin_with_pages_they_do_not_see(d, page):
+    """A list that names the run's last page first, one twice, and none between: order does not matter, twice counts twice."""
+    b = Batch([90], [190], 2, 1, d, page)
+    last = 189 // page
+    odd = torch.tensor([last, -1, 0, 0, 5000, last - 1], dtype=torch.int32).expand(2, 1, -1).contiguous()
+    want = _attention(b, odd, 64)
+    _close(b.to("cuda").attend(odd.cuda(), run=64), want)
+
+
 @pytest.mark.parametrize("dev", BOTH)
-def test_values_that_a_query_does_not_see_may_be_anything(dev):
+@pytest.mark.parametrize("hq", [3, 8])
+def test_values_that_a_query_does_not_see_may_be_anything(dev, hq):
     """Infinite and no numbers in a run's own page: they reach the queries that see them and no others."""
-    b = Batch([6], [38], 8, 1, 128, 16)
+    b = Batch([6], [38], hq, 1, 128, 16)
     want, bound = _attention(b, torch.tensor([[[0, 1, 2]]]), 6)
     b.v[b.table[0, 2].long(), 0, 4, 7] = math.inf          # position 36: the last two queries
     b.v[b.table[0, 2].long(), 0, 5, 9] = math.nan          # position 37: the last query
