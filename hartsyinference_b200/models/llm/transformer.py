@@ -138,6 +138,7 @@ class DecoderModel:
         # sliding-window layers of Gemma 3 rotate with their own base and no long-context scaling
         self.inv_freq_local = (build_inv_freq(rot, cfg.rope_local_theta, RopeScaling(), self.device)[0]
                                if cfg.rope_local_theta > 0 else None)
+        self.rope_axes: Optional[torch.Tensor] = None     # axis of every rotary pair (three-axis positions), see _rope_axes
         self.final_norm_b: Optional[torch.Tensor] = None
         self.pos_embed: Optional[torch.Tensor] = None      # learned absolute positions (GPT-2)
         self.embed_norm_w: Optional[torch.Tensor] = None   # LayerNorm on the embedding output (BLOOM)
@@ -706,9 +707,15 @@ class DecoderModel:
         rot = cfg.rotary_dim if cfg.use_rope and not (cfg.nope_global and window == 0) else 0
         if cfg.rope_layers and not cfg.rope_layers[self.layer0 + li]:
             rot = 0
-        if cfg.mrope_section and batch.positions3 is not None and rot > 0:
-            qkv = self._mrope(qkv, batch.positions3, inv_freq)       # rotated here; the kernel below only writes the cache
-            rot = 0
+        three = cfg.mrope_section and batch.positions3 is not None and rot > 0
+        if three and (kv4 is not None or cfg.qk_norm_after_rope):
+            # rotated here (the heads' norm comes first, unless the model has it behind), stored by the op below
+            before = not cfg.qk_norm_after_rope
+            parts = ops.rope_axes_kv(qkv, batch.positions3, self.hq, self.hkv, d, axes=self._rope_axes(inv_freq.numel()), inv_freq=inv_freq, style=cfg.rope_style,
+                                     q_norm_w=q_norm_w if before else None, k_norm_w=k_norm_w if before else None, eps=cfg.rms_eps, want_kv=True)
+            qkv = torch.cat([x.reshape(t, -1) for x in parts], 1)
+            q_norm_w, k_norm_w = (None, None) if before else (q_norm_w, k_norm_w)
+            rot, three = 0, False
         if cfg.qk_norm_after_rope and q_norm_w is not None:
             # rotate first (no cache write), normalise the rotated heads, then run the same kernel with
             # no rotation for the cache write
@@ -721,10 +728,14 @@ class DecoderModel:
             rot = 0
         if kv4 is not None:
             return self._attention_kv4(lw, kv4, qkv, q_norm_w, k_norm_w, rot, inv_freq, batch, scale, window)
-        q, _, _ = ops.rope_kv(qkv, batch.positions, self.hq, self.hkv, d, k_cache=kc, v_cache=vc,
-                              slot_mapping=batch.slot_mapping, rot=rot, theta=cfg.rope_theta,
-                              inv_freq=inv_freq, style=cfg.rope_style, q_norm_w=q_norm_w,
-                              k_norm_w=k_norm_w, eps=cfg.rms_eps)
+        if three:
+            q, _, _ = ops.rope_axes_kv(qkv, batch.positions3, self.hq, self.hkv, d, axes=self._rope_axes(inv_freq.numel()), inv_freq=inv_freq, k_cache=kc, v_cache=vc,
+                                       slot_mapping=batch.slot_mapping if kc is not None else None, style=cfg.rope_style, q_norm_w=q_norm_w, k_norm_w=k_norm_w, eps=cfg.rms_eps)
+        else:
+            q, _, _ = ops.rope_kv(qkv, batch.positions, self.hq, self.hkv, d, k_cache=kc, v_cache=vc,
+                                  slot_mapping=batch.slot_mapping, rot=rot, theta=cfg.rope_theta,
+                                  inv_freq=inv_freq, style=cfg.rope_style, q_norm_w=q_norm_w,
+                                  k_norm_w=k_norm_w, eps=cfg.rms_eps)
         if self.alibi_slopes is not None or lw.sinks is not None:
             att = ops.attn_paged_biased(q, kc, vc, batch.block_table, batch.kv_lens,
                                         None if batch.is_decode else batch.cu_q, scale=scale,
@@ -765,27 +776,14 @@ class DecoderModel:
             att = ops.attn_prefill_kv4(q, cache, batch.block_table, batch.kv_lens, batch.cu_q, batch.max_q_len, max_kv_len=batch.max_kv_len or None, **kw)
         return att.reshape(t, self.hq * d)
 
-    def _mrope(self, qkv: torch.Tensor, positions3: torch.Tensor, inv_freq: torch.Tensor) -> torch.Tensor:
-        """Rotary embedding whose frequency pairs are split into three sections, driven by the time,
-        row and column position of each token (split-half pairing). Rotates q and k inside the
-        packed [T, (hq + 2 hkv) d] activation."""
-        cfg, d = self.cfg, self.cfg.head_dim
-        t = qkv.shape[0]
-        if cfg.mrope_interleaved:         # pair j follows axis j % 3 while that axis has pairs left, else time
-            j = torch.arange(d // 2, device=qkv.device)
-            lim = torch.tensor([0, cfg.mrope_section[1] * 3, cfg.mrope_section[2] * 3], device=qkv.device)
-            axis = torch.where(j < lim[j % 3], j % 3, torch.zeros_like(j))
-        else:
-            axis = torch.repeat_interleave(torch.arange(3, device=qkv.device),
-                                           torch.tensor(cfg.mrope_section, device=qkv.device))      # [d / 2]
-        ang = positions3.to(qkv.device).float()[:, :, None] * inv_freq.float()[None, None, :]        # [3, T, d / 2]
-        ang = ang.gather(0, axis[None, None, :].expand(1, t, -1))[0]                                 # [T, d / 2]
-        cos, sin = ang.cos()[:, None, :], ang.sin()[:, None, :]
-        x = qkv.float().reshape(t, self.hq + 2 * self.hkv, d)
-        nr = self.hq + self.hkv
-        x1, x2 = x[:, :nr, : d // 2], x[:, :nr, d // 2:]
-        rotd = torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin], -1)
-        return torch.cat([rotd, x[:, nr:]], 1).reshape(t, -1).to(qkv.dtype).contiguous()
+    def _rope_axes(self, pairs: int) -> torch.Tensor:
+        """The axis that turns every rotary pair (time, row, column), made once."""
+        if self.rope_axes is None or self.rope_axes.numel() != pairs:
+            sections = self.cfg.mrope_section
+            if self.cfg.mrope_interleaved:
+                sections = (pairs - sum(sections[1:]), *sections[1:])
+            self.rope_axes = ops.rope_axes(sections, self.cfg.mrope_interleaved, self.device)
+        return self.rope_axes
 
     def _block_norm(self, x: torch.Tensor, w: Optional[torch.Tensor], b: Optional[torch.Tensor]) -> torch.Tensor:
         cfg = self.cfg

@@ -24,6 +24,8 @@ from typing import Callable, Optional, Sequence
 import torch
 import torch.nn.functional as F
 
+from ... import ops
+
 
 @dataclass(frozen=True)
 class QwenVisionConfig:
@@ -64,6 +66,23 @@ def merge_block_coords(gh: int, gw: int, merge: int) -> tuple[torch.Tensor, torc
     rows = torch.arange(gh)[:, None].expand(gh, gw).reshape(gh // merge, merge, gw // merge, merge).permute(0, 2, 1, 3).flatten()
     cols = torch.arange(gw)[None, :].expand(gh, gw).reshape(gh // merge, merge, gw // merge, merge).permute(0, 2, 1, 3).flatten()
     return rows, cols
+
+
+class _Turns:
+    """The 2-D rotation of a tower's patches: rows turn the first half of the pairs, columns the second."""
+
+    def __init__(self, rows: torch.Tensor, cols: torch.Tensor, inv_freq: torch.Tensor, device: torch.device):
+        self.positions = torch.stack([rows, cols]).to(torch.int32).to(device)
+        self.axes = ops.rope_axes((inv_freq.numel(),) * 2, device=device)
+        self.inv_freq = torch.cat([inv_freq, inv_freq]).to(device)
+
+    def __call__(self, qkv: torch.Tensor, heads: int) -> tuple:
+        """q, k, v [n, heads, d] of packed rows [n, 3 heads d]; 32-bit towers on a device turn by tensor ops."""
+        d = qkv.shape[1] // (3 * heads)
+        if qkv.is_cuda and qkv.dtype != torch.bfloat16:
+            q, k, v = ops.reference.rope_axes(qkv, self.positions, heads, heads, d, self.axes, self.inv_freq, 0, None, None, 0.0)
+            return q.to(qkv.dtype), k.to(qkv.dtype), v.to(qkv.dtype)
+        return ops.rope_axes_kv(qkv, self.positions, heads, heads, d, axes=self.axes, inv_freq=self.inv_freq, want_kv=True)
 
 
 def patchify(image: torch.Tensor, cfg, max_pixels: int = 1280 * 28 * 28) -> tuple[torch.Tensor, int, int]:
@@ -107,18 +126,10 @@ class _Block:
         self.up_w, self.up_b = t(p + "mlp.up_proj.weight"), t(p + "mlp.up_proj.bias")
         self.down_w, self.down_b = t(p + "mlp.down_proj.weight"), t(p + "mlp.down_proj.bias")
 
-    def __call__(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, mask: Optional[torch.Tensor], heads: int, eps: float):
+    def __call__(self, x: torch.Tensor, turns: _Turns, mask: Optional[torch.Tensor], heads: int, eps: float):
         n, c = x.shape
-        d = c // heads
-        q, k, v = F.linear(_norm(x, self.n1, self.n1_b, eps), self.qkv_w, self.qkv_b).reshape(n, 3, heads, d).unbind(1)
-
-        def rot(u):
-            uf = u.float()
-            u1, u2 = uf[..., : d // 2], uf[..., d // 2:]
-            return (uf * cos[:, None] + torch.cat([-u2, u1], -1) * sin[:, None]).to(u.dtype)
-
-        a = F.scaled_dot_product_attention(rot(q).transpose(0, 1)[None], rot(k).transpose(0, 1)[None], v.transpose(0, 1)[None],
-                                           attn_mask=mask)[0]
+        q, k, v = turns(F.linear(_norm(x, self.n1, self.n1_b, eps), self.qkv_w, self.qkv_b), heads)
+        a = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.transpose(0, 1)[None], v.transpose(0, 1)[None], attn_mask=mask)[0]
         x = x + F.linear(a.transpose(0, 1).reshape(n, c), self.proj_w, self.proj_b)
         h = _norm(x, self.n2, self.n2_b, eps)
         if self.legacy:
@@ -152,16 +163,14 @@ class QwenVisionTower:
         cfg = self.cfg
         x = F.linear(patches.to(self.device, self.dtype), self.patch_w)
         rows, cols = merge_block_coords(gh, gw, cfg.merge)
-        fr = torch.cat([rows[:, None].float() * self.inv_freq[None], cols[:, None].float() * self.inv_freq[None]], -1)
-        emb = torch.cat([fr, fr], -1).to(self.device)
-        cos, sin = emb.cos(), emb.sin()
+        turns = _Turns(rows, cols, self.inv_freq, self.device)
         wmask = None
         if cfg.window > 0:
             cells = cfg.window // cfg.merge // cfg.patch                     # window side in merged cells
             win = ((rows // cfg.merge) // cells) * (gw // cfg.merge // cells + 1) + (cols // cfg.merge) // cells
             wmask = (win[:, None] == win[None, :]).to(self.device)
         for i, blk in enumerate(self.blocks):
-            x = blk(x, cos, sin, None if (i in cfg.full_blocks or wmask is None) else wmask, cfg.heads, cfg.eps)
+            x = blk(x, turns, None if (i in cfg.full_blocks or wmask is None) else wmask, cfg.heads, cfg.eps)
         g = cfg.merge * cfg.merge
         y = _norm(x, self.ln_q, self.ln_q_b, cfg.eps).reshape(-1, g * cfg.hidden)
         return F.linear(F.gelu(F.linear(y, self.m0_w, self.m0_b)), self.m2_w, self.m2_b)
@@ -256,21 +265,13 @@ class Qwen3VisionTower:
         cfg = self.cfg
         x = F.linear(patches.to(self.device, self.dtype), self.patch_w, self.patch_b) + self._positions(gh, gw)
         rows, cols = merge_block_coords(gh, gw, cfg.merge)
-        fr = torch.cat([rows[:, None].float() * self.inv_freq[None], cols[:, None].float() * self.inv_freq[None]], -1)
-        emb = torch.cat([fr, fr], -1).to(self.device)
-        cos, sin = emb.cos()[:, None], emb.sin()[:, None]
+        turns = _Turns(rows, cols, self.inv_freq, self.device)
         n, c = x.shape
-        d = c // cfg.heads
         g = cfg.merge * cfg.merge
-
-        def rot(u):
-            uf = u.float()
-            return (uf * cos + torch.cat([-uf[..., d // 2:], uf[..., : d // 2]], -1) * sin).to(u.dtype)
-
         taps = []
         for i, b in enumerate(self.blocks):
-            q, k, v = F.linear(_norm(x, b["n1"], b["n1b"], cfg.eps), b["qkv"], b["qkvb"]).reshape(n, 3, cfg.heads, d).unbind(1)
-            a = F.scaled_dot_product_attention(rot(q).transpose(0, 1)[None], rot(k).transpose(0, 1)[None], v.transpose(0, 1)[None])[0]
+            q, k, v = turns(F.linear(_norm(x, b["n1"], b["n1b"], cfg.eps), b["qkv"], b["qkvb"]), cfg.heads)
+            a = F.scaled_dot_product_attention(q.transpose(0, 1)[None], k.transpose(0, 1)[None], v.transpose(0, 1)[None])[0]
             x = x + F.linear(a.transpose(0, 1).reshape(n, c), b["proj"], b["projb"])
             h = _norm(x, b["n2"], b["n2b"], cfg.eps)
             x = x + F.linear(F.gelu(F.linear(h, b["f1"], b["f1b"]), approximate="tanh"), b["f2"], b["f2b"])
