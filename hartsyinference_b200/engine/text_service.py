@@ -564,7 +564,7 @@ class TextService:
                 n = len(ids)
                 dev = m.device
                 pages = (n + 15) // 16
-                saved, saved_state = m.kv_cache, (getattr(m, "mixer_state", None), getattr(m, "input_state", None))
+                saved, saved_bounds, saved_state = m.kv_cache, getattr(m, "key_bounds", None), (getattr(m, "mixer_state", None), getattr(m, "input_state", None))
                 m.alloc_kv(max(pages, 1), 16)
                 recurrent = getattr(m.cfg, "recurrent", False)
                 if recurrent:
@@ -577,7 +577,7 @@ class TextService:
                                  cu_q=torch.tensor([0, n], dtype=torch.int32, device=dev), max_q_len=n, max_kv_len=n, runs=[(n, n)],
                                  state_slots=torch.zeros(1, dtype=torch.int32, device=dev) if recurrent else None)
                 hid = m.forward_hidden(b)[:, :m.cfg.hidden_size].float().mean(0)
-                m.kv_cache = saved
+                m.kv_cache, m.key_bounds = saved, saved_bounds
                 if recurrent:
                     m.mixer_state, m.input_state = saved_state
                 outs.append(torch.nn.functional.normalize(hid, dim=0).cpu())

@@ -102,7 +102,7 @@ def x_is_cuda(x) -> bool:
 class DecoderModel:
     def __init__(self, cfg: TransformerConfig, device: torch.device | str = "cpu", comm: Optional[Comm] = None,
                  fp8: bool = False, layer_range: Optional[tuple[int, int]] = None, dp_attention: bool = False,
-                 dtype: torch.dtype = torch.bfloat16, kv_dtype: Optional[str] = None):
+                 dtype: torch.dtype = torch.bfloat16, kv_dtype: Optional[str] = None, attn_pages: Optional[int] = None):
         self.cfg = cfg
         # what the cache holds keys and values in: "bf16", or "int4" with a scale of 8 bits per 32 values (ops.kv4)
         self.kv_dtype = config.get("kv_dtype") if kv_dtype is None else kv_dtype
@@ -110,6 +110,13 @@ class DecoderModel:
             raise ValueError(f"KV cache dtype bf16 or int4, got '{self.kv_dtype}'")
         if self.kv_dtype == "int4" and (cfg.mla is not None or cfg.mixed_layers or cfg.head_dim not in (64, 128)):
             raise ValueError(f"{cfg.arch}: a 4-bit KV cache takes plain attention with heads of 64 or 128")
+        # attention over chosen pages of a long cache (ops.picked): how many of the scored ones a query keeps, 0: all of the cache
+        self.attn_pages = config.get("attn_pages") if attn_pages is None else int(attn_pages)
+        if self.attn_pages < 0 or self.attn_pages > ops.picked.WIDTH // 2:
+            raise ValueError(f"attention over 0 (all) to {ops.picked.WIDTH // 2} chosen pages, got {self.attn_pages}")
+        if self.attn_pages and (cfg.mla is not None or cfg.mixed_layers or self.kv_dtype != "bf16" or cfg.head_dim not in (64, 128)):
+            raise ValueError(f"{cfg.arch}: attention over chosen pages takes plain attention over a bf16 cache with heads of 64 or 128")
+        self.key_bounds: Optional[torch.Tensor] = None    # [layers, pages, hkv_local, 2 d + 16], with attn_pages
         # activation dtype: bf16, or fp32 (32-bit products and caches) where the layers have that form
         if dtype != torch.bfloat16 and not (cfg.mixed_layers and dtype == torch.float32):
             raise ValueError(f"{cfg.arch}: activations run in bfloat16")
@@ -595,7 +602,8 @@ class DecoderModel:
             return (self.layer1 - self.layer0) * page * (self.cfg.mla.kv_lora_rank + self.cfg.mla.qk_rope_head_dim) * 2
         if self.kv_dtype == "int4":
             return (self.layer1 - self.layer0) * self.hkv * page * self.cfg.head_dim * 17 // 16
-        return (self.layer1 - self.layer0) * 2 * self.hkv * page * self.cfg.head_dim * 2
+        bounds = (2 * self.cfg.head_dim + 16) if self.attn_pages else 0
+        return (self.layer1 - self.layer0) * self.hkv * (2 * page * self.cfg.head_dim * 2 + bounds)
 
     def alloc_kv(self, num_pages: int, page: int = 16) -> torch.Tensor:
         """[layers, 2, pages, hkv_local, page, head_dim] bf16, or with multi-head latent attention
@@ -617,6 +625,11 @@ class DecoderModel:
             return self.kv_cache
         self.kv_cache = torch.zeros(self.layer1 - self.layer0, 2, num_pages, self.hkv, page, self.cfg.head_dim,
                                     dtype=torch.bfloat16, device=self.device)
+        if self.attn_pages:
+            if page not in (16, 32, 64, 128):
+                raise ValueError(f"attention over chosen pages takes pages of 16, 32, 64 or 128 tokens, got {page}")
+            one = ops.key_bounds(1, self.hkv, self.cfg.head_dim, "cpu")
+            self.key_bounds = torch.zeros(self.layer1 - self.layer0, num_pages, *one.shape[1:], dtype=torch.uint8, device=self.device)
         return self.kv_cache
 
     def alloc_state(self, slots: int) -> None:
@@ -736,6 +749,10 @@ class DecoderModel:
                                   slot_mapping=batch.slot_mapping, rot=rot, theta=cfg.rope_theta,
                                   inv_freq=inv_freq, style=cfg.rope_style, q_norm_w=q_norm_w,
                                   k_norm_w=k_norm_w, eps=cfg.rms_eps)
+        if self._picks_pages(lw, window):
+            att = self._attention_picked(lw, li, q, kc, vc, batch, scale)
+            if att is not None:
+                return att
         if self.alibi_slopes is not None or lw.sinks is not None:
             att = ops.attn_paged_biased(q, kc, vc, batch.block_table, batch.kv_lens,
                                         None if batch.is_decode else batch.cu_q, scale=scale,
@@ -756,6 +773,29 @@ class DecoderModel:
                                          batch.max_q_len, causal=True, scale=scale,
                                          softcap=cfg.attn_softcap, window=window, max_kv_len=batch.max_kv_len or None)
         return att.reshape(t, self.hq * d)
+
+    def _picks_pages(self, lw: LayerWeights, window: int) -> bool:
+        """Whether a layer attends over chosen pages: with ``attn_pages``, where its attention has no window and no biases."""
+        return self.attn_pages > 0 and self.key_bounds is not None and window == 0 and self.alibi_slopes is None and lw.sinks is None
+
+    def _attention_picked(self, lw: LayerWeights, li: int, q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, batch: ForwardBatch, scale: float):
+        """Attention over chosen pages, behind the store of the batch's keys: their pages are bounded, and where some sequence may be longer than what a query
+        keeps (the first page, the two last and ``attn_pages`` between), pages are chosen. None: no sequence is, the whole cache is read."""
+        t, page, group = q.shape[0], kc.shape[2], self.hq // self.hkv
+        cu_q = None if batch.is_decode else batch.cu_q
+        bounds = ops.key_bounds_(self.key_bounds[li], kc, batch.block_table, batch.kv_lens, cu_q, batch.max_q_len)
+        first, last = 1, 2
+        if (batch.max_kv_len or batch.block_table.shape[1] * page) <= (first + last + self.attn_pages) * page or group > 128:
+            return None
+        # tokens of a prompt choose together, as many as fill a tile of 128 rows; a few (drafts to be verified) by themselves, as decoded ones do
+        run = 1
+        if cu_q is not None and batch.max_q_len > 16:
+            run = 1 << (128 // group).bit_length() - 1
+        picked = ops.pick_pages(q, bounds, batch.block_table, batch.kv_lens, cu_q, page=page, top=self.attn_pages, first=first, last=last, run=run)
+        fp8 = batch.is_decode and self.fp8 and q.is_cuda and lw.o is not None and lw.o.is_fp8 and self.cfg.head_dim == 128
+        att = ops.attn_picked(q, kc, vc, batch.block_table, batch.kv_lens, picked, cu_q, run=run, scale=scale, softcap=self.cfg.attn_softcap, emit_fp8=fp8,
+                              emit_bf16=not fp8)
+        return att[1] if fp8 else att.reshape(t, self.hq * self.cfg.head_dim)
 
     def _attention_kv4(self, lw: LayerWeights, cache: torch.Tensor, qkv, q_norm_w, k_norm_w, rot: int, inv_freq: torch.Tensor,
                        batch: ForwardBatch, scale: float, window: int):
@@ -1083,7 +1123,7 @@ class DecoderModel:
         cfg = self.cfg
         if (not x.is_cuda or self.tp > 1 or self.fp8 or cfg.residual_multiplier != 1.0 or cfg.mixed_layers or not (self.first_stage and self.last_stage)
                 or self.alibi_slopes is not None or self.inv_freq_local is not None or batch.slot_mapping is None or self.kv_cache is None
-                or self.kv_dtype != "bf16" or not x.is_contiguous() or batch.positions.dtype != torch.int32 or batch.slot_mapping.dtype != torch.int64
+                or self.kv_dtype != "bf16" or self.attn_pages or not x.is_contiguous() or batch.positions.dtype != torch.int32 or batch.slot_mapping.dtype != torch.int64
                 or self.inv_freq.dtype != torch.float32 or self.kv_cache.dim() != 6 or not self.kv_cache.is_contiguous() or cfg.rotary_dim % 2):
             return False
         rows = (self.hq + 2 * self.hkv) * cfg.head_dim
