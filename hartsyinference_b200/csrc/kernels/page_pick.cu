@@ -90,8 +90,9 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
 }
 
 // ------------------------------------------------------------------------------------------ the choice
-constexpr int kPickThreads = 256, kPickWarps = 8, kPickBins = 256;
+constexpr int kPickThreads = 512, kPickWarps = 16, kPickBins = 2048;
 constexpr int kPickRows = 128;          // queries of a run, heads counted
+constexpr int kPickStep = 16;           // pages that a warp scores at a time
 
 struct PickParams {
   const __nv_bfloat16* q;      // [tokens][hq][D]
@@ -99,18 +100,53 @@ struct PickParams {
   const int *block_table, *kv_lens, *cu_q;
   int* out;                    // [rows][hkv][width]
   long long pages;
-  int seqs, hq, hkv, run, page_shift, max_pages, top, first, last, width, parts, cap;
+  int seqs, hq, hkv, run, page_shift, max_pages, top, first, last, width, parts;
   DeviceStatus* status;
 };
 
 struct PickShared {
-  unsigned hist[2][kPickBins];
-  unsigned meet[2];                 // smallest and largest key of this block
-  unsigned counts[2];               // this block's selected and tied ones
+  unsigned hist[kPickBins];
+  unsigned least[8 * kPickWarps], most[8 * kPickWarps];      // smallest and largest key of every warp of the row's blocks
   unsigned warp_a[kPickWarps], warp_b[kPickWarps];
+  unsigned counts[2];               // this block's selected and tied ones
   unsigned bin, want, in_bin;
-  float2 row[kPickRows];            // 2^e and 0, or 0 and -inf for rows that pad
+  __align__(16) float2 row[kPickRows];      // 2^e and 0, or 0 and -inf for rows that pad
 };
+
+// What a row of runs chooses between: pages first .. first + n are scored, if there are more of them than `top`.
+struct PickRange {
+  RunOfRow run;
+  int n;
+};
+
+// The pages that are kept whatever the scores (written by the block of rank 0); false: nothing is left to choose.
+__device__ __forceinline__ bool pick_range(const PickParams& p, int row, int* out, bool writes, PickRange& x) {
+  x.run = run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)));
+  const int end = x.run.begin + x.run.tokens - 1;
+  if (x.run.tokens <= 0 || end < 0) {
+    if (writes)
+      for (int i = threadIdx.x; i < p.width; i += blockDim.x) out[i] = -1;
+    return false;
+  }
+  const int page0 = max(x.run.begin, 0) >> p.page_shift, page1 = end >> p.page_shift;
+  const int hi = max(p.first, page0 - p.last + 1);
+  x.n = hi - p.first;
+  if (x.n <= p.top) {                                                        // every page is kept
+    if (writes)
+      for (int i = threadIdx.x; i < p.width; i += blockDim.x) out[i] = i <= page1 ? i : -1;
+    return false;
+  }
+  // (from here on first < hi <= page1)
+  if (writes) {
+    const int tail = page1 - hi + 1;
+    for (int i = threadIdx.x; i < p.first; i += blockDim.x) out[i] = i;
+    for (int i = p.first + p.top + threadIdx.x; i < p.width; i += blockDim.x) {
+      const int j = i - p.first - p.top;
+      out[i] = j < tail ? hi + j : -1;
+    }
+  }
+  return p.top > 0;
+}
 
 __device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -129,194 +165,54 @@ __device__ __forceinline__ unsigned pick_peer_load(const void* local, int block)
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(pick_peer(local, block)) : "memory");
   return v;
 }
-
-// Barrier over the blocks of a row.
-__device__ __forceinline__ void pick_sync(int parts) {
-  if (parts > 1) cluster_sync_all();
-  else __syncthreads();
+__device__ __forceinline__ void pick_peer_store(const void* local, int block, unsigned v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(pick_peer(local, block)), "r"(v) : "memory");
 }
 
-// A cluster of `parts` blocks per row of runs and key head; each scores a share of the pages.
-template <int D>
-__global__ void __launch_bounds__(kPickThreads) pick_pages_kernel(const PickParams p) {
-  pdl_wait();
-  pdl_trigger();
-  extern __shared__ __align__(16) uint8_t pick_smem[];
-  PickShared& sh = *reinterpret_cast<PickShared*>(pick_smem);
-  constexpr int kPitch = 2 * D + 64;      // of a query's codes: rows of eight lanes keep apart in the banks
-  uint8_t* codes = pick_smem + (sizeof(PickShared) + 15) / 16 * 16;
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, group = p.hq / p.hkv;
-  const int row = blockIdx.x / p.parts, rank = blockIdx.x % p.parts, h = blockIdx.y;
-  const int tiles = (p.run * group + 15) / 16;
-  float* scores = reinterpret_cast<float*>(codes + tiles * 16 * kPitch);
-  int* out = p.out + (static_cast<long long>(row) * p.hkv + h) * p.width;
-  const RunOfRow r = run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)));
-  const int end = r.begin + r.tokens - 1;
-  if (r.tokens <= 0 || end < 0) {
-    if (rank == 0)
-      for (int i = threadIdx.x; i < p.width; i += kPickThreads) out[i] = -1;
-    return;
-  }
-  const int page0 = max(r.begin, 0) >> p.page_shift, page1 = end >> p.page_shift;
-  const int hi = max(p.first, page0 - p.last + 1), n = hi - p.first;       // pages first .. hi are scored
-  if (n <= p.top) {                                                        // every page is kept
-    if (rank == 0)
-      for (int i = threadIdx.x; i < p.width; i += kPickThreads) out[i] = i <= page1 ? i : -1;
-    return;
-  }
-  // (from here on first < hi <= page1)
-  if (rank == 0) {
-    const int tail = page1 - hi + 1;
-    for (int i = threadIdx.x; i < p.first; i += kPickThreads) out[i] = i;
-    for (int i = p.first + p.top + threadIdx.x; i < p.width; i += kPickThreads) {
-      const int j = i - p.first - p.top;
-      out[i] = j < tail ? hi + j : -1;
-    }
-  }
-  if (p.top == 0) return;
+// Keys order like scores.
+__device__ __forceinline__ unsigned pick_key(float score) {
+  const unsigned u = __float_as_uint(score);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
 
-  // ---- codes of the queries: a+ against the largest values, a- against the smallest
-  for (int i = wid; i < tiles * 16; i += kPickWarps) {
-    constexpr int kEach = D / 32;
-    const bool real = i < r.tokens * group && r.begin + i / group >= 0;
-    float v[kEach], amax = 0.f;
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) v[k] = 0.f;
-    if (real) {
-      const __nv_bfloat16* src = p.q + (static_cast<long long>(r.q_off + i / group) * p.hq + h * group + i % group) * D + lane * kEach;
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        v[k] = __bfloat162float(src[k]);
-        v[k] = v[k] == v[k] ? v[k] : 0.f;
-        amax = fmaxf(amax, fabsf(v[k]));
-      }
-    }
-    const int e = bounds_exponent(warp_max(amax));
-    const float f = bounds_pow2(-e);
-    uint8_t* dst = codes + i * kPitch + lane * kEach;
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      const int a = static_cast<int>(fminf(fmaxf(rintf(v[k] * f), -127.f), 127.f));
-      dst[k] = static_cast<uint8_t>(max(a, 0));
-      dst[D + k] = static_cast<uint8_t>(min(a, 0));
-    }
-    if (lane == 0) sh.row[i] = real ? make_float2(bounds_pow2(e), 0.f) : make_float2(0.f, -INFINITY);
-  }
-  __syncthreads();
-
-  // ---- scores of this block's share
-  const int per = (n + p.parts - 1) / p.parts, a0 = min(n, rank * per), mine = min(n, a0 + per) - a0;
-  const int* ids = p.block_table + static_cast<long long>(r.seq) * p.max_pages + p.first + a0;
-  const int g = lane >> 2, kq = lane & 3;
-  for (int base = wid * 32; base < mine; base += kPickWarps * 32) {
-    // operands: channels are taken in an order of their own, 16 bytes a lane of every 64; sums do not mind
-    uint4 b[4][2 * D / 64];
-    float unit[4];
-#pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
-      const int at = min(base + nb * 8 + g, mine - 1);
-      int id = ids[at];
-      const bool ok = id >= 0 && id < p.pages;
-      if (!ok) {
-        report_status(p.status, kBadArgument, kKernelPicked, 2, static_cast<uint32_t>(r.seq));
-        id = 0;
-      }
-      const uint8_t* src = p.bounds + (static_cast<long long>(id) * p.hkv + h) * (2 * D + kBoundsTail);
-#pragma unroll
-      for (int c = 0; c < 2 * D / 64; ++c) b[nb][c] = __ldg(reinterpret_cast<const uint4*>(src + c * 64 + kq * 16));
-      unit[nb] = ok ? bounds_pow2(min(50, max(-50, static_cast<int>(__ldg(src + 2 * D)) - kBoundsBias))) : 0.f;
-    }
-    float best[4][2];
-#pragma unroll
-    for (int nb = 0; nb < 4; ++nb) best[nb][0] = best[nb][1] = -INFINITY;
-    for (int mt = 0; mt < tiles; ++mt) {
-      int acc[4][4];
-#pragma unroll
-      for (int nb = 0; nb < 4; ++nb) acc[nb][0] = acc[nb][1] = acc[nb][2] = acc[nb][3] = 0;
-      const uint8_t* src = codes + (mt * 16 + g) * kPitch + kq * 16;
-#pragma unroll
-      for (int c = 0; c < 2 * D / 64; ++c) {
-        const uint4 x = *reinterpret_cast<const uint4*>(src + c * 64), y = *reinterpret_cast<const uint4*>(src + 8 * kPitch + c * 64);
-#pragma unroll
-        for (int nb = 0; nb < 4; ++nb) {
-          mma_s8_16832(acc[nb], x.x, y.x, x.y, y.y, b[nb][c].x, b[nb][c].y);
-          mma_s8_16832(acc[nb], x.z, y.z, x.w, y.w, b[nb][c].z, b[nb][c].w);
-        }
-      }
-      const float2 f0 = sh.row[mt * 16 + g], f1 = sh.row[mt * 16 + 8 + g];
-#pragma unroll
-      for (int nb = 0; nb < 4; ++nb)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          best[nb][i] = fmaxf(best[nb][i], fmaxf(fmaf(static_cast<float>(acc[nb][i]), f0.x, f0.y), fmaf(static_cast<float>(acc[nb][2 + i]), f1.x, f1.y)));
-    }
-#pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) best[nb][i] = fmaxf(best[nb][i], __shfl_xor_sync(0xffffffffu, best[nb][i], o));
-      // column g of the tile is with the lanes of quarter g / 2
-      const float x = __shfl_sync(0xffffffffu, best[nb][0], g >> 1), y = __shfl_sync(0xffffffffu, best[nb][1], g >> 1);
-      const int at = base + nb * 8 + g;
-      if (kq == nb && at < mine) scores[at] = unit[nb] > 0.f ? (g & 1 ? y : x) * unit[nb] : -INFINITY;
-    }
-  }
-  __syncthreads();
-
-  // ---- the `top` largest: keys order like scores; digits of 8 bits of what they lie above the smallest
-  const auto key_of = [&](int i) {
-    const unsigned u = __float_as_uint(scores[i]);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-  };
-  unsigned least = 0xffffffffu, most = 0u;
-  for (int i = threadIdx.x; i < mine; i += kPickThreads) {
-    const unsigned k = key_of(i);
-    least = min(least, k);
-    most = max(most, k);
-  }
-  least = __reduce_min_sync(0xffffffffu, least);
-  most = __reduce_max_sync(0xffffffffu, most);
-  if (lane == 0) { sh.warp_a[wid] = least; sh.warp_b[wid] = most; }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kPickWarps; ++w) { least = min(least, sh.warp_a[w]); most = max(most, sh.warp_b[w]); }
-    sh.meet[0] = least;
-    sh.meet[1] = most;
-  }
-  pick_sync(p.parts);
-  if (p.parts > 1) {
-    least = 0xffffffffu;
-    most = 0u;
-    for (int k = 0; k < p.parts; ++k) {
-      least = min(least, pick_peer_load(&sh.meet[0], k));
-      most = max(most, pick_peer_load(&sh.meet[1], k));
-    }
-  } else {
-    least = sh.meet[0];
-    most = sh.meet[1];
-  }
+// The `top` largest of more than `top` scores, of which this block holds the `mine` from number `a0` on, ties to the lowest number: first + number, in order, to
+// out[0 .. top). `least` and `most` bound all keys. Digits of what keys lie above the smallest, as many as it takes: 11 bits where one block holds all
+// scores; 9 in a cluster, whose blocks read one another's counts. All threads of all blocks of the row.
+template <bool kCluster>
+__device__ __forceinline__ void pick_select(PickShared& sh, const float* scores, int mine, int a0, int rank, int parts, int top, unsigned least, unsigned most,
+                                            int first, int* out) {
+  constexpr int kDigit = kCluster ? 9 : 11, kBins = 1 << kDigit, kEach = kBins / kPickThreads;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   int shift = 32 - __clz(static_cast<int>(most - least));        // bits that differ
-  unsigned prefix = 0u, want = static_cast<unsigned>(p.top);
+  unsigned prefix = 0u, want = static_cast<unsigned>(top);
   for (int pass = 0;; ++pass) {
-    const int bits = min(8, shift);
+    const int bits = min(kDigit, shift);
     shift -= bits;
-    unsigned* hist = sh.hist[pass & 1];
-    hist[threadIdx.x] = 0u;                                        // 256 threads, 256 bins
+    unsigned* hist = sh.hist + (kCluster ? (pass & 1) * kBins : 0);      // (a peer may still read those of the pass before)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) hist[i * kPickThreads + threadIdx.x] = 0u;
     __syncthreads();
     for (int i = threadIdx.x; i < mine; i += kPickThreads) {
-      const unsigned k = key_of(i) - least, digit = (k >> shift) & ((1u << bits) - 1u);
-      if ((static_cast<unsigned long long>(k) >> (shift + bits)) == prefix) atomicAdd(hist + digit, 1u);
+      const unsigned k = pick_key(scores[i]) - least;
+      if ((static_cast<unsigned long long>(k) >> (shift + bits)) == prefix) atomicAdd(hist + ((k >> shift) & ((1u << bits) - 1u)), 1u);
     }
-    pick_sync(p.parts);
-    unsigned count = 0;
-    if (p.parts > 1) {
-      for (int k = 0; k < p.parts; ++k) count += pick_peer_load(hist + threadIdx.x, k);
-    } else {
-      count = hist[threadIdx.x];
+    if (kCluster) cluster_sync_all();
+    else __syncthreads();
+    // a thread owns neighbouring bins; how many lie in them and above
+    unsigned own[kEach], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      own[i] = 0;
+      if (kCluster) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < parts) own[i] += pick_peer_load(hist + threadIdx.x * kEach + i, k);
+      } else {
+        own[i] = hist[threadIdx.x * kEach + i];
+      }
+      sum += own[i];
     }
-    // how many lie in this bin and above it
-    unsigned upto = count;
+    unsigned upto = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned x = __shfl_down_sync(0xffffffffu, upto, o);
@@ -325,24 +221,29 @@ __global__ void __launch_bounds__(kPickThreads) pick_pages_kernel(const PickPara
     if (lane == 0) sh.warp_a[wid] = upto;
     __syncthreads();
     for (int w = wid + 1; w < kPickWarps; ++w) upto += sh.warp_a[w];
-    if (upto >= want && upto - count < want) {
-      sh.bin = threadIdx.x;
-      sh.want = want - (upto - count);
-      sh.in_bin = count;
+    unsigned above = upto - sum;
+    if (above < want && upto >= want) {
+#pragma unroll
+      for (int i = kEach - 1; i >= 0; --i) {
+        if (above < want && above + own[i] >= want) {
+          sh.bin = threadIdx.x * kEach + i;
+          sh.want = want - above;
+          sh.in_bin = own[i];
+        }
+        above += own[i];
+      }
     }
     __syncthreads();
     prefix = (prefix << bits) | sh.bin;
     want = sh.want;
-    const bool done = sh.in_bin == want || shift == 0;
-    if (done) break;                     // (the same in every block of the row)
+    if (sh.in_bin == want || shift == 0) break;      // (alike in all blocks)
   }
-
-  // ---- kept: larger prefixes, and the first `want` of the equal ones
+  // kept: larger prefixes, and the first `want` of the equal ones
   const int seg = ((mine + kPickWarps - 1) / kPickWarps + 31) & ~31, s0 = min(mine, wid * seg), s1 = min(mine, s0 + seg);
   unsigned over = 0, tied = 0;
   for (int i0 = s0; i0 < s1; i0 += 32) {
     const int i = i0 + lane;
-    const unsigned k = i < s1 ? (key_of(i) - least) >> shift : 0u;
+    const unsigned k = i < s1 ? (pick_key(scores[i]) - least) >> shift : 0u;
     over += __popc(__ballot_sync(0xffffffffu, i < s1 && k > prefix));
     tied += __popc(__ballot_sync(0xffffffffu, i < s1 && k == prefix));
   }
@@ -350,24 +251,197 @@ __global__ void __launch_bounds__(kPickThreads) pick_pages_kernel(const PickPara
   __syncthreads();
   unsigned over0 = 0, tied0 = 0;
   for (int w = 0; w < wid; ++w) { over0 += sh.warp_a[w]; tied0 += sh.warp_b[w]; }
-  if (threadIdx.x == kPickThreads - 1) { sh.counts[0] = over0 + over; sh.counts[1] = tied0 + tied; }
-  pick_sync(p.parts);
-  if (p.parts > 1)
-    for (int k = 0; k < rank; ++k) {
-      over0 += pick_peer_load(&sh.counts[0], k);
-      tied0 += pick_peer_load(&sh.counts[1], k);
-    }
+  if (kCluster) {
+    if (threadIdx.x == kPickThreads - 1) { sh.counts[0] = over0 + over; sh.counts[1] = tied0 + tied; }
+    cluster_sync_all();
+    unsigned x = 0, y = 0;
+    if (lane < rank) { x = pick_peer_load(&sh.counts[0], lane); y = pick_peer_load(&sh.counts[1], lane); }
+    over0 += __reduce_add_sync(0xffffffffu, x);
+    tied0 += __reduce_add_sync(0xffffffffu, y);
+  }
   for (int i0 = s0; i0 < s1; i0 += 32) {
     const int i = i0 + lane;
-    const unsigned k = i < s1 ? (key_of(i) - least) >> shift : 0u, below = (1u << lane) - 1u;
+    const unsigned k = i < s1 ? (pick_key(scores[i]) - least) >> shift : 0u, below = (1u << lane) - 1u;
     const unsigned more = __ballot_sync(0xffffffffu, i < s1 && k > prefix), same = __ballot_sync(0xffffffffu, i < s1 && k == prefix);
     const unsigned o = over0 + __popc(more & below), t = tied0 + __popc(same & below);
     const bool kept = (more >> lane & 1u) || ((same >> lane & 1u) && t < want);
-    if (kept) out[p.first + o + min(t, want)] = p.first + a0 + i;
+    if (kept) out[o + min(t, want)] = first + a0 + i;
     over0 += __popc(more);
     tied0 += __popc(same);
   }
-  if (p.parts > 1) cluster_sync_all();     // nobody leaves while a peer may still read its words
+}
+
+// A cluster of `parts` blocks per row of runs and key head; each scores a share of the pages, a warp 16 at a time. Pages are rows of the product
+// and queries (with their heads) its columns, eight a tile: groups of up to eight heads fill one, and the maximum over them is two exchanges. The bounds of the
+// next 16 pages are on their way into registers while some are multiplied. One token of 16 sequences of 2000 to 6000 tokens: 16.8 us with queries as
+// rows, 256 threads and digits of 8 bits.
+template <int D>
+__global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickParams p) {
+  pdl_wait();
+  pdl_trigger();
+  extern __shared__ __align__(16) uint8_t pick_smem[];
+  PickShared& sh = *reinterpret_cast<PickShared*>(pick_smem);
+  constexpr int kPitch = 2 * D + 64;      // of a query's codes: rows of eight lanes keep apart in the banks
+  constexpr int kC = 2 * D / 64, kRow = 2 * D + kBoundsTail;
+  uint8_t* codes = pick_smem + (sizeof(PickShared) + 15) / 16 * 16;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, group = p.hq / p.hkv;
+  const int row = blockIdx.x / p.parts, rank = blockIdx.x % p.parts, h = blockIdx.y;
+  const int tiles = (p.run * group + 7) / 8;
+  float* scores = reinterpret_cast<float*>(codes + tiles * 8 * kPitch);
+  int* out = p.out + (static_cast<long long>(row) * p.hkv + h) * p.width;
+  PickRange x;
+  if (!pick_range(p, row, out, rank == 0, x)) return;            // (alike in all blocks of a cluster)
+  const RunOfRow& r = x.run;
+
+  // ---- the first bounds on their way
+  const int per = (x.n + p.parts - 1) / p.parts, a0 = min(x.n, rank * per), mine = min(x.n, a0 + per) - a0;
+  const int* ids = p.block_table + static_cast<long long>(r.seq) * p.max_pages + p.first + a0;
+  const int g = lane >> 2, kq = lane & 3;
+  constexpr int kAll = kPickWarps * kPickStep;
+  // of pages g and g + 8 of a step; channels are taken in an order of their own, 16 bytes a lane of every 64: sums do not mind
+  int id[2];
+  const auto load_ids = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) id[i] = ids[min(base + i * 8 + g, mine - 1)];
+  };
+  const auto load_bounds = [&](uint4 (&to)[2][kC], float (&u)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool ok = id[i] >= 0 && id[i] < p.pages;
+      if (!ok) report_status(p.status, kBadArgument, kKernelPicked, 2, static_cast<uint32_t>(r.seq));
+      const uint8_t* src = p.bounds + (static_cast<long long>(ok ? id[i] : 0) * p.hkv + h) * kRow;
+#pragma unroll
+      for (int c = 0; c < kC; ++c) to[i][c] = __ldg(reinterpret_cast<const uint4*>(src + c * 64 + kq * 16));
+      u[i] = ok ? bounds_pow2(min(50, max(-50, static_cast<int>(__ldg(src + 2 * D)) - kBoundsBias))) : 0.f;
+    }
+  };
+  uint4 a[2][kC];
+  float unit[2];
+  int base = wid * kPickStep;
+  if (base < mine) {
+    load_ids(base);
+    load_bounds(a, unit);
+    load_ids(base + kAll);
+  }
+
+  // ---- codes of the queries: a+ against the largest values, a- against the smallest
+  for (int i = wid; i < tiles * 8; i += kPickWarps) {
+    constexpr int kEach = D / 32;
+    const bool real = i < r.tokens * group && r.begin + i / group >= 0;
+    float v[kEach], amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) v[k] = 0.f;
+    if (real) {
+      const __nv_bfloat16* src = p.q + (static_cast<long long>(r.q_off + i / group) * p.hq + h * group + i % group) * D + lane * kEach;
+#pragma unroll
+      for (int k = 0; k < kEach; k += 2) {
+        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + k));
+        v[k] = f.x == f.x ? f.x : 0.f;
+        v[k + 1] = f.y == f.y ? f.y : 0.f;
+        amax = fmaxf(amax, fmaxf(fabsf(v[k]), fabsf(v[k + 1])));
+      }
+    }
+    const int e = bounds_exponent(warp_max(amax));
+    const float f = bounds_pow2(-e);
+    uint32_t up = 0, down = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int c = static_cast<int>(fminf(fmaxf(rintf(v[k] * f), -127.f), 127.f));
+      up |= static_cast<uint32_t>(max(c, 0)) << (8 * k);
+      down |= (static_cast<uint32_t>(min(c, 0)) & 0xffu) << (8 * k);
+    }
+    uint8_t* dst = codes + i * kPitch + lane * kEach;
+    if (kEach == 4) {
+      *reinterpret_cast<uint32_t*>(dst) = up;
+      *reinterpret_cast<uint32_t*>(dst + D) = down;
+    } else {
+      *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(up);
+      *reinterpret_cast<uint16_t*>(dst + D) = static_cast<uint16_t>(down);
+    }
+    if (lane == 0) sh.row[i] = real ? make_float2(bounds_pow2(e), 0.f) : make_float2(0.f, -INFINITY);
+  }
+  if (p.parts > 1) cluster_sync_all();          // (the peers' memory is there)
+  else __syncthreads();
+
+  // ---- scores of this block's share
+  unsigned least = 0xffffffffu, most = 0u;
+  for (; base < mine; base += kAll) {
+    uint4 next[2][kC];
+    float next_unit[2];
+    if (base + kAll < mine) {
+      load_bounds(next, next_unit);
+      load_ids(base + 2 * kAll);
+    }
+    float best[2] = {-INFINITY, -INFINITY};
+    for (int t = 0; t < tiles; ++t) {
+      int acc[2][4];                           // even and odd halves of the channels
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[0][i] = acc[1][i] = 0;
+      const uint8_t* src = codes + (t * 8 + g) * kPitch + kq * 16;
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        const uint4 b = *reinterpret_cast<const uint4*>(src + c * 64);
+        mma_s8_16832(acc[0], a[0][c].x, a[1][c].x, a[0][c].y, a[1][c].y, b.x, b.y);
+        mma_s8_16832(acc[1], a[0][c].z, a[1][c].z, a[0][c].w, a[1][c].w, b.z, b.w);
+      }
+      const float4 f = *reinterpret_cast<const float4*>(sh.row + t * 8 + 2 * kq);      // of queries 2 kq and 2 kq + 1
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        best[i] = fmaxf(best[i], fmaxf(fmaf(static_cast<float>(acc[0][2 * i] + acc[1][2 * i]), f.x, f.y),
+                                       fmaf(static_cast<float>(acc[0][2 * i + 1] + acc[1][2 * i + 1]), f.z, f.w)));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 1));
+      best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 2));
+      const int at = base + i * 8 + g;
+      if (kq == 0 && at < mine) {
+        const float score = unit[i] > 0.f ? best[i] * unit[i] : -INFINITY;
+        const unsigned k = pick_key(score);
+        least = min(least, k);
+        most = max(most, k);
+        scores[at] = score;
+      }
+    }
+    if (base + kAll < mine) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        unit[i] = next_unit[i];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) a[i][c] = next[i][c];
+      }
+    }
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  const int slot = rank * kPickWarps + wid;
+  if (p.parts > 1) {
+    if (lane < p.parts) {
+      pick_peer_store(sh.least + slot, lane, least);
+      pick_peer_store(sh.most + slot, lane, most);
+    }
+    cluster_sync_all();
+  } else {
+    if (lane == 0) {
+      sh.least[slot] = least;
+      sh.most[slot] = most;
+    }
+    __syncthreads();
+  }
+  least = 0xffffffffu;
+  most = 0u;
+  for (int i = lane; i < p.parts * kPickWarps; i += 32) {
+    least = min(least, sh.least[i]);
+    most = max(most, sh.most[i]);
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (p.parts > 1) {
+    pick_select<true>(sh, scores, mine, a0, rank, p.parts, p.top, least, most, p.first, out + p.first);
+    cluster_sync_all();                        // nobody leaves while a peer may still read its words
+  } else {
+    pick_select<false>(sh, scores, mine, 0, 0, 1, p.top, least, most, p.first, out + p.first);
+  }
 }
 
 template <int D>
@@ -442,13 +516,14 @@ B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block
   p.seqs = seqs; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages;
   p.top = top; p.first = first; p.last = last; p.width = width;
   p.status = static_cast<DeviceStatus*>(status);
-  const int codes = (run * (hq / hkv) + 15) / 16 * 16 * (2 * d + 64), fixed = (static_cast<int>(sizeof(PickShared)) + 15) / 16 * 16 + codes;
-  // blocks of a row: until the processors have two each, as long as a block has 256 pages to score; at least as many as hold the scores
+  const int fixed = (static_cast<int>(sizeof(PickShared)) + 15) / 16 * 16 + (run * (hq / hkv) + 7) / 8 * 8 * (2 * d + 64);
+  // blocks of a row: as long as every processor has one at most and a block 256 pages to score; at least as many as hold the scores
   p.parts = 1;
-  while (p.parts < 8 && static_cast<long long>(rows) * hkv * p.parts < num_sms() && max_pages > p.parts * 256) p.parts *= 2;
-  while (p.parts < 8 && fixed + static_cast<long long>((max_pages + p.parts - 1) / p.parts) * 4 > 100000) p.parts *= 2;
-  p.cap = (max_pages + p.parts - 1) / p.parts;
-  if (fixed + 4ll * p.cap > 232448) return -6;
+  while (p.parts < 8 && static_cast<long long>(rows) * hkv * p.parts * 2 <= num_sms() && max_pages > p.parts * 256) p.parts *= 2;
+  const auto scores = [&] { return 4ll * ((max_pages + p.parts - 1) / p.parts); };
+  while (p.parts < 8 && fixed + scores() > 232448) p.parts *= 2;
+  if (fixed + scores() > 232448) return -6;
   if (static_cast<long long>(rows) * p.parts >= (1ll << 31)) return -3;
-  return d == 128 ? launch_pick<128>(p, rows, fixed + 4 * p.cap, stream) : launch_pick<64>(p, rows, fixed + 4 * p.cap, stream);
+  const int smem = fixed + static_cast<int>(scores());
+  return d == 128 ? launch_pick<128>(p, rows, smem, stream) : launch_pick<64>(p, rows, smem, stream);
 }
