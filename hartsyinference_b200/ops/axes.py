@@ -34,22 +34,25 @@ def rope_axes_kv(qkv: torch.Tensor, positions: torch.Tensor, hq: int, hkv: int, 
     not stored). ``positions`` int32 [A, T]; pair j of the rotated part (the first 2 * len(axes) channels) turns by
     ``positions[axes[j]] * inv_freq[j]``, in angles of 64 bits; ``axes`` int32 as of :func:`rope_axes`, ``inv_freq`` fp32, both [pairs]. Heads of an
     even size up to 256; style 0 pairs channel j with j + pairs, 1 channel 2 j with 2 j + 1. Returns (q [T, hq, d], k [T, hkv, d] or None, v or None)."""
-    if positions.dim() != 2 or qkv.dim() != 2 or positions.shape[1] != qkv.shape[0]:
-        raise ValueError(f"rope_axes_kv: positions [A, T] of qkv [T, (hq + 2 hkv) d], got {tuple(positions.shape)} and {tuple(qkv.shape)}")
-    t, pairs = qkv.shape[0], axes.numel()
-    if hq < 1 or hkv < 1 or qkv.shape[1] != (hq + 2 * hkv) * d or not 2 <= d <= 256 or d % 2 or 2 * pairs > d or style not in (0, 1):
-        raise ValueError(f"rope_axes_kv: heads of an even size up to 256, at most d / 2 pairs, style 0 or 1; got {tuple(qkv.shape)} for {hq} + 2 * {hkv} heads of {d}, {pairs} pairs")
-    if positions.shape[0] < 1 or inv_freq.numel() != pairs:
+    shape, where, pairs, device = qkv.shape, positions.shape, axes.numel(), qkv.get_device()
+    if len(where) != 2 or len(shape) != 2 or where[1] != shape[0]:
+        raise ValueError(f"rope_axes_kv: positions [A, T] of qkv [T, (hq + 2 hkv) d], got {tuple(where)} and {tuple(shape)}")
+    t = shape[0]
+    if hq < 1 or hkv < 1 or shape[1] != (hq + 2 * hkv) * d or not 2 <= d <= 256 or d % 2 or 2 * pairs > d or style not in (0, 1):
+        raise ValueError(f"rope_axes_kv: heads of an even size up to 256, at most d / 2 pairs, style 0 or 1; got {tuple(shape)} for {hq} + 2 * {hkv} heads of {d}, {pairs} pairs")
+    if where[0] < 1 or inv_freq.numel() != pairs:
         raise ValueError("rope_axes_kv: an axis and a frequency for every pair")
     if (k_cache is None) != (v_cache is None) or (slot_mapping is not None and k_cache is None):
         raise ValueError("rope_axes_kv: caches of keys and of values, and slots only with them")
     if slot_mapping is not None and slot_mapping.numel() != t:
         raise ValueError("rope_axes_kv: a slot for every token")
-    device = qkv.get_device()
+    pages, page = 0, 1
     if k_cache is not None:
-        for c in (k_cache, v_cache):
-            if c.dim() != 4 or c.shape != k_cache.shape or c.shape[1] != hkv or c.shape[3] != d or not c.is_contiguous() or c.get_device() != device or c.dtype != qkv.dtype:
-                raise ValueError("rope_axes_kv: contiguous caches [pages, hkv, page, d] of the type and on the device of qkv")
+        pool = k_cache.shape
+        if (len(pool) != 4 or v_cache.shape != pool or pool[1] != hkv or pool[3] != d or not k_cache.is_contiguous() or not v_cache.is_contiguous()
+                or k_cache.get_device() != device or v_cache.get_device() != device or k_cache.dtype is not qkv.dtype or v_cache.dtype is not qkv.dtype):
+            raise ValueError("rope_axes_kv: contiguous caches [pages, hkv, page, d] of the type and on the device of qkv")
+        pages, page = pool[0], pool[2]
     for w in (q_norm_w, k_norm_w):
         if w is not None and (w.numel() != d or w.get_device() != device or (device >= 0 and w.dtype != torch.bfloat16)):
             raise ValueError("rope_axes_kv: norm weights are bf16 [d] on the device of qkv")
@@ -66,13 +69,13 @@ def rope_axes_kv(qkv: torch.Tensor, positions: torch.Tensor, hq: int, hkv: int, 
         raise ValueError(f"rope_axes_kv: bf16 activations, got {qkv.dtype}")
     with _on(device):
         qkv = _dense(qkv)
-        q_norm_w, k_norm_w = (None if w is None else w.contiguous() for w in (q_norm_w, k_norm_w))
-        q = torch.empty(t, hq, d, dtype=torch.bfloat16, device=qkv.device)
-        k = torch.empty(t, hkv, d, dtype=torch.bfloat16, device=qkv.device) if want_kv else None
-        v = torch.empty_like(k) if want_kv else None
-        pages, page = (0, 1) if k_cache is None else (k_cache.shape[0], k_cache.shape[2])
+        if q_norm_w is not None or k_norm_w is not None:
+            q_norm_w, k_norm_w = (None if w is None else w.contiguous() for w in (q_norm_w, k_norm_w))
+        q = qkv.new_empty((t, hq, d))
+        k = qkv.new_empty((t, hkv, d)) if want_kv else None
+        v = qkv.new_empty((t, hkv, d)) if want_kv else None
         rc = N.lib().b200_rope_axes(qkv.data_ptr(), q.data_ptr(), N.ptr(k_cache), N.ptr(v_cache), N.ptr(k), N.ptr(v), positions.data_ptr(), axes.data_ptr(),
-                                    inv_freq.data_ptr(), N.ptr(slot_mapping), N.ptr(q_norm_w), N.ptr(k_norm_w), t, positions.shape[0], hq, hkv, d, 2 * pairs, style,
+                                    inv_freq.data_ptr(), N.ptr(slot_mapping), N.ptr(q_norm_w), N.ptr(k_norm_w), t, where[0], hq, hkv, d, 2 * pairs, style,
                                     page, pages, eps, N.state(qkv.device).status.data_ptr(), N.stream())
         N.check(rc, "b200_rope_axes")
     return q, k, v

@@ -22,6 +22,12 @@ from .core import quant_fp8_act
 from .kv4 import _dense, _ints, _on
 
 WIDTH = 4096          # pages that a run can choose
+_PAGES, _HEADS, _I32 = (16, 32, 64, 128), (64, 128), torch.int32
+
+
+def _plain(x: torch.Tensor, device: int, n: int) -> bool:
+    """Whether x is n neighbouring numbers of 32 bits on the device."""
+    return x.dtype is _I32 and x.get_device() == device and x.numel() == n and x.is_contiguous()
 
 
 def key_bounds(pages: int, hkv: int, d: int, device="cuda") -> torch.Tensor:
@@ -34,16 +40,15 @@ def key_bounds(pages: int, hkv: int, d: int, device="cuda") -> torch.Tensor:
 def _pool_of(what: str, cache: torch.Tensor, device: int, d: Optional[int] = None) -> tuple:
     """(pages, hkv, page, d) of a pool of keys or values."""
     shape = cache.shape
-    if len(shape) != 4 or shape[2] not in (16, 32, 64, 128) or shape[3] not in (64, 128) or (d is not None and shape[3] != d):
+    if len(shape) != 4 or shape[2] not in _PAGES or shape[3] not in _HEADS or (d is not None and shape[3] != d):
         raise ValueError(f"{what}: pools [pages, hkv, page, d] with pages of 16, 32, 64 or 128 tokens and heads of 64 or 128, got {tuple(shape)}")
-    if not cache.is_contiguous() or cache.get_device() != device or (device >= 0 and (cache.dtype is not torch.bfloat16 or cache.data_ptr() % 16)):
+    if not cache.is_contiguous() or cache.get_device() != device or (device >= 0 and cache.dtype is not torch.bfloat16):
         raise ValueError(f"{what}: a contiguous pool, bf16 on a device, on that of the other tensors")
     return tuple(shape)
 
 
 def _bounds_of(what: str, bounds: torch.Tensor, device: int, hkv: int, d: int) -> int:
-    if bounds.dtype is not torch.uint8 or bounds.dim() != 3 or bounds.shape[1] != hkv or bounds.shape[2] != 2 * d + 16 or not bounds.is_contiguous() or bounds.get_device() != device \
-            or (device >= 0 and bounds.data_ptr() % 16):
+    if bounds.dtype is not torch.uint8 or bounds.dim() != 3 or bounds.shape[1] != hkv or bounds.shape[2] != 2 * d + 16 or not bounds.is_contiguous() or bounds.get_device() != device:
         raise ValueError(f"{what}: contiguous bounds uint8 [pages, {hkv}, {2 * d + 16}] on the device of the other tensors (key_bounds makes them), got {bounds.dtype} {tuple(bounds.shape)}")
     return bounds.shape[0]
 
@@ -76,23 +81,33 @@ def key_bounds_(bounds: torch.Tensor, k_cache: torch.Tensor, block_table: torch.
     """Bounds of the pages that the last tokens of every sequence filled, written into ``bounds``: ``cu_q[s + 1] - cu_q[s]`` tokens (one without ``cu_q``, at most
     ``max_q_len``) of ``kv_lens[s]`` that the cache holds. Pages that are not full are left as they are: whoever attends
     has them among its last ones. A page that is cut back and filled again is bounded again."""
-    device = bounds.get_device()
-    pages, hkv, page, d = _pool_of("key_bounds_", k_cache, device)
-    if _bounds_of("key_bounds_", bounds, device, hkv, d) != pages:
-        raise ValueError(f"key_bounds_: bounds of {bounds.shape[0]} pages for a pool of {pages}")
-    block_table, kv_lens, cu_q = _batch("key_bounds_", block_table, kv_lens, cu_q, device)
+    device, shape, table = bounds.get_device(), k_cache.shape, block_table.shape
+    seqs = kv_lens.numel()
+    if not (device >= 0 and len(shape) == 4 and len(table) == 2 and table[0] == seqs and shape[2] in _PAGES and shape[3] in _HEADS and bounds.dtype is torch.uint8
+            and k_cache.dtype is torch.bfloat16 and block_table.dtype is _I32 and kv_lens.dtype is _I32 and (cu_q is None or _plain(cu_q, device, seqs + 1))
+            and bounds.shape == (shape[0], shape[1], 2 * shape[3] + 16) and device == k_cache.get_device() == block_table.get_device() == kv_lens.get_device()
+            and bounds.is_contiguous() and k_cache.is_contiguous() and block_table.is_contiguous() and kv_lens.is_contiguous()):
+        # not the ordinary call: say what is wrong, or make it one
+        pages, hkv, page, d = _pool_of("key_bounds_", k_cache, device)
+        if _bounds_of("key_bounds_", bounds, device, hkv, d) != pages:
+            raise ValueError(f"key_bounds_: bounds of {bounds.shape[0]} pages for a pool of {pages}")
+        block_table, kv_lens, cu_q = _batch("key_bounds_", block_table, kv_lens, cu_q, device)
+    pages, hkv, page, d = shape
     if device < 0:
-        cuts = list(range(kv_lens.numel() + 1)) if cu_q is None else cu_q.tolist()
+        cuts = list(range(seqs + 1)) if cu_q is None else cu_q.tolist()
         for s, n in enumerate(kv_lens.tolist()):
             n, count = min(n, block_table.shape[1] * page), cuts[s + 1] - cuts[s]
             if count > 0 and n > 0:
                 ids = block_table[s, max(0, n - count) // page:n // page].long()
                 bounds[ids] = R.page_bounds(k_cache[ids])
         return bounds
-    if kv_lens.numel() and pages and block_table.shape[1]:
+    to, keys = bounds.data_ptr(), k_cache.data_ptr()
+    if (to | keys) % 16:
+        raise ValueError("key_bounds_: bounds and pool from 16-byte boundaries")
+    if seqs and pages and table[1]:
         with _on(device):
-            rc = N.lib().b200_key_bounds(k_cache.data_ptr(), bounds.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), N.ptr(cu_q), kv_lens.numel(),
-                                         max_q_len if cu_q is not None else 1, hkv, d, page, block_table.shape[1], pages, N.state(bounds.device).status.data_ptr(), N.stream())
+            rc = N.lib().b200_key_bounds(keys, to, block_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), seqs,
+                                         max_q_len if cu_q is not None else 1, hkv, d, page, table[1], pages, N.state(bounds.device).status.data_ptr(), N.stream())
             N.check(rc, "b200_key_bounds")
     return bounds
 
@@ -105,16 +120,21 @@ def pick_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor,
     group, of ``2^(e_q + e_page) * sum_c max(a_c high_c, a_c low_c)`` with the query's codes ``a = round(q / 2^e_q)`` (its own
     exponent, as for bounds). Sums are whole numbers below 2^22, so scores are exact and the choice does not depend on how they are computed.
     The queries of a sequence are its last tokens; ``cu_q`` None: one per sequence. Rows of no run are -1."""
-    device = q.get_device()
-    if q.dim() != 3 or (device >= 0 and q.dtype is not torch.bfloat16) or q.shape[2] not in (64, 128):
-        raise ValueError(f"pick_pages: q is [tokens, hq, 64 or 128], bf16 on a device; got {q.dtype} {tuple(q.shape)}")
-    tokens, hq, d = q.shape
-    hkv = bounds.shape[1] if bounds.dim() == 3 else 0
-    if hkv < 1 or hq < 1 or hq % hkv or page not in (16, 32, 64, 128):
-        raise ValueError(f"pick_pages: {hq} query heads on {hkv} key heads, pages of 16, 32, 64 or 128 tokens, got {page}")
-    pages = _bounds_of("pick_pages", bounds, device, hkv, d)
-    block_table, kv_lens, cu_q = _batch("pick_pages", block_table, kv_lens, cu_q, device)
+    device, shape, rows_of, table = q.get_device(), q.shape, bounds.shape, block_table.shape
     seqs = kv_lens.numel()
+    if not (device >= 0 and len(shape) == 3 and len(rows_of) == 3 and len(table) == 2 and table[0] == seqs and shape[2] in _HEADS and page in _PAGES
+            and rows_of[2] == 2 * shape[2] + 16 and shape[1] > 0 and rows_of[1] > 0 and shape[1] % rows_of[1] == 0 and q.dtype is torch.bfloat16
+            and bounds.dtype is torch.uint8 and block_table.dtype is _I32 and kv_lens.dtype is _I32 and (cu_q is None or _plain(cu_q, device, seqs + 1))
+            and device == bounds.get_device() == block_table.get_device() == kv_lens.get_device()
+            and bounds.is_contiguous() and block_table.is_contiguous() and kv_lens.is_contiguous()):
+        if q.dim() != 3 or (device >= 0 and q.dtype is not torch.bfloat16) or q.shape[2] not in _HEADS:
+            raise ValueError(f"pick_pages: q is [tokens, hq, 64 or 128], bf16 on a device; got {q.dtype} {tuple(q.shape)}")
+        hkv = bounds.shape[1] if bounds.dim() == 3 else 0
+        if hkv < 1 or shape[1] < 1 or shape[1] % hkv or page not in _PAGES:
+            raise ValueError(f"pick_pages: {shape[1]} query heads on {hkv} key heads, pages of 16, 32, 64 or 128 tokens, got {page}")
+        _bounds_of("pick_pages", bounds, device, hkv, shape[2])
+        block_table, kv_lens, cu_q = _batch("pick_pages", block_table, kv_lens, cu_q, device)
+    (tokens, hq, d), (pages, hkv, _) = shape, rows_of
     rows = _rows("pick_pages", tokens, seqs, run, hq // hkv, cu_q)
     width = first + top + last + (run + page - 2) // page
     if top < 0 or first < 0 or last < 1 or width > WIDTH:
@@ -137,13 +157,15 @@ def pick_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor,
             else:
                 out[row, :, :len(kept)] = torch.tensor(kept, dtype=torch.int32)
         return out
-    out = torch.empty(rows, hkv, width, dtype=torch.int32, device=q.device)
+    out = q.new_empty((rows, hkv, width), dtype=_I32)
     with _on(device):
-        if pages == 0 or block_table.shape[1] == 0 or seqs == 0:
+        if pages == 0 or table[1] == 0 or seqs == 0:
             return out.fill_(-1)
+        if bounds.data_ptr() % 16:
+            raise ValueError("pick_pages: bounds from a 16-byte boundary")
         q = _dense(q)
-        rc = N.lib().b200_pick_pages(q.data_ptr(), bounds.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), N.ptr(cu_q), out.data_ptr(), seqs, rows, hq, hkv, d,
-                                     page, block_table.shape[1], pages, run, top, first, last, width, N.state(q.device).status.data_ptr(), N.stream())
+        rc = N.lib().b200_pick_pages(q.data_ptr(), bounds.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), out.data_ptr(),
+                                     seqs, rows, hq, hkv, d, page, table[1], pages, run, top, first, last, width, N.state(q.device).status.data_ptr(), N.stream())
         N.check(rc, "b200_pick_pages")
     return out
 
@@ -155,19 +177,28 @@ def attn_picked(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     queries of a sequence are its last tokens; ``cu_q`` None: one per sequence. A query that sees no key gives zeros; rows behind the last sequence's are undefined. Page numbers below 0 or
     behind the run's last query are none; one that is named twice counts twice. With ``emit_fp8`` the result is ``(out, Fp8Act of out.reshape(tokens, hq * d))``
     as of :func:`.core.attn_decode`."""
-    device = q.get_device()
-    if q.dim() != 3 or (device >= 0 and q.dtype is not torch.bfloat16):
-        raise ValueError(f"attn_picked: q is [tokens, hq, d], bf16 on a device; got {q.dtype} {tuple(q.shape)}")
-    tokens, hq, d = q.shape
-    pages, hkv, page, _ = _pool_of("attn_picked", k_cache, device, d)
-    if _pool_of("attn_picked", v_cache, device, d) != (pages, hkv, page, d) or hkv < 1 or hq < 1 or hq % hkv:
-        raise ValueError(f"attn_picked: pools of keys and of values alike, {hq} query heads on {hkv} key heads")
-    block_table, kv_lens, cu_q = _batch("attn_picked", block_table, kv_lens, cu_q, device)
+    device, shape, pool, table, chosen = q.get_device(), q.shape, k_cache.shape, block_table.shape, picked.shape
     seqs = kv_lens.numel()
+    if not (device >= 0 and len(shape) == 3 and len(pool) == 4 and len(table) == 2 and len(chosen) == 3 and table[0] == seqs and pool[2] in _PAGES and pool[3] in _HEADS
+            and shape[2] == pool[3] and shape[1] > 0 and pool[1] > 0 and shape[1] % pool[1] == 0 and v_cache.shape == pool
+            and q.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16 and block_table.dtype is _I32 and kv_lens.dtype is _I32
+            and picked.dtype is _I32 and (cu_q is None or _plain(cu_q, device, seqs + 1))
+            and device == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == kv_lens.get_device() == picked.get_device()
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and block_table.is_contiguous() and kv_lens.is_contiguous() and picked.is_contiguous()):
+        if q.dim() != 3 or (device >= 0 and q.dtype is not torch.bfloat16):
+            raise ValueError(f"attn_picked: q is [tokens, hq, d], bf16 on a device; got {q.dtype} {tuple(q.shape)}")
+        hkv = _pool_of("attn_picked", k_cache, device, shape[2])[1]
+        if _pool_of("attn_picked", v_cache, device, shape[2]) != tuple(pool) or hkv < 1 or shape[1] < 1 or shape[1] % hkv:
+            raise ValueError(f"attn_picked: pools of keys and of values alike, {shape[1]} query heads on {hkv} key heads")
+        block_table, kv_lens, cu_q = _batch("attn_picked", block_table, kv_lens, cu_q, device)
+        if picked.dim() != 3:
+            raise ValueError(f"attn_picked: picked [rows, {hkv}, width], got {tuple(picked.shape)}")
+        picked = _ints("picked", picked, device)
+    (tokens, hq, d), (pages, hkv, page, _) = shape, pool
     rows = _rows("attn_picked", tokens, seqs, run, hq // hkv, cu_q)
-    if picked.dim() != 3 or tuple(picked.shape[:2]) != (rows, hkv) or not 1 <= picked.shape[2] <= WIDTH:
-        raise ValueError(f"attn_picked: picked [{rows}, {hkv}, 1 to {WIDTH}], got {tuple(picked.shape)}")
-    picked = _ints("picked", picked, device)
+    width = chosen[2]
+    if chosen[0] != rows or chosen[1] != hkv or not 1 <= width <= WIDTH:
+        raise ValueError(f"attn_picked: picked [{rows}, {hkv}, 1 to {WIDTH}], got {tuple(chosen)}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if device < 0:
         out = torch.zeros_like(q)
@@ -186,15 +217,17 @@ def attn_picked(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
         with _on(device):
             q = _dense(q)
             out = torch.empty_like(q)
-            if block_table.shape[1] == 0 or pages == 0:
+            if table[1] == 0 or pages == 0:
                 out.zero_()
             elif seqs:
-                L, status, width = N.lib(), N.state(q.device).status.data_ptr(), picked.shape[2]
-                ptrs = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), picked.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), N.ptr(cu_q))
+                L, status, keys, values = N.lib(), N.state(q.device).status.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+                if (keys | values) % 16:
+                    raise ValueError("attn_picked: pools from 16-byte boundaries")
+                ptrs = (q.data_ptr(), keys, values, out.data_ptr(), picked.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr())
                 if run > 1 and L.b200_attn_picked_form(rows, run * (hq // hkv), hkv, page, width, pages, scale, softcap):
-                    rc = L.b200_attn_picked_tc(*ptrs, seqs, rows, tokens, hq, hkv, d, page, block_table.shape[1], pages, run, width, scale, status, N.stream())
+                    rc = L.b200_attn_picked_tc(*ptrs, seqs, rows, tokens, hq, hkv, d, page, table[1], pages, run, width, scale, status, N.stream())
                 else:
-                    rc = L.b200_attn_picked(*ptrs, seqs, rows, hq, hkv, d, page, block_table.shape[1], pages, run, width, scale, float(softcap), status, N.stream())
+                    rc = L.b200_attn_picked(*ptrs, seqs, rows, hq, hkv, d, page, table[1], pages, run, width, scale, float(softcap), status, N.stream())
                 N.check(rc, "b200_attn_picked")
     if not emit_fp8:
         return out
