@@ -22,7 +22,6 @@ struct RopeAxesParams {
   long long slots_end;             // slots of the pool
   int tokens, n_axes, hq, hkv, d, rot, style, page, block_tokens;
   float eps;
-  int norms_aligned;               // to 16 bytes
   DeviceStatus* status;
 };
 
@@ -76,147 +75,133 @@ __device__ __forceinline__ void axes_unpack(const typename AxesVec<V>::T& raw, f
   }
 }
 
-// Norm weights, which may lie anywhere.
-template <int V>
-__device__ __forceinline__ void axes_weights(const __nv_bfloat16* src, bool aligned, float (&v)[V]) {
-  if (aligned) {
-    axes_unpack<V>(__ldg(reinterpret_cast<const typename AxesVec<V>::T*>(src)), v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = __bfloat162float(__ldg(src + i));
-  }
-}
-
 // `lanes` lanes share a head (as many as it has units of work; a power of two of them where a norm's sum is exchanged), two vectors of V neighbouring
-// values each: with split halves the two that turn together, else neighbours (what lies behind the rotated part always so). A block walks the heads of a few
-// tokens, the next vectors on their way while some are turned, the first ones while the angles are worked out. Bound by HBM.
+// values each: with split halves the two that turn together, else neighbours (what lies behind the rotated part always so). A thread keeps its place
+// in the head and walks the heads of a few tokens, the next vectors on their way while some are turned, the first ones while the angles are worked out.
+// 8192 tokens of 32 + 16 heads of 128 with norms: 56.6 us with a division per vector and norm weights loaded one by one (495 instructions a unit, issued in
+// 77 % of the cycles).
 template <int V>
 __global__ void __launch_bounds__(256, 4) rope_axes_kernel(const RopeAxesParams p, int lanes) {
   using Vec = typename AxesVec<V>::T;
   pdl_wait();
   pdl_trigger();
-  extern __shared__ __align__(16) float axes_table[];      // [block_tokens][cos of rot / 2, then sin; each part padded to 4]
+  extern __shared__ __align__(16) float axes_table[];      // [block_tokens][cos of rot / 2, then sin; each part padded to 4], norm weights of q, of k
   __shared__ long long cache_row[8];
   const int heads = p.hq + 2 * p.hkv, half = p.rot >> 1, pitch = (half + 3) & ~3;
   const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.tokens - t0);
   const int units = p.d / (2 * V), split = half / V;       // units whose two vectors turn together
-  const int slots = heads * lanes, step = 256 * gridDim.y, first = blockIdx.y * 256 + threadIdx.x;
-  const int rounds = (slots - (first & ~31) + step - 1) / step;      // (of the warp; its lanes make the same ones)
-  // place r of the walk: token, head and unit
-  int tt = 0, rr = 0;
-  Vec na, nb;
-  const auto ends = [&](int u, int& ca, int& cb) {
-    ca = (p.style == 0 && u < split ? u : 2 * u) * V;
-    cb = p.style == 0 && u < split ? ca + half : ca + V;
-  };
-  const auto fetch = [&](int t, int round) {
-    const int s = min(first + round * step, slots - 1), h = s / lanes, u = min(s - h * lanes, units - 1);
-    int ca, cb;
-    ends(u, ca, cb);
-    const __nv_bfloat16* src = p.qkv + (static_cast<long long>(t0 + t) * heads + h) * p.d;
-    na = __ldg(reinterpret_cast<const Vec*>(src + ca));
-    nb = __ldg(reinterpret_cast<const Vec*>(src + cb));
-  };
-  if (rounds > 0) fetch(0, 0);
+  const int each = 256 / lanes, mine = threadIdx.x / lanes, u = threadIdx.x - mine * lanes;
+  const int h0 = blockIdx.y * each + mine, step = each * gridDim.y, rounds = (heads - static_cast<int>(blockIdx.y) * each + step - 1) / step;
+  const bool on = mine < each && u < units, turns = on && u * V < half, norms = p.q_norm_w || p.k_norm_w;
+  const int at = min(u, units - 1), ca = (p.style == 0 && at < split ? at : 2 * at) * V, cb = p.style == 0 && at < split ? ca + half : ca + V;
+  const __nv_bfloat16* src = p.qkv + (static_cast<long long>(t0) * heads + min(h0, heads - 1)) * p.d;
+  Vec na = __ldg(reinterpret_cast<const Vec*>(src + ca)), nb = __ldg(reinterpret_cast<const Vec*>(src + cb));
   for (int i = threadIdx.x; i < nt * half; i += 256) {
     const int t = i / half, j = i - t * half;
     const float2 cs = axes_turn(p, t0 + t, j);
     axes_table[2 * t * pitch + j] = cs.x;
     axes_table[(2 * t + 1) * pitch + j] = cs.y;
   }
+  float* const weights = axes_table + 2 * p.block_tokens * pitch;
+  if (norms)
+    for (int i = threadIdx.x; i < 2 * p.d; i += 256) {
+      const __nv_bfloat16* w = i < p.d ? p.q_norm_w : p.k_norm_w;
+      weights[i] = w ? __bfloat162float(w[i < p.d ? i : i - p.d]) : 0.f;
+    }
   if (threadIdx.x < nt) cache_row[threadIdx.x] = axes_row(p, t0 + threadIdx.x, blockIdx.y == 0);
   __syncthreads();
-  if (rounds <= 0) return;
-  while (tt < nt) {
-    const int s = first + rr * step, at = min(s, slots - 1), h = at / lanes, u = at - h * lanes, t = t0 + tt;
-    const bool mine = u < units, active = s < slots && mine, turns = mine && u * V < half;
-    const int kind = h < p.hq ? 0 : (h < p.hq + p.hkv ? 1 : 2);
-    int ca, cb;
-    ends(min(u, units - 1), ca, cb);
-    float a[V], b[V];
-    axes_unpack<V>(na, a);
-    axes_unpack<V>(nb, b);
-    const float* cosv = axes_table + 2 * tt * pitch;
+  const auto floats = [](const float* from, float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(from + i);
+      v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+    }
+  };
+  for (int tt = 0; tt < nt; ++tt) {
+    const int t = t0 + tt;
+    const float* cosv = axes_table + 2 * tt * pitch + u * V;
     const long long stored = cache_row[tt];
-    if (++rr == rounds) { rr = 0; ++tt; }
-    if (tt < nt) fetch(tt, rr);
-    if (p.q_norm_w || p.k_norm_w) {
-      float ss = 0.f;
-      if (mine) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) ss += a[i] * a[i] + b[i] * b[i];
+    for (int r = 0, h = h0; r < rounds; ++r, h += step) {
+      const int kind = h < p.hq ? 0 : (h < p.hq + p.hkv ? 1 : 2);
+      float a[V], b[V];
+      axes_unpack<V>(na, a);
+      axes_unpack<V>(nb, b);
+      if (r + 1 < rounds || tt + 1 < nt) {
+        const bool same = r + 1 < rounds;
+        src = p.qkv + (static_cast<long long>(same ? t : t + 1) * heads + min(same ? h + step : h0, heads - 1)) * p.d;
+        na = __ldg(reinterpret_cast<const Vec*>(src + ca));
+        nb = __ldg(reinterpret_cast<const Vec*>(src + cb));
       }
-      for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const __nv_bfloat16* nw = kind == 0 ? p.q_norm_w : (kind == 1 ? p.k_norm_w : nullptr);
-      if (nw) {
-        const float rstd = rsqrtf(ss / p.d + p.eps);
-        float w[V];
-        axes_weights<V>(nw + ca, p.norms_aligned, w);
+      if (norms) {
+        float ss = 0.f;
+        if (on) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) a[i] = a[i] * rstd * w[i];
-        axes_weights<V>(nw + cb, p.norms_aligned, w);
-#pragma unroll
-        for (int i = 0; i < V; ++i) b[i] = b[i] * rstd * w[i];
-      }
-    }
-    if (turns && kind != 2) {
-      float cs[V], sn[V];
-      if ((half & 3) == 0) {
-#pragma unroll
-        for (int i = 0; i < V; i += 4) {
-          const int j = min(u * V + i, half - 4);             // (behind the last pair: not used)
-          const float4 c = *reinterpret_cast<const float4*>(cosv + j), n = *reinterpret_cast<const float4*>(cosv + pitch + j);
-          cs[i] = c.x; cs[i + 1] = c.y; cs[i + 2] = c.z; cs[i + 3] = c.w;
-          sn[i] = n.x; sn[i + 1] = n.y; sn[i + 2] = n.z; sn[i + 3] = n.w;
+          for (int i = 0; i < V; ++i) ss += a[i] * a[i] + b[i] * b[i];
         }
+        for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (kind == 0 ? p.q_norm_w != nullptr : kind == 1 && p.k_norm_w) {
+          const float rstd = rsqrtf(ss / p.d + p.eps);
+          const float* nw = weights + kind * p.d;
+          float w[V];
+          floats(nw + ca, w);
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (u * V + i >= half) { cs[i] = 1.f; sn[i] = 0.f; }
+          for (int i = 0; i < V; ++i) a[i] = a[i] * rstd * w[i];
+          floats(nw + cb, w);
+#pragma unroll
+          for (int i = 0; i < V; ++i) b[i] = b[i] * rstd * w[i];
+        }
+      }
+      if (turns && kind != 2) {
+        float cs[V], sn[V];
+        if ((u + 1) * V <= half && (half & 3) == 0) {
+          floats(cosv, cs);
+          floats(cosv + pitch, sn);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const bool real = u * V + i < half;
+            cs[i] = real ? cosv[i] : 1.f;
+            sn[i] = real ? cosv[pitch + i] : 0.f;
+          }
+        }
+        if (p.style == 0) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float x = a[i], y = b[i];
+            a[i] = x * cs[i] - y * sn[i];
+            b[i] = y * cs[i] + x * sn[i];
+          }
+        } else {
+          // pairs (2 i, 2 i + 1) of the unit's 2 V neighbours: the first V / 2 pairs lie in a, the others in b
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) {
+            const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
+            a[2 * i] = x * cs[i] - y * sn[i];
+            a[2 * i + 1] = y * cs[i] + x * sn[i];
+            b[2 * i] = z * cs[V / 2 + i] - w * sn[V / 2 + i];
+            b[2 * i + 1] = w * cs[V / 2 + i] + z * sn[V / 2 + i];
+          }
+        }
+      }
+      if (!on || h >= heads) continue;
+      __nv_bfloat16 *dst = nullptr, *dense = nullptr;
+      if (kind == 0) {
+        dst = p.q_out + (static_cast<long long>(t) * p.hq + h) * p.d;
       } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const bool on = u * V + i < half;
-          cs[i] = on ? cosv[u * V + i] : 1.f;
-          sn[i] = on ? cosv[pitch + u * V + i] : 0.f;
-        }
+        const int hk = kind == 1 ? h - p.hq : h - p.hq - p.hkv;
+        __nv_bfloat16* cache = kind == 1 ? p.k_cache : p.v_cache;
+        if (cache && stored >= 0) dst = cache + (stored + static_cast<long long>(hk) * p.page) * p.d;
+        dense = kind == 1 ? p.k_out : p.v_out;
+        if (dense) dense += (static_cast<long long>(t) * p.hkv + hk) * p.d;
       }
-      if (p.style == 0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float x = a[i], y = b[i];
-          a[i] = x * cs[i] - y * sn[i];
-          b[i] = y * cs[i] + x * sn[i];
-        }
-      } else {
-        // pairs (2 i, 2 i + 1) of the unit's 2 V neighbours: the first V / 2 pairs lie in a, the others in b
-#pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-          const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
-          a[2 * i] = x * cs[i] - y * sn[i];
-          a[2 * i + 1] = y * cs[i] + x * sn[i];
-          b[2 * i] = z * cs[V / 2 + i] - w * sn[V / 2 + i];
-          b[2 * i + 1] = w * cs[V / 2 + i] + z * sn[V / 2 + i];
-        }
+      if (dst) {
+        axes_store<V>(dst + ca, a);
+        axes_store<V>(dst + cb, b);
       }
-    }
-    if (!active) continue;
-    __nv_bfloat16 *dst = nullptr, *dense = nullptr;
-    if (kind == 0) {
-      dst = p.q_out + (static_cast<long long>(t) * p.hq + h) * p.d;
-    } else {
-      const int hk = kind == 1 ? h - p.hq : h - p.hq - p.hkv;
-      __nv_bfloat16* cache = kind == 1 ? p.k_cache : p.v_cache;
-      if (cache && stored >= 0) dst = cache + (stored + static_cast<long long>(hk) * p.page) * p.d;
-      dense = kind == 1 ? p.k_out : p.v_out;
-      if (dense) dense += (static_cast<long long>(t) * p.hkv + hk) * p.d;
-    }
-    if (dst) {
-      axes_store<V>(dst + ca, a);
-      axes_store<V>(dst + cb, b);
-    }
-    if (dense) {
-      axes_store<V>(dense + ca, a);
-      axes_store<V>(dense + cb, b);
+      if (dense) {
+        axes_store<V>(dense + ca, a);
+        axes_store<V>(dense + cb, b);
+      }
     }
   }
 }
@@ -277,10 +262,10 @@ static cudaError_t launch_rope_axes(RopeAxesParams p, cudaStream_t stream) {
   int lanes = p.d / (2 * V);
   if (norm)
     for (lanes = 1; lanes * 2 * V < p.d;) lanes *= 2;
-  const int chunks = ((p.hq + 2 * p.hkv) * lanes + 255) / 256;
+  const int each = 256 / lanes, chunks = (p.hq + 2 * p.hkv + each - 1) / each;
   p.block_tokens = p.tokens >= 148 * 8 ? 4 : 1;      // more tokens a block once every processor has several
   return launch_pdl(rope_axes_kernel<V>, dim3((p.tokens + p.block_tokens - 1) / p.block_tokens, p.block_tokens == 1 ? chunks : 1), dim3(256),
-                    static_cast<size_t>(p.block_tokens) * 2 * (((p.rot >> 1) + 3) & ~3) * sizeof(float), stream, p, lanes);
+                    (p.block_tokens * 2 * (((p.rot >> 1) + 3) & ~3) + (norm ? 2 * p.d : 0)) * sizeof(float), stream, p, lanes);
 }
 
 }  // namespace b200
@@ -312,7 +297,6 @@ B200_API int b200_rope_axes(const void* qkv, void* q_out, void* k_cache, void* v
   p.tokens = tokens; p.n_axes = n_axes; p.hq = hq; p.hkv = hkv; p.d = d; p.rot = rot; p.style = style; p.page = page;
   p.eps = eps;
   p.status = static_cast<DeviceStatus*>(status);
-  p.norms_aligned = ((reinterpret_cast<uintptr_t>(q_norm_w) | reinterpret_cast<uintptr_t>(k_norm_w)) & 15) == 0;
   uintptr_t all = 0;
   for (const void* x : {qkv, static_cast<const void*>(q_out), static_cast<const void*>(k_cache), static_cast<const void*>(v_cache), static_cast<const void*>(k_out), static_cast<const void*>(v_out)})
     all |= reinterpret_cast<uintptr_t>(x);
