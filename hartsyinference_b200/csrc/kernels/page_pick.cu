@@ -7,6 +7,7 @@
 //                   score(page) = max over queries of 2^(e_q + e_page) * sum_c max(a_c high_c, a_c low_c),
 //                 a bound of every product of a with a key of the page. max(a h, a l) is a+ h + a- l, so the sum is an integer product of 2 D
 //                 codes: mma.sync on 8-bit integers, exact, below 2^22 and scaled by a power of two. What is kept does not depend on any order.
+#include "mma_sync.cuh"
 #include "picked.cuh"
 
 namespace b200 {
@@ -92,6 +93,7 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
 // ------------------------------------------------------------------------------------------ the choice
 constexpr int kPickThreads = 512, kPickWarps = 16, kPickBins = 2048;
 constexpr int kPickRows = 128;          // queries of a run, heads counted
+constexpr int kPickFew = 32;            // of which so many are multiplied by mma.sync
 constexpr int kPickStep = 16;           // pages that a warp scores at a time
 
 struct PickParams {
@@ -178,10 +180,10 @@ __device__ __forceinline__ unsigned pick_key(float score) {
 // The `top` largest of more than `top` scores, of which this block holds the `mine` from number `a0` on, ties to the lowest number: first + number, in order, to
 // out[0 .. top). `least` and `most` bound all keys. Digits of what keys lie above the smallest, as many as it takes: 11 bits where one block holds all
 // scores; 9 in a cluster, whose blocks read one another's counts. All threads of all blocks of the row.
-template <bool kCluster>
+template <bool kCluster, int kThreads>
 __device__ __forceinline__ void pick_select(PickShared& sh, const float* scores, int mine, int a0, int rank, int parts, int top, unsigned least, unsigned most,
                                             int first, int* out) {
-  constexpr int kDigit = kCluster ? 9 : 11, kBins = 1 << kDigit, kEach = kBins / kPickThreads;
+  constexpr int kWarps = kThreads / 32, kDigit = kCluster ? 9 : 11, kBins = 1 << kDigit, kEach = kBins / kThreads;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   int shift = 32 - __clz(static_cast<int>(most - least));        // bits that differ
   unsigned prefix = 0u, want = static_cast<unsigned>(top);
@@ -190,9 +192,9 @@ __device__ __forceinline__ void pick_select(PickShared& sh, const float* scores,
     shift -= bits;
     unsigned* hist = sh.hist + (kCluster ? (pass & 1) * kBins : 0);      // (a peer may still read those of the pass before)
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) hist[i * kPickThreads + threadIdx.x] = 0u;
+    for (int i = 0; i < kEach; ++i) hist[i * kThreads + threadIdx.x] = 0u;
     __syncthreads();
-    for (int i = threadIdx.x; i < mine; i += kPickThreads) {
+    for (int i = threadIdx.x; i < mine; i += kThreads) {
       const unsigned k = pick_key(scores[i]) - least;
       if ((static_cast<unsigned long long>(k) >> (shift + bits)) == prefix) atomicAdd(hist + ((k >> shift) & ((1u << bits) - 1u)), 1u);
     }
@@ -220,7 +222,7 @@ __device__ __forceinline__ void pick_select(PickShared& sh, const float* scores,
     }
     if (lane == 0) sh.warp_a[wid] = upto;
     __syncthreads();
-    for (int w = wid + 1; w < kPickWarps; ++w) upto += sh.warp_a[w];
+    for (int w = wid + 1; w < kWarps; ++w) upto += sh.warp_a[w];
     unsigned above = upto - sum;
     if (above < want && upto >= want) {
 #pragma unroll
@@ -239,7 +241,7 @@ __device__ __forceinline__ void pick_select(PickShared& sh, const float* scores,
     if (sh.in_bin == want || shift == 0) break;      // (alike in all blocks)
   }
   // kept: larger prefixes, and the first `want` of the equal ones
-  const int seg = ((mine + kPickWarps - 1) / kPickWarps + 31) & ~31, s0 = min(mine, wid * seg), s1 = min(mine, s0 + seg);
+  const int seg = ((mine + kWarps - 1) / kWarps + 31) & ~31, s0 = min(mine, wid * seg), s1 = min(mine, s0 + seg);
   unsigned over = 0, tied = 0;
   for (int i0 = s0; i0 < s1; i0 += 32) {
     const int i = i0 + lane;
@@ -252,7 +254,7 @@ __device__ __forceinline__ void pick_select(PickShared& sh, const float* scores,
   unsigned over0 = 0, tied0 = 0;
   for (int w = 0; w < wid; ++w) { over0 += sh.warp_a[w]; tied0 += sh.warp_b[w]; }
   if (kCluster) {
-    if (threadIdx.x == kPickThreads - 1) { sh.counts[0] = over0 + over; sh.counts[1] = tied0 + tied; }
+    if (threadIdx.x == kThreads - 1) { sh.counts[0] = over0 + over; sh.counts[1] = tied0 + tied; }
     cluster_sync_all();
     unsigned x = 0, y = 0;
     if (lane < rank) { x = pick_peer_load(&sh.counts[0], lane); y = pick_peer_load(&sh.counts[1], lane); }
@@ -437,10 +439,10 @@ __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickP
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
   if (p.parts > 1) {
-    pick_select<true>(sh, scores, mine, a0, rank, p.parts, p.top, least, most, p.first, out + p.first);
+    pick_select<true, kPickThreads>(sh, scores, mine, a0, rank, p.parts, p.top, least, most, p.first, out + p.first);
     cluster_sync_all();                        // nobody leaves while a peer may still read its words
   } else {
-    pick_select<false>(sh, scores, mine, 0, 0, 1, p.top, least, most, p.first, out + p.first);
+    pick_select<false, kPickThreads>(sh, scores, mine, 0, 0, 1, p.top, least, most, p.first, out + p.first);
   }
 }
 
@@ -462,6 +464,239 @@ static int launch_pick(const PickParams& p, int rows, int smem, cudaStream_t str
   cfg.attrs = attr;
   cfg.numAttrs = p.parts > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, pick_pages_kernel<D>, p);
+  return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
+}
+
+// The same for runs whose queries (with their heads) are many: a block scores 128 pages at a time for up to 128 queries on the 5th-generation tensor cores.
+// Pages are rows of the product, so a thread of the epilogue owns a page and takes the maximum over the queries by itself.
+//   warps 0..3   copy the codes of 128 pages into one of two stages, 16 bytes a lane, in the layout of a 128-byte swizzle; one thread
+//                issues the products of the stage before
+//   warps 4..7   scores: a page a thread, its 16 to 128 sums from one of two halves of TMEM
+// Bound by the reads of the bounds, 2 D bytes a page and run, from L2. mma.sync has 8-bit products at a fifth of the rate (2048 queries behind 30720: 307 us).
+constexpr int kPtThreads = 256, kPtTile = 128;
+
+struct PickTcShared {
+  uint64_t a_empty[2], s_full[2], s_empty[2];
+  uint32_t tmem_base, abort_flag;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kPtThreads, 2) pick_pages_tc_kernel(const PickParams p) {
+  pdl_wait();
+  pdl_trigger();
+  extern __shared__ uint8_t pick_raw[];
+  constexpr int kAtoms = 2 * D / 128, kRow = 2 * D + kBoundsTail, kStage = kPtTile * 2 * D;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pick_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, group = p.hq / p.hkv;
+  const int row = blockIdx.x, h = blockIdx.y, cols = (p.run * group + 15) & ~15;
+  uint8_t* stages = smem;                                    // [2][atom][128 pages][128 bytes]; the choice works here afterwards
+  uint8_t* codes = stages + 2 * kStage;                      // [atom][128 queries][128 bytes]
+  float2* factor = reinterpret_cast<float2*>(codes + kStage);                    // of a query: 2^e and 0, or 0 and -inf for those that pad
+  PickTcShared& bars = *reinterpret_cast<PickTcShared*>(factor + kPickRows);
+  float* scores = reinterpret_cast<float*>(&bars + 1);
+  int* out = p.out + (static_cast<long long>(row) * p.hkv + h) * p.width;
+  PickRange x;
+  if (!pick_range(p, row, out, true, x)) return;
+  const RunOfRow& r = x.run;
+  const int n_tiles = (x.n + kPtTile - 1) / kPtTile;
+  const int* ids = p.block_table + static_cast<long long>(r.seq) * p.max_pages + p.first;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.a_empty[i], 1);
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.s_empty[i], 4);
+    }
+    bars.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (wid == 4) {
+    tmem_alloc(&bars.tmem_base, 256);
+    tmem_relinquish();
+  }
+  volatile uint32_t* abort_flag = &bars.abort_flag;
+  // sixteen (D = 128) or eight lanes a page
+  constexpr int kLanes = 2 * D / 16, kPages = 128 / kLanes;      // pages that warps 0..3 copy at a time
+  const int piece = threadIdx.x % kLanes;
+  const auto copy = [&](int j) {
+#pragma unroll 4
+    for (int i = 0; i < kPtTile / kPages; ++i) {
+      const int at = i * kPages + threadIdx.x / kLanes, id = ids[min(j * kPtTile + at, x.n - 1)];
+      const bool ok = id >= 0 && id < p.pages;
+      cp_async_16(smem_u32(stages + (j & 1) * kStage + (piece >> 3) * (kPtTile * 128) + at * 128 + (((piece & 7) ^ (at & 7)) << 4)),
+                  p.bounds + (static_cast<long long>(ok ? id : 0) * p.hkv + h) * kRow + piece * 16, ok);
+    }
+    cp_async_commit();
+  };
+  if (wid < 4) copy(0);
+
+  // ---- codes of the queries, four at a time
+  for (int i0 = wid * 4; i0 < cols; i0 += 32) {
+    constexpr int kEach = D / 32;
+    float v[4][kEach];
+    bool real[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u;
+      real[u] = i < r.tokens * group && r.begin + i / group >= 0;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) v[u][k] = 0.f;
+      if (real[u]) {
+        const __nv_bfloat16* src = p.q + (static_cast<long long>(r.q_off + i / group) * p.hq + h * group + i % group) * D + lane * kEach;
+#pragma unroll
+        for (int k = 0; k < kEach; k += 2) {
+          const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + k));
+          v[u][k] = f.x;
+          v[u][k + 1] = f.y;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u;
+      float amax = 0.f;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        v[u][k] = v[u][k] == v[u][k] ? v[u][k] : 0.f;
+        amax = fmaxf(amax, fabsf(v[u][k]));
+      }
+      const int e = bounds_exponent(warp_max(amax));
+      const float f = bounds_pow2(-e);
+      uint32_t up = 0, down = 0;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) {
+        const int c = static_cast<int>(fminf(fmaxf(rintf(v[u][k] * f), -127.f), 127.f));
+        up |= static_cast<uint32_t>(max(c, 0)) << (8 * k);
+        down |= (static_cast<uint32_t>(min(c, 0)) & 0xffu) << (8 * k);
+      }
+      const auto place = [&](int byte) {
+        return codes + (byte >> 7) * (kPtTile * 128) + i * 128 + ((((byte >> 4) & 7) ^ (i & 7)) << 4) + (byte & 15);
+      };
+      if (kEach == 4) {
+        *reinterpret_cast<uint32_t*>(place(lane * 4)) = up;
+        *reinterpret_cast<uint32_t*>(place(D + lane * 4)) = down;
+      } else {
+        *reinterpret_cast<uint16_t*>(place(lane * 2)) = static_cast<uint16_t>(up);
+        *reinterpret_cast<uint16_t*>(place(D + lane * 2)) = static_cast<uint16_t>(down);
+      }
+      if (lane == 0) factor[i] = real[u] ? make_float2(bounds_pow2(e), 0.f) : make_float2(0.f, -INFINITY);
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
+  unsigned least = 0xffffffffu, most = 0u;
+
+  if (wid < 4) {
+    // every thread makes all rounds, whatever runs out: the group's barrier counts on it
+    const uint32_t idesc = make_idesc(128, cols, kFmtS8, kFmtS8, 2);
+    const auto multiply = [&](int j) {
+      fence_proxy_async_smem();
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (threadIdx.x != 0) return;
+      if (j >= 2 && !mbar_wait(&bars.s_empty[j & 1], static_cast<uint32_t>(((j >> 1) - 1) & 1), abort_flag)) {
+        report_status(p.status, kWaitTimeout, kKernelPicked, 22, blockIdx.x);
+        return;
+      }
+      tc_fence_after_sync();
+#pragma unroll
+      for (int a = 0; a < kAtoms; ++a) {
+        const uint64_t ad = make_desc_sw128(smem_u32(stages + (j & 1) * kStage + a * (kPtTile * 128)));
+        const uint64_t bd = make_desc_sw128(smem_u32(codes + a * (kPtTile * 128)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_i8_ss(tmem_base + (j & 1) * 128, ad + 2 * k, bd + 2 * k, idesc, (a | k) != 0);
+      }
+      tc_commit(&bars.s_full[j & 1]);
+      tc_commit(&bars.a_empty[j & 1]);
+    };
+    for (int j = 1; j < n_tiles; ++j) {
+      if (j >= 2 && !mbar_wait(&bars.a_empty[j & 1], static_cast<uint32_t>(((j >> 1) - 1) & 1), abort_flag) && threadIdx.x == 0)
+        report_status(p.status, kWaitTimeout, kKernelPicked, 23, blockIdx.x);
+      copy(j);
+      cp_async_wait<1>();
+      multiply(j - 1);
+    }
+    cp_async_wait<0>();
+    multiply(n_tiles - 1);
+  } else {
+    const int mine = threadIdx.x - 128;                      // page of a tile = TMEM lane
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>((wid & 3) * 32) << 16);
+    // the exponent of the tile's page, one tile ahead
+    const auto unit_of = [&](int j) {
+      const int at = j * kPtTile + mine;
+      if (at >= x.n) return 0.f;
+      const int id = ids[at];
+      if (id < 0 || id >= p.pages) {
+        report_status(p.status, kBadArgument, kKernelPicked, 2, static_cast<uint32_t>(r.seq));
+        return 0.f;
+      }
+      return bounds_pow2(min(50, max(-50, static_cast<int>(__ldg(p.bounds + (static_cast<long long>(id) * p.hkv + h) * kRow + 2 * D)) - kBoundsBias)));
+    };
+    float unit = unit_of(0);
+    for (int j = 0; j < n_tiles; ++j) {
+      const float next = j + 1 < n_tiles ? unit_of(j + 1) : 0.f;
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars.s_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag))) {
+        if (lane == 0) report_status(p.status, kWaitTimeout, kKernelPicked, 24, blockIdx.x);
+        break;
+      }
+      tc_fence_after_sync();
+      float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      for (int c0 = 0; c0 < cols; c0 += 32) {                // (behind the last column TMEM holds anything: not used)
+        uint32_t s[32];
+        tmem_ld_32x32(lane_base + (j & 1) * 128 + c0, s);
+        tmem_ld_wait();
+        if (c0 + 32 >= cols) {                               // the products of the tile after the next may take these columns
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.s_empty[j & 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          if (i == 16 && c0 + 16 >= cols) break;
+          const float4 f = *reinterpret_cast<const float4*>(factor + c0 + i);
+          best[i & 2] = fmaxf(best[i & 2], fmaf(static_cast<float>(static_cast<int>(s[i])), f.x, f.y));
+          best[(i & 2) + 1] = fmaxf(best[(i & 2) + 1], fmaf(static_cast<float>(static_cast<int>(s[i + 1])), f.z, f.w));
+        }
+      }
+      const int at = j * kPtTile + mine;
+      if (at < x.n) {
+        const float score = unit > 0.f ? fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * unit : -INFINITY;
+        const unsigned k = pick_key(score);
+        least = min(least, k);
+        most = max(most, k);
+        scores[at] = score;
+      }
+      unit = next;
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  if (wid == 4) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 256);
+  }
+  if (*abort_flag) {                                         // nothing is chosen
+    for (int i = threadIdx.x; i < p.top; i += kPtThreads) out[p.first + i] = -1;
+    return;
+  }
+  PickShared& sh = *reinterpret_cast<PickShared*>(stages);   // (the last products have been waited for)
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) { sh.least[wid] = least; sh.most[wid] = most; }
+  __syncthreads();
+  least = __reduce_min_sync(0xffffffffu, sh.least[lane & 7]);
+  most = __reduce_max_sync(0xffffffffu, sh.most[lane & 7]);
+  pick_select<false, kPtThreads>(sh, scores, x.n, 0, 0, 1, p.top, least, most, p.first, out + p.first);
+}
+
+template <int D>
+static int launch_pick_tc(const PickParams& p, int rows, int smem, cudaStream_t stream) {
+  static PerDeviceOnce configured;
+  if (configured.first_time() && cudaFuncSetAttribute(pick_pages_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return -200;
+  const cudaError_t e = launch_pdl(pick_pages_tc_kernel<D>, dim3(rows, p.hkv), dim3(kPtThreads), smem, stream, p);
   return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
 }
 
@@ -516,6 +751,10 @@ B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block
   p.seqs = seqs; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages;
   p.top = top; p.first = first; p.last = last; p.width = width;
   p.status = static_cast<DeviceStatus*>(status);
+  // Runs of many queries: blocks of their own, as long as their scores fit.
+  const int smem_tc = 1024 + 3 * kPtTile * 2 * d + kPickRows * 8 + static_cast<int>(sizeof(PickTcShared));
+  if (run * (hq / hkv) > kPickFew && smem_tc + 4ll * max_pages <= 232448 && rows < (1 << 30))
+    return d == 128 ? launch_pick_tc<128>(p, rows, smem_tc + 4 * max_pages, stream) : launch_pick_tc<64>(p, rows, smem_tc + 4 * max_pages, stream);
   const int fixed = (static_cast<int>(sizeof(PickShared)) + 15) / 16 * 16 + (run * (hq / hkv) + 7) / 8 * 8 * (2 * d + 64);
   // blocks of a row: as long as every processor has one at most and a block 256 pages to score; at least as many as hold the scores
   p.parts = 1;
