@@ -7,10 +7,11 @@
 //                   score(page) = max over queries of 2^(e_q + e_page) * sum_c max(a_c high_c, a_c low_c),
 //                 a bound of every product of a with a key of the page. max(a h, a l) is a+ h + a- l, so the sum is an integer product of 2 D
 //                 codes: mma.sync on 8-bit integers, exact, below 2^22 and scaled by a power of two. What is kept does not depend on any order.
-#include "mma_sync.cuh"
 #include "picked.cuh"
 
 namespace b200 {
+
+int make_kmajor_map(CUtensorMap* out, const void* base, int elem_bytes, long long rows, long long k, long long ld, int box_rows);
 
 struct BoundsParams {
   const __nv_bfloat16* k;      // [pages][hkv][page][D]
@@ -121,9 +122,12 @@ struct PickRange {
   int n;
 };
 
-// The pages that are kept whatever the scores (written by the block of rank 0); false: nothing is left to choose.
-__device__ __forceinline__ bool pick_range(const PickParams& p, int row, int* out, bool writes, PickRange& x) {
-  x.run = run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)));
+__device__ __forceinline__ RunOfRow pick_run(const PickParams& p, int row) {
+  return run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)));
+}
+
+// The pages that are kept whatever the scores, of run x.run (written by the block of rank 0); false: nothing is left to choose.
+__device__ __forceinline__ bool pick_range(const PickParams& p, int* out, bool writes, PickRange& x) {
   const int end = x.run.begin + x.run.tokens - 1;
   if (x.run.tokens <= 0 || end < 0) {
     if (writes)
@@ -179,12 +183,14 @@ __device__ __forceinline__ unsigned pick_key(float score) {
 
 // The `top` largest of more than `top` scores, of which this block holds the `mine` from number `a0` on, ties to the lowest number: first + number, in order, to
 // out[0 .. top). `least` and `most` bound all keys. Digits of what keys lie above the smallest, as many as it takes: 11 bits where one block holds all
-// scores; 9 in a cluster, whose blocks read one another's counts. All threads of all blocks of the row.
+// scores; 9 in a cluster, whose blocks read one another's counts. All threads of all blocks of the row, or `kThreads` threads
+// (tid) of a block that share barrier `bar`.
 template <bool kCluster, int kThreads>
-__device__ __forceinline__ void pick_select(PickShared& sh, const float* scores, int mine, int a0, int rank, int parts, int top, unsigned least, unsigned most,
+__device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, const float* scores, int mine, int a0, int rank, int parts, int top, unsigned least, unsigned most,
                                             int first, int* out) {
   constexpr int kWarps = kThreads / 32, kDigit = kCluster ? 9 : 11, kBins = 1 << kDigit, kEach = kBins / kThreads;
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int lane = tid & 31, wid = tid >> 5;
+  const auto sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(kThreads) : "memory"); };
   int shift = 32 - __clz(static_cast<int>(most - least));        // bits that differ
   unsigned prefix = 0u, want = static_cast<unsigned>(top);
   for (int pass = 0;; ++pass) {
@@ -192,14 +198,14 @@ __device__ __forceinline__ void pick_select(PickShared& sh, const float* scores,
     shift -= bits;
     unsigned* hist = sh.hist + (kCluster ? (pass & 1) * kBins : 0);      // (a peer may still read those of the pass before)
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) hist[i * kThreads + threadIdx.x] = 0u;
-    __syncthreads();
-    for (int i = threadIdx.x; i < mine; i += kThreads) {
+    for (int i = 0; i < kEach; ++i) hist[i * kThreads + tid] = 0u;
+    sync();
+    for (int i = tid; i < mine; i += kThreads) {
       const unsigned k = pick_key(scores[i]) - least;
       if ((static_cast<unsigned long long>(k) >> (shift + bits)) == prefix) atomicAdd(hist + ((k >> shift) & ((1u << bits) - 1u)), 1u);
     }
     if (kCluster) cluster_sync_all();
-    else __syncthreads();
+    else sync();
     // a thread owns neighbouring bins; how many lie in them and above
     unsigned own[kEach], sum = 0;
 #pragma unroll
@@ -208,9 +214,9 @@ __device__ __forceinline__ void pick_select(PickShared& sh, const float* scores,
       if (kCluster) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (k < parts) own[i] += pick_peer_load(hist + threadIdx.x * kEach + i, k);
+          if (k < parts) own[i] += pick_peer_load(hist + tid * kEach + i, k);
       } else {
-        own[i] = hist[threadIdx.x * kEach + i];
+        own[i] = hist[tid * kEach + i];
       }
       sum += own[i];
     }
@@ -221,21 +227,21 @@ __device__ __forceinline__ void pick_select(PickShared& sh, const float* scores,
       if (lane + o < 32) upto += x;
     }
     if (lane == 0) sh.warp_a[wid] = upto;
-    __syncthreads();
+    sync();
     for (int w = wid + 1; w < kWarps; ++w) upto += sh.warp_a[w];
     unsigned above = upto - sum;
     if (above < want && upto >= want) {
 #pragma unroll
       for (int i = kEach - 1; i >= 0; --i) {
         if (above < want && above + own[i] >= want) {
-          sh.bin = threadIdx.x * kEach + i;
+          sh.bin = tid * kEach + i;
           sh.want = want - above;
           sh.in_bin = own[i];
         }
         above += own[i];
       }
     }
-    __syncthreads();
+    sync();
     prefix = (prefix << bits) | sh.bin;
     want = sh.want;
     if (sh.in_bin == want || shift == 0) break;      // (alike in all blocks)
@@ -250,11 +256,11 @@ __device__ __forceinline__ void pick_select(PickShared& sh, const float* scores,
     tied += __popc(__ballot_sync(0xffffffffu, i < s1 && k == prefix));
   }
   if (lane == 0) { sh.warp_a[wid] = over; sh.warp_b[wid] = tied; }
-  __syncthreads();
+  sync();
   unsigned over0 = 0, tied0 = 0;
   for (int w = 0; w < wid; ++w) { over0 += sh.warp_a[w]; tied0 += sh.warp_b[w]; }
   if (kCluster) {
-    if (threadIdx.x == kThreads - 1) { sh.counts[0] = over0 + over; sh.counts[1] = tied0 + tied; }
+    if (tid == kThreads - 1) { sh.counts[0] = over0 + over; sh.counts[1] = tied0 + tied; }
     cluster_sync_all();
     unsigned x = 0, y = 0;
     if (lane < rank) { x = pick_peer_load(&sh.counts[0], lane); y = pick_peer_load(&sh.counts[1], lane); }
@@ -291,8 +297,8 @@ __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickP
   const int tiles = (p.run * group + 7) / 8;
   float* scores = reinterpret_cast<float*>(codes + tiles * 8 * kPitch);
   int* out = p.out + (static_cast<long long>(row) * p.hkv + h) * p.width;
-  PickRange x;
-  if (!pick_range(p, row, out, rank == 0, x)) return;            // (alike in all blocks of a cluster)
+  PickRange x{pick_run(p, row), 0};
+  if (!pick_range(p, out, rank == 0, x)) return;                 // (alike in all blocks of a cluster)
   const RunOfRow& r = x.run;
 
   // ---- the first bounds on their way
@@ -439,10 +445,10 @@ __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickP
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
   if (p.parts > 1) {
-    pick_select<true, kPickThreads>(sh, scores, mine, a0, rank, p.parts, p.top, least, most, p.first, out + p.first);
+    pick_select<true, kPickThreads>(sh, threadIdx.x, 0, scores, mine, a0, rank, p.parts, p.top, least, most, p.first, out + p.first);
     cluster_sync_all();                        // nobody leaves while a peer may still read its words
   } else {
-    pick_select<false, kPickThreads>(sh, scores, mine, 0, 0, 1, p.top, least, most, p.first, out + p.first);
+    pick_select<false, kPickThreads>(sh, threadIdx.x, 0, scores, mine, 0, 0, 1, p.top, least, most, p.first, out + p.first);
   }
 }
 
@@ -467,119 +473,158 @@ static int launch_pick(const PickParams& p, int rows, int smem, cudaStream_t str
   return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
 }
 
-// The same for runs whose queries (with their heads) are many: a block scores 128 pages at a time for up to 128 queries on the 5th-generation tensor cores.
-// Pages are rows of the product, so a thread of the epilogue owns a page and takes the maximum over the queries by itself.
-//   warps 0..3   copy the codes of 128 pages into one of two stages, 16 bytes a lane, in the layout of a 128-byte swizzle; one thread
-//                issues the products of the stage before
-//   warps 4..7   scores: a page a thread, its 16 to 128 sums from one of two halves of TMEM
-// Bound by the reads of the bounds, 2 D bytes a page and run, from L2. mma.sync has 8-bit products at a fifth of the rate (2048 queries behind 30720: 307 us).
-constexpr int kPtThreads = 256, kPtTile = 128;
+// The same for runs whose queries (with their heads) are many, on the 5th-generation tensor cores: a block scores 128 pages at a time for two neighbouring
+// runs of a sequence, up to 128 queries each. Pages are rows of the product, so a thread of the epilogue owns a page and takes the maximum over a run's queries by itself.
+//   warp 0        TMA producer: the codes of 128 pages into one of three stages, four pages a gather
+//   warp 1        one thread issues the products
+//   warps 8..15   scores: a page a thread, its 16 to 128 sums of one of the runs from one of two halves of TMEM; then half of the block chooses for each run
+// Bound by the gathers: a row of 2 D bytes lies on any 16-byte boundary, and a processor fetches 14 bytes of such rows a cycle, by TMA as by copies of 16 bytes a
+// lane. So a tile serves two runs (one: 218 us for 2048 queries behind 30720; with copies 198; mma.sync, whose 8-bit products have a fifth of the rate, 307).
+constexpr int kPtThreads = 512, kPtTile = 128, kPtStages = 3;
 
 struct PickTcShared {
-  uint64_t a_empty[2], s_full[2], s_empty[2];
+  uint64_t a_full[kPtStages], a_empty[kPtStages], s_full[2], s_empty[2];
   uint32_t tmem_base, abort_flag;
 };
 
+// Four rows of a tensor of bytes, 128 of each from column c on; completion counts bytes on `bar`.
+__device__ __forceinline__ void pick_gather4(void* dst, const CUtensorMap* m, uint64_t* bar, int c, const int (&row)[4]) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3])
+      : "memory");
+}
+
 template <int D>
-__global__ void __launch_bounds__(kPtThreads, 2) pick_pages_tc_kernel(const PickParams p) {
+__global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const PickParams p, const __grid_constant__ CUtensorMap tm) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ uint8_t pick_raw[];
-  constexpr int kAtoms = 2 * D / 128, kRow = 2 * D + kBoundsTail, kStage = kPtTile * 2 * D;
+  constexpr int kAtoms = 2 * D / 128, kRow = 2 * D + kBoundsTail, kStage = kPtTile * 2 * D, kAtom = 2 * kPickRows * 128;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pick_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, group = p.hq / p.hkv;
-  const int row = blockIdx.x, h = blockIdx.y, cols = (p.run * group + 15) & ~15;
-  uint8_t* stages = smem;                                    // [2][atom][128 pages][128 bytes]; the choice works here afterwards
-  uint8_t* codes = stages + 2 * kStage;                      // [atom][128 queries][128 bytes]
-  float2* factor = reinterpret_cast<float2*>(codes + kStage);                    // of a query: 2^e and 0, or 0 and -inf for those that pad
-  PickTcShared& bars = *reinterpret_cast<PickTcShared*>(factor + kPickRows);
-  float* scores = reinterpret_cast<float*>(&bars + 1);
-  int* out = p.out + (static_cast<long long>(row) * p.hkv + h) * p.width;
-  PickRange x;
-  if (!pick_range(p, row, out, true, x)) return;
-  const RunOfRow& r = x.run;
-  const int n_tiles = (x.n + kPtTile - 1) / kPtTile;
-  const int* ids = p.block_table + static_cast<long long>(r.seq) * p.max_pages + p.first;
+  const int row = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, cols = (p.run * group + 15) & ~15;
+  uint8_t* stages = smem;                                    // [3][atom][128 pages][128 bytes]; the choice works here afterwards
+  uint8_t* codes = stages + kPtStages * kStage;              // [atom][256 queries][128 bytes]
+  float2* factor = reinterpret_cast<float2*>(codes + kAtoms * kAtom);            // of a query: 2^e and 0, or 0 and -inf for those that pad
+  PickTcShared& bars = *reinterpret_cast<PickTcShared*>(factor + 2 * kPickRows);
+  float* scores = reinterpret_cast<float*>(&bars + 1);       // [2][pages]
+  const auto out_of = [&](int i) { return p.out + (static_cast<long long>(i) * p.hkv + h) * p.width; };
+  // the runs of this block: an even one of a sequence and the one behind it (whose own block leaves). Rows of no run are written by their own blocks.
+  PickRange x[2];
+  int rows[2], runs = 0;
+  {
+    PickRange y{pick_run(p, row), 0};
+    const int len = y.run.kv_len - y.run.begin, rest = len - y.run.tokens;      // queries from the run's first on, and behind the run
+    const int first_q = p.cu_q ? p.cu_q[y.run.seq] : y.run.seq;
+    if (y.run.tokens > 0 && ((y.run.q_off - first_q) / p.run & 1)) return;
+    if (pick_range(p, out_of(row), true, y)) { x[runs] = y; rows[runs++] = row; }
+    if (y.run.tokens > 0 && rest > 0) {
+      y.run.q_off += p.run;
+      y.run.begin += p.run;
+      y.run.tokens = min(p.run, rest);
+      if (pick_range(p, out_of(row + 1), true, y)) { x[runs] = y; rows[runs++] = row + 1; }
+    }
+    if (runs == 0) return;
+    if (runs == 1) { x[1] = x[0]; rows[1] = rows[0]; }
+  }
+  const int n = max(x[0].n, x[1].n), n_tiles = (n + kPtTile - 1) / kPtTile;
+  const int* ids = p.block_table + static_cast<long long>(x[0].run.seq) * p.max_pages + p.first;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kPtStages; ++i) {
+      mbar_init(&bars.a_full[i], 4);
       mbar_init(&bars.a_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.s_empty[i], 4);
+      mbar_init(&bars.s_empty[i], 4 * runs);
     }
     bars.abort_flag = 0;
     fence_mbar_init();
+    prefetch_tensormap(&tm);
   }
-  if (wid == 4) {
-    tmem_alloc(&bars.tmem_base, 256);
+  if (wid == 2) {
+    tmem_alloc(&bars.tmem_base, 512);
     tmem_relinquish();
   }
   volatile uint32_t* abort_flag = &bars.abort_flag;
-  // sixteen (D = 128) or eight lanes a page
-  constexpr int kLanes = 2 * D / 16, kPages = 128 / kLanes;      // pages that warps 0..3 copy at a time
-  const int piece = threadIdx.x % kLanes;
-  const auto copy = [&](int j) {
-#pragma unroll 4
-    for (int i = 0; i < kPtTile / kPages; ++i) {
-      const int at = i * kPages + threadIdx.x / kLanes, id = ids[min(j * kPtTile + at, x.n - 1)];
-      const bool ok = id >= 0 && id < p.pages;
-      cp_async_16(smem_u32(stages + (j & 1) * kStage + (piece >> 3) * (kPtTile * 128) + at * 128 + (((piece & 7) ^ (at & 7)) << 4)),
-                  p.bounds + (static_cast<long long>(ok ? id : 0) * p.hkv + h) * kRow + piece * 16, ok);
+  __syncthreads();
+  // rows of the pool of bounds: of four neighbouring pages of a tile (one that is no page lies behind the end and arrives as zeros)
+  const int quad = (wid & 3) * 8 + (lane & 7);
+  const auto rows_of = [&](int j, int (&to)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int id = ids[min(j * kPtTile + quad * 4 + i, n - 1)];
+      to[i] = id >= 0 && id < p.pages ? id * p.hkv + h : static_cast<int>(p.pages * p.hkv);
     }
-    cp_async_commit();
   };
-  if (wid < 4) copy(0);
-
-  // ---- codes of the queries, four at a time
-  for (int i0 = wid * 4; i0 < cols; i0 += 32) {
-    constexpr int kEach = D / 32;
-    float v[4][kEach];
-    bool real[4];
+  const auto gather = [&](int j, const int (&from)[4]) {
+    const int s = j % kPtStages;
+    if (lane == 0) mbar_arrive_expect_tx(&bars.a_full[s], kStage / 4);
+    __syncwarp();
+    if (lane < 8) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u;
-      real[u] = i < r.tokens * group && r.begin + i / group >= 0;
-#pragma unroll
-      for (int k = 0; k < kEach; ++k) v[u][k] = 0.f;
-      if (real[u]) {
-        const __nv_bfloat16* src = p.q + (static_cast<long long>(r.q_off + i / group) * p.hq + h * group + i % group) * D + lane * kEach;
-#pragma unroll
-        for (int k = 0; k < kEach; k += 2) {
-          const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + k));
-          v[u][k] = f.x;
-          v[u][k + 1] = f.y;
-        }
-      }
+      for (int a = 0; a < kAtoms; ++a) pick_gather4(stages + s * kStage + a * (kPtTile * 128) + quad * 512, &tm, &bars.a_full[s], a * 128, from);
     }
+  };
+  int next[4];
+  if (wid >= 4 && wid < 8) {                                 // the first tiles are on their way while the queries are coded
+    for (int j = 0; j < min(n_tiles, kPtStages); ++j) {
+      rows_of(j, next);
+      gather(j, next);
+    }
+    rows_of(kPtStages < n_tiles ? kPtStages : 0, next);
+  }
+
+  // ---- codes of the queries: D / 8 lanes a query, 16 bytes each, half of the loads of a warp ahead of their use
+  {
+    constexpr int kQLanes = D / 8, kQueries = 32 / kQLanes, kRounds = kPickRows / (16 * kQueries);
+    const int u = lane % kQLanes;
+    for (int w = 0; w < runs; ++w) {
+      const RunOfRow& r = x[w].run;
+      uint4 raw[kRounds];
+      bool real[kRounds];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u;
-      float amax = 0.f;
+      for (int k = 0; k < kRounds; ++k) {
+        const int i = (k * 16 + wid) * kQueries + lane / kQLanes, token = i / group;
+        real[k] = token < r.tokens && r.begin + token >= 0;
+        raw[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (real[k]) raw[k] = __ldg(reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(r.q_off + token) * p.hq + h * group + i - token * group) * D + u * 8));
+      }
 #pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        v[u][k] = v[u][k] == v[u][k] ? v[u][k] : 0.f;
-        amax = fmaxf(amax, fabsf(v[u][k]));
-      }
-      const int e = bounds_exponent(warp_max(amax));
-      const float f = bounds_pow2(-e);
-      uint32_t up = 0, down = 0;
+      for (int k = 0; k < kRounds; ++k) {
+        const int i = (k * 16 + wid) * kQueries + lane / kQLanes, at = w * cols + i;
+        const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw[k]);
+        float v[8], amax = 0.f;
 #pragma unroll
-      for (int k = 0; k < kEach; ++k) {
-        const int c = static_cast<int>(fminf(fmaxf(rintf(v[u][k] * f), -127.f), 127.f));
-        up |= static_cast<uint32_t>(max(c, 0)) << (8 * k);
-        down |= (static_cast<uint32_t>(min(c, 0)) & 0xffu) << (8 * k);
+        for (int y = 0; y < 4; ++y) {
+          const float2 f = __bfloat1622float2(b[y]);
+          v[2 * y] = f.x == f.x ? f.x : 0.f;
+          v[2 * y + 1] = f.y == f.y ? f.y : 0.f;
+          amax = fmaxf(amax, fmaxf(fabsf(v[2 * y]), fabsf(v[2 * y + 1])));
+        }
+#pragma unroll
+        for (int o = kQLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const int e = bounds_exponent(amax);
+        const float f = bounds_pow2(-e);
+        uint2 up = make_uint2(0u, 0u), down = make_uint2(0u, 0u);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int c = static_cast<int>(fminf(fmaxf(rintf(v[y] * f), -127.f), 127.f)), d = static_cast<int>(fminf(fmaxf(rintf(v[4 + y] * f), -127.f), 127.f));
+          up.x |= static_cast<uint32_t>(max(c, 0)) << (8 * y);
+          down.x |= (static_cast<uint32_t>(min(c, 0)) & 0xffu) << (8 * y);
+          up.y |= static_cast<uint32_t>(max(d, 0)) << (8 * y);
+          down.y |= (static_cast<uint32_t>(min(d, 0)) & 0xffu) << (8 * y);
+        }
+        if (i >= cols) continue;
+        const auto place = [&](int byte) {
+          return reinterpret_cast<uint2*>(codes + (byte >> 7) * kAtom + at * 128 + ((((byte >> 4) & 7) ^ (at & 7)) << 4) + (byte & 15));
+        };
+        *place(u * 8) = up;
+        *place(D + u * 8) = down;
+        if (u == 0) factor[at] = real[k] ? make_float2(bounds_pow2(e), 0.f) : make_float2(0.f, -INFINITY);
       }
-      const auto place = [&](int byte) {
-        return codes + (byte >> 7) * (kPtTile * 128) + i * 128 + ((((byte >> 4) & 7) ^ (i & 7)) << 4) + (byte & 15);
-      };
-      if (kEach == 4) {
-        *reinterpret_cast<uint32_t*>(place(lane * 4)) = up;
-        *reinterpret_cast<uint32_t*>(place(D + lane * 4)) = down;
-      } else {
-        *reinterpret_cast<uint16_t*>(place(lane * 2)) = static_cast<uint16_t>(up);
-        *reinterpret_cast<uint16_t*>(place(D + lane * 2)) = static_cast<uint16_t>(down);
-      }
-      if (lane == 0) factor[i] = real[u] ? make_float2(bounds_pow2(e), 0.f) : make_float2(0.f, -INFINITY);
     }
   }
   fence_proxy_async_smem();
@@ -589,63 +634,69 @@ __global__ void __launch_bounds__(kPtThreads, 2) pick_pages_tc_kernel(const Pick
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_base);
   unsigned least = 0xffffffffu, most = 0u;
 
-  if (wid < 4) {
-    // every thread makes all rounds, whatever runs out: the group's barrier counts on it
-    const uint32_t idesc = make_idesc(128, cols, kFmtS8, kFmtS8, 2);
-    const auto multiply = [&](int j) {
-      fence_proxy_async_smem();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (threadIdx.x != 0) return;
-      if (j >= 2 && !mbar_wait(&bars.s_empty[j & 1], static_cast<uint32_t>(((j >> 1) - 1) & 1), abort_flag)) {
-        report_status(p.status, kWaitTimeout, kKernelPicked, 22, blockIdx.x);
-        return;
+  if (wid >= 4 && wid < 8) {
+    for (int j = kPtStages; j < n_tiles; ++j) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars.a_empty[j % kPtStages], static_cast<uint32_t>((j / kPtStages - 1) & 1), abort_flag))) {
+        if (lane == 0) report_status(p.status, kWaitTimeout, kKernelPicked, 22, blockIdx.x);
+        // copies on their way land before the shared memory is given back
+        uint32_t none = 0;
+        for (int i = j - kPtStages; i < j; ++i) mbar_wait(&bars.a_full[i % kPtStages], static_cast<uint32_t>((i / kPtStages) & 1), &none);
+        break;
       }
-      tc_fence_after_sync();
-#pragma unroll
-      for (int a = 0; a < kAtoms; ++a) {
-        const uint64_t ad = make_desc_sw128(smem_u32(stages + (j & 1) * kStage + a * (kPtTile * 128)));
-        const uint64_t bd = make_desc_sw128(smem_u32(codes + a * (kPtTile * 128)));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mma_i8_ss(tmem_base + (j & 1) * 128, ad + 2 * k, bd + 2 * k, idesc, (a | k) != 0);
-      }
-      tc_commit(&bars.s_full[j & 1]);
-      tc_commit(&bars.a_empty[j & 1]);
-    };
-    for (int j = 1; j < n_tiles; ++j) {
-      if (j >= 2 && !mbar_wait(&bars.a_empty[j & 1], static_cast<uint32_t>(((j >> 1) - 1) & 1), abort_flag) && threadIdx.x == 0)
-        report_status(p.status, kWaitTimeout, kKernelPicked, 23, blockIdx.x);
-      copy(j);
-      cp_async_wait<1>();
-      multiply(j - 1);
+      gather(j, next);
+      if (j + 1 < n_tiles) rows_of(j + 1, next);
     }
-    cp_async_wait<0>();
-    multiply(n_tiles - 1);
-  } else {
-    const int mine = threadIdx.x - 128;                      // page of a tile = TMEM lane
-    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>((wid & 3) * 32) << 16);
+  } else if (wid == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = make_idesc(128, runs * cols, kFmtS8, kFmtS8, 2);
+      for (int j = 0; j < n_tiles; ++j) {
+        const int s = j % kPtStages;
+        if (!mbar_wait(&bars.a_full[s], static_cast<uint32_t>((j / kPtStages) & 1), abort_flag) ||
+            (j >= 2 && !mbar_wait(&bars.s_empty[j & 1], static_cast<uint32_t>(((j >> 1) - 1) & 1), abort_flag))) {
+          report_status(p.status, kWaitTimeout, kKernelPicked, 23, blockIdx.x);
+          break;
+        }
+        tc_fence_after_sync();
+#pragma unroll
+        for (int a = 0; a < kAtoms; ++a) {
+          const uint64_t ad = make_desc_sw128(smem_u32(stages + s * kStage + a * (kPtTile * 128)));
+          const uint64_t bd = make_desc_sw128(smem_u32(codes + a * kAtom));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_i8_ss(tmem_base + (j & 1) * 256, ad + 2 * k, bd + 2 * k, idesc, (a | k) != 0);
+        }
+        tc_commit(&bars.s_full[j & 1]);
+        tc_commit(&bars.a_empty[s]);
+      }
+    }
+    __syncwarp();
+  } else if (wid >= 8 && wid < 8 + 4 * runs) {
+    const int w = (wid - 8) >> 2, mine = threadIdx.x & 127;  // run, page of a tile = TMEM lane
+    const uint32_t column = tmem_base + (static_cast<uint32_t>((wid & 3) * 32) << 16) + w * cols;
+    const float2* const mult = factor + w * cols;
+    float* const to = scores + w * p.max_pages;
     // the exponent of the tile's page, one tile ahead
     const auto unit_of = [&](int j) {
       const int at = j * kPtTile + mine;
-      if (at >= x.n) return 0.f;
+      if (at >= x[w].n) return 0.f;
       const int id = ids[at];
       if (id < 0 || id >= p.pages) {
-        report_status(p.status, kBadArgument, kKernelPicked, 2, static_cast<uint32_t>(r.seq));
+        report_status(p.status, kBadArgument, kKernelPicked, 2, static_cast<uint32_t>(x[0].run.seq));
         return 0.f;
       }
       return bounds_pow2(min(50, max(-50, static_cast<int>(__ldg(p.bounds + (static_cast<long long>(id) * p.hkv + h) * kRow + 2 * D)) - kBoundsBias)));
     };
     float unit = unit_of(0);
     for (int j = 0; j < n_tiles; ++j) {
-      const float next = j + 1 < n_tiles ? unit_of(j + 1) : 0.f;
+      const float ahead = j + 1 < n_tiles ? unit_of(j + 1) : 0.f;
       if (!__all_sync(0xffffffffu, mbar_wait(&bars.s_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag))) {
         if (lane == 0) report_status(p.status, kWaitTimeout, kKernelPicked, 24, blockIdx.x);
         break;
       }
       tc_fence_after_sync();
       float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      for (int c0 = 0; c0 < cols; c0 += 32) {                // (behind the last column TMEM holds anything: not used)
+      for (int c0 = 0; c0 < cols; c0 += 32) {                // (columns behind the run's are read, not used; the last ones end with TMEM)
         uint32_t s[32];
-        tmem_ld_32x32(lane_base + (j & 1) * 128 + c0, s);
+        tmem_ld_32x32(column + (j & 1) * 256 + c0, s);
         tmem_ld_wait();
         if (c0 + 32 >= cols) {                               // the products of the tile after the next may take these columns
           tc_fence_before_sync();
@@ -655,48 +706,57 @@ __global__ void __launch_bounds__(kPtThreads, 2) pick_pages_tc_kernel(const Pick
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           if (i == 16 && c0 + 16 >= cols) break;
-          const float4 f = *reinterpret_cast<const float4*>(factor + c0 + i);
+          const float4 f = *reinterpret_cast<const float4*>(mult + c0 + i);
           best[i & 2] = fmaxf(best[i & 2], fmaf(static_cast<float>(static_cast<int>(s[i])), f.x, f.y));
           best[(i & 2) + 1] = fmaxf(best[(i & 2) + 1], fmaf(static_cast<float>(static_cast<int>(s[i + 1])), f.z, f.w));
         }
       }
       const int at = j * kPtTile + mine;
-      if (at < x.n) {
+      if (at < x[w].n) {
         const float score = unit > 0.f ? fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * unit : -INFINITY;
         const unsigned k = pick_key(score);
         least = min(least, k);
         most = max(most, k);
-        scores[at] = score;
+        to[at] = score;
       }
-      unit = next;
+      unit = ahead;
     }
   }
   __syncwarp();
   tc_fence_before_sync();
   __syncthreads();
-  if (wid == 4) {
+  if (wid == 2) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem_base, 256);
+    tmem_dealloc(tmem_base, 512);
   }
+  const int w = wid >> 3;                                    // the run that this half of the block chooses for
   if (*abort_flag) {                                         // nothing is chosen
-    for (int i = threadIdx.x; i < p.top; i += kPtThreads) out[p.first + i] = -1;
+    if (w < runs)
+      for (int i = threadIdx.x & 255; i < p.top; i += 256) out_of(rows[w])[p.first + i] = -1;
     return;
   }
-  PickShared& sh = *reinterpret_cast<PickShared*>(stages);   // (the last products have been waited for)
+  PickShared* sh = reinterpret_cast<PickShared*>(stages);    // [2] (the last products have been waited for)
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
-  if (lane == 0) { sh.least[wid] = least; sh.most[wid] = most; }
+  if (wid >= 8 && lane == 0) {
+    sh[(wid - 8) >> 2].least[wid & 3] = least;
+    sh[(wid - 8) >> 2].most[wid & 3] = most;
+  }
   __syncthreads();
-  least = __reduce_min_sync(0xffffffffu, sh.least[lane & 7]);
-  most = __reduce_max_sync(0xffffffffu, sh.most[lane & 7]);
-  pick_select<false, kPtThreads>(sh, scores, x.n, 0, 0, 1, p.top, least, most, p.first, out + p.first);
+  if (w >= runs) return;
+  least = __reduce_min_sync(0xffffffffu, sh[w].least[lane & 3]);
+  most = __reduce_max_sync(0xffffffffu, sh[w].most[lane & 3]);
+  pick_select<false, 256>(sh[w], threadIdx.x & 255, 1 + w, scores + w * p.max_pages, x[w].n, 0, 0, 1, p.top, least, most, p.first, out_of(rows[w]) + p.first);
 }
 
 template <int D>
 static int launch_pick_tc(const PickParams& p, int rows, int smem, cudaStream_t stream) {
   static PerDeviceOnce configured;
   if (configured.first_time() && cudaFuncSetAttribute(pick_pages_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return -200;
-  const cudaError_t e = launch_pdl(pick_pages_tc_kernel<D>, dim3(rows, p.hkv), dim3(kPtThreads), smem, stream, p);
+  CUtensorMap tm;
+  const int rc = make_kmajor_map(&tm, p.bounds, 1, p.pages * p.hkv, 2 * D, 2 * D + kBoundsTail, 1);
+  if (rc) return rc;
+  const cudaError_t e = launch_pdl(pick_pages_tc_kernel<D>, dim3(static_cast<unsigned>(rows) * p.hkv), dim3(kPtThreads), smem, stream, p, tm);
   return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
 }
 
@@ -752,9 +812,9 @@ B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block
   p.top = top; p.first = first; p.last = last; p.width = width;
   p.status = static_cast<DeviceStatus*>(status);
   // Runs of many queries: blocks of their own, as long as their scores fit.
-  const int smem_tc = 1024 + 3 * kPtTile * 2 * d + kPickRows * 8 + static_cast<int>(sizeof(PickTcShared));
-  if (run * (hq / hkv) > kPickFew && smem_tc + 4ll * max_pages <= 232448 && rows < (1 << 30))
-    return d == 128 ? launch_pick_tc<128>(p, rows, smem_tc + 4 * max_pages, stream) : launch_pick_tc<64>(p, rows, smem_tc + 4 * max_pages, stream);
+  const long long smem_tc = 1024 + (kPtStages * kPtTile + 2 * kPickRows) * 2 * d + 2 * kPickRows * 8 + static_cast<int>(sizeof(PickTcShared)) + 8ll * max_pages;
+  if (run * (hq / hkv) > kPickFew && smem_tc <= 232448 && static_cast<long long>(rows) * hkv < (1ll << 31) && pages * hkv < (1ll << 31))
+    return d == 128 ? launch_pick_tc<128>(p, rows, static_cast<int>(smem_tc), stream) : launch_pick_tc<64>(p, rows, static_cast<int>(smem_tc), stream);
   const int fixed = (static_cast<int>(sizeof(PickShared)) + 15) / 16 * 16 + (run * (hq / hkv) + 7) / 8 * 8 * (2 * d + 64);
   // blocks of a row: as long as every processor has one at most and a block 256 pages to score; at least as many as hold the scores
   p.parts = 1;
