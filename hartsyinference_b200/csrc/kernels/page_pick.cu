@@ -113,7 +113,7 @@ struct PickShared {
   unsigned warp_a[kPickWarps], warp_b[kPickWarps];
   unsigned counts[2];               // this block's selected and tied ones
   unsigned bin, want, in_bin;
-  __align__(16) float2 row[kPickRows];      // 2^e and 0, or 0 and -inf for rows that pad
+  __align__(16) float2 row[kPickRows];      // of a query (pick_factor)
 };
 
 // What a row of runs chooses between: pages first .. first + n are scored, if there are more of them than `top`.
@@ -175,6 +175,14 @@ __device__ __forceinline__ void pick_peer_store(const void* local, int block, un
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(pick_peer(local, block)), "r"(v) : "memory");
 }
 
+// A sum times 2^e, where f = (2^e, -1.5 * 2^(23 + e)), or -inf where f = (0, -inf): sums are below 2^22, so 1.5 * 2^23 + sum is a float with the sum
+// in its last bits, and the fused product takes the large number off again, exactly (a conversion takes four times as long).
+__device__ __forceinline__ float pick_scaled(int sum, float f, float off) { return fmaf(__int_as_float(sum + 0x4b400000), f, off); }
+__device__ __forceinline__ float2 pick_factor(bool real, int e) {
+  const float f = bounds_pow2(e);
+  return real ? make_float2(f, -12582912.f * f) : make_float2(0.f, -INFINITY);
+}
+
 // Keys order like scores.
 __device__ __forceinline__ unsigned pick_key(float score) {
   const unsigned u = __float_as_uint(score);
@@ -197,8 +205,13 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
     const int bits = min(kDigit, shift);
     shift -= bits;
     unsigned* hist = sh.hist + (kCluster ? (pass & 1) * kBins : 0);      // (a peer may still read those of the pass before)
+    if (kEach >= 4) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) hist[i * kThreads + tid] = 0u;
+      for (int i = 0; i < kEach / 4; ++i) reinterpret_cast<uint4*>(hist)[i * kThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) hist[i * kThreads + tid] = 0u;
+    }
     sync();
     for (int i = tid; i < mine; i += kThreads) {
       const unsigned k = pick_key(scores[i]) - least;
@@ -210,13 +223,14 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
     unsigned own[kEach], sum = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      own[i] = 0;
       if (kCluster) {
+        own[i] = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           if (k < parts) own[i] += pick_peer_load(hist + tid * kEach + i, k);
-      } else {
-        own[i] = hist[tid * kEach + i];
+      } else if (i % 4 == 0) {                 // (four bins at a time: one by one the lanes would meet in the banks)
+        const uint4 x = *reinterpret_cast<const uint4*>(hist + tid * kEach + i);
+        own[i] = x.x; own[i + 1] = x.y; own[i + 2] = x.z; own[i + 3] = x.w;
       }
       sum += own[i];
     }
@@ -366,7 +380,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickP
       *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(up);
       *reinterpret_cast<uint16_t*>(dst + D) = static_cast<uint16_t>(down);
     }
-    if (lane == 0) sh.row[i] = real ? make_float2(bounds_pow2(e), 0.f) : make_float2(0.f, -INFINITY);
+    if (lane == 0) sh.row[i] = pick_factor(real, e);
   }
   if (p.parts > 1) cluster_sync_all();          // (the peers' memory is there)
   else __syncthreads();
@@ -395,8 +409,8 @@ __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickP
       const float4 f = *reinterpret_cast<const float4*>(sh.row + t * 8 + 2 * kq);      // of queries 2 kq and 2 kq + 1
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        best[i] = fmaxf(best[i], fmaxf(fmaf(static_cast<float>(acc[0][2 * i] + acc[1][2 * i]), f.x, f.y),
-                                       fmaf(static_cast<float>(acc[0][2 * i + 1] + acc[1][2 * i + 1]), f.z, f.w)));
+        best[i] = fmaxf(best[i], fmaxf(pick_scaled(acc[0][2 * i] + acc[1][2 * i], f.x, f.y),
+                                       pick_scaled(acc[0][2 * i + 1] + acc[1][2 * i + 1], f.z, f.w)));
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -506,7 +520,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
   const int row = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, cols = (p.run * group + 15) & ~15;
   uint8_t* stages = smem;                                    // [3][atom][128 pages][128 bytes]; the choice works here afterwards
   uint8_t* codes = stages + kPtStages * kStage;              // [atom][256 queries][128 bytes]
-  float2* factor = reinterpret_cast<float2*>(codes + kAtoms * kAtom);            // of a query: 2^e and 0, or 0 and -inf for those that pad
+  float2* factor = reinterpret_cast<float2*>(codes + kAtoms * kAtom);            // of a query (pick_factor)
   PickTcShared& bars = *reinterpret_cast<PickTcShared*>(factor + 2 * kPickRows);
   float* scores = reinterpret_cast<float*>(&bars + 1);       // [2][pages]
   const auto out_of = [&](int i) { return p.out + (static_cast<long long>(i) * p.hkv + h) * p.width; };
@@ -580,14 +594,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
   // ---- codes of the queries: D / 8 lanes a query, 16 bytes each, half of the loads of a warp ahead of their use
   {
     constexpr int kQLanes = D / 8, kQueries = 32 / kQLanes, kRounds = kPickRows / (16 * kQueries);
-    const int u = lane % kQLanes;
+    const int u = lane % kQLanes, inverse = (65536 + group - 1) / group;      // i / group for i < 128 is a product and a shift
     for (int w = 0; w < runs; ++w) {
       const RunOfRow& r = x[w].run;
       uint4 raw[kRounds];
       bool real[kRounds];
 #pragma unroll
       for (int k = 0; k < kRounds; ++k) {
-        const int i = (k * 16 + wid) * kQueries + lane / kQLanes, token = i / group;
+        const int i = (k * 16 + wid) * kQueries + lane / kQLanes, token = i * inverse >> 16;
         real[k] = token < r.tokens && r.begin + token >= 0;
         raw[k] = make_uint4(0u, 0u, 0u, 0u);
         if (real[k]) raw[k] = __ldg(reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(r.q_off + token) * p.hq + h * group + i - token * group) * D + u * 8));
@@ -623,7 +637,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
         };
         *place(u * 8) = up;
         *place(D + u * 8) = down;
-        if (u == 0) factor[at] = real[k] ? make_float2(bounds_pow2(e), 0.f) : make_float2(0.f, -INFINITY);
+        if (u == 0) factor[at] = pick_factor(real[k], e);
       }
     }
   }
@@ -674,52 +688,54 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
     const uint32_t column = tmem_base + (static_cast<uint32_t>((wid & 3) * 32) << 16) + w * cols;
     const float2* const mult = factor + w * cols;
     float* const to = scores + w * p.max_pages;
-    // the exponent of the tile's page, one tile ahead
-    const auto unit_of = [&](int j) {
-      const int at = j * kPtTile + mine;
-      if (at >= x[w].n) return 0.f;
-      const int id = ids[at];
-      if (id < 0 || id >= p.pages) {
-        report_status(p.status, kBadArgument, kKernelPicked, 2, static_cast<uint32_t>(x[0].run.seq));
-        return 0.f;
-      }
-      return bounds_pow2(min(50, max(-50, static_cast<int>(__ldg(p.bounds + (static_cast<long long>(id) * p.hkv + h) * kRow + 2 * D)) - kBoundsBias)));
+    // the exponent of the tile's page, one tile ahead, and the page's number two ahead
+    const int count = x[w].n;
+    const auto id_of = [&](int j) { return ids[min(j * kPtTile + mine, count - 1)]; };
+    // (a loaded value is first looked at a tile later: a test of it here would wait for it)
+    const auto exponent_of = [&](int id) {
+      return static_cast<int>(__ldg(p.bounds + (static_cast<long long>(id >= 0 && id < p.pages ? id : 0) * p.hkv + h) * kRow + 2 * D));
     };
-    float unit = unit_of(0);
+    int id = id_of(0), behind = id_of(1), exponent = exponent_of(id);
     for (int j = 0; j < n_tiles; ++j) {
-      const float ahead = j + 1 < n_tiles ? unit_of(j + 1) : 0.f;
+      const int ahead = exponent_of(behind), far = id_of(j + 2);
       if (!__all_sync(0xffffffffu, mbar_wait(&bars.s_full[j & 1], static_cast<uint32_t>((j >> 1) & 1), abort_flag))) {
         if (lane == 0) report_status(p.status, kWaitTimeout, kKernelPicked, 24, blockIdx.x);
         break;
       }
       tc_fence_after_sync();
       float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      for (int c0 = 0; c0 < cols; c0 += 32) {                // (columns behind the run's are read, not used; the last ones end with TMEM)
-        uint32_t s[32];
-        tmem_ld_32x32(column + (j & 1) * 256 + c0, s);
+      // 64 columns a time (those behind the run's are read, not used; the last ones end with TMEM)
+      for (int c0 = 0; c0 < cols; c0 += 64) {
+        uint32_t s[64];
+        tmem_ld_32x32(column + (j & 1) * 256 + c0, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        if (c0 + 32 < cols) tmem_ld_32x32(column + (j & 1) * 256 + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
         tmem_ld_wait();
-        if (c0 + 32 >= cols) {                               // the products of the tile after the next may take these columns
+        if (c0 + 64 >= cols) {                               // the products of the tile after the next may take these columns
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars.s_empty[j & 1]);
         }
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          if (i == 16 && c0 + 16 >= cols) break;
+        for (int i = 0; i < 64; i += 2) {
+          if (i % 16 == 0 && c0 + i >= cols) break;
           const float4 f = *reinterpret_cast<const float4*>(mult + c0 + i);
-          best[i & 2] = fmaxf(best[i & 2], fmaf(static_cast<float>(static_cast<int>(s[i])), f.x, f.y));
-          best[(i & 2) + 1] = fmaxf(best[(i & 2) + 1], fmaf(static_cast<float>(static_cast<int>(s[i + 1])), f.z, f.w));
+          best[(i >> 1) & 3] = fmaxf(best[(i >> 1) & 3], fmaxf(pick_scaled(static_cast<int>(s[i]), f.x, f.y), pick_scaled(static_cast<int>(s[i + 1]), f.z, f.w)));
         }
       }
       const int at = j * kPtTile + mine;
-      if (at < x[w].n) {
-        const float score = unit > 0.f ? fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * unit : -INFINITY;
+      if (at < count) {
+        const bool ok = id >= 0 && id < p.pages;
+        if (!ok) report_status(p.status, kBadArgument, kKernelPicked, 2, static_cast<uint32_t>(x[0].run.seq));
+        const float unit = bounds_pow2(min(50, max(-50, exponent - kBoundsBias)));
+        const float score = ok ? fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * unit : -INFINITY;
         const unsigned k = pick_key(score);
         least = min(least, k);
         most = max(most, k);
         to[at] = score;
       }
-      unit = ahead;
+      exponent = ahead;
+      id = behind;
+      behind = far;
     }
   }
   __syncwarp();
