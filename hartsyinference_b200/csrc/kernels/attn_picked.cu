@@ -397,8 +397,8 @@ using namespace b200;
 constexpr int kPickedWidth = 4096;
 
 // Whether rows of `cols` columns (queries times heads of a group) go through the tensor-core tiles of attn_picked_tc.cu (1) or b200_attn_picked (0).
-B200_API int b200_attn_picked_form(int rows, int cols, int hkv, int page, int width, long long pages, float scale, float softcap) {
-  if (width > 1024 || !(scale > 0.f) || softcap > 0.f || pages * hkv * page >= (1ll << 31)) return 0;
+B200_API int b200_attn_picked_form(int rows, int cols, int hkv, int d, int page, int width, long long pages, float scale, float softcap) {
+  if (cols <= 16 || width > 1024 || !(scale > 0.f) || softcap > 0.f || pages * hkv * page >= (1ll << 31)) return 0;
   return cols >= 48;
 }
 

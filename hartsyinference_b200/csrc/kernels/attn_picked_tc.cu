@@ -30,7 +30,7 @@ struct TpBarriers {
   uint64_t v_ask, v_clean;                // the V tile at hand has landed; its rows are cleared
   uint64_t s_full[2], p_ready[2], o_done;
   uint32_t tmem_base, abort_flag;
-  int entries, odd;                       // pages up to the last real one; keys that rows add by themselves
+  int entries, free_entries, odd;         // pages up to the last real one; those in front of the first that not all rows see; keys that rows add by themselves
   int odd_keys[kTpOdd];                   // place in the list of keys
 };
 
@@ -90,6 +90,7 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
     }
     bars->abort_flag = 0;
     bars->entries = 0;
+    bars->free_entries = p.width;
     bars->odd = 0;
     fence_mbar_init();
     prefetch_tensormap(&tm_q);
@@ -103,7 +104,7 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
   __syncthreads();
   {
     const int* mine = p.picked + (static_cast<long long>(row_id) * p.hkv + h) * p.width;
-    int last = 0;
+    int last = 0, partly = p.width;
     for (int i = threadIdx.x; i < p.width; i += kTpThreads) {
       const int at = mine[i];
       int2 e = make_int2(p.pool_rows, kTpFar);
@@ -117,9 +118,14 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
         }
       }
       list[i] = e;
+      if (e.y + (1 << p.page_shift) > r.begin + 1) partly = min(partly, i);
     }
     last = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0) atomicMax(&bars->entries, last);
+    partly = __reduce_min_sync(0xffffffffu, partly);
+    if (lane == 0) {
+      atomicMax(&bars->entries, last);
+      atomicMin(&bars->free_entries, partly);
+    }
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -139,7 +145,9 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
   };
   const int free_keys = r.begin + 1;                    // keys that every row sees
   // whether a tile has keys that some row does not see
+  const int free_tiles = min(bars->free_entries << per_page, pieces) >> per_tile_shift;
   const auto masked = [&](int j) {
+    if (j < free_tiles) return false;
     bool some = false;
     for (int i = 0; i < 1 << per_tile_shift; ++i) some |= piece((j << per_tile_shift) + i).y + box > free_keys;
     return some;

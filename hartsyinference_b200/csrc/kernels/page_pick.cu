@@ -94,7 +94,6 @@ __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
 // ------------------------------------------------------------------------------------------ the choice
 constexpr int kPickThreads = 512, kPickWarps = 16, kPickBins = 2048;
 constexpr int kPickRows = 128;          // queries of a run, heads counted
-constexpr int kPickFew = 32;            // of which so many are multiplied by mma.sync
 constexpr int kPickStep = 16;           // pages that a warp scores at a time
 
 struct PickParams {
@@ -113,7 +112,7 @@ struct PickShared {
   unsigned warp_a[kPickWarps], warp_b[kPickWarps];
   unsigned counts[2];               // this block's selected and tied ones
   unsigned bin, want, in_bin;
-  __align__(16) float2 row[kPickRows];      // of a query (pick_factor)
+  __align__(16) float row[kPickRows];       // of a query: 2^e
 };
 
 // What a row of runs chooses between: pages first .. first + n are scored, if there are more of them than `top`.
@@ -175,12 +174,30 @@ __device__ __forceinline__ void pick_peer_store(const void* local, int block, un
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(pick_peer(local, block)), "r"(v) : "memory");
 }
 
-// A sum times 2^e, where f = (2^e, -1.5 * 2^(23 + e)), or -inf where f = (0, -inf): sums are below 2^22, so 1.5 * 2^23 + sum is a float with the sum
-// in its last bits, and the fused product takes the large number off again, exactly (a conversion takes four times as long).
-__device__ __forceinline__ float pick_scaled(int sum, float f, float off) { return fmaf(__int_as_float(sum + 0x4b400000), f, off); }
-__device__ __forceinline__ float2 pick_factor(bool real, int e) {
-  const float f = bounds_pow2(e);
-  return real ? make_float2(f, -12582912.f * f) : make_float2(0.f, -INFINITY);
+// Sums are below 2^22, so 1.5 * 2^23 + sum is a float with the sum in its last bits, and that number taken off again leaves the sum as a float, exactly
+// (conversions take four times as long; so do roundings, which the same addition makes).
+constexpr float kPickLarge = 12582912.f;
+constexpr int kPickLargeBits = 0x4b400000;
+__device__ __forceinline__ float pick_float(int sum) { return __int_as_float(sum + kPickLargeBits) - kPickLarge; }
+// Two sums at a time, times two factors.
+__device__ __forceinline__ float2 pick_scaled2(int a, int b, float2 f) {
+  float2 r;
+  asm("{\n\t"
+      ".reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 y, {%4, %4};\n\t"
+      "mov.b64 z, {%5, %6};\n\t"
+      "add.rn.f32x2 x, x, y;\n\t"
+      "mul.rn.f32x2 x, x, z;\n\t"
+      "mov.b64 {%0, %1}, x;\n\t"
+      "}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(__int_as_float(a + kPickLargeBits)), "f"(__int_as_float(b + kPickLargeBits)), "f"(-kPickLarge), "f"(f.x), "f"(f.y));
+  return r;
+}
+// Code of a channel: v times f, a power of two, to the nearest whole number from -127 to 127.
+__device__ __forceinline__ int pick_code(float v, float f) {
+  return __float_as_int(fminf(fmaxf(v * f, -127.f), 127.f) + kPickLarge) - kPickLargeBits;
 }
 
 // Keys order like scores.
@@ -349,26 +366,23 @@ __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickP
   // ---- codes of the queries: a+ against the largest values, a- against the smallest
   for (int i = wid; i < tiles * 8; i += kPickWarps) {
     constexpr int kEach = D / 32;
-    const bool real = i < r.tokens * group && r.begin + i / group >= 0;
+    // (rows that pad, and queries in front of the first key, repeat one that counts)
+    const int token = min(max(i / group, -r.begin), r.tokens - 1);
     float v[kEach], amax = 0.f;
+    const __nv_bfloat16* src = p.q + (static_cast<long long>(r.q_off + token) * p.hq + h * group + i % group) * D + lane * kEach;
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) v[k] = 0.f;
-    if (real) {
-      const __nv_bfloat16* src = p.q + (static_cast<long long>(r.q_off + i / group) * p.hq + h * group + i % group) * D + lane * kEach;
-#pragma unroll
-      for (int k = 0; k < kEach; k += 2) {
-        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + k));
-        v[k] = f.x == f.x ? f.x : 0.f;
-        v[k + 1] = f.y == f.y ? f.y : 0.f;
-        amax = fmaxf(amax, fmaxf(fabsf(v[k]), fabsf(v[k + 1])));
-      }
+    for (int k = 0; k < kEach; k += 2) {
+      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src + k));
+      v[k] = f.x == f.x ? f.x : 0.f;
+      v[k + 1] = f.y == f.y ? f.y : 0.f;
+      amax = fmaxf(amax, fmaxf(fabsf(v[k]), fabsf(v[k + 1])));
     }
     const int e = bounds_exponent(warp_max(amax));
     const float f = bounds_pow2(-e);
     uint32_t up = 0, down = 0;
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      const int c = static_cast<int>(fminf(fmaxf(rintf(v[k] * f), -127.f), 127.f));
+      const int c = pick_code(v[k], f);
       up |= static_cast<uint32_t>(max(c, 0)) << (8 * k);
       down |= (static_cast<uint32_t>(min(c, 0)) & 0xffu) << (8 * k);
     }
@@ -380,7 +394,7 @@ __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickP
       *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(up);
       *reinterpret_cast<uint16_t*>(dst + D) = static_cast<uint16_t>(down);
     }
-    if (lane == 0) sh.row[i] = pick_factor(real, e);
+    if (lane == 0) sh.row[i] = bounds_pow2(e);
   }
   if (p.parts > 1) cluster_sync_all();          // (the peers' memory is there)
   else __syncthreads();
@@ -406,11 +420,11 @@ __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickP
         mma_s8_16832(acc[0], a[0][c].x, a[1][c].x, a[0][c].y, a[1][c].y, b.x, b.y);
         mma_s8_16832(acc[1], a[0][c].z, a[1][c].z, a[0][c].w, a[1][c].w, b.z, b.w);
       }
-      const float4 f = *reinterpret_cast<const float4*>(sh.row + t * 8 + 2 * kq);      // of queries 2 kq and 2 kq + 1
+      const float2 f = *reinterpret_cast<const float2*>(sh.row + t * 8 + 2 * kq);      // of queries 2 kq and 2 kq + 1
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        best[i] = fmaxf(best[i], fmaxf(pick_scaled(acc[0][2 * i] + acc[1][2 * i], f.x, f.y),
-                                       pick_scaled(acc[0][2 * i + 1] + acc[1][2 * i + 1], f.z, f.w)));
+        best[i] = fmaxf(best[i], fmaxf(pick_float(acc[0][2 * i] + acc[1][2 * i]) * f.x,
+                                       pick_float(acc[0][2 * i + 1] + acc[1][2 * i + 1]) * f.y));
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -520,7 +534,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
   const int row = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, cols = (p.run * group + 15) & ~15;
   uint8_t* stages = smem;                                    // [3][atom][128 pages][128 bytes]; the choice works here afterwards
   uint8_t* codes = stages + kPtStages * kStage;              // [atom][256 queries][128 bytes]
-  float2* factor = reinterpret_cast<float2*>(codes + kAtoms * kAtom);            // of a query (pick_factor)
+  float* factor = reinterpret_cast<float*>(codes + kAtoms * kAtom);              // of a query: 2^e
   PickTcShared& bars = *reinterpret_cast<PickTcShared*>(factor + 2 * kPickRows);
   float* scores = reinterpret_cast<float*>(&bars + 1);       // [2][pages]
   const auto out_of = [&](int i) { return p.out + (static_cast<long long>(i) * p.hkv + h) * p.width; };
@@ -584,11 +598,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
   };
   int next[4];
   if (wid >= 4 && wid < 8) {                                 // the first tiles are on their way while the queries are coded
-    for (int j = 0; j < min(n_tiles, kPtStages); ++j) {
-      rows_of(j, next);
-      gather(j, next);
-    }
+    int from[kPtStages][4];
+#pragma unroll
+    for (int j = 0; j < kPtStages; ++j) rows_of(min(j, n_tiles - 1), from[j]);
     rows_of(kPtStages < n_tiles ? kPtStages : 0, next);
+#pragma unroll
+    for (int j = 0; j < kPtStages; ++j)
+      if (j < n_tiles) gather(j, from[j]);
   }
 
   // ---- codes of the queries: D / 8 lanes a query, 16 bytes each, half of the loads of a warp ahead of their use
@@ -598,13 +614,11 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
     for (int w = 0; w < runs; ++w) {
       const RunOfRow& r = x[w].run;
       uint4 raw[kRounds];
-      bool real[kRounds];
 #pragma unroll
       for (int k = 0; k < kRounds; ++k) {
-        const int i = (k * 16 + wid) * kQueries + lane / kQLanes, token = i * inverse >> 16;
-        real[k] = token < r.tokens && r.begin + token >= 0;
-        raw[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (real[k]) raw[k] = __ldg(reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(r.q_off + token) * p.hq + h * group + i - token * group) * D + u * 8));
+        // (rows that pad, and queries in front of the first key, repeat one that counts)
+        const int i = (k * 16 + wid) * kQueries + lane / kQLanes, at = i * inverse >> 16, token = min(max(at, -r.begin), r.tokens - 1);
+        raw[k] = __ldg(reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(r.q_off + token) * p.hq + h * group + i - at * group) * D + u * 8));
       }
 #pragma unroll
       for (int k = 0; k < kRounds; ++k) {
@@ -625,7 +639,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
         uint2 up = make_uint2(0u, 0u), down = make_uint2(0u, 0u);
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          const int c = static_cast<int>(fminf(fmaxf(rintf(v[y] * f), -127.f), 127.f)), d = static_cast<int>(fminf(fmaxf(rintf(v[4 + y] * f), -127.f), 127.f));
+          const int c = pick_code(v[y], f), d = pick_code(v[4 + y], f);
           up.x |= static_cast<uint32_t>(max(c, 0)) << (8 * y);
           down.x |= (static_cast<uint32_t>(min(c, 0)) & 0xffu) << (8 * y);
           up.y |= static_cast<uint32_t>(max(d, 0)) << (8 * y);
@@ -637,7 +651,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
         };
         *place(u * 8) = up;
         *place(D + u * 8) = down;
-        if (u == 0) factor[at] = pick_factor(real[k], e);
+        if (u == 0) factor[at] = bounds_pow2(e);
       }
     }
   }
@@ -686,7 +700,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
   } else if (wid >= 8 && wid < 8 + 4 * runs) {
     const int w = (wid - 8) >> 2, mine = threadIdx.x & 127;  // run, page of a tile = TMEM lane
     const uint32_t column = tmem_base + (static_cast<uint32_t>((wid & 3) * 32) << 16) + w * cols;
-    const float2* const mult = factor + w * cols;
+    const float* const mult = factor + w * cols;
     float* const to = scores + w * p.max_pages;
     // the exponent of the tile's page, one tile ahead, and the page's number two ahead
     const int count = x[w].n;
@@ -716,10 +730,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
           if (lane == 0) mbar_arrive(&bars.s_empty[j & 1]);
         }
 #pragma unroll
-        for (int i = 0; i < 64; i += 2) {
+        for (int i = 0; i < 64; i += 4) {
           if (i % 16 == 0 && c0 + i >= cols) break;
           const float4 f = *reinterpret_cast<const float4*>(mult + c0 + i);
-          best[(i >> 1) & 3] = fmaxf(best[(i >> 1) & 3], fmaxf(pick_scaled(static_cast<int>(s[i]), f.x, f.y), pick_scaled(static_cast<int>(s[i + 1]), f.z, f.w)));
+          const float2 a = pick_scaled2(static_cast<int>(s[i]), static_cast<int>(s[i + 1]), make_float2(f.x, f.y));
+          const float2 b = pick_scaled2(static_cast<int>(s[i + 2]), static_cast<int>(s[i + 3]), make_float2(f.z, f.w));
+          best[(i >> 1) & 2] = fmaxf(best[(i >> 1) & 2], fmaxf(a.x, a.y));
+          best[((i >> 1) & 2) + 1] = fmaxf(best[((i >> 1) & 2) + 1], fmaxf(b.x, b.y));
         }
       }
       const int at = j * kPtTile + mine;
@@ -827,9 +844,12 @@ B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block
   p.seqs = seqs; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages;
   p.top = top; p.first = first; p.last = last; p.width = width;
   p.status = static_cast<DeviceStatus*>(status);
-  // Runs of many queries: blocks of their own, as long as their scores fit.
-  const long long smem_tc = 1024 + (kPtStages * kPtTile + 2 * kPickRows) * 2 * d + 2 * kPickRows * 8 + static_cast<int>(sizeof(PickTcShared)) + 8ll * max_pages;
-  if (run * (hq / hkv) > kPickFew && smem_tc <= 232448 && static_cast<long long>(rows) * hkv < (1ll << 31) && pages * hkv < (1ll << 31))
+  // Tiles of 128 queries pay from 17 on, once there are more rows than processors: below that the other kernel's blocks share a row, and few queries leave most
+  // of a tile empty. us, tiles / mma.sync, heads of 128 (queries of a run, rows x key heads, pages): 8, 8000, 1920 799 / 859; 16, 4000, 190 172 / 161;
+  // 32, 600, 270 37 / 37; 32, 2000, 1920 213 / 294; 64, 304, 270 26 / 28; 64, 64, 1880 30 / 22; 128, 152, 270 18 / 27; 128, 32, 1880 37 / 22; 128, 504, 1920
+  // 77 / 163; heads of 64: 28, 500, 1920 51 / 66; 56, 76, 270 13 / 10; 112, 126, 1920 36 / 29.
+  const long long smem_tc = 1024 + (kPtStages * kPtTile + 2 * kPickRows) * 2 * d + 2 * kPickRows * 4 + static_cast<int>(sizeof(PickTcShared)) + 8ll * max_pages;
+  if (run * (hq / hkv) > 16 && static_cast<long long>(rows) * hkv > num_sms() && smem_tc <= 232448 && static_cast<long long>(rows) * hkv < (1ll << 31) && pages * hkv < (1ll << 31))
     return d == 128 ? launch_pick_tc<128>(p, rows, static_cast<int>(smem_tc), stream) : launch_pick_tc<64>(p, rows, static_cast<int>(smem_tc), stream);
   const int fixed = (static_cast<int>(sizeof(PickShared)) + 15) / 16 * 16 + (run * (hq / hkv) + 7) / 8 * 8 * (2 * d + 64);
   // blocks of a row: as long as every processor has one at most and a block 256 pages to score; at least as many as hold the scores

@@ -169,6 +169,21 @@ def test_the_choice_is_that_of_the_host(each, lens, hq, hkv, d, top, first, last
 
 
 @gpu
+@pytest.mark.parametrize("hq,hkv,d,run", [(14, 2, 64, 18), (8, 1, 128, 16), (28, 4, 128, 5), (100, 1, 128, 1), (33, 1, 64, 3), (40, 2, 128, 6)])
+@pytest.mark.parametrize("each,lens", [([2500, 0, 3, 1], [2900, 50, 3000, 1]), ([17, 2600], [17, 2650])])
+def test_the_choice_of_many_runs_is_that_of_the_host(each, lens, hq, hkv, d, run):
+    """More rows than processors, so that tiles of queries score them: runs in pairs of a sequence, one by themselves at its end, sequences of a token."""
+    if run < 16:
+        each = [m // (2 if run > 2 else 8) for m in each]
+        each = [max(m, 1) if n else 0 for m, n in zip(each, lens)]
+    b = Batch(each, lens, hq, hkv, d, 16, seed=run).fill_bounds()
+    assert ((sum(each) + len(each) * (run - 1)) // run) * hkv > 148
+    want = b.pick(top=9, run=run)
+    assert torch.equal(b.to("cuda").pick(top=9, run=run).cpu(), want)
+    N.check_status()
+
+
+@gpu
 @pytest.mark.parametrize("pages,extra,top", [(3000, 0, 100), (9000, 3000, 1), (9000, 0, 2500), (2100, 60000, 300)])
 def test_a_long_table_is_shared_by_blocks(pages, extra, top):
     """One sequence; wide tables whose scores no single block holds. Bounds are random bytes."""
