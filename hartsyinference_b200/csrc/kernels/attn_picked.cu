@@ -6,6 +6,8 @@
 // registers: the channels of K are taken in the order in which 16-byte loads deal them to the lanes (Q likewise; sums do not mind), those of V
 // fall into tiles so that a lane's 16 bytes are four pairs of rows, which two neighbouring keys' words make by byte permutes. P is turned by
 // movmatrix. Nothing goes through shared memory but Q and, once, the warps' results, so no barrier stands between a load and its use.
+// Rows of more than 32 columns are walked by two or four warps at a time, each with columns of its own: the first to load a unit brings it to L1 for the others
+// (in blocks of their own, each reading all pages: 46 us for 16 x 5 tokens of 32 heads on 8 over 2112 keys).
 // Maxima and sums are in 32 bits, of unrounded probabilities; P is rounded to bf16 once.
 //
 // A row whose pages are too many for one block's warps is shared by a cluster of up to eight blocks (every eighth page each), which meet
@@ -21,7 +23,7 @@ struct PickedParams {
   const int* picked;           // [rows][hkv][width]
   const int *block_table, *kv_lens, *cu_q;
   long long pages;
-  int seqs, hq, hkv, run, page_shift, max_pages, width, parts, col_groups, cap;
+  int seqs, hq, hkv, run, page_shift, max_pages, width, parts, cap;
   float scale_log2, cap_in, cap_out;   // softcap: cap_out - 2 cap_out / (1 + 2^(cap_in s)), or cap_out = 0
   DeviceStatus* status;
 };
@@ -60,34 +62,37 @@ __device__ __forceinline__ float pk_peer(const float* local, int block) {
 }
 
 // Shared memory: list of pages, limits of the columns, Q; the results of warps, then of the block, lie over Q.
-template <int D, int NT>
+template <int D, int NT, int CG>
 struct PkLayout {
-  static constexpr int kCols = 8 * NT;
+  static constexpr int kCols = 8 * NT;                           // of a warp
+  static constexpr int kAll = kCols * CG;                        // of the block
   static constexpr int kQPitch = 2 * D + 64;                     // bytes; eight lanes' pieces of 16 bytes keep apart
   static constexpr int kOPitch = D + 4;                          // floats
   static constexpr int kWarpO = kCols * kOPitch;                 // floats of a warp's O
-  static constexpr int head(int cap) { return (cap * 8 + kCols * 4 + 15) / 16 * 16; }
+  static constexpr int head(int cap) { return (cap * 8 + kAll * 4 + 15) / 16 * 16; }
   static constexpr int bytes(int cap) {
-    const int q = kCols * kQPitch, join = kPkWarps * (kWarpO + 2 * kCols) * 4;
+    const int q = kAll * kQPitch, join = kPkWarps * (kWarpO + 2 * kCols) * 4;
     return head(cap) + (q > join ? q : join);
   }
 };
 
-template <int D, int NT>
+template <int D, int NT, int CG>
 __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kernel(const PickedParams p) {
   pdl_wait();
   pdl_trigger();
-  using L = PkLayout<D, NT>;
+  using L = PkLayout<D, NT, CG>;
   constexpr int kK = D / 32, kHalves = D / 64;
   extern __shared__ __align__(16) uint8_t pk_smem[];
   int2* list = reinterpret_cast<int2*>(pk_smem);                 // page id (-1: none), first key
   int* limits = reinterpret_cast<int*>(pk_smem + p.cap * 8);
   uint8_t* work = pk_smem + L::head(p.cap);
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, g = lane >> 2, kq = lane & 3, group = p.hq / p.hkv;
-  const int row = blockIdx.x / p.parts, rank = blockIdx.x % p.parts, h = blockIdx.y / p.col_groups, col0 = blockIdx.y % p.col_groups * L::kCols;
+  const int row = blockIdx.x / p.parts, rank = blockIdx.x % p.parts, h = blockIdx.y;
+  const int mate = wid % CG, walker = wid / CG;                  // whose columns, whose units
+  constexpr int kWalkers = kPkWarps / CG;
   const RunOfRow r = run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)));
-  const int cols = min(L::kCols, r.tokens * group - col0);       // of this block
-  if (r.tokens <= 0 || cols <= 0) return;                        // (alike in all blocks of a cluster)
+  const int cols = r.tokens * group;
+  if (r.tokens <= 0) return;                        // (alike in all blocks of a cluster)
   const int end = r.begin + r.tokens;                            // keys that the run's last query sees
 
   const int* mine = p.picked + (static_cast<long long>(row) * p.hkv + h) * p.width;
@@ -104,22 +109,24 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
     }
     list[i] = make_int2(id, id < 0 ? 0 : at << p.page_shift);
   }
-  for (int c = threadIdx.x; c < L::kCols; c += kPkThreads) limits[c] = c < cols ? r.begin + (col0 + c) / group + 1 : 0;
-  for (int i = threadIdx.x; i < L::kCols * (D / 8); i += kPkThreads) {
+  for (int c = threadIdx.x; c < L::kAll; c += kPkThreads) limits[c] = c < cols ? r.begin + c / group + 1 : 0;
+  for (int i = threadIdx.x; i < L::kAll * (D / 8); i += kPkThreads) {
     const int c = i / (D / 8), x = i - c * (D / 8);
     uint4 w = make_uint4(0u, 0u, 0u, 0u);
-    if (c < cols) w = *reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(r.q_off + (col0 + c) / group) * p.hq + h * group + (col0 + c) % group) * D + x * 8);
+    if (c < cols) w = *reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(r.q_off + c / group) * p.hq + h * group + c % group) * D + x * 8);
     *reinterpret_cast<uint4*>(work + c * L::kQPitch + x * 16) = w;
   }
   __syncthreads();
 
-  const int free_keys = r.begin + col0 / group + 1;              // keys that every column sees
+  const uint8_t* const mine_q = work + mate * L::kCols * L::kQPitch;
+  const int* const mine_limits = limits + mate * L::kCols;
+  const int free_keys = r.begin + mate * L::kCols / group + 1;   // keys that every column of the warp sees
   const int unit_shift = p.page_shift - 4, units = n << unit_shift;
   int lim[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) lim[t][i] = limits[t * 8 + 2 * kq + i];
+    for (int i = 0; i < 2; ++i) lim[t][i] = mine_limits[t * 8 + 2 * kq + i];
   float o[kHalves][4][NT][4];                                    // [half][tile][columns][row g | row g + 8 of two columns]
   float m[NT][2], l[NT][2];
 #pragma unroll
@@ -135,7 +142,7 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
   }
   // the warp's next unit at or after u: its offset in the pool and first key
   const auto next_unit = [&](int& u, long long& at, int& key0) {
-    for (; u < units; u += kPkWarps) {
+    for (; u < units; u += kWalkers) {
       const int2 e = list[u >> unit_shift];
       const int sub = u & ((1 << unit_shift) - 1);
       key0 = e.y + sub * 16;
@@ -153,7 +160,7 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
 #pragma unroll
       for (int c = 0; c < kK; ++c) ka[i][c] = pk_load(p.k + at + (g + 8 * i) * D + c * 32 + kq * 8);
   };
-  int u = wid, key0 = 0;
+  int u = walker, key0 = 0;
   long long at = 0;
   bool on = next_unit(u, at, key0);
   if (on) load_k(at);
@@ -169,13 +176,13 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
       s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
 #pragma unroll
       for (int c = 0; c < kK; ++c) {
-        const uint4 b = *reinterpret_cast<const uint4*>(work + (t * 8 + g) * L::kQPitch + c * 64 + kq * 16);
+        const uint4 b = *reinterpret_cast<const uint4*>(mine_q + (t * 8 + g) * L::kQPitch + c * 64 + kq * 16);
         pk_mma(s[t], ka[0][c].x, ka[1][c].x, ka[0][c].y, ka[1][c].y, b.x, b.y);
         pk_mma(s[t], ka[0][c].z, ka[1][c].z, ka[0][c].w, ka[1][c].w, b.z, b.w);
       }
     }
     const int key = key0;
-    u += kPkWarps;
+    u += kWalkers;
     on = next_unit(u, at, key0);
     if (on) load_k(at);
     const bool masked = key + 16 > free_keys;
@@ -244,8 +251,8 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
       // one column at a time, over the values that it sees
 #pragma unroll 1
       for (int c = 0; c < L::kCols; ++c) {
-        const int seen = limits[c];
-        if (c >= cols) break;
+        const int seen = mine_limits[c];
+        if (mate * L::kCols + c >= cols) break;
         uint32_t keep[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) keep[i] = key + 2 * kq + (i & 1) + (i >> 1) * 8 < seen ? 0xffffffffu : 0u;
@@ -289,21 +296,24 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
       }
     }
   __syncthreads();
-  // a thread owns neighbouring pairs of values of a column; weights of the warps first
-  constexpr int kPairs = L::kCols * D / 2, kEach = (kPairs + kPkThreads - 1) / kPkThreads;
+  // a thread owns neighbouring pairs of values of a column
+  constexpr int kPairs = L::kAll * D / 2, kEach = (kPairs + kPkThreads - 1) / kPkThreads;
   float2 sums[kEach];
   float tops[kEach], totals[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int i = e * kPkThreads + threadIdx.x, c = min(i / (D / 2), L::kCols - 1), x = i % (D / 2) * 2;
+    const int i = e * kPkThreads + threadIdx.x, all = min(i / (D / 2), L::kAll - 1), x = i % (D / 2) * 2, c = all % L::kCols, first = all / L::kCols;
     float top = -INFINITY, total = 0.f;
-    for (int w = 0; w < kPkWarps; ++w) top = fmaxf(top, wm[w * L::kCols + c]);
+#pragma unroll
+    for (int w = 0; w < kWalkers; ++w) top = fmaxf(top, wm[(w * CG + first) * L::kCols + c]);
     float2 sum = make_float2(0.f, 0.f);
-    for (int w = 0; w < kPkWarps; ++w) {
-      const float mw = wm[w * L::kCols + c], lw = wl[w * L::kCols + c];
+#pragma unroll
+    for (int w = 0; w < kWalkers; ++w) {
+      const int at = (w * CG + first) * L::kCols + c;
+      const float mw = wm[at], lw = wl[at];
       if (mw == -INFINITY && lw == 0.f) continue;                // (NaN scores have no maximum, but a sum)
       const float f = pk_exp2(mw - (top == -INFINITY ? 0.f : top));
-      const float2 y = *reinterpret_cast<const float2*>(wo + w * L::kWarpO + c * L::kOPitch + x);
+      const float2 y = *reinterpret_cast<const float2*>(wo + (w * CG + first) * L::kWarpO + c * L::kOPitch + x);
       sum.x += f * y.x;
       sum.y += f * y.y;
       total += f * lw;
@@ -315,7 +325,7 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
   const auto store = [&](int c, int x, float2 sum, float total) {
     if (c >= cols) return;
     const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;       // nothing seen: zeros; NaN stays
-    *reinterpret_cast<uint32_t*>(p.out + (static_cast<long long>(r.q_off + (col0 + c) / group) * p.hq + h * group + (col0 + c) % group) * D + x) =
+    *reinterpret_cast<uint32_t*>(p.out + (static_cast<long long>(r.q_off + c / group) * p.hq + h * group + c % group) * D + x) =
         pack_bf16x2(sum.x * inv, sum.y * inv);
   };
   if (p.parts == 1) {
@@ -328,13 +338,15 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
   }
   // ---- and those of the blocks: each joins a share of the columns' values
   __syncthreads();
+  float* const bm = wo + L::kAll * L::kOPitch;                   // [columns] maxima, then sums, behind the columns' values
+  float* const bl = bm + L::kAll;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const int i = e * kPkThreads + threadIdx.x;
     if (i >= kPairs) continue;
     const int c = i / (D / 2), x = i % (D / 2) * 2;
     *reinterpret_cast<float2*>(wo + c * L::kOPitch + x) = sums[e];
-    if (x == 0) { wm[c] = tops[e]; wl[c] = totals[e]; }
+    if (x == 0) { bm[c] = tops[e]; bl[c] = totals[e]; }
   }
   cluster_sync_all();
   for (int i = rank * kPkThreads + threadIdx.x; i < kPairs; i += p.parts * kPkThreads) {
@@ -342,11 +354,11 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
     float top = -INFINITY, total = 0.f, ms[8];
     float2 sum = make_float2(0.f, 0.f);
     for (int k = 0; k < p.parts; ++k) {
-      ms[k] = pk_peer(wm + c, k);
+      ms[k] = pk_peer(bm + c, k);
       top = fmaxf(top, ms[k]);
     }
     for (int k = 0; k < p.parts; ++k) {
-      const float lk = pk_peer(wl + c, k);
+      const float lk = pk_peer(bl + c, k);
       if (ms[k] == -INFINITY && lk == 0.f) continue;
       const float f = pk_exp2(ms[k] - (top == -INFINITY ? 0.f : top));
       sum.x += f * pk_peer(wo + c * L::kOPitch + x, k);
@@ -358,23 +370,20 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
   cluster_sync_all();                       // nobody leaves while a peer may still read its words
 }
 
-template <int D, int NT>
+template <int D, int NT, int CG>
 static int launch_picked(PickedParams p, int rows, cudaStream_t stream) {
   static PerDeviceOnce configured;
-  if (configured.first_time() && cudaFuncSetAttribute(attn_picked_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return -200;
-  const int cols = p.run * (p.hq / p.hkv);
-  p.col_groups = (cols + 8 * NT - 1) / (8 * NT);
-  if (static_cast<long long>(p.hkv) * p.col_groups > 65535) return -2;
-  const long long blocks = static_cast<long long>(rows) * p.hkv * p.col_groups, units = static_cast<long long>(p.width) << (p.page_shift - 4);
+  if (configured.first_time() && cudaFuncSetAttribute(attn_picked_kernel<D, NT, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return -200;
+  const long long blocks = static_cast<long long>(rows) * p.hkv, units = static_cast<long long>(p.width) << (p.page_shift - 4);
   // blocks of a row: until the processors have two each, as long as every warp has a unit of its own
   p.parts = 1;
-  while (p.parts < 8 && blocks * p.parts * 2 <= 2 * num_sms() && units > p.parts * kPkWarps) p.parts *= 2;
+  while (p.parts < 8 && blocks * p.parts * 2 <= 2 * num_sms() && units > p.parts * (kPkWarps / CG)) p.parts *= 2;
   p.cap = (p.width + p.parts - 1) / p.parts;
-  const int smem = PkLayout<D, NT>::bytes(p.cap);
+  const int smem = PkLayout<D, NT, CG>::bytes(p.cap);
   if (smem > 232448) return -6;
   if (static_cast<long long>(rows) * p.parts >= (1ll << 31)) return -3;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(rows) * p.parts, p.hkv * p.col_groups);
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * p.parts, p.hkv);
   cfg.blockDim = dim3(kPkThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -386,8 +395,22 @@ static int launch_picked(PickedParams p, int rows, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.parts > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_picked_kernel<D, NT>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_picked_kernel<D, NT, CG>, p);
   return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
+}
+
+// Columns of a warp in eights, as few as hold the row's with one, two or four warps side by side.
+template <int D>
+static int launch_columns(const PickedParams& p, int rows, cudaStream_t stream) {
+  const int eights = (p.run * (p.hq / p.hkv) + 7) / 8;
+  if (eights <= 1) return launch_picked<D, 1, 1>(p, rows, stream);
+  if (eights <= 2) return launch_picked<D, 2, 1>(p, rows, stream);
+  if (eights <= 3) return launch_picked<D, 3, 1>(p, rows, stream);
+  if (eights <= 4) return launch_picked<D, 2, 2>(p, rows, stream);
+  if (eights <= 6) return launch_picked<D, 3, 2>(p, rows, stream);
+  if (eights <= 8) return launch_picked<D, 2, 4>(p, rows, stream);
+  if (eights <= 12) return launch_picked<D, 3, 4>(p, rows, stream);
+  return launch_picked<D, 4, 4>(p, rows, stream);
 }
 
 }  // namespace b200
@@ -410,7 +433,7 @@ B200_API int b200_attn_picked(const void* q, const void* k, const void* v, void*
   if (rows <= 0 || seqs <= 0) return 0;
   PickedParams p{};
   p.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1;
-  if (p.page_shift < 0 || hkv < 1 || hq < 1 || hq % hkv || pages < 1 || max_pages < 1 || (d != 64 && d != 128)) return -2;
+  if (p.page_shift < 0 || hkv < 1 || hkv > 65535 || hq < 1 || hq % hkv || pages < 1 || max_pages < 1 || (d != 64 && d != 128)) return -2;
   if (run < 1 || static_cast<long long>(run) * (hq / hkv) > 128 || (!cu_q && (run != 1 || rows != seqs))) return -3;
   if (width < 1 || width > kPickedWidth) return -5;
   uintptr_t all = 0;
@@ -427,8 +450,5 @@ B200_API int b200_attn_picked(const void* q, const void* k, const void* v, void*
   p.cap_out = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
   p.cap_in = softcap > 0.f ? 2.f * scale / softcap * 1.4426950408889634f : 0.f;
   p.status = static_cast<DeviceStatus*>(status);
-  const int cols = run * (hq / hkv);
-  if (cols <= 8) return d == 128 ? launch_picked<128, 1>(p, rows, stream) : launch_picked<64, 1>(p, rows, stream);
-  if (cols <= 16) return d == 128 ? launch_picked<128, 2>(p, rows, stream) : launch_picked<64, 2>(p, rows, stream);
-  return d == 128 ? launch_picked<128, 4>(p, rows, stream) : launch_picked<64, 4>(p, rows, stream);
+  return d == 128 ? launch_columns<128>(p, rows, stream) : launch_columns<64>(p, rows, stream);
 }
