@@ -12,6 +12,8 @@
 //
 // A row whose pages are too many for one block's warps is shared by a cluster of up to eight blocks (every eighth page each), which meet
 // through distributed shared memory: one launch, no scratch.
+#include <math.h>
+
 #include "picked.cuh"
 
 namespace b200 {
@@ -375,9 +377,9 @@ static int launch_picked(PickedParams p, int rows, cudaStream_t stream) {
   static PerDeviceOnce configured;
   if (configured.first_time() && cudaFuncSetAttribute(attn_picked_kernel<D, NT, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return -200;
   const long long blocks = static_cast<long long>(rows) * p.hkv, units = static_cast<long long>(p.width) << (p.page_shift - 4);
-  // blocks of a row: until the processors have two each, as long as every warp has a unit of its own
+  // blocks of a row: as long as all fit the processors at once (two each where the registers allow it) and every warp has a unit of its own
   p.parts = 1;
-  while (p.parts < 8 && blocks * p.parts * 2 <= 2 * num_sms() && units > p.parts * (kPkWarps / CG)) p.parts *= 2;
+  while (p.parts < 8 && blocks * p.parts * 2 <= (NT == 1 ? 2 : 1) * num_sms() && units > p.parts * (kPkWarps / CG)) p.parts *= 2;
   p.cap = (p.width + p.parts - 1) / p.parts;
   const int smem = PkLayout<D, NT, CG>::bytes(p.cap);
   if (smem > 232448) return -6;
@@ -419,10 +421,20 @@ using namespace b200;
 
 constexpr int kPickedWidth = 4096;
 
-// Whether rows of `cols` columns (queries times heads of a group) go through the tensor-core tiles of attn_picked_tc.cu (1) or b200_attn_picked (0).
+// Whether rows of `cols` columns (queries times heads of a group) go through the tensor-core tiles of attn_picked_tc.cu (1) or b200_attn_picked (0). A tile takes
+// 128 rows whatever the columns, 40 us for 2112 keys with a processor to itself and 53 with another beside it (heads of 64: 34 and 42); here a block takes 10 us
+// and 9 for every eight columns (7 and 5.3), and few rows are shared by several blocks. us, here / tiles, rows x key heads in front: heads of 128, 24 columns: 144 36 / 56,
+// 192 65 / 57, 400 99 / 112; 40 columns: 32 39 / 41, 64 60 / 45, 144 63 / 57, 288 122 / 68; 64 columns: 16 33 / 41, 32 56 / 41, 400 283 / 116; 128 columns: 8 37 / 40,
+// 16 53 / 41; heads of 64, 35 columns: 24 26 / 35, 48 39 / 35; 112 columns: 16 33 / 35, 24 54 / 35. Up to 16 columns there is little between the two from 200 rows on.
 B200_API int b200_attn_picked_form(int rows, int cols, int hkv, int d, int page, int width, long long pages, float scale, float softcap) {
   if (cols <= 16 || width > 1024 || !(scale > 0.f) || softcap > 0.f || pages * hkv * page >= (1ll << 31)) return 0;
-  return cols >= 48;
+  const double r = static_cast<double>(rows) * hkv, sms = num_sms(), keys = width * static_cast<double>(page) / 2112.;
+  const int eights = (cols + 7) / 8, held = eights <= 4 ? eights : eights <= 6 ? 6 : eights <= 8 ? 8 : eights <= 12 ? 12 : 16;
+  const double block = d == 128 ? 10. + 9. * held : 7. + 5.3 * held;
+  const double here = 5. + keys * block * fmin(1., fmax(0.3, r * 3. / sms)) * ceil(r / sms);
+  const double one = d == 128 ? 32. : 26., two = d == 128 ? 49. : 40.;
+  const double tiles = 8. + keys * (r <= sms ? one + (two - one) * r / sms : two * ceil(r / (2. * sms)));
+  return tiles < here;
 }
 
 // q, out [tokens][hq][d], k, v [pages][hkv][page][d] bf16; picked int32 [rows][hkv][width] (see picked.cuh), rows = (tokens + seqs (run - 1)) / run.

@@ -325,8 +325,10 @@ def test_rows_without_pages_and_queries_in_front_of_their_pages_give_zeros(dev):
 @pytest.mark.parametrize("each,lens", BATCHES + [([130, 0, 61, 1], [700, 0, 61, 200])])
 @pytest.mark.parametrize("hq,hkv,d", HEADS)
 @pytest.mark.parametrize("page,width", [(16, 30), (32, 5), (64, 9), (128, 7), (16, 1000)])
-def test_attention_of_long_runs(each, lens, hq, hkv, d, page, width):
-    """As many tokens a run as it may have: tiles of up to 128 rows."""
+@pytest.mark.parametrize("tiles", [0, 1])
+def test_attention_of_long_runs(each, lens, hq, hkv, d, page, width, tiles, monkeypatch):
+    """As many tokens a run as it may have, by each of the two kernels, whichever the rule would take for the size."""
+    monkeypatch.setattr(N.lib(), "b200_attn_picked_form", lambda *a: tiles)
     run = 128 // (hq // hkv)
     b = Batch(each, lens, hq, hkv, d, page, seed=width)
     picked = _some(b, run, width)
@@ -337,8 +339,10 @@ def test_attention_of_long_runs(each, lens, hq, hkv, d, page, width):
 
 @gpu
 @pytest.mark.parametrize("d,page", [(128, 16), (64, 128)])
-def test_rows_of_a_long_run_that_begin_with_pages_they_do_not_see(d, page):
+@pytest.mark.parametrize("tiles", [0, 1])
+def test_rows_of_a_long_run_that_begin_with_pages_they_do_not_see(d, page, tiles, monkeypatch):
     """A list that names the run's last page first, one twice, and none between: order does not matter, twice counts twice."""
+    monkeypatch.setattr(N.lib(), "b200_attn_picked_form", lambda *a: tiles)
     b = Batch([90], [190], 2, 1, d, page)
     last = 189 // page
     odd = torch.tensor([last, -1, 0, 0, 5000, last - 1], dtype=torch.int32).expand(2, 1, -1).contiguous()
@@ -346,10 +350,12 @@ def test_rows_of_a_long_run_that_begin_with_pages_they_do_not_see(d, page):
     _close(b.to("cuda").attend(odd.cuda(), run=64), want)
 
 
-@pytest.mark.parametrize("dev", BOTH)
+@pytest.mark.parametrize("dev,tiles", [("cpu", 0), pytest.param("cuda", 0, marks=gpu), pytest.param("cuda", 1, marks=gpu)])
 @pytest.mark.parametrize("hq", [3, 8])
-def test_values_that_a_query_does_not_see_may_be_anything(dev, hq):
+def test_values_that_a_query_does_not_see_may_be_anything(dev, tiles, hq, monkeypatch):
     """Infinite and no numbers in a run's own page: they reach the queries that see them and no others."""
+    if dev == "cuda":
+        monkeypatch.setattr(N.lib(), "b200_attn_picked_form", lambda *a: tiles)
     b = Batch([6], [38], hq, 1, 128, 16)
     want, bound = _attention(b, torch.tensor([[[0, 1, 2]]]), 6)
     b.v[b.table[0, 2].long(), 0, 4, 7] = math.inf          # position 36: the last two queries
@@ -370,6 +376,16 @@ def test_a_query_that_is_no_number_gives_none(dev, softcap):
     if dev == "cuda":                                      # (the host's statement gives zeros for such a row)
         assert got[0, 1].isnan().all()
     assert torch.isfinite(got[0, [0, 2, 3]]).all() and torch.isfinite(got[1]).all()
+
+
+# both kernels measured: tiles of 128 rows where they are faster
+@pytest.mark.skipif(not N.available(), reason="kernels library not built")
+@pytest.mark.parametrize("d,cols,rows,tiles", [(128, 16, 4000, 0), (128, 24, 144, 0), (128, 24, 192, 1), (128, 40, 64, 1), (128, 64, 16, 0), (128, 64, 32, 1), (128, 128, 1024, 1),
+                                               (64, 35, 24, 0), (64, 35, 48, 1), (64, 112, 16, 0), (64, 112, 24, 1)])
+def test_the_rule_between_the_kernels(d, cols, rows, tiles):
+    form = N.lib().b200_attn_picked_form
+    assert form(rows // 8, cols, 8, d, 16, 132, 10000, 0.1, 0.0) == tiles
+    assert form(1024, 128, 8, d, 16, 1025, 10000, 0.1, 0.0) == form(1024, 128, 8, d, 16, 132, 10000, 0.1, 30.0) == form(1024, 128, 8, d, 16, 132, 10000, 0.0, 0.0) == 0
 
 
 @pytest.mark.parametrize("dev", BOTH)
