@@ -25,7 +25,7 @@ struct PickedParams {
   const int* picked;           // [rows][hkv][width]
   const int *block_table, *kv_lens, *cu_q;
   long long pages;
-  int seqs, hq, hkv, run, page_shift, max_pages, width, parts, cap;
+  int seqs, tokens, hq, hkv, run, page_shift, max_pages, width, parts, cap;
   float scale_log2, cap_in, cap_out;   // softcap: cap_out - 2 cap_out / (1 + 2^(cap_in s)), or cap_out = 0
   DeviceStatus* status;
 };
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kPkThreads, NT == 1 ? 2 : 1) attn_picked_kerne
   const int row = blockIdx.x / p.parts, rank = blockIdx.x % p.parts, h = blockIdx.y;
   const int mate = wid % CG, walker = wid / CG;                  // whose columns, whose units
   constexpr int kWalkers = kPkWarps / CG;
-  const RunOfRow r = run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)));
+  const RunOfRow r = run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)), p.tokens);
   const int cols = r.tokens * group;
   if (r.tokens <= 0) return;                        // (alike in all blocks of a cluster)
   const int end = r.begin + r.tokens;                            // keys that the run's last query sees
@@ -440,13 +440,13 @@ B200_API int b200_attn_picked_form(int rows, int cols, int hkv, int d, int page,
 // q, out [tokens][hq][d], k, v [pages][hkv][page][d] bf16; picked int32 [rows][hkv][width] (see picked.cuh), rows = (tokens + seqs (run - 1)) / run.
 // Causal; entries below 0 or behind the run's last query are no pages. A page named twice counts twice.
 B200_API int b200_attn_picked(const void* q, const void* k, const void* v, void* out, const int* picked, const int* block_table, const int* kv_lens,
-                              const int* cu_q, int seqs, int rows, int hq, int hkv, int d, int page, int max_pages, long long pages, int run, int width,
-                              float scale, float softcap, void* status, cudaStream_t stream) {
-  if (rows <= 0 || seqs <= 0) return 0;
+                              const int* cu_q, int seqs, int rows, int tokens, int hq, int hkv, int d, int page, int max_pages, long long pages, int run,
+                              int width, float scale, float softcap, void* status, cudaStream_t stream) {
+  if (rows <= 0 || seqs <= 0 || tokens <= 0) return 0;
   PickedParams p{};
   p.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1;
   if (p.page_shift < 0 || hkv < 1 || hkv > 65535 || hq < 1 || hq % hkv || pages < 1 || max_pages < 1 || (d != 64 && d != 128)) return -2;
-  if (run < 1 || static_cast<long long>(run) * (hq / hkv) > 128 || (!cu_q && (run != 1 || rows != seqs))) return -3;
+  if (run < 1 || static_cast<long long>(run) * (hq / hkv) > 128 || (!cu_q && (run != 1 || rows != seqs || tokens != seqs))) return -3;
   if (width < 1 || width > kPickedWidth) return -5;
   uintptr_t all = 0;
   for (const void* x : {q, k, v, static_cast<const void*>(out)}) all |= reinterpret_cast<uintptr_t>(x);
@@ -457,7 +457,7 @@ B200_API int b200_attn_picked(const void* q, const void* k, const void* v, void*
   p.out = static_cast<__nv_bfloat16*>(out);
   p.picked = picked; p.block_table = block_table; p.kv_lens = kv_lens; p.cu_q = cu_q;
   p.pages = pages;
-  p.seqs = seqs; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages; p.width = width;
+  p.seqs = seqs; p.tokens = tokens; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages; p.width = width;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.cap_out = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
   p.cap_in = softcap > 0.f ? 2.f * scale / softcap * 1.4426950408889634f : 0.f;

@@ -44,7 +44,7 @@ struct TpParams {
   const int* picked;           // [rows][hkv][width]
   const int *block_table, *kv_lens, *cu_q;
   long long pages;
-  int seqs, hq, hkv, run, page_shift, box_shift, max_pages, width, pool_rows;
+  int seqs, tokens, hq, hkv, run, page_shift, box_shift, max_pages, width, pool_rows;
   float scale_log2;
   DeviceStatus* status;
 };
@@ -73,7 +73,7 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
   const int row_id = blockIdx.x, h = blockIdx.y;
   pdl_wait();
   pdl_trigger();
-  const RunOfRow r = run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row_id, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x3fffffffll)));
+  const RunOfRow r = run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row_id, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x3fffffffll)), p.tokens);
   if (r.tokens <= 0) return;
   const int end = r.begin + r.tokens, real_rows = r.tokens * group;
 
@@ -447,7 +447,7 @@ B200_API int b200_attn_picked_tc(const void* q, const void* k, const void* v, vo
   TpParams p{};
   p.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : -1;
   if (p.page_shift < 0 || hkv < 1 || hkv > 65535 || hq < 1 || hq % hkv || pages < 1 || max_pages < 1 || (d != 64 && d != 128)) return -2;
-  if (run < 1 || static_cast<long long>(run) * (hq / hkv) > 128 || (!cu_q && (run != 1 || rows != seqs))) return -3;
+  if (run < 1 || static_cast<long long>(run) * (hq / hkv) > 128 || (!cu_q && (run != 1 || rows != seqs || tokens != seqs))) return -3;
   if (width < 1 || width > kTpWidth || !(scale > 0.f)) return -5;
   const long long pool_rows = pages * hkv * page;
   if (pool_rows >= (1ll << 31)) return -7;
@@ -461,7 +461,7 @@ B200_API int b200_attn_picked_tc(const void* q, const void* k, const void* v, vo
   p.out = static_cast<__nv_bfloat16*>(out);
   p.picked = picked; p.block_table = block_table; p.kv_lens = kv_lens; p.cu_q = cu_q;
   p.pages = pages;
-  p.seqs = seqs; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages; p.width = width;
+  p.seqs = seqs; p.tokens = tokens; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages; p.width = width;
   p.pool_rows = static_cast<int>(pool_rows);
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = static_cast<DeviceStatus*>(status);

@@ -102,7 +102,7 @@ struct PickParams {
   const int *block_table, *kv_lens, *cu_q;
   int* out;                    // [rows][hkv][width]
   long long pages;
-  int seqs, hq, hkv, run, page_shift, max_pages, top, first, last, width, parts;
+  int seqs, tokens, hq, hkv, run, page_shift, max_pages, top, first, last, width, parts;
   DeviceStatus* status;
 };
 
@@ -122,7 +122,7 @@ struct PickRange {
 };
 
 __device__ __forceinline__ RunOfRow pick_run(const PickParams& p, int row) {
-  return run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)));
+  return run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)), p.tokens);
 }
 
 // The pages that are kept whatever the scores, of run x.run (written by the block of rank 0); false: nothing is left to choose.
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
     if (y.run.tokens > 0 && rest > 0) {
       y.run.q_off += p.run;
       y.run.begin += p.run;
-      y.run.tokens = min(p.run, rest);
+      y.run.tokens = min(min(p.run, rest), p.tokens - y.run.q_off);
       if (pick_range(p, out_of(row + 1), true, y)) { x[runs] = y; rows[runs++] = row + 1; }
     }
     if (runs == 0) return;
@@ -827,13 +827,13 @@ B200_API int b200_key_bounds(const void* k, void* bounds, const int* block_table
 // q [tokens][hq][d] bf16, out int32 [rows][hkv][width] (see picked.cuh), rows = (tokens + seqs (run - 1)) / run,
 // width >= first + top + last + (run + page - 2) / page.
 B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block_table, const int* kv_lens, const int* cu_q, int* out, int seqs,
-                             int rows, int hq, int hkv, int d, int page, int max_pages, long long pages, int run, int top, int first, int last,
+                             int rows, int tokens, int hq, int hkv, int d, int page, int max_pages, long long pages, int run, int top, int first, int last,
                              int width, void* status, cudaStream_t stream) {
   if (rows <= 0 || seqs <= 0) return 0;
   PickParams p{};
   p.page_shift = picked_page_shift(page);
   if (p.page_shift < 0 || hkv < 1 || hq < 1 || hq % hkv || pages < 1 || max_pages < 1 || (d != 64 && d != 128) || hkv > 65535) return -2;
-  if (run < 1 || static_cast<long long>(run) * (hq / hkv) > kPickRows || (!cu_q && (run != 1 || rows != seqs))) return -3;
+  if (run < 1 || static_cast<long long>(run) * (hq / hkv) > kPickRows || (!cu_q && (run != 1 || rows != seqs || tokens != seqs))) return -3;
   if (top < 0 || first < 0 || last < 1 || static_cast<long long>(first) + top + last + (run + page - 2) / page > width) return -5;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(bounds)) & 15) return -4;
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -841,7 +841,7 @@ B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block
   p.block_table = block_table; p.kv_lens = kv_lens; p.cu_q = cu_q;
   p.out = out;
   p.pages = pages;
-  p.seqs = seqs; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages;
+  p.seqs = seqs; p.tokens = tokens; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages;
   p.top = top; p.first = first; p.last = last; p.width = width;
   p.status = static_cast<DeviceStatus*>(status);
   // Tiles of 128 queries pay from 17 on, once there are more rows than processors: below that the other kernel's blocks share a row, and few queries leave most

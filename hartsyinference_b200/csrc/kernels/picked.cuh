@@ -47,14 +47,15 @@ struct RunOfRow {
   int begin, kv_len;  // position of its first query (may be negative: such queries see nothing), keys of the sequence
 };
 
-__device__ __forceinline__ RunOfRow run_of_row(const int* __restrict__ cu_q, const int* __restrict__ kv_lens, int seqs, int run, int row, int most_keys) {
+// (tokens: rows of q, behind which no run reaches whatever cu_q holds)
+__device__ __forceinline__ RunOfRow run_of_row(const int* __restrict__ cu_q, const int* __restrict__ kv_lens, int seqs, int run, int row, int most_keys, int tokens) {
   RunOfRow r;
   r.seq = row_sequence(cu_q, seqs, run, row);
   const int off = cu_q ? cu_q[r.seq] : r.seq, len = cu_q ? cu_q[r.seq + 1] - off : 1;
   const int first = static_cast<int>((off + static_cast<long long>(r.seq) * (run - 1)) / run);
   const int skip = (row - first) * run;            // queries of the sequence in front of the run
   r.q_off = off + skip;
-  r.tokens = min(run, len - skip);
+  r.tokens = skip < 0 ? 0 : min(min(run, len - skip), tokens - r.q_off);
   r.kv_len = min(kv_lens[r.seq], most_keys);
   r.begin = r.kv_len - len + skip;
   return r;

@@ -128,8 +128,8 @@ _SIGNATURES = {
     "b200_attn_kv4": (i32, [vp] * 6 + [i32] * 7 + [i64, i32, i32, f32, f32, vp, vp]),
     "b200_rope_axes": (i32, [vp] * 12 + [i32] * 8 + [i64, f32, vp, vp]),
     "b200_key_bounds": (i32, [vp] * 5 + [i32] * 6 + [i64, vp, vp]),
-    "b200_pick_pages": (i32, [vp] * 6 + [i32] * 7 + [i64] + [i32] * 5 + [vp, vp]),
-    "b200_attn_picked": (i32, [vp] * 8 + [i32] * 7 + [i64, i32, i32, f32, f32, vp, vp]),
+    "b200_pick_pages": (i32, [vp] * 6 + [i32] * 8 + [i64] + [i32] * 5 + [vp, vp]),
+    "b200_attn_picked": (i32, [vp] * 8 + [i32] * 8 + [i64, i32, i32, f32, f32, vp, vp]),
     "b200_attn_picked_form": (i32, [i32] * 6 + [i64, f32, f32]),
     "b200_attn_picked_tc": (i32, [vp] * 8 + [i32] * 8 + [i64, i32, i32, f32, vp, vp]),
     "b200_attn_prefill": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp]),

@@ -6,7 +6,7 @@ from -50 to 50 with max |value| <= 127 * 2^e; NaN counts as 0. A forward pass st
 (:func:`key_bounds_`), chooses (:func:`pick_pages`) and attends (:func:`attn_picked`).
 
 Queries choose in runs of ``run`` neighbouring tokens of a sequence; the rows of runs are packed, run r of sequence s in row
-``(cu_q[s] + s * (run - 1)) // run + r`` of ``(tokens + S * (run - 1)) // run``. Pages of 16, 32, 64 or 128 tokens, heads of 64 or 128, any number of query heads per key
+``(cu_q[s] + s * (run - 1)) // run + r`` of ``(tokens + S * (run - 1)) // run`` (``cu_q`` from 0). Pages of 16, 32, 64 or 128 tokens, heads of 64 or 128, any number of query heads per key
 head as long as a run has at most 128 of them. CUDA tensors are bf16, block tables and lengths int32; CPU tensors go to the statements here and in :mod:`.reference`.
 """
 from __future__ import annotations
@@ -77,12 +77,14 @@ def _runs(kv_lens: torch.Tensor, cu_q: Optional[torch.Tensor], run: int, most: i
 
 
 def key_bounds_(bounds: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, cu_q: Optional[torch.Tensor] = None,
-                max_q_len: int = 1) -> torch.Tensor:
+                max_q_len: Optional[int] = None) -> torch.Tensor:
     """Bounds of the pages that the last tokens of every sequence filled, written into ``bounds``: ``cu_q[s + 1] - cu_q[s]`` tokens (one without ``cu_q``, at most
-    ``max_q_len``) of ``kv_lens[s]`` that the cache holds. Pages that are not full are left as they are: whoever attends
+    ``max_q_len``) of ``kv_lens[s]`` that the cache holds; ``max_q_len`` is asked for with ``cu_q``, since pages behind it would keep old bounds. Pages that are not full are left as they are: whoever attends
     has them among its last ones. A page that is cut back and filled again is bounded again."""
     device, shape, table = bounds.get_device(), k_cache.shape, block_table.shape
     seqs = kv_lens.numel()
+    if cu_q is not None and max_q_len is None:
+        raise ValueError("key_bounds_: cu_q with the longest run of new tokens, max_q_len")
     if not (device >= 0 and len(shape) == 4 and len(table) == 2 and table[0] == seqs and shape[2] in _PAGES and shape[3] in _HEADS and bounds.dtype is torch.uint8
             and k_cache.dtype is torch.bfloat16 and block_table.dtype is _I32 and kv_lens.dtype is _I32 and (cu_q is None or _plain(cu_q, device, seqs + 1))
             and bounds.shape == (shape[0], shape[1], 2 * shape[3] + 16) and device == k_cache.get_device() == block_table.get_device() == kv_lens.get_device()
@@ -165,7 +167,7 @@ def pick_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor,
             raise ValueError("pick_pages: bounds from a 16-byte boundary")
         q = _dense(q)
         rc = N.lib().b200_pick_pages(q.data_ptr(), bounds.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), out.data_ptr(),
-                                     seqs, rows, hq, hkv, d, page, table[1], pages, run, top, first, last, width, N.state(q.device).status.data_ptr(), N.stream())
+                                     seqs, rows, tokens, hq, hkv, d, page, table[1], pages, run, top, first, last, width, N.state(q.device).status.data_ptr(), N.stream())
         N.check(rc, "b200_pick_pages")
     return out
 
@@ -227,7 +229,7 @@ def attn_picked(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
                 if run > 1 and L.b200_attn_picked_form(rows, run * (hq // hkv), hkv, d, page, width, pages, scale, softcap):
                     rc = L.b200_attn_picked_tc(*ptrs, seqs, rows, tokens, hq, hkv, d, page, table[1], pages, run, width, scale, status, N.stream())
                 else:
-                    rc = L.b200_attn_picked(*ptrs, seqs, rows, hq, hkv, d, page, table[1], pages, run, width, scale, float(softcap), status, N.stream())
+                    rc = L.b200_attn_picked(*ptrs, seqs, rows, tokens, hq, hkv, d, page, table[1], pages, run, width, scale, float(softcap), status, N.stream())
                 N.check(rc, "b200_attn_picked")
     if not emit_fp8:
         return out

@@ -520,6 +520,7 @@ def test_refusals(dev):
            lambda: ops.key_bounds_(b.bounds, b.k[:, :, :8].contiguous(), b.table, b.kv_lens, b.cu_q, 3),
            lambda: ops.key_bounds_(b.bounds, b.k.transpose(1, 2), b.table, b.kv_lens, b.cu_q, 3),
            lambda: ops.key_bounds_(b.bounds, b.k, b.table, b.kv_lens[:1], b.cu_q, 3),
+           lambda: ops.key_bounds_(b.bounds, b.k, b.table, b.kv_lens, b.cu_q),
            lambda: b.pick(top=2, run=0), lambda: b.pick(top=2, run=33), lambda: b.pick(top=2, last=0), lambda: b.pick(top=-1), lambda: b.pick(top=5000),
            lambda: b.pick(top=2, step=True),
            lambda: ops.pick_pages(b.q, b.bounds, b.table, b.kv_lens, b.cu_q, page=24, top=2),
@@ -539,6 +540,26 @@ def test_refusals(dev):
                      lambda: ops.attn_picked(b.q, b.k, b.v, b.table, b.kv_lens, rows.long(), b.cu_q, run=2)):
             with pytest.raises((ValueError, RuntimeError)):
                 call()
+
+
+@pytest.mark.parametrize("dev", BOTH)
+@pytest.mark.parametrize("run", [1, 4, 16])
+def test_rows_in_front_of_the_first_sequence_and_behind_the_last(dev, run):
+    """A padded batch: q has rows that no sequence has. Their rows of pages are -1, and the sequences' results are those without them."""
+    b = Batch([9, 1], [300, 170], 8, 2, 64, 16).fill_bounds().to(dev)
+    want_p, want = b.pick(top=4, run=run), b.attend(b.pick(top=4, run=run), run=run)
+    for front, behind in ((0, 40), (33, 0), (5, 17)):
+        q = torch.cat([b.q[:1].expand(front, -1, -1), b.q, b.q[:1].expand(behind, -1, -1)])
+        cu = b.cu_q + front
+        p = ops.pick_pages(q, b.bounds, b.table, b.kv_lens, cu, page=16, top=4, run=run)
+        first = [(int(c) + i * (run - 1)) // run for i, c in enumerate(cu)]
+        rows = [x for i, m in enumerate(b.each) for x in range(first[i], first[i] + -(-m // run))]
+        was = [x for i, m in enumerate(b.each) for x in range((int(b.cu_q[i]) + i * (run - 1)) // run, (int(b.cu_q[i]) + i * (run - 1)) // run + -(-m // run))]
+        assert torch.equal(p[rows], want_p[was])
+        rest = [x for x in range(p.shape[0]) if x not in rows]
+        assert (p[rest] == -1).all()
+        got = ops.attn_picked(q, b.k, b.v, b.table, b.kv_lens, p, cu, run=run)
+        assert torch.equal(got[front:front + 10], want)
 
 
 @pytest.mark.parametrize("dev", BOTH)
