@@ -22,7 +22,8 @@ struct BoundsParams {
   DeviceStatus* status;
 };
 
-// A warp per page and head; four channels a lane, D / 4 lanes a key.
+// A warp per page and head; four channels a lane, D / 4 lanes a key. Bound by latency: a warp has few loads and one page. The pages of 2048 new tokens, 8 heads
+// of 128, take 3.1 us, one token of 16 sequences 1.3.
 template <int D>
 __global__ void __launch_bounds__(256) key_bounds_kernel(const BoundsParams p) {
   pdl_wait();
@@ -312,8 +313,9 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
 
 // A cluster of `parts` blocks per row of runs and key head; each scores a share of the pages, a warp 16 at a time. Pages are rows of the product
 // and queries (with their heads) its columns, eight a tile: groups of up to eight heads fill one, and the maximum over them is two exchanges. The bounds of the
-// next 16 pages are on their way into registers while some are multiplied. One token of 16 sequences of 2000 to 6000 tokens: 16.8 us with queries as
-// rows, 256 threads and digits of 8 bits.
+// next 16 pages are on their way into registers while some are multiplied. One token of 16 sequences of 2000 to 6000 tokens, 32 heads on 8: 7.7 us, of which the
+// loads' latencies one after the other (length, page number, bounds) and the choice's barriers are the most; 16.8 with queries as
+// rows, 256 threads and digits of 8 bits. One token behind 131072, 64 heads on 8: 15.1 us, the cluster's counts among them (1.2 TB/s).
 template <int D>
 __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickParams p) {
   pdl_wait();
@@ -506,8 +508,10 @@ static int launch_pick(const PickParams& p, int rows, int smem, cudaStream_t str
 //   warp 0        TMA producer: the codes of 128 pages into one of three stages, four pages a gather
 //   warp 1        one thread issues the products
 //   warps 8..15   scores: a page a thread, its 16 to 128 sums of one of the runs from one of two halves of TMEM; then half of the block chooses for each run
-// Bound by the gathers: a row of 2 D bytes lies on any 16-byte boundary, and a processor fetches 14 bytes of such rows a cycle, by TMA as by copies of 16 bytes a
-// lane. So a tile serves two runs (one: 218 us for 2048 queries behind 30720; with copies 198; mma.sync, whose 8-bit products have a fifth of the rate, 307).
+// 2048 queries of 64 heads on 8, runs of 16, behind 30720: 146 us, 3.5 blocks a processor one after the other. A block's time is that of its gathers (a row of 2 D
+// bytes lies on any 16-byte boundary, and a processor fetches 14 bytes of such rows a cycle, by TMA as by copies of 16 bytes a lane), of the maxima beside them, and of what
+// neither hides, the coding of the queries and the choice. A tile serves two runs for the gathers' sake (one: 218 us; mma.sync, whose 8-bit products have a fifth of the
+// rate, 307).
 constexpr int kPtThreads = 512, kPtTile = 128, kPtStages = 3;
 
 struct PickTcShared {
