@@ -112,7 +112,8 @@ struct PickShared {
   unsigned least[8 * kPickWarps], most[8 * kPickWarps];      // smallest and largest key of every warp of the row's blocks
   unsigned warp_a[kPickWarps], warp_b[kPickWarps];
   unsigned counts[2];               // this block's selected and tied ones
-  unsigned bin, want, in_bin;
+  unsigned bin, want, in_bin, listed;
+  unsigned list[32];                // keys of a bin that is nearly all that is left
   __align__(16) float row[kPickRows];       // of a query: 2^e
 };
 
@@ -209,8 +210,8 @@ __device__ __forceinline__ unsigned pick_key(float score) {
 
 // The `top` largest of more than `top` scores, of which this block holds the `mine` from number `a0` on, ties to the lowest number: first + number, in order, to
 // out[0 .. top). `least` and `most` bound all keys. Digits of what keys lie above the smallest, as many as it takes: 11 bits where one block holds all
-// scores; 9 in a cluster, whose blocks read one another's counts. All threads of all blocks of the row, or `kThreads` threads
-// (tid) of a block that share barrier `bar`.
+// scores; 9 in a cluster, whose blocks read one another's counts. Once a digit leaves 32 keys at most, every warp ranks them by itself. All threads of all blocks
+// of the row, or `kThreads` threads (tid) of a block that share barrier `bar`; sh.hist is zero before, for all of them to see.
 template <bool kCluster, int kThreads>
 __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, const float* scores, int mine, int a0, int rank, int parts, int top, unsigned least, unsigned most,
                                             int first, int* out) {
@@ -223,14 +224,17 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
     const int bits = min(kDigit, shift);
     shift -= bits;
     unsigned* hist = sh.hist + (kCluster ? (pass & 1) * kBins : 0);      // (a peer may still read those of the pass before)
-    if (kEach >= 4) {
+    if (pass >= (kCluster ? 2 : 1)) {
+      if (kEach >= 4) {
 #pragma unroll
-      for (int i = 0; i < kEach / 4; ++i) reinterpret_cast<uint4*>(hist)[i * kThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
-    } else {
+        for (int i = 0; i < kEach / 4; ++i) reinterpret_cast<uint4*>(hist)[i * kThreads + tid] = make_uint4(0u, 0u, 0u, 0u);
+      } else {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) hist[i * kThreads + tid] = 0u;
+        for (int i = 0; i < kEach; ++i) hist[i * kThreads + tid] = 0u;
+      }
+      sync();
     }
-    sync();
+#pragma unroll 4
     for (int i = tid; i < mine; i += kThreads) {
       const unsigned k = pick_key(scores[i]) - least;
       if ((static_cast<unsigned long long>(k) >> (shift + bits)) == prefix) atomicAdd(hist + ((k >> shift) & ((1u << bits) - 1u)), 1u);
@@ -260,7 +264,7 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
     }
     if (lane == 0) sh.warp_a[wid] = upto;
     sync();
-    for (int w = wid + 1; w < kWarps; ++w) upto += sh.warp_a[w];
+    upto += __reduce_add_sync(0xffffffffu, lane > wid && lane < kWarps ? sh.warp_a[lane] : 0u);
     unsigned above = upto - sum;
     if (above < want && upto >= want) {
 #pragma unroll
@@ -269,6 +273,7 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
           sh.bin = tid * kEach + i;
           sh.want = want - above;
           sh.in_bin = own[i];
+          sh.listed = 0;
         }
         above += own[i];
       }
@@ -276,11 +281,49 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
     sync();
     prefix = (prefix << bits) | sh.bin;
     want = sh.want;
-    if (sh.in_bin == want || shift == 0) break;      // (alike in all blocks)
+    const unsigned left = sh.in_bin;
+    if (left == want || shift == 0) break;           // (alike in all blocks)
+    if (left > 32) continue;
+#pragma unroll 4
+    for (int i = tid; i < mine; i += kThreads) {
+      const unsigned k = pick_key(scores[i]) - least;
+      if (k >> shift == prefix) sh.list[atomicAdd(&sh.listed, 1u)] = k;
+    }
+    if (kCluster) cluster_sync_all();
+    else sync();
+    unsigned key = 0;
+    if (kCluster) {
+      unsigned to = lane < parts ? pick_peer_load(&sh.listed, lane) : 0u, from;
+      const unsigned count = to;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, to, o);
+        if (lane >= o) to += x;
+      }
+      from = to - count;
+      for (int k = 0; k < parts; ++k) {
+        const int a = static_cast<int>(__shfl_sync(0xffffffffu, from, k)), b = static_cast<int>(__shfl_sync(0xffffffffu, to, k));
+        if (lane >= a && lane < b) key = pick_peer_load(sh.list + (lane - a), k);
+      }
+    } else if (lane < static_cast<int>(left)) {
+      key = sh.list[lane];
+    }
+    unsigned larger = 0, alike = 0;
+    for (int i = 0; i < static_cast<int>(left); ++i) {
+      const unsigned x = __shfl_sync(0xffffffffu, key, i);
+      larger += x > key;
+      alike += x == key;
+    }
+    const int at = __ffs(__ballot_sync(0xffffffffu, lane < static_cast<int>(left) && larger < want && larger + alike >= want)) - 1;
+    prefix = __shfl_sync(0xffffffffu, key, at);
+    want -= __shfl_sync(0xffffffffu, larger, at);
+    shift = 0;
+    break;
   }
   // kept: larger prefixes, and the first `want` of the equal ones
   const int seg = ((mine + kWarps - 1) / kWarps + 31) & ~31, s0 = min(mine, wid * seg), s1 = min(mine, s0 + seg);
   unsigned over = 0, tied = 0;
+#pragma unroll 4
   for (int i0 = s0; i0 < s1; i0 += 32) {
     const int i = i0 + lane;
     const unsigned k = i < s1 ? (pick_key(scores[i]) - least) >> shift : 0u;
@@ -289,8 +332,7 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
   }
   if (lane == 0) { sh.warp_a[wid] = over; sh.warp_b[wid] = tied; }
   sync();
-  unsigned over0 = 0, tied0 = 0;
-  for (int w = 0; w < wid; ++w) { over0 += sh.warp_a[w]; tied0 += sh.warp_b[w]; }
+  unsigned over0 = __reduce_add_sync(0xffffffffu, lane < wid ? sh.warp_a[lane] : 0u), tied0 = __reduce_add_sync(0xffffffffu, lane < wid ? sh.warp_b[lane] : 0u);
   if (kCluster) {
     if (tid == kThreads - 1) { sh.counts[0] = over0 + over; sh.counts[1] = tied0 + tied; }
     cluster_sync_all();
@@ -299,6 +341,7 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
     over0 += __reduce_add_sync(0xffffffffu, x);
     tied0 += __reduce_add_sync(0xffffffffu, y);
   }
+#pragma unroll 4
   for (int i0 = s0; i0 < s1; i0 += 32) {
     const int i = i0 + lane;
     const unsigned k = i < s1 ? (pick_key(scores[i]) - least) >> shift : 0u, below = (1u << lane) - 1u;
@@ -364,6 +407,8 @@ __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickP
     load_bounds(a, unit);
     load_ids(base + kAll);
   }
+
+  for (int i = threadIdx.x; i < kPickBins / 4; i += kPickThreads) reinterpret_cast<uint4*>(sh.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
 
   // ---- codes of the queries: a+ against the largest values, a- against the smallest
   for (int i = wid; i < tiles * 8; i += kPickWarps) {
@@ -773,6 +818,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
     return;
   }
   PickShared* sh = reinterpret_cast<PickShared*>(stages);    // [2] (the last products have been waited for)
+  for (int i = threadIdx.x & 255; i < kPickBins / 4; i += 256) reinterpret_cast<uint4*>(sh[w].hist)[i] = make_uint4(0u, 0u, 0u, 0u);
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
   if (wid >= 8 && lane == 0) {
