@@ -103,7 +103,8 @@ struct PickParams {
   const int *block_table, *kv_lens, *cu_q;
   int* out;                    // [rows][hkv][width]
   long long pages;
-  int seqs, tokens, hq, hkv, run, page_shift, max_pages, top, first, last, width, parts;
+  int seqs, rows, tokens, hq, hkv, run, page_shift, max_pages, top, first, last, width, parts;
+  int pairs;                   // rows of runs of twice as many queries
   DeviceStatus* status;
 };
 
@@ -123,8 +124,8 @@ struct PickRange {
   int n;
 };
 
-__device__ __forceinline__ RunOfRow pick_run(const PickParams& p, int row) {
-  return run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)), p.tokens);
+__device__ __forceinline__ RunOfRow pick_run(const PickParams& p, int row, int runs = 1) {
+  return run_of_row(p.cu_q, p.kv_lens, p.seqs, runs * p.run, row, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x7fffffffll)), p.tokens);
 }
 
 // The pages that are kept whatever the scores, of run x.run (written by the block of rank 0); false: nothing is left to choose.
@@ -356,9 +357,9 @@ __device__ __forceinline__ void pick_select(PickShared& sh, int tid, int bar, co
 
 // A cluster of `parts` blocks per row of runs and key head; each scores a share of the pages, a warp 16 at a time. Pages are rows of the product
 // and queries (with their heads) its columns, eight a tile: groups of up to eight heads fill one, and the maximum over them is two exchanges. The bounds of the
-// next 16 pages are on their way into registers while some are multiplied. One token of 16 sequences of 2000 to 6000 tokens, 32 heads on 8: 7.7 us, of which the
+// next 16 pages are on their way into registers while some are multiplied. One token of 16 sequences of 2000 to 6000 tokens, 32 heads on 8: 6.7 us, of which the
 // loads' latencies one after the other (length, page number, bounds) and the choice's barriers are the most; 16.8 with queries as
-// rows, 256 threads and digits of 8 bits. One token behind 131072, 64 heads on 8: 15.1 us, the cluster's counts among them (1.2 TB/s).
+// rows, 256 threads and digits of 8 bits. One token behind 131072, 64 heads on 8: 14.9 us, the cluster's counts among them (1.2 TB/s).
 template <int D>
 __global__ void __launch_bounds__(kPickThreads, 1) pick_pages_kernel(const PickParams p) {
   pdl_wait();
@@ -552,11 +553,12 @@ static int launch_pick(const PickParams& p, int rows, int smem, cudaStream_t str
 // runs of a sequence, up to 128 queries each. Pages are rows of the product, so a thread of the epilogue owns a page and takes the maximum over a run's queries by itself.
 //   warp 0        TMA producer: the codes of 128 pages into one of three stages, four pages a gather
 //   warp 1        one thread issues the products
+//   warp 3        rows of no run
 //   warps 8..15   scores: a page a thread, its 16 to 128 sums of one of the runs from one of two halves of TMEM; then half of the block chooses for each run
-// 2048 queries of 64 heads on 8, runs of 16, behind 30720: 146 us, 3.5 blocks a processor one after the other. A block's time is that of its gathers (a row of 2 D
-// bytes lies on any 16-byte boundary, and a processor fetches 14 bytes of such rows a cycle, by TMA as by copies of 16 bytes a lane), of the maxima beside them, and of what
-// neither hides, the coding of the queries and the choice. A tile serves two runs for the gathers' sake (one: 218 us; mma.sync, whose 8-bit products have a fifth of the
-// rate, 307).
+// 2048 queries of 64 heads on 8, runs of 16, behind 30720: 137 us, 3.5 blocks a processor one after the other. A block takes about 11 us for its start, the coding of
+// the queries and the choice, and 1.4 a tile: the way from a gather (16 bytes of such rows a processor and cycle) over products and TMEM to the maxima, whose instructions are 0.4 of
+// them. A tile serves two runs (one: 218 us; mma.sync, whose 8-bit products have a fifth of the rate, 307); loads of 32 columns ahead of the maxima 159, a fourth stage 150, gathers
+// from rows of 256 bytes 150, all against 146.
 constexpr int kPtThreads = 512, kPtTile = 128, kPtStages = 3;
 
 struct PickTcShared {
@@ -580,29 +582,40 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
   constexpr int kAtoms = 2 * D / 128, kRow = 2 * D + kBoundsTail, kStage = kPtTile * 2 * D, kAtom = 2 * kPickRows * 128;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pick_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, group = p.hq / p.hkv;
-  const int row = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, cols = (p.run * group + 15) & ~15;
+  const int pair = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, cols = (p.run * group + 15) & ~15;
   uint8_t* stages = smem;                                    // [3][atom][128 pages][128 bytes]; the choice works here afterwards
   uint8_t* codes = stages + kPtStages * kStage;              // [atom][256 queries][128 bytes]
   float* factor = reinterpret_cast<float*>(codes + kAtoms * kAtom);              // of a query: 2^e
   PickTcShared& bars = *reinterpret_cast<PickTcShared*>(factor + 2 * kPickRows);
   float* scores = reinterpret_cast<float*>(&bars + 1);       // [2][pages]
   const auto out_of = [&](int i) { return p.out + (static_cast<long long>(i) * p.hkv + h) * p.width; };
-  // the runs of this block: an even one of a sequence and the one behind it (whose own block leaves). Rows of no run are written by their own blocks.
+  // rows of no run: one warp of a block looks some up, beside the others' work
+  const auto leave_out = [&] {
+    for (int row = pair; row < p.rows; row += p.pairs) {
+      if (pick_run(p, row).tokens > 0) continue;
+      for (int i = lane; i < p.width; i += 32) out_of(row)[i] = -1;
+    }
+  };
+  // the runs of this block: two neighbouring ones of a sequence, which are one of twice as many queries
   PickRange x[2];
   int rows[2], runs = 0;
   {
-    PickRange y{pick_run(p, row), 0};
-    const int len = y.run.kv_len - y.run.begin, rest = len - y.run.tokens;      // queries from the run's first on, and behind the run
-    const int first_q = p.cu_q ? p.cu_q[y.run.seq] : y.run.seq;
-    if (y.run.tokens > 0 && ((y.run.q_off - first_q) / p.run & 1)) return;
-    if (pick_range(p, out_of(row), true, y)) { x[runs] = y; rows[runs++] = row; }
-    if (y.run.tokens > 0 && rest > 0) {
-      y.run.q_off += p.run;
-      y.run.begin += p.run;
-      y.run.tokens = min(min(p.run, rest), p.tokens - y.run.q_off);
+    PickRange y{pick_run(p, pair, 2), 0};
+    RunOfRow& r = y.run;
+    const int first_q = p.cu_q ? p.cu_q[r.seq] : r.seq, rest = r.tokens - p.run;
+    const int row = static_cast<int>((first_q + static_cast<long long>(r.seq) * (p.run - 1)) / p.run) + (r.q_off - first_q) / p.run;
+    r.tokens = min(r.tokens, p.run);
+    if (r.tokens > 0 && pick_range(p, out_of(row), true, y)) { x[runs] = y; rows[runs++] = row; }
+    if (rest > 0) {
+      r.q_off += p.run;
+      r.begin += p.run;
+      r.tokens = rest;
       if (pick_range(p, out_of(row + 1), true, y)) { x[runs] = y; rows[runs++] = row + 1; }
     }
-    if (runs == 0) return;
+    if (runs == 0) {
+      if (wid == 3) leave_out();
+      return;
+    }
     if (runs == 1) { x[1] = x[0]; rows[1] = rows[0]; }
   }
   const int n = max(x[0].n, x[1].n), n_tiles = (n + kPtTile - 1) / kPtTile;
@@ -746,6 +759,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
       }
     }
     __syncwarp();
+  } else if (wid == 3) {
+    leave_out();
   } else if (wid >= 8 && wid < 8 + 4 * runs) {
     const int w = (wid - 8) >> 2, mine = threadIdx.x & 127;  // run, page of a tile = TMEM lane
     const uint32_t column = tmem_base + (static_cast<uint32_t>((wid & 3) * 32) << 16) + w * cols;
@@ -833,13 +848,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
 }
 
 template <int D>
-static int launch_pick_tc(const PickParams& p, int rows, int smem, cudaStream_t stream) {
+static int launch_pick_tc(const PickParams& p, int smem, cudaStream_t stream) {
   static PerDeviceOnce configured;
   if (configured.first_time() && cudaFuncSetAttribute(pick_pages_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448) != cudaSuccess) return -200;
   CUtensorMap tm;
   const int rc = make_kmajor_map(&tm, p.bounds, 1, p.pages * p.hkv, 2 * D, 2 * D + kBoundsTail, 1);
   if (rc) return rc;
-  const cudaError_t e = launch_pdl(pick_pages_tc_kernel<D>, dim3(static_cast<unsigned>(rows) * p.hkv), dim3(kPtThreads), smem, stream, p, tm);
+  const cudaError_t e = launch_pdl(pick_pages_tc_kernel<D>, dim3(static_cast<unsigned>(p.pairs) * p.hkv), dim3(kPtThreads), smem, stream, p, tm);
   return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
 }
 
@@ -891,7 +906,7 @@ B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block
   p.block_table = block_table; p.kv_lens = kv_lens; p.cu_q = cu_q;
   p.out = out;
   p.pages = pages;
-  p.seqs = seqs; p.tokens = tokens; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages;
+  p.seqs = seqs; p.rows = rows; p.tokens = tokens; p.hq = hq; p.hkv = hkv; p.run = run; p.max_pages = max_pages;
   p.top = top; p.first = first; p.last = last; p.width = width;
   p.status = static_cast<DeviceStatus*>(status);
   // Tiles of 128 queries pay from 17 on, once there are more rows than processors: below that the other kernel's blocks share a row, and few queries leave most
@@ -899,8 +914,10 @@ B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block
   // 32, 600, 270 37 / 37; 32, 2000, 1920 213 / 294; 64, 304, 270 26 / 28; 64, 64, 1880 30 / 22; 128, 152, 270 18 / 27; 128, 32, 1880 37 / 22; 128, 504, 1920
   // 77 / 163; heads of 64: 28, 500, 1920 51 / 66; 56, 76, 270 13 / 10; 112, 126, 1920 36 / 29.
   const long long smem_tc = 1024 + (kPtStages * kPtTile + 2 * kPickRows) * 2 * d + 2 * kPickRows * 4 + static_cast<int>(sizeof(PickTcShared)) + 8ll * max_pages;
-  if (run * (hq / hkv) > 16 && static_cast<long long>(rows) * hkv > num_sms() && smem_tc <= 232448 && static_cast<long long>(rows) * hkv < (1ll << 31) && pages * hkv < (1ll << 31))
-    return d == 128 ? launch_pick_tc<128>(p, rows, static_cast<int>(smem_tc), stream) : launch_pick_tc<64>(p, rows, static_cast<int>(smem_tc), stream);
+  if (run * (hq / hkv) > 16 && static_cast<long long>(rows) * hkv > num_sms() && smem_tc <= 232448 && static_cast<long long>(rows) * hkv < (1ll << 31) && pages * hkv < (1ll << 31)) {
+    p.pairs = static_cast<int>((tokens + static_cast<long long>(seqs) * (2 * run - 1)) / (2 * run));
+    return d == 128 ? launch_pick_tc<128>(p, static_cast<int>(smem_tc), stream) : launch_pick_tc<64>(p, static_cast<int>(smem_tc), stream);
+  }
   const int fixed = (static_cast<int>(sizeof(PickShared)) + 15) / 16 * 16 + (run * (hq / hkv) + 7) / 8 * 8 * (2 * d + 64);
   // blocks of a row: as long as every processor has one at most and a block 256 pages to score; at least as many as hold the scores
   p.parts = 1;

@@ -55,7 +55,7 @@ __device__ __forceinline__ RunOfRow run_of_row(const int* __restrict__ cu_q, con
   const int first = static_cast<int>((off + static_cast<long long>(r.seq) * (run - 1)) / run);
   const int skip = (row - first) * run;            // queries of the sequence in front of the run
   r.q_off = off + skip;
-  r.tokens = skip < 0 ? 0 : min(min(run, len - skip), tokens - r.q_off);
+  r.tokens = skip < 0 || off < 0 ? 0 : min(min(run, len - skip), tokens - r.q_off);
   r.kv_len = min(kv_lens[r.seq], most_keys);
   r.begin = r.kv_len - len + skip;
   return r;
