@@ -184,6 +184,24 @@ def test_the_choice_of_many_runs_is_that_of_the_host(each, lens, hq, hkv, d, run
 
 
 @gpu
+@pytest.mark.parametrize("front,behind", [(0, 0), (50, 0), (0, 700), (3, 21)])
+@pytest.mark.parametrize("run,group", [(5, 4), (16, 4), (16, 2), (21, 6)])
+def test_the_choice_of_many_short_sequences_is_that_of_the_host(front, behind, run, group):
+    """Sequences of no, one, two and three runs, whole ones and not, and rows of q that no sequence has: rows of no run lie between the others, and are -1 too."""
+    each = [(17 * i + i // 5) % (2 * run + 7) if i % 7 else 0 for i in range(60)]
+    b = Batch(each, [m + (37 * i) % 300 for i, m in enumerate(each)], 3 * group, 3, 64, 16, seed=run).fill_bounds()
+    b.q = torch.cat([b.q[:1].expand(front, -1, -1), b.q, b.q[:1].expand(behind, -1, -1)])
+    b.cu_q += front
+    want = b.pick(top=4, run=run)
+    assert want.shape[0] * 3 > 148 and (want == -1).all(-1).all(-1).sum() > len(each) // 3
+    b.to("cuda")
+    full_of_sevens = torch.full_like(want, 7, device="cuda")
+    del full_of_sevens                               # its memory is likely to be the result's
+    assert torch.equal(b.pick(top=4, run=run).cpu(), want)
+    N.check_status()
+
+
+@gpu
 @pytest.mark.parametrize("pages,extra,top", [(3000, 0, 100), (9000, 3000, 1), (9000, 0, 2500), (2100, 60000, 300)])
 def test_a_long_table_is_shared_by_blocks(pages, extra, top):
     """One sequence; wide tables whose scores no single block holds. Bounds are random bytes."""
