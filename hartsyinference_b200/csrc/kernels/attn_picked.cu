@@ -13,7 +13,7 @@
 // A row whose pages are too many for one block's warps is shared by a cluster of up to eight blocks (every eighth page each), which meet
 // through distributed shared memory: one launch, no scratch.
 //
-// One token of 64 sequences, 64 heads on 8, 2096 keys each: 92 us, 6.0 TB/s of keys and values. One token behind 131001, 32 heads on 8, 4096 keys: 11.5 us, the
+// One token of 64 sequences, 64 heads on 8, 2096 keys each: 89 us, 6.2 TB/s of keys and values. One token behind 131001, 32 heads on 8, 4096 keys: 11.5 us, the
 // latencies of pages chosen, page numbers, keys, values and the join one after the other.
 #include <math.h>
 

@@ -555,7 +555,7 @@ static int launch_pick(const PickParams& p, int rows, int smem, cudaStream_t str
 //   warp 1        one thread issues the products
 //   warp 3        rows of no run
 //   warps 8..15   scores: a page a thread, its 16 to 128 sums of one of the runs from one of two halves of TMEM; then half of the block chooses for each run
-// 2048 queries of 64 heads on 8, runs of 16, behind 30720: 137 us, 3.5 blocks a processor one after the other. A block takes about 11 us for its start, the coding of
+// 2048 queries of 64 heads on 8, runs of 16, behind 30720: 135 us, 3.5 blocks a processor one after the other. A block takes about 11 us for its start, the coding of
 // the queries and the choice, and 1.4 a tile: the way from a gather (16 bytes of such rows a processor and cycle) over products and TMEM to the maxima, whose instructions are 0.4 of
 // them. A tile serves two runs (one: 218 us; mma.sync, whose 8-bit products have a fifth of the rate, 307); loads of 32 columns ahead of the maxima 159, a fourth stage 150, gathers
 // from rows of 256 bytes 150, all against 146.
@@ -621,6 +621,21 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
   const int n = max(x[0].n, x[1].n), n_tiles = (n + kPtTile - 1) / kPtTile;
   const int* ids = p.block_table + static_cast<long long>(x[0].run.seq) * p.max_pages + p.first;
 
+  // the queries on their way: D / 8 lanes a query, 16 bytes each
+  constexpr int kQLanes = D / 8, kQueries = 32 / kQLanes, kRounds = kPickRows / (16 * kQueries);
+  const int u = lane % kQLanes, inverse = (65536 + group - 1) / group;      // i / group for i < 128 is a product and a shift
+  uint4 raw[2][kRounds];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const RunOfRow& r = x[w].run;
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      // (rows that pad, and queries in front of the first key, repeat one that counts)
+      const int i = (k * 16 + wid) * kQueries + lane / kQLanes, at = i * inverse >> 16, token = min(max(at, -r.begin), r.tokens - 1);
+      raw[w][k] = __ldg(reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(r.q_off + token) * p.hq + h * group + i - at * group) * D + u * 8));
+    }
+  }
+
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPtStages; ++i) {
       mbar_init(&bars.a_full[i], 4);
@@ -669,23 +684,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
       if (j < n_tiles) gather(j, from[j]);
   }
 
-  // ---- codes of the queries: D / 8 lanes a query, 16 bytes each, half of the loads of a warp ahead of their use
+  // ---- codes of the queries
   {
-    constexpr int kQLanes = D / 8, kQueries = 32 / kQLanes, kRounds = kPickRows / (16 * kQueries);
-    const int u = lane % kQLanes, inverse = (65536 + group - 1) / group;      // i / group for i < 128 is a product and a shift
-    for (int w = 0; w < runs; ++w) {
-      const RunOfRow& r = x[w].run;
-      uint4 raw[kRounds];
 #pragma unroll
-      for (int k = 0; k < kRounds; ++k) {
-        // (rows that pad, and queries in front of the first key, repeat one that counts)
-        const int i = (k * 16 + wid) * kQueries + lane / kQLanes, at = i * inverse >> 16, token = min(max(at, -r.begin), r.tokens - 1);
-        raw[k] = __ldg(reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(r.q_off + token) * p.hq + h * group + i - at * group) * D + u * 8));
-      }
+    for (int w = 0; w < 2; ++w) {
+      if (w >= runs) break;
 #pragma unroll
       for (int k = 0; k < kRounds; ++k) {
         const int i = (k * 16 + wid) * kQueries + lane / kQLanes, at = w * cols + i;
-        const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw[k]);
+        const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&raw[w][k]);
         float v[8], amax = 0.f;
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
@@ -910,9 +917,10 @@ B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block
   p.top = top; p.first = first; p.last = last; p.width = width;
   p.status = static_cast<DeviceStatus*>(status);
   // Tiles of 128 queries pay from 17 on, once there are more rows than processors: below that the other kernel's blocks share a row, and few queries leave most
-  // of a tile empty. us, tiles / mma.sync, heads of 128 (queries of a run, rows x key heads, pages): 8, 8000, 1920 799 / 859; 16, 4000, 190 172 / 161;
-  // 32, 600, 270 37 / 37; 32, 2000, 1920 213 / 294; 64, 304, 270 26 / 28; 64, 64, 1880 30 / 22; 128, 152, 270 18 / 27; 128, 32, 1880 37 / 22; 128, 504, 1920
-  // 77 / 163; heads of 64: 28, 500, 1920 51 / 66; 56, 76, 270 13 / 10; 112, 126, 1920 36 / 29.
+  // of a tile empty. us, tiles / mma.sync, heads of 128 (queries of a run, rows x key heads, pages): 8, 200, 200 11.8 / 12.0; 8, 1000, 200 42 / 38; 8, 1000, 1000 70 / 73;
+  // 16, 1000, 200 42 / 40; 16, 1000, 1000 70 / 78; 24, 160, 1000 19 / 25; 24, 300, 500 25 / 25; 32, 600, 270 33 / 34; 32, 2000, 1920 182 / 285; 64, 304, 270 23 / 25;
+  // 64, 64, 1880 28 / 21; 128, 152, 270 15 / 25; 128, 32, 1880 33 / 21; 128, 504, 1920 67 / 157; heads of 64: 28, 500, 1920 43 / 62; 56, 76, 270 12 / 9;
+  // 112, 126, 1920 32 / 27.
   const long long smem_tc = 1024 + (kPtStages * kPtTile + 2 * kPickRows) * 2 * d + 2 * kPickRows * 4 + static_cast<int>(sizeof(PickTcShared)) + 8ll * max_pages;
   if (run * (hq / hkv) > 16 && static_cast<long long>(rows) * hkv > num_sms() && smem_tc <= 232448 && static_cast<long long>(rows) * hkv < (1ll << 31) && pages * hkv < (1ll << 31)) {
     p.pairs = static_cast<int>((tokens + static_cast<long long>(seqs) * (2 * run - 1)) / (2 * run));
