@@ -31,7 +31,7 @@ def rope_axes_kv(qkv: torch.Tensor, positions: torch.Tensor, hq: int, hkv: int, 
                  want_kv: bool = False):
     """:func:`.core.rope_kv` with positions on several axes: optional QK RMSNorm, then rotary embedding on a packed qkv activation
     [T, (hq + 2 hkv) d], and the K/V write into the page pool ([pages, hkv, page, d]; ``slot_mapping`` int64 [T], page_index * page + offset, below 0:
-    not stored). ``positions`` int32 [A, T]; pair j of the rotated part (the first 2 * len(axes) channels) turns by
+    not stored; no slot twice). ``positions`` int32 [A, T]; pair j of the rotated part (the first 2 * len(axes) channels) turns by
     ``positions[axes[j]] * inv_freq[j]``, in angles of 64 bits; ``axes`` int32 as of :func:`rope_axes`, ``inv_freq`` fp32, both [pairs]. Heads of an
     even size up to 256; style 0 pairs channel j with j + pairs, 1 channel 2 j with 2 j + 1. Returns (q [T, hq, d], k [T, hkv, d] or None, v or None)."""
     shape, where, pairs, device = qkv.shape, positions.shape, axes.numel(), qkv.get_device()

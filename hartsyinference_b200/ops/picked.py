@@ -22,7 +22,7 @@ from .core import quant_fp8_act
 from .kv4 import _dense, _ints, _on
 
 WIDTH = 4096          # pages that a run can choose
-_PAGES, _HEADS, _I32 = (16, 32, 64, 128), (64, 128), torch.int32
+_PAGES, _HEADS, _I32, _BF16 = (16, 32, 64, 128), (64, 128), torch.int32, torch.bfloat16
 
 
 def _plain(x: torch.Tensor, device: int, n: int) -> bool:
@@ -86,7 +86,7 @@ def key_bounds_(bounds: torch.Tensor, k_cache: torch.Tensor, block_table: torch.
     if cu_q is not None and max_q_len is None:
         raise ValueError("key_bounds_: cu_q with the longest run of new tokens, max_q_len")
     if not (device >= 0 and len(shape) == 4 and len(table) == 2 and table[0] == seqs and shape[2] in _PAGES and shape[3] in _HEADS and bounds.dtype is torch.uint8
-            and k_cache.dtype is torch.bfloat16 and block_table.dtype is _I32 and kv_lens.dtype is _I32 and (cu_q is None or _plain(cu_q, device, seqs + 1))
+            and k_cache.dtype is _BF16 and block_table.dtype is _I32 and kv_lens.dtype is _I32 and (cu_q is None or _plain(cu_q, device, seqs + 1))
             and bounds.shape == (shape[0], shape[1], 2 * shape[3] + 16) and device == k_cache.get_device() == block_table.get_device() == kv_lens.get_device()
             and bounds.is_contiguous() and k_cache.is_contiguous() and block_table.is_contiguous() and kv_lens.is_contiguous()):
         # not the ordinary call: say what is wrong, or make it one
@@ -125,11 +125,11 @@ def pick_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor,
     device, shape, rows_of, table = q.get_device(), q.shape, bounds.shape, block_table.shape
     seqs = kv_lens.numel()
     if not (device >= 0 and len(shape) == 3 and len(rows_of) == 3 and len(table) == 2 and table[0] == seqs and shape[2] in _HEADS and page in _PAGES
-            and rows_of[2] == 2 * shape[2] + 16 and shape[1] > 0 and rows_of[1] > 0 and shape[1] % rows_of[1] == 0 and q.dtype is torch.bfloat16
+            and rows_of[2] == 2 * shape[2] + 16 and shape[1] > 0 and rows_of[1] > 0 and shape[1] % rows_of[1] == 0 and q.dtype is _BF16
             and bounds.dtype is torch.uint8 and block_table.dtype is _I32 and kv_lens.dtype is _I32 and (cu_q is None or _plain(cu_q, device, seqs + 1))
             and device == bounds.get_device() == block_table.get_device() == kv_lens.get_device()
             and bounds.is_contiguous() and block_table.is_contiguous() and kv_lens.is_contiguous()):
-        if q.dim() != 3 or (device >= 0 and q.dtype is not torch.bfloat16) or q.shape[2] not in _HEADS:
+        if q.dim() != 3 or (device >= 0 and q.dtype is not _BF16) or q.shape[2] not in _HEADS:
             raise ValueError(f"pick_pages: q is [tokens, hq, 64 or 128], bf16 on a device; got {q.dtype} {tuple(q.shape)}")
         hkv = bounds.shape[1] if bounds.dim() == 3 else 0
         if hkv < 1 or shape[1] < 1 or shape[1] % hkv or page not in _PAGES:
@@ -159,7 +159,7 @@ def pick_pages(q: torch.Tensor, bounds: torch.Tensor, block_table: torch.Tensor,
             else:
                 out[row, :, :len(kept)] = torch.tensor(kept, dtype=torch.int32)
         return out
-    out = q.new_empty((rows, hkv, width), dtype=_I32)
+    out = kv_lens.new_empty((rows, hkv, width))
     with _on(device):
         if pages == 0 or table[1] == 0 or seqs == 0:
             return out.fill_(-1)
@@ -183,11 +183,10 @@ def attn_picked(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
     seqs = kv_lens.numel()
     if not (device >= 0 and len(shape) == 3 and len(pool) == 4 and len(table) == 2 and len(chosen) == 3 and table[0] == seqs and pool[2] in _PAGES and pool[3] in _HEADS
             and shape[2] == pool[3] and shape[1] > 0 and pool[1] > 0 and shape[1] % pool[1] == 0 and v_cache.shape == pool
-            and q.dtype is torch.bfloat16 and k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16 and block_table.dtype is _I32 and kv_lens.dtype is _I32
-            and picked.dtype is _I32 and (cu_q is None or _plain(cu_q, device, seqs + 1))
+            and q.dtype is k_cache.dtype is v_cache.dtype is _BF16 and block_table.dtype is kv_lens.dtype is picked.dtype is _I32 and (cu_q is None or _plain(cu_q, device, seqs + 1))
             and device == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == kv_lens.get_device() == picked.get_device()
             and k_cache.is_contiguous() and v_cache.is_contiguous() and block_table.is_contiguous() and kv_lens.is_contiguous() and picked.is_contiguous()):
-        if q.dim() != 3 or (device >= 0 and q.dtype is not torch.bfloat16):
+        if q.dim() != 3 or (device >= 0 and q.dtype is not _BF16):
             raise ValueError(f"attn_picked: q is [tokens, hq, d], bf16 on a device; got {q.dtype} {tuple(q.shape)}")
         hkv = _pool_of("attn_picked", k_cache, device, shape[2])[1]
         if _pool_of("attn_picked", v_cache, device, shape[2]) != tuple(pool) or hkv < 1 or shape[1] < 1 or shape[1] % hkv:
