@@ -32,7 +32,7 @@ constexpr float kTpRescaleGap = 8.f;
 struct TpBarriers {
   uint64_t q_full, k_full[kTpStages], k_empty[kTpStages], v_full[kTpStages], v_empty[kTpStages];
   uint64_t v_ask, v_clean;                // the V tile at hand has landed; its rows are cleared
-  uint64_t s_full[2], p_ready[2], o_done;
+  uint64_t s_full[2], p_ready[2], o_done, o_last;      // (o_done: of all products but the last)
   uint32_t tmem_base, abort_flag;
   int entries, free_entries, odd;         // pages up to the last real one; those in front of the first that not all rows see; keys that rows add by themselves
   int odd_keys[kTpOdd];                   // place in the list of keys
@@ -82,6 +82,7 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
     mbar_init(&bars->v_ask, 1);
     mbar_init(&bars->v_clean, 1);
     mbar_init(&bars->o_done, 1);
+    mbar_init(&bars->o_last, 1);
     for (int i = 0; i < kTpStages; ++i) {
       mbar_init(&bars->k_full[i], 1);
       mbar_init(&bars->k_empty[i], 1);
@@ -238,7 +239,7 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
 #pragma unroll
           for (int k = 0; k < kTpTile / 16; ++k)
             mma_bf16_ts(tmem_base + 128, tmem_base + (j & 1) * 64 + k * 8, bd + k * (2048 >> 4), kIdescPV, (j | k) != 0);
-          tc_commit(&bars->o_done);
+          tc_commit(j + 1 < n_tiles ? &bars->o_done : &bars->o_last);
           tc_commit(&bars->v_empty[s]);
         }
         if (!ok) report_status(p.status, kWaitTimeout, kKernelPicked, 42, blockIdx.x);
@@ -358,9 +359,9 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->p_ready[j & 1]);
     }
-    // the last scores told of all products but two: each of those is waited for, since a wait for the last alone would take the
-    // phase of the one before the other for it
-    for (int j = max(0, n_tiles - 2); j < n_tiles && ok; ++j) ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_done, j & 1, abort_flag));
+    // The last product has a barrier of its own, with a single phase: the last scores told of all products but two, and a warp that comes late
+    // to o_done's last two phases finds both gone by, which looks like the first of them still to come.
+    if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_last, 0, abort_flag));
     if (!ok) {
       if (lane == 0) report_status(p.status, kWaitTimeout, kKernelPicked, 43, blockIdx.x);
     } else {
