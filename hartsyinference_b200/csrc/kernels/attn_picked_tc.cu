@@ -25,7 +25,6 @@ constexpr int kTpThreads = 256;
 constexpr int kTpTile = 64;               // keys
 constexpr int kTpStages = 2;
 constexpr int kTpWidth = 1024;            // pages of a row that the list in shared memory holds
-constexpr int kTpOdd = 128;
 constexpr int kTpFar = 0x40000000;        // first key of what is no page
 constexpr float kTpRescaleGap = 8.f;
 
@@ -34,8 +33,7 @@ struct TpBarriers {
   uint64_t v_ask, v_clean;                // the V tile at hand has landed; its rows are cleared
   uint64_t s_full[2], p_ready[2], o_done, o_last;      // (o_done: of all products but the last)
   uint32_t tmem_base, abort_flag;
-  int entries, free_entries, odd;         // pages up to the last real one; those in front of the first that not all rows see; keys that rows add by themselves
-  int odd_keys[kTpOdd];                   // place in the list of keys
+  int entries, free_entries, odd;         // pages up to the last real one; those in front of the first that not all rows see; whether there are keys that rows add by themselves
 };
 
 struct TpParams {
@@ -54,6 +52,9 @@ __device__ __forceinline__ float tp_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Whether one of two bf16 is not finite.
+__device__ __forceinline__ bool tp_not_finite(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 
 template <int D>
 __global__ void __launch_bounds__(kTpThreads, 2)
@@ -264,17 +265,12 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
               const uint4 w = *at;
               const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-              for (int u = 0; u < 4; ++u) odd |= (x[u] & 0x7f80u) == 0x7f80u || (x[u] & 0x7f800000u) == 0x7f800000u;
+              for (int u = 0; u < 4; ++u) odd |= tp_not_finite(x[u]);
             }
-            odd = __any_sync(0xffffffffu, odd) && e.y + c < end;
-            const int n = bars->odd;
-            if (e.y + c >= end || (odd && n < kTpOdd)) {
+            odd = __any_sync(0xffffffffu, odd);
+            if (e.y + c >= end || odd) {
               if (lane < 8 * kHalves) *at = make_uint4(0u, 0u, 0u, 0u);
-              __syncwarp();
-              if (odd && lane == 0) {
-                bars->odd_keys[n] = (j << 6) + (i << p.box_shift) + c;
-                bars->odd = n + 1;
-              }
+              if (e.y + c < end && lane == 0) bars->odd = 1;
               __syncwarp();
             }
           }
@@ -367,7 +363,7 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
     } else {
       tc_fence_after_sync();
       const float inv = l_run > 0.f ? 1.f / l_run : l_run == 0.f ? 0.f : l_run;       // nothing seen: zeros; NaN stays
-      const int odd = *reinterpret_cast<volatile int*>(&bars->odd);
+      const bool odd = *reinterpret_cast<volatile int*>(&bars->odd) != 0;
       // The Q tile is no longer read: 32 rows of 128 bytes per warp turn the rows that the lanes hold into
       // 128-byte runs. 16-byte pieces are placed by (piece xor row), which keeps the banks apart.
       uint8_t* strip = sq + quarter * 32 * 128;
@@ -377,20 +373,24 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
         tmem_ld_32x32(o_col + hc * 64, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
         tmem_ld_32x32(o_col + hc * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
         tmem_ld_wait();
-        for (int n = 0; n < odd; ++n) {
-          // a key whose values are not all finite: this row's probability of it, once more
-          const int place = *reinterpret_cast<volatile int*>(&bars->odd_keys[n]);
-          const int2 e = piece(place >> p.box_shift);
-          const int sub = place & (box - 1);
-          if (e.y + sub >= lim) continue;
-          const __nv_bfloat16* qr = p.q + (static_cast<long long>(r.q_off + row / group) * p.hq + h * group + row % group) * D;
-          const __nv_bfloat16* kr = p.k + static_cast<long long>(e.x + sub) * D;
-          const __nv_bfloat16* vr = p.v + static_cast<long long>(e.x + sub) * D + hc * 64;
-          float s = 0.f;
-          for (int i = 0; i < D; ++i) s += __bfloat162float(qr[i]) * __bfloat162float(kr[i]);
-          const float w = tp_exp2(fmaf(s, c, -(m_run == -INFINITY ? 0.f : m_run)));
+        // keys whose values are not all finite: this row's probability of them, once more (all that were cleared are looked for again, however
+        // often their page is named)
+        for (int n = odd ? free_tiles << per_tile_shift : pieces; n < pieces; ++n) {
+          const int2 e = piece(n);
+          if (e.y == kTpFar) continue;
+          for (int sub = max(0, free_keys - e.y); sub < box && e.y + sub < lim; ++sub) {
+            const __nv_bfloat16* vr = p.v + static_cast<long long>(e.x + sub) * D;
+            bool some = false;
+            for (int i = 0; i < D / 2; ++i) some |= tp_not_finite(reinterpret_cast<const uint32_t*>(vr)[i]);
+            if (!some) continue;
+            const __nv_bfloat16* qr = p.q + (static_cast<long long>(r.q_off + row / group) * p.hq + h * group + row % group) * D;
+            const __nv_bfloat16* kr = p.k + static_cast<long long>(e.x + sub) * D;
+            float s = 0.f;
+            for (int i = 0; i < D; ++i) s += __bfloat162float(qr[i]) * __bfloat162float(kr[i]);
+            const float w = tp_exp2(fmaf(s, c, -(m_run == -INFINITY ? 0.f : m_run)));
 #pragma unroll
-          for (int i = 0; i < 64; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + w * __bfloat162float(vr[i]));
+            for (int i = 0; i < 64; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) + w * __bfloat162float(vr[hc * 64 + i]));
+          }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

@@ -1,10 +1,12 @@
 """Attention over chosen pages where its parts meet."""
+import math
+
 import pytest
 import torch
 
 from hartsyinference_b200.ops import _native as N
 
-from .test_picked import Batch
+from .test_picked import Batch, _attention
 
 gpu = pytest.mark.gpu
 
@@ -23,3 +25,28 @@ def test_many_blocks_one_after_the_other_end_without_a_wait_that_runs_out(hq, hk
         got = b.attend(picked, run=run)
     N.check_status()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dev,tiles", [("cpu", 0), pytest.param("cuda", 0, marks=gpu), pytest.param("cuda", 1, marks=gpu)])
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 16), (128, 64), (64, 128)])
+@pytest.mark.parametrize("times", [1, 2, 5])
+def test_many_values_that_are_not_finite_in_pages_named_several_times(dev, tiles, d, page, times, monkeypatch):
+    """A run of 128 queries whose own keys all have an infinite value, each in a channel of its own; its own pages are named up to five times, which makes
+    up to 880 such keys. Every query has them in the channels of the keys that it sees, and the other channels are those of finite values."""
+    if dev == "cuda":
+        monkeypatch.setattr(N.lib(), "b200_attn_picked_form", lambda *a: tiles)
+    before = 47
+    b = Batch([128], [before + 128], 1, 1, d, page)
+    last = (before + 127) // page
+    own = list(range(before // page, last + 1))
+    picked = torch.tensor([[[0] * (before >= page) + own * times + [last + 1, -1]]], dtype=torch.int32)
+    want, bound = _attention(b, picked, 128)
+    infinite = torch.zeros(128, d, dtype=torch.bool)
+    for t in range(128):
+        at = before + t
+        b.v[b.table[0, at // page].long(), 0, at % page, t % d] = math.inf
+        infinite[t:, t % d] = True
+    got = b.to(dev).attend(picked.to(dev), run=128).double().cpu()[:, 0]
+    assert (got[infinite] == math.inf).all()
+    off = (got - want[:, 0]).abs()
+    assert (off[~infinite] <= bound[:, 0][~infinite]).all()
