@@ -1,4 +1,4 @@
-// Attention over chosen pages (rows of page numbers: picked.cuh), for decoded tokens, a few queries, and runs of a prompt.
+// Attention over chosen pages (rows of page numbers: picked.cuh), for decoded tokens, a few queries, and runs of a prompt that have a cap or few columns.
 //
 // A block owns 8 or more columns, a column being a query head of a token of one run, all on one key head, and walks the chosen pages in units of
 // 16 keys, every warp units of its own. Products are mma.sync with the keys as rows (S = K Q^T, O^T = V^T P^T): eight columns fill a tile of eight,
@@ -429,6 +429,9 @@ constexpr int kPickedWidth = 4096;
 // and 9 for every eight columns (7 and 5.3), and few rows are shared by several blocks. us, here / tiles, rows x key heads in front: heads of 128, 24 columns: 144 36 / 56,
 // 192 65 / 57, 400 99 / 112; 40 columns: 32 39 / 41, 64 60 / 45, 144 63 / 57, 288 122 / 68; 64 columns: 16 33 / 41, 32 56 / 41, 400 283 / 116; 128 columns: 8 37 / 40,
 // 16 53 / 41; heads of 64, 35 columns: 24 26 / 35, 48 39 / 35; 112 columns: 16 33 / 35, 24 54 / 35. Up to 16 columns there is little between the two from 200 rows on.
+// (Sequences of one run, which leave every other row of the grid without one.) One query of each sequence, whose heads are the columns and whose rows all have a run:
+// heads of 128, 24 columns: 144 34 / 48, 192 64 / 55; 64 columns: 16 43 / 39, 32 32 / 39, 148 97 / 50, 400 282 / 109; 128 columns: 8 35 / 39, 16 69 / 39, 300 420 / 104;
+// heads of 64, 112 columns: 8 22 / 33, 24 32 / 33, 200 184 / 45.
 B200_API int b200_attn_picked_form(int rows, int cols, int hkv, int d, int page, int width, long long pages, float scale, float softcap) {
   if (cols <= 16 || width > 1024 || !(scale > 0.f) || softcap > 0.f || pages * hkv * page >= (1ll << 31)) return 0;
   const double r = static_cast<double>(rows) * hkv, sms = num_sms(), keys = width * static_cast<double>(page) / 2112.;

@@ -1,4 +1,4 @@
-// Attention over chosen pages (picked.cuh) for runs of a prompt, on the 5th-generation tensor cores.
+// Attention over chosen pages (picked.cuh) for runs of a prompt, and for single queries with many heads on a key head, on the 5th-generation tensor cores.
 //
 // One CTA owns one row of pages: the queries of a run times the heads of a group, up to 128 rows of Q, walk the keys of the pages that they chose
 // together in tiles of 64. Rows have pages of their own, so two of them share nothing; two CTAs lie on a processor instead, and one's products

@@ -6,7 +6,7 @@ import torch
 
 from hartsyinference_b200.ops import _native as N
 
-from .test_picked import Batch, _attention
+from .test_picked import Batch, _attention, _close, _some
 
 gpu = pytest.mark.gpu
 
@@ -50,3 +50,28 @@ def test_many_values_that_are_not_finite_in_pages_named_several_times(dev, tiles
     assert (got[infinite] == math.inf).all()
     off = (got - want[:, 0]).abs()
     assert (off[~infinite] <= bound[:, 0][~infinite]).all()
+
+
+@gpu
+@pytest.mark.parametrize("tiles", [0, 1])
+@pytest.mark.parametrize("hq,hkv,d,page", [(48, 2, 128, 16), (100, 1, 128, 32), (33, 1, 64, 16), (254, 2, 64, 128), (128, 1, 128, 64)])
+def test_single_tokens_of_many_heads_on_a_key_head(hq, hkv, d, page, tiles, monkeypatch):
+    """Decoded tokens without cu_q by each of the two kernels: sequences of no keys, one key, ends inside a page and on its border."""
+    monkeypatch.setattr(N.lib(), "b200_attn_picked_form", lambda *a: tiles)
+    b = Batch([1] * 7, [0, 1, page, page + 1, 700, 333, 2 * page - 1], hq, hkv, d, page, seed=hq)
+    picked = _some(b, 1, 9)
+    want = _attention(b, picked, 1)
+    _close(b.to("cuda").attend(picked.cuda(), step=True), want)
+    N.check_status()
+
+
+@gpu
+def test_the_rule_decides_for_single_tokens_too(monkeypatch):
+    called = []
+    for name in ("b200_attn_picked", "b200_attn_picked_tc"):
+        monkeypatch.setattr(N.lib(), name, lambda *a, name=name, call=getattr(N.lib(), name): called.append(name) or call(*a))
+    for n, group in ((160, 64), (160, 8), (2, 64)):
+        b = Batch([1] * n, [40] * n, group, 1, 128, 16).to("cuda")
+        b.attend(torch.arange(132, dtype=torch.int32, device="cuda").expand(n, 1, -1).contiguous(), step=True)
+    N.check_status()
+    assert called == ["b200_attn_picked_tc", "b200_attn_picked", "b200_attn_picked"]
