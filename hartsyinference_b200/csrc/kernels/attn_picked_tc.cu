@@ -73,7 +73,6 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = p.hq / p.hkv;
   const int row_id = blockIdx.x, h = blockIdx.y;
   pdl_wait();
-  pdl_trigger();
   const RunOfRow r = run_of_row(p.cu_q, p.kv_lens, p.seqs, p.run, row_id, static_cast<int>(min(static_cast<long long>(p.max_pages) << p.page_shift, 0x3fffffffll)), p.tokens);
   if (r.tokens <= 0) return;
   const int end = r.begin + r.tokens, real_rows = r.tokens * group;
@@ -136,6 +135,7 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  pdl_trigger();                                        // (not before this block has its TMEM: a kernel that starts early may take what it waits for, and wait for this grid)
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
   volatile uint32_t* abort_flag = &bars->abort_flag;
   const int box = 1 << p.box_shift, per_page = p.page_shift - p.box_shift;      // boxes of a page, as a shift

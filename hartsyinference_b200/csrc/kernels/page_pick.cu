@@ -577,7 +577,6 @@ __device__ __forceinline__ void pick_gather4(void* dst, const CUtensorMap* m, ui
 template <int D>
 __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const PickParams p, const __grid_constant__ CUtensorMap tm) {
   pdl_wait();
-  pdl_trigger();
   extern __shared__ uint8_t pick_raw[];
   constexpr int kAtoms = 2 * D / 128, kRow = 2 * D + kBoundsTail, kStage = kPtTile * 2 * D, kAtom = 2 * kPickRows * 128;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pick_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -655,6 +654,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
   }
   volatile uint32_t* abort_flag = &bars.abort_flag;
   __syncthreads();
+  pdl_trigger();                                             // (not before this block has its TMEM: a kernel that starts early may take what it waits for, and wait for this grid)
   // rows of the pool of bounds: of four neighbouring pages of a tile (one that is no page lies behind the end and arrives as zeros)
   const int quad = (wid & 3) * 8 + (lane & 7);
   const auto rows_of = [&](int j, int (&to)[4]) {
