@@ -32,6 +32,7 @@ struct TpBarriers {
   uint64_t q_full, k_full[kTpStages], k_empty[kTpStages], v_full[kTpStages], v_empty[kTpStages];
   uint64_t v_ask, v_clean;                // the V tile at hand has landed; its rows are cleared
   uint64_t s_full[2], p_ready[2], o_done, o_last;      // (o_done: of all products but the last)
+  uint64_t drain;                         // all products have been carried out
   uint32_t tmem_base, abort_flag;
   int entries, free_entries, odd;         // pages up to the last real one; those in front of the first that not all rows see; whether there are keys that rows add by themselves
 };
@@ -83,6 +84,7 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
     mbar_init(&bars->v_clean, 1);
     mbar_init(&bars->o_done, 1);
     mbar_init(&bars->o_last, 1);
+    mbar_init(&bars->drain, 1);
     for (int i = 0; i < kTpStages; ++i) {
       mbar_init(&bars->k_full[i], 1);
       mbar_init(&bars->k_empty[i], 1);
@@ -189,10 +191,15 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
         if (lane < boxes) tma_load_2d(at + (sv - sk), &tm_v, &bars->v_full[s], half * 64, e.x);
         ++v_sent;
       }
+      for (int j = max(0, n_tiles - kTpStages); j < n_tiles && ok; ++j) {      // until the last tiles have been read, or somebody gives up
+        const uint32_t ph = static_cast<uint32_t>((j / kTpStages) & 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_empty[j % kTpStages], ph, abort_flag) && mbar_wait(&bars->v_empty[j % kTpStages], ph, abort_flag));
+      }
       if (!ok) {
         if (lane == 0) report_status(p.status, kWaitTimeout, kKernelPicked, 41, blockIdx.x);
         // copies on their way land before the shared memory is given back
         uint32_t none = 0;
+        mbar_wait(&bars->q_full, 0, &none);
         for (int b = 0; b < kTpStages; ++b) {
           const int k_last = (k_sent - 1 - b) >= 0 ? k_sent - 1 - b : -1, v_last = (v_sent - 1 - b) >= 0 ? v_sent - 1 - b : -1;
           if (k_last >= 0) mbar_wait(&bars->k_full[k_last % kTpStages], static_cast<uint32_t>((k_last / kTpStages) & 1), &none);
@@ -244,6 +251,10 @@ attn_picked_tc_kernel(const TpParams p, const __grid_constant__ CUtensorMap tm_q
           tc_commit(&bars->v_empty[s]);
         }
         if (!ok) report_status(p.status, kWaitTimeout, kKernelPicked, 42, blockIdx.x);
+        // no product reads shared memory or writes TMEM when they are given back, whoever gave up
+        uint32_t none = 0;
+        tc_commit(&bars->drain);
+        mbar_wait(&bars->drain, 0, &none);
       }
     } else if (warp == 2) {
       // ----------------------------------------------------------------------- rows of V that not all rows of P may touch

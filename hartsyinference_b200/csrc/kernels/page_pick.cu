@@ -563,6 +563,7 @@ constexpr int kPtThreads = 512, kPtTile = 128, kPtStages = 3;
 
 struct PickTcShared {
   uint64_t a_full[kPtStages], a_empty[kPtStages], s_full[2], s_empty[2];
+  uint64_t drain;                   // all products have been carried out
   uint32_t tmem_base, abort_flag;
 };
 
@@ -644,6 +645,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.s_empty[i], 4 * runs);
     }
+    mbar_init(&bars.drain, 1);
     bars.abort_flag = 0;
     fence_mbar_init();
     prefetch_tensormap(&tm);
@@ -732,16 +734,21 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
   unsigned least = 0xffffffffu, most = 0u;
 
   if (wid >= 4 && wid < 8) {
-    for (int j = kPtStages; j < n_tiles; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars.a_empty[j % kPtStages], static_cast<uint32_t>((j / kPtStages - 1) & 1), abort_flag))) {
-        if (lane == 0) report_status(p.status, kWaitTimeout, kKernelPicked, 22, blockIdx.x);
-        // copies on their way land before the shared memory is given back
-        uint32_t none = 0;
-        for (int i = j - kPtStages; i < j; ++i) mbar_wait(&bars.a_full[i % kPtStages], static_cast<uint32_t>((i / kPtStages) & 1), &none);
-        break;
-      }
-      gather(j, next);
-      if (j + 1 < n_tiles) rows_of(j + 1, next);
+    bool ok = true;
+    int sent = min(kPtStages, n_tiles);
+    const auto read = [&](int j) {                           // whether the products of tile j have read its stage
+      return __all_sync(0xffffffffu, mbar_wait(&bars.a_empty[j % kPtStages], static_cast<uint32_t>((j / kPtStages) & 1), abort_flag)) != 0;
+    };
+    for (; sent < n_tiles && (ok = read(sent - kPtStages)); ++sent) {
+      gather(sent, next);
+      if (sent + 1 < n_tiles) rows_of(sent + 1, next);
+    }
+    for (int j = max(0, n_tiles - kPtStages); j < n_tiles && ok; ++j) ok = read(j);      // until the last tiles have been read, or somebody gives up
+    if (!ok) {
+      if (lane == 0) report_status(p.status, kWaitTimeout, kKernelPicked, 22, blockIdx.x);
+      // copies on their way land before the shared memory is given back
+      uint32_t none = 0;
+      for (int i = max(0, sent - kPtStages); i < sent; ++i) mbar_wait(&bars.a_full[i % kPtStages], static_cast<uint32_t>((i / kPtStages) & 1), &none);
     }
   } else if (wid == 1) {
     if (lane == 0) {
@@ -764,6 +771,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) pick_pages_tc_kernel(const Pick
         tc_commit(&bars.s_full[j & 1]);
         tc_commit(&bars.a_empty[s]);
       }
+      // no product reads shared memory or writes TMEM when they are given back, whoever gave up
+      uint32_t none = 0;
+      tc_commit(&bars.drain);
+      mbar_wait(&bars.drain, 0, &none);
     }
     __syncwarp();
   } else if (wid == 3) {

@@ -96,3 +96,15 @@ def test_kernels_let_the_next_one_start_only_once_they_hold_their_tmem():
                 seen += 1
                 assert trigger.start() > alloc.start(), path.name
     assert seen >= 4
+
+
+@pytest.mark.parametrize("name", ["attn_picked_tc", "page_pick"])
+def test_a_block_whose_wait_ran_out_leaves_nothing_on_its_way(name):
+    """(Read from the sources: no wait of a sound block runs out.) Products are waited for before TMEM is given back; whoever sends tiles stays until the last ones
+    have been read, and waits for those on their way where somebody has given up."""
+    text = (Path(ops.__file__).parents[1] / "csrc" / "kernels" / f"{name}.cu").read_text()
+    products, end = re.search(r"tc_commit\(&bars(->|\.)drain\);\s+mbar_wait\(&bars(->|\.)drain, 0, &none\);", text), text.rindex("tmem_dealloc(")
+    assert products and products.start() < end
+    given_up = text.index("copies on their way land")
+    assert text.index("until the last tiles have been read, or somebody gives up") < given_up < end
+    assert re.search(r"mbar_wait\([^;]*_full[^;]*&none\)", text[given_up:end])
