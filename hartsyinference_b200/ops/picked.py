@@ -225,7 +225,8 @@ def attn_picked(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, b
                 if (keys | values) % 16:
                     raise ValueError("attn_picked: pools from 16-byte boundaries")
                 ptrs = (q.data_ptr(), keys, values, out.data_ptr(), picked.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr())
-                if L.b200_attn_picked_form(rows, run * (hq // hkv), hkv, d, page, width, pages, scale, softcap):
+                cols = run * (hq // hkv)          # (few of them never take the tiles: small calls do without the question)
+                if cols > 16 and L.b200_attn_picked_form(rows, cols, hkv, d, page, width, pages, scale, softcap):
                     rc = L.b200_attn_picked_tc(*ptrs, seqs, rows, tokens, hq, hkv, d, page, table[1], pages, run, width, scale, status, N.stream())
                 else:
                     rc = L.b200_attn_picked(*ptrs, seqs, rows, tokens, hq, hkv, d, page, table[1], pages, run, width, scale, float(softcap), status, N.stream())
