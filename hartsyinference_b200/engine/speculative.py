@@ -50,7 +50,7 @@ def find_draft(tokens: Sequence[int], ngram: int = 3, max_draft: int = 8, lookba
     return []
 
 
-def _forward_chunk(engine, seq: int, toks: Sequence[int], start: int) -> torch.Tensor:
+def _forward_chunk(engine, seq: int, toks: Sequence[int], start: int, drafts: bool = False) -> torch.Tensor:
     """Appends ``toks`` at positions [start, start + len) of sequence ``seq`` and returns the hidden
     states of all their rows."""
     count = len(toks)
@@ -70,7 +70,7 @@ def _forward_chunk(engine, seq: int, toks: Sequence[int], start: int) -> torch.T
                          slot_mapping=engine._to_device(engine.h_slots, count),
                          block_table=engine._to_device(engine.h_table, 1),
                          kv_lens=engine._to_device(engine.h_kv_lens, 1), is_decode=False,
-                         cu_q=engine._to_device(engine.h_cu_q, 2), max_q_len=count, max_kv_len=start + count)
+                         cu_q=engine._to_device(engine.h_cu_q, 2), max_q_len=count, max_kv_len=start + count, drafts=drafts)
     return engine.model.forward_hidden(batch)
 
 
@@ -114,7 +114,7 @@ def generate_speculative(engine, prompt: Sequence[int], params: Optional[Samplin
             draft = find_draft(ctx, ngram, max_draft, lookback)
             draft = draft[:max(0, limit - len(out) - 1)]
             # rows: [last emitted token, draft...]; row i predicts the token after position cached + i
-            hidden = _forward_chunk(engine, seq, [out[-1]] + draft, cached)
+            hidden = _forward_chunk(engine, seq, [out[-1]] + draft, cached, drafts=True)
             stats.forward_passes += 1
             stats.drafted += len(draft)
             pred = engine.model.greedy_tokens(hidden.contiguous()).tolist()

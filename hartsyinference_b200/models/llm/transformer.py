@@ -54,6 +54,7 @@ class ForwardBatch:
     cross_row_mask: Optional[torch.Tensor] = None   # Mllama: [T], 0 for text rows that precede every image
     state_slots: Optional[torch.Tensor] = None      # [S] int32 recurrent-state slot of every sequence (-1: none)
     runs: Optional[list] = None                     # ragged batch, host copy: (query tokens, keys) of every sequence
+    drafts: bool = False                            # ragged batch of guessed tokens: each attends to what it would as a decode step
     plan: Optional[object] = None                   # what a mixer works out once per batch for all its layers
 
 
@@ -787,9 +788,9 @@ class DecoderModel:
         first, last = 1, 2
         if (batch.max_kv_len or batch.block_table.shape[1] * page) <= (first + last + self.attn_pages) * page or group > 128:
             return None
-        # tokens of a prompt choose together, as many as fill a tile of 128 rows; a few (drafts to be verified) by themselves, as decoded ones do
+        # tokens of a prompt choose together, as many as fill a tile of 128 rows, whatever else is in the batch; drafts to be verified by themselves, as decoded ones do
         run = 1
-        if cu_q is not None and batch.max_q_len > 16:
+        if cu_q is not None and not batch.drafts:
             run = 1 << (128 // group).bit_length() - 1
         picked = ops.pick_pages(q, bounds, batch.block_table, batch.kv_lens, cu_q, page=page, top=self.attn_pages, first=first, last=last, run=run)
         fp8 = batch.is_decode and self.fp8 and q.is_cuda and lw.o is not None and lw.o.is_fp8 and self.cfg.head_dim == 128

@@ -130,7 +130,7 @@ class PipelinedModel:
                                       slot_mapping=batch.slot_mapping[r0:r1].contiguous(),
                                       block_table=batch.block_table[s0:s1].contiguous(), kv_lens=batch.kv_lens[s0:s1].contiguous(),
                                       is_decode=batch.is_decode, cu_q=cu_q,
-                                      max_q_len=batch.max_q_len, max_kv_len=batch.max_kv_len, logit_rows=lr))
+                                      max_q_len=batch.max_q_len, max_kv_len=batch.max_kv_len, logit_rows=lr, drafts=batch.drafts))
         return parts or [batch]
 
     # -- forward
