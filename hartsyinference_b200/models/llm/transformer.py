@@ -722,10 +722,13 @@ class DecoderModel:
         if cfg.rope_layers and not cfg.rope_layers[self.layer0 + li]:
             rot = 0
         three = cfg.mrope_section and batch.positions3 is not None and rot > 0
+        if three:
+            pos3 = batch.positions3.to(qkv.device)
+            pos3 = pos3 if pos3.is_floating_point() else pos3.to(torch.int32)      # (the op refuses others)
         if three and (kv4 is not None or cfg.qk_norm_after_rope):
             # rotated here (the heads' norm comes first, unless the model has it behind), stored by the op below
             before = not cfg.qk_norm_after_rope
-            parts = ops.rope_axes_kv(qkv, batch.positions3, self.hq, self.hkv, d, axes=self._rope_axes(inv_freq.numel()), inv_freq=inv_freq, style=cfg.rope_style,
+            parts = ops.rope_axes_kv(qkv, pos3, self.hq, self.hkv, d, axes=self._rope_axes(inv_freq.numel()), inv_freq=inv_freq, style=cfg.rope_style,
                                      q_norm_w=q_norm_w if before else None, k_norm_w=k_norm_w if before else None, eps=cfg.rms_eps, want_kv=True)
             qkv = torch.cat([x.reshape(t, -1) for x in parts], 1)
             q_norm_w, k_norm_w = (None, None) if before else (q_norm_w, k_norm_w)
@@ -743,7 +746,7 @@ class DecoderModel:
         if kv4 is not None:
             return self._attention_kv4(lw, kv4, qkv, q_norm_w, k_norm_w, rot, inv_freq, batch, scale, window)
         if three:
-            q, _, _ = ops.rope_axes_kv(qkv, batch.positions3, self.hq, self.hkv, d, axes=self._rope_axes(inv_freq.numel()), inv_freq=inv_freq, k_cache=kc, v_cache=vc,
+            q, _, _ = ops.rope_axes_kv(qkv, pos3, self.hq, self.hkv, d, axes=self._rope_axes(inv_freq.numel()), inv_freq=inv_freq, k_cache=kc, v_cache=vc,
                                        slot_mapping=batch.slot_mapping if kc is not None else None, style=cfg.rope_style, q_norm_w=q_norm_w, k_norm_w=k_norm_w, eps=cfg.rms_eps)
         else:
             q, _, _ = ops.rope_kv(qkv, batch.positions, self.hq, self.hkv, d, k_cache=kc, v_cache=vc,
