@@ -4,10 +4,12 @@
 //   angle(t, j) = positions[axes[j]][t] * inv_freq[j]         (a, b) -> (a cos - b sin, b cos + a sin)
 //
 // Angles are the tokens', not the heads': a block works out those of its tokens once, as whole and broken turns in 64 bits, since a position of
-// 100000 would leave 32 bits 8 bits behind the point; what is left of the turn, at most half of it, goes through the 32-bit functions.
+// 100000 would leave 32 bits 7 bits behind the point; what is left of the turn, at most half of it, goes through the 32-bit functions.
 #include "common.cuh"
 
 namespace b200 {
+
+int num_sms();      // of the current device, see gemm_tcgen05.cu
 
 struct RopeAxesParams {
   const __nv_bfloat16* qkv;        // [tokens][(hq + 2 hkv) d]
@@ -263,7 +265,7 @@ static cudaError_t launch_rope_axes(RopeAxesParams p, cudaStream_t stream) {
   if (norm)
     for (lanes = 1; lanes * 2 * V < p.d;) lanes *= 2;
   const int each = 256 / lanes, chunks = (p.hq + 2 * p.hkv + each - 1) / each;
-  p.block_tokens = p.tokens >= 148 * 8 ? 4 : 1;      // more tokens a block once every processor has several
+  p.block_tokens = p.tokens >= num_sms() * 8 ? 4 : 1;      // more tokens a block once every processor has several
   return launch_pdl(rope_axes_kernel<V>, dim3((p.tokens + p.block_tokens - 1) / p.block_tokens, p.block_tokens == 1 ? chunks : 1), dim3(256),
                     (p.block_tokens * 2 * (((p.rot >> 1) + 3) & ~3) + (norm ? 2 * p.d : 0)) * sizeof(float), stream, p, lanes);
 }

@@ -1,4 +1,7 @@
 """Rotary positions on several axes: calls that a model takes in other forms."""
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -26,3 +29,10 @@ def test_a_models_positions_are_whole_numbers_of_any_type_on_any_device(dev, kv_
     assert all(torch.equal(x, outs[0]) for x in outs)
     if dev == "cuda":
         N.check_status()
+
+
+@pytest.mark.parametrize("name", ["rope_axes", "page_pick", "attn_picked", "attn_picked_tc"])
+def test_rules_ask_how_many_processors_there_are(name):
+    text = (Path(qwen_vl.__file__).parents[2] / "csrc" / "kernels" / f"{name}.cu").read_text()
+    code = "\n".join(line.split("//")[0] for line in text.splitlines())
+    assert not re.search(r"\b148\b", code)
