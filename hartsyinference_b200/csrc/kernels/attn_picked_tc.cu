@@ -24,6 +24,7 @@ int make_heads_map(CUtensorMap* out, const void* base, long long tokens, int hea
 constexpr int kTpThreads = 256;
 constexpr int kTpTile = 64;               // keys
 constexpr int kTpStages = 2;
+constexpr int kTpRegisters = 128;         // of a thread at launch; the first four warps give 64 of them to the softmax warps
 constexpr int kTpWidth = 1024;            // pages of a row that the list in shared memory holds
 constexpr int kTpFar = 0x40000000;        // first key of what is no page
 constexpr float kTpRescaleGap = 8.f;
@@ -443,6 +444,13 @@ static int launch_picked_tc(const TpParams& p, int rows, int tokens, cudaStream_
   static PerDeviceOnce configured;
   if (configured.first_time() && cudaFuncSetAttribute(attn_picked_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 115712) != cudaSuccess) return -200;
   if (smem > 115712) return -6;
+  static int registers;                   // of the kernel as it was built
+  if (registers == 0) {
+    cudaFuncAttributes has{};
+    if (cudaFuncGetAttributes(&has, attn_picked_tc_kernel<D>) != cudaSuccess) return -200;
+    registers = has.numRegs;
+  }
+  if (registers != kTpRegisters) return -8;      // the softmax warps would wait for registers that nobody gives back
   const cudaError_t e = launch_pdl(attn_picked_tc_kernel<D>, dim3(rows, p.hkv), dim3(kTpThreads), smem, stream, p, tq, tk, tv);
   return e == cudaSuccess ? 0 : -static_cast<int>(e) - 300;
 }

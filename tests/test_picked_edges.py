@@ -108,3 +108,12 @@ def test_a_block_whose_wait_ran_out_leaves_nothing_on_its_way(name):
     given_up = text.index("copies on their way land")
     assert text.index("until the last tiles have been read, or somebody gives up") < given_up < end
     assert re.search(r"mbar_wait\([^;]*_full[^;]*&none\)", text[given_up:end])
+
+
+def test_a_build_with_other_registers_is_refused():
+    """Warps that take more registers wait for those that others give back: 4 warps from 128 to 64, 4 from 128 to 192. The launch asks what the kernel was built with."""
+    text = (Path(ops.__file__).parents[1] / "csrc" / "kernels" / "attn_picked_tc.cu").read_text()
+    held = int(re.search(r"kTpRegisters = (\d+);", text)[1])
+    dec, inc = (int(re.search(rf"setmaxnreg\.{x}\.sync\.aligned\.u32 (\d+);", text)[1]) for x in ("dec", "inc"))
+    assert dec + inc == 2 * held
+    assert text.index("has.numRegs") < text.index("registers != kTpRegisters) return") < text.index("launch_pdl(attn_picked_tc_kernel")
