@@ -117,3 +117,16 @@ def test_a_build_with_other_registers_is_refused():
     dec, inc = (int(re.search(rf"setmaxnreg\.{x}\.sync\.aligned\.u32 (\d+);", text)[1]) for x in ("dec", "inc"))
     assert dec + inc == 2 * held
     assert text.index("has.numRegs") < text.index("registers != kTpRegisters) return") < text.index("launch_pdl(attn_picked_tc_kernel")
+
+
+@gpu
+@pytest.mark.parametrize("hq,hkv,d,run", [(8, 1, 128, 16), (14, 2, 64, 18), (64, 1, 128, 2)])
+def test_many_runs_under_a_table_too_wide_for_the_tiles(hq, hkv, d, run):
+    """A table of 40000 columns, of which a sequence uses 180: its scores have no room beside the tiles, and the other kernel chooses the same pages."""
+    b = Batch([2800], [2880], hq, hkv, d, 16, seed=run).fill_bounds()
+    assert ((sum(b.each) + run - 1) // run) * hkv > 148
+    want = b.pick(top=9, run=run)
+    narrow = b.to("cuda").pick(top=9, run=run)
+    b.table = torch.cat([b.table, torch.full((1, 40000), -1, dtype=torch.int32, device="cuda")], 1)
+    assert torch.equal(narrow.cpu(), want) and torch.equal(b.pick(top=9, run=run).cpu(), want)
+    N.check_status()
