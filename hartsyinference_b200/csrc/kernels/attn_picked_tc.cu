@@ -9,7 +9,8 @@
 //                read from TMEM, V is consumed as it lies in the pages (an MN-major operand)
 //   warp 2       in tiles with keys that not all rows see: clears the rows of V behind the last key (what a page held before may not be
 //                finite, and its probability is zero), and rows with values that are not finite, which the rows that see them add by themselves
-//   warps 4..7   softmax, one row per thread, lazy rescale: the running maximum is raised only when it grows by more than 2^8
+//   warps 4..7   softmax, one row per thread, lazy rescale: the running maximum is raised only when it grows by more than 2^8; sums in 32 bits, of unrounded
+//                probabilities, which are rounded to bf16 once: the second product takes them in the type of V
 //
 // 2048 queries of 64 heads on 8, runs of 16, 2144 keys each behind 30720: 197 us (711 TFLOP/s; 1134 by mma.sync). Bound by the two CTAs' products and the softmax
 // about equally: a product of 16 channels takes as long for 64 keys as for 128, since Q is read from shared memory for each. Tiles of 128 keys with one set of

@@ -932,6 +932,8 @@ B200_API int b200_pick_pages(const void* q, const void* bounds, const int* block
   // 16, 1000, 200 42 / 40; 16, 1000, 1000 70 / 78; 24, 160, 1000 19 / 25; 24, 300, 500 25 / 25; 32, 600, 270 33 / 34; 32, 2000, 1920 182 / 285; 64, 304, 270 23 / 25;
   // 64, 64, 1880 28 / 21; 128, 152, 270 15 / 25; 128, 32, 1880 33 / 21; 128, 504, 1920 67 / 157; heads of 64: 28, 500, 1920 43 / 62; 56, 76, 270 12 / 9;
   // 112, 126, 1920 32 / 27.
+  // The scores of two runs lie in shared memory, 8 bytes for every column of the block table, however few of them a sequence uses (how many that is only the device
+  // knows): heads of 128 leave room for 8300 columns, and under wider tables the other kernel chooses (2048 queries of 64 heads behind 30720: 140 us under 8048 columns, 285 under 9048).
   const long long smem_tc = 1024 + (kPtStages * kPtTile + 2 * kPickRows) * 2 * d + 2 * kPickRows * 4 + static_cast<int>(sizeof(PickTcShared)) + 8ll * max_pages;
   if (run * (hq / hkv) > 16 && static_cast<long long>(rows) * hkv > num_sms() && smem_tc <= 232448 && static_cast<long long>(rows) * hkv < (1ll << 31) && pages * hkv < (1ll << 31)) {
     p.pairs = static_cast<int>((tokens + static_cast<long long>(seqs) * (2 * run - 1)) / (2 * run));
